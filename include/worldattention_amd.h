@@ -717,6 +717,35 @@ typedef struct wa_hkv_gather_rotate_args {
 } wa_hkv_gather_rotate_args;
 int wa_hkv_gather_rotate(const wa_hkv_gather_rotate_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------ */
+/* Token-by-token operators (no reference counterpart)                                         */
+/* ------------------------------------------------------------------------------------------ */
+
+/* Rotary positions with several axes on a BLHD query tensor and (k not NULL) a key tensor with its
+ * own number of heads, in one launch. Pair p of a head turns by the angle
+ * positions[b, t, axis(p)] * inv_freq[p] (its negative with `inverse`: the gradient); the pairs are
+ * dealt to the axes in runs of sections[0], sections[1], ... pairs (n_axes of them, 4 at most).
+ * Pair p holds channels (2p, 2p + 1) with `interleaved`, else (p, p + P) of P pairs; channels from
+ * 2P on are copied. The angle is formed and reduced in fp64, its sine and cosine and the rotation
+ * are fp32, the result is rounded once to the tensors' dtype. positions: device int64 (pos_int64)
+ * or int32 with element strides (p_sb = 0: shared by the batch). q_out / k_out must not overlap
+ * the inputs. */
+#define WA_ROPE_MAX_AXES 4
+#define WA_ROPE_MAX_DIM 1024
+typedef struct wa_rope_axes_args {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  void* q_out; int64_t qo_sb, qo_st, qo_sh;
+  const void* k; int64_t k_sb, k_st, k_sh;
+  void* k_out; int64_t ko_sb, ko_st, ko_sh;
+  int32_t dtype;
+  int64_t B, L, Hq, Hk, D;
+  const void* positions; int64_t p_sb, p_st, p_sa; int32_t pos_int64;
+  const double* inv_freq;
+  int64_t n_axes; int64_t sections[WA_ROPE_MAX_AXES];
+  int32_t interleaved, inverse;
+} wa_rope_axes_args;
+int wa_rope_axes(const wa_rope_axes_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,9 @@ reference's attention path:
   (reference: ``wan/modules/hsa/{routing,block_sparse_torch,attention}.py``,
   ``trainer/hsa_stage.py``);
 * ``oracle.hkv`` — page summaries, temporal re-rotation, two-stage retrieval, install planning and
-  the LRU tier (reference: ``pipeline/hkv/{retrieval,rope,cache,tiering}.py``).
+  the LRU tier (reference: ``pipeline/hkv/{retrieval,rope,cache,tiering}.py``);
+* ``oracle.token`` — the token-by-token operators in fp64 from their definitions (no reference
+  counterpart).
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and the ``cpu_baseline`` leg of ``bench.py`` may
 import this package, and only as the checker or the reported CPU baseline. The product package

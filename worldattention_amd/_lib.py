@@ -339,6 +339,21 @@ HkvCopy = _struct("wa_hkv_copy", [
     ("width", c_int64), ("rows", c_int64),
 ])
 
+ROPE_MAX_AXES, ROPE_MAX_DIM = 4, 1024
+
+RopeAxesArgs = _struct("wa_rope_axes_args", [
+    ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+    ("q_out", c_void_p), ("qo_sb", c_int64), ("qo_st", c_int64), ("qo_sh", c_int64),
+    ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
+    ("k_out", c_void_p), ("ko_sb", c_int64), ("ko_st", c_int64), ("ko_sh", c_int64),
+    ("dtype", c_int32),
+    ("B", c_int64), ("L", c_int64), ("Hq", c_int64), ("Hk", c_int64), ("D", c_int64),
+    ("positions", c_void_p), ("p_sb", c_int64), ("p_st", c_int64), ("p_sa", c_int64), ("pos_int64", c_int32),
+    ("inv_freq", c_void_p),
+    ("n_axes", c_int64), ("sections", c_int64 * ROPE_MAX_AXES),
+    ("interleaved", c_int32), ("inverse", c_int32),
+])
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "wa_version": (c_int, []),
@@ -385,6 +400,7 @@ SIGNATURES = {
     "wa_hkv_page_summary": (c_int, [POINTER(HkvSummaryArgs), c_void_p]),
     "wa_hkv_score_topk": (c_int, [POINTER(HkvTopkArgs), c_void_p]),
     "wa_rerope": (c_int, [POINTER(RopeArgs), c_void_p]),
+    "wa_rope_axes": (c_int, [POINTER(RopeAxesArgs), c_void_p]),
     "wa_hkv_gather_async": (c_int, [POINTER(HkvCopy), c_int64, c_void_p, c_void_p]),
     "wa_hkv_store_async": (c_int, [POINTER(HkvCopy), c_int64, c_void_p, c_void_p]),
 }
@@ -414,6 +430,16 @@ def call(name: str, *args) -> None:
         if rc < 0:
             raise ValueError(f"{name}: {msg}")
         raise RuntimeError(f"{name} failed (hip error {rc}): {msg}")
+
+
+def launch(name: str, args, dev: torch.device) -> None:
+    """:func:`call` on ``dev``'s current stream, with ``dev`` made the current device around it (a kernel
+    launch takes the current device's)."""
+    if dev.index == torch.cuda.current_device():
+        call(name, args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, args, torch.cuda.current_stream(dev).cuda_stream)
 
 
 # ----------------------------------------------------------------------------------------------

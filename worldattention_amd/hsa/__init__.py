@@ -10,6 +10,7 @@ from .attention import (
 )
 from .kvcache import kv_append, new_block_sums
 from .block_sparse import block_sparse_attention, block_sparse_attention_reference, map_to_index
+from .rope import axis_frequencies, rope_axes
 from .routing import (
     BlockRouting,
     block_attention_map,
@@ -35,4 +36,6 @@ __all__ = [
     "block_mean_pool",
     "kv_append",
     "new_block_sums",
+    "rope_axes",
+    "axis_frequencies",
 ]
