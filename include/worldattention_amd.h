@@ -746,6 +746,74 @@ typedef struct wa_rope_axes_args {
 } wa_rope_axes_args;
 int wa_rope_axes(const wa_rope_axes_args* args, void* stream);
 
+/* Linear attention with a decay for each head, causal, over BLHD tensors of one dtype (fp32 or bf16)
+ * and head dim D = 64 or 128:
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   S_{-1} = initial (NULL: 0).
+ * log_decay: device fp32 [H], meant to be <= 0 (-inf: a head without memory). lengths (optional):
+ * device int32 [B], clamped to [0, L]: tokens from lengths[b] on are not read, their outputs (and
+ * gradients) are 0 and the state ends at the last token before them.
+ * The sequence is cut into wa_decay_segments(B, L, H) segments. `states` (device fp32
+ * [B, H, segments, D, D]) receives the state before each, which the backward takes back;
+ * initial / final: fp32 [B, H, D, D] (key channel, value channel), contiguous; final may be NULL.
+ * Rows must be 16-byte aligned. The state is kept and summed in fp32. */
+int64_t wa_decay_segments(int64_t B, int64_t L, int64_t H);
+typedef struct wa_decay_fwd_args {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const void* k; int64_t k_sb, k_st, k_sh;
+  const void* v; int64_t v_sb, v_st, v_sh;
+  void* o; int64_t o_sb, o_st, o_sh;
+  int32_t dtype;
+  int64_t B, L, H, D;
+  const float* log_decay;
+  const int32_t* lengths;
+  const float* initial;
+  float* final_state;
+  float* states;
+  float scale;
+} wa_decay_fwd_args;
+int wa_decay_fwd(const wa_decay_fwd_args* args, void* stream);
+
+/* Gradients of wa_decay_fwd. dfinal (NULL: 0): the gradient of the final state. dq, dk, dv are
+ * written in the inputs' dtype; dinitial (fp32) and dlog_decay (fp32 [H], summed in a fixed order)
+ * are optional. The workspace (device, wa_decay_bwd_workspace_bytes) holds the gradient states. */
+int64_t wa_decay_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D);
+typedef struct wa_decay_bwd_args {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const void* k; int64_t k_sb, k_st, k_sh;
+  const void* v; int64_t v_sb, v_st, v_sh;
+  const void* dout; int64_t d_sb, d_st, d_sh;
+  void* dq; int64_t dq_sb, dq_st, dq_sh;
+  void* dk; int64_t dk_sb, dk_st, dk_sh;
+  void* dv; int64_t dv_sb, dv_st, dv_sh;
+  int32_t dtype;
+  int64_t B, L, H, D;
+  const float* log_decay;
+  const int32_t* lengths;
+  const float* states;
+  const float* dfinal;
+  float* dinitial;
+  float* dlog_decay;
+  void* workspace;
+  float scale;
+} wa_decay_bwd_args;
+int wa_decay_bwd(const wa_decay_bwd_args* args, void* stream);
+
+/* The same recurrence for L tokens (one, as a decoding step makes it, or a few), one after the other,
+ * with the fp32 state [B, H, D, Dv] (strides st_sb, st_sh; rows contiguous) updated in place. Any
+ * head dims 1 .. 256; bf16 or fp32 tensors of any strides with contiguous channels. */
+typedef struct wa_decay_step_args {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const void* k; int64_t k_sb, k_st, k_sh;
+  const void* v; int64_t v_sb, v_st, v_sh;
+  void* o; int64_t o_sb, o_st, o_sh;
+  int32_t dtype;
+  int64_t B, L, H, D, Dv;
+  const float* log_decay;
+  float* state; int64_t st_sb, st_sh;
+  float scale;
+} wa_decay_step_args;
+int wa_decay_step(const wa_decay_step_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

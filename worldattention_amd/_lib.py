@@ -354,6 +354,41 @@ RopeAxesArgs = _struct("wa_rope_axes_args", [
     ("interleaved", c_int32), ("inverse", c_int32),
 ])
 
+DecayFwdArgs = _struct("wa_decay_fwd_args", [
+    ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+    ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
+    ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64), ("v_sh", c_int64),
+    ("o", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
+    ("dtype", c_int32),
+    ("B", c_int64), ("L", c_int64), ("H", c_int64), ("D", c_int64),
+    ("log_decay", c_void_p), ("lengths", c_void_p), ("initial", c_void_p), ("final_state", c_void_p),
+    ("states", c_void_p), ("scale", c_float),
+])
+
+DecayBwdArgs = _struct("wa_decay_bwd_args", [
+    ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+    ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
+    ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64), ("v_sh", c_int64),
+    ("dout", c_void_p), ("d_sb", c_int64), ("d_st", c_int64), ("d_sh", c_int64),
+    ("dq", c_void_p), ("dq_sb", c_int64), ("dq_st", c_int64), ("dq_sh", c_int64),
+    ("dk", c_void_p), ("dk_sb", c_int64), ("dk_st", c_int64), ("dk_sh", c_int64),
+    ("dv", c_void_p), ("dv_sb", c_int64), ("dv_st", c_int64), ("dv_sh", c_int64),
+    ("dtype", c_int32),
+    ("B", c_int64), ("L", c_int64), ("H", c_int64), ("D", c_int64),
+    ("log_decay", c_void_p), ("lengths", c_void_p), ("states", c_void_p), ("dfinal", c_void_p),
+    ("dinitial", c_void_p), ("dlog_decay", c_void_p), ("workspace", c_void_p), ("scale", c_float),
+])
+
+DecayStepArgs = _struct("wa_decay_step_args", [
+    ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+    ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
+    ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64), ("v_sh", c_int64),
+    ("o", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
+    ("dtype", c_int32),
+    ("B", c_int64), ("L", c_int64), ("H", c_int64), ("D", c_int64), ("Dv", c_int64),
+    ("log_decay", c_void_p), ("state", c_void_p), ("st_sb", c_int64), ("st_sh", c_int64), ("scale", c_float),
+])
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "wa_version": (c_int, []),
@@ -401,6 +436,11 @@ SIGNATURES = {
     "wa_hkv_score_topk": (c_int, [POINTER(HkvTopkArgs), c_void_p]),
     "wa_rerope": (c_int, [POINTER(RopeArgs), c_void_p]),
     "wa_rope_axes": (c_int, [POINTER(RopeAxesArgs), c_void_p]),
+    "wa_decay_segments": (c_int64, [c_int64] * 3),
+    "wa_decay_fwd": (c_int, [POINTER(DecayFwdArgs), c_void_p]),
+    "wa_decay_bwd_workspace_bytes": (c_int64, [c_int64] * 4),
+    "wa_decay_bwd": (c_int, [POINTER(DecayBwdArgs), c_void_p]),
+    "wa_decay_step": (c_int, [POINTER(DecayStepArgs), c_void_p]),
     "wa_hkv_gather_async": (c_int, [POINTER(HkvCopy), c_int64, c_void_p, c_void_p]),
     "wa_hkv_store_async": (c_int, [POINTER(HkvCopy), c_int64, c_void_p, c_void_p]),
 }

@@ -10,6 +10,7 @@ from .attention import (
 )
 from .kvcache import kv_append, new_block_sums
 from .block_sparse import block_sparse_attention, block_sparse_attention_reference, map_to_index
+from .decay import decay_linear_attention, decay_linear_step
 from .rope import axis_frequencies, rope_axes
 from .routing import (
     BlockRouting,
@@ -38,4 +39,6 @@ __all__ = [
     "new_block_sums",
     "rope_axes",
     "axis_frequencies",
+    "decay_linear_attention",
+    "decay_linear_step",
 ]
