@@ -814,6 +814,52 @@ typedef struct wa_decay_step_args {
 } wa_decay_step_args;
 int wa_decay_step(const wa_decay_step_args* args, void* stream);
 
+/* Key blocks of a cache for single queries. The n queries of sequence b are its last n tokens: query i
+ * sits at token kv_len[b] - n + i and sees the tokens up to its own, the blocks up to the one its own
+ * token is in (none if that is before token 0). Shared key heads (GQA): query heads
+ * hk (H / Hk) .. (hk + 1)(H / Hk) - 1 read key head hk and share its choice. Chosen are the first
+ * sink_blocks and the last local_blocks (>= 1) seen blocks and, up to topk in all, those whose
+ *   score_j = (sum of the group's queries) . k_sums[b, hk, j]
+ * is largest (formed in fp64, so neither the launch's shape nor the batch moves a border; ties take
+ * the lowest id, NaN counts as the largest). Every scored block is whole, so the sums need no division.
+ * k_sums: fp32 [B, Hk, n_blocks, D] as wa_kv_append keeps them. kv_len: device int32 [B] (NULL:
+ * kv_len_all), clamped to [0, cap]; cap <= n_blocks * block_size (0: that).
+ * index: int32 [B, n, Hk, topk], ascending, -1 behind; num: int32 [B, n, Hk]. D = 64 or 128. */
+#define WA_SELECT_MAX_BLOCKS 32768
+int64_t wa_select_blocks_workspace_bytes(int64_t B, int64_t n, int64_t Hk, int64_t n_blocks);
+typedef struct wa_select_blocks_args {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const float* k_sums; int64_t n_blocks;
+  const int32_t* kv_len; int64_t kv_len_all, cap;
+  int64_t B, n, H, Hk, D;
+  int64_t block_size, topk, sink_blocks, local_blocks;
+  int32_t* index; int32_t* num;
+  void* workspace;
+} wa_select_blocks_args;
+int wa_select_blocks(const wa_select_blocks_args* args, void* stream);
+
+/* Attention of the same queries over the listed blocks' seen tokens: softmax(scale q K^T) V, bf16
+ * tensors, fp32 statistics. index / num as above (any int32 lists: an id that names no seen block adds
+ * nothing, one listed twice counts twice). A query that sees nothing gets 0 and a log-sum-exp of
+ * -inf. Keys and values behind a sequence's end are not used, whatever they hold. k, v: BLHD
+ * [B, cap, Hk, D] with 16-byte aligned rows; lse: fp32 [B, H, n] or NULL; block_size 64 or 128. */
+int64_t wa_selected_attn_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t Hk, int64_t D, int64_t topk,
+                                         int64_t block_size);
+typedef struct wa_selected_attn_args {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const void* k; int64_t k_sb, k_st, k_sh;
+  const void* v; int64_t v_sb, v_st, v_sh;
+  void* o; int64_t o_sb, o_st, o_sh;
+  float* lse;
+  const int32_t* index; const int32_t* num; int64_t topk;
+  const int32_t* kv_len; int64_t kv_len_all;
+  int64_t B, n, cap, H, Hk, D;
+  int64_t block_size;
+  float scale;
+  void* workspace;
+} wa_selected_attn_args;
+int wa_selected_attn(const wa_selected_attn_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -55,8 +55,8 @@ def select_key_blocks(q, k_block_sums, kv_len, *, block_size, topk, sink_blocks=
             blocks = -(-seen // block_size)
             forced = {j for j in range(blocks) if j < sink_blocks or j >= blocks - local_blocks}
             for hi in range(hk):
-                row = scores[bi, hi, i]
-                key = lambda j: (0 if math.isnan(row[j]) else 1, -float(row[j]), j)  # noqa: E731  NaN first, as the largest
+                row = scores[bi, hi, i].tolist()
+                key = lambda j: (0 if math.isnan(row[j]) else 1, -row[j], j)  # noqa: E731  NaN first, as the largest
                 rest = sorted((j for j in range(blocks) if j not in forced), key=key)
                 pick = sorted(forced | set(rest[:topk - len(forced)]))
                 num[bi, i, hi] = len(pick)

@@ -114,3 +114,74 @@ def test_decay_entry_points_refuse():
     s = _lib.DecayStepArgs()
     s.B, s.L, s.H, s.D, s.Dv, s.dtype = 1, 1, 2, 300, 64, _lib.WA_F32
     assert lib.wa_decay_step(ctypes.byref(s), None) == _lib.WA_ERR_ARG and b"1 .. 256" in lib.wa_last_error()
+
+
+def _bf(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+def _selected(which, **kw):
+    a = dict(q=_bf(2, 3, 8, 64), k=_bf(2, 200, 2, 64), v=_bf(2, 200, 2, 64), sums=torch.zeros(2, 2, 4, 64), kv_len=200,
+             block_size=64, topk=4, sink=1, local=1, index=torch.zeros(2, 3, 2, 4, dtype=torch.int32),
+             num=torch.zeros(2, 3, 2, dtype=torch.int32), scale=None)
+    a.update(kw)
+    if which == "select":
+        return W.select_key_blocks(a["q"], a["sums"], a["kv_len"], block_size=a["block_size"], topk=a["topk"],
+                                   sink_blocks=a["sink"], local_blocks=a["local"])
+    if which == "attend":
+        return W.selected_attention(a["q"], a["k"], a["v"], a["index"], a["num"], a["kv_len"], block_size=a["block_size"],
+                                    scale=a["scale"])
+    cache = {"k": a["k"], "v": a["v"], "k_block_sums": a["sums"], "k_block_sums_block_size": a["block_size"]}
+    return W.attend_selected(a["q"], cache, a["kv_len"], topk=a["topk"], sink_blocks=a["sink"], local_blocks=a["local"],
+                             scale=a["scale"])
+
+
+@pytest.mark.parametrize("which,bad,match", [(w, b, m) for ws, b, m in [
+    ("select attend both", dict(q=_bf(3, 3, 8, 64)), "q must be"), ("select attend both", dict(q=_bf(2, 3, 7, 64)), "do not share"),
+    ("select attend both", dict(q=torch.zeros(2, 3, 8, 64)), "bf16"), ("select attend both", dict(block_size=32), "block_size"),
+    ("select attend both", dict(kv_len=torch.zeros(2, dtype=torch.int64)), "kv_len"),
+    ("select attend both", dict(kv_len=torch.zeros(3, dtype=torch.int32)), "kv_len"),
+    ("select both", dict(topk=1), "must hold"), ("select both", dict(local=0), "must hold"), ("select both", dict(sink=-1), "must hold"),
+    ("select both", dict(topk=32769), "at most"), ("select both", dict(sums=torch.zeros(2, 2, 4, 64).double()), "fp32"),
+    ("select both", dict(sums=torch.zeros(2, 2, 64, 4).transpose(-1, -2)), "contiguous"), ("both", dict(sums=torch.zeros(2, 2, 5, 64)), "k_block_sums"),
+    ("select", dict(sums=torch.zeros(2, 2, 0, 64)), "blocks"), ("select", dict(q=_bf(2, 3, 8, 96), sums=torch.zeros(2, 2, 4, 96)), "64 or 128"),
+    ("attend both", dict(v=_bf(2, 200, 1, 64)), "matching"), ("attend both", dict(k=_bf(2, 200, 2, 64).float()), "bf16"),
+    ("attend both", dict(k=_bf(2, 200, 64, 2).transpose(2, 3)), "in place"), ("attend both", dict(scale=0.0), "scale"),
+    ("attend", dict(index=torch.zeros(2, 3, 1, 4, dtype=torch.int32)), "index / num"), ("attend", dict(num=torch.zeros(2, 3, 2)), "int32"),
+    ("attend", dict(index=torch.zeros(2, 3, 2, 0, dtype=torch.int32)), "ids a row")] for w in ws.split()])
+def test_selected_attention_refuses(which, bad, match):
+    with pytest.raises(ValueError, match=match):
+        _selected(which, **bad)
+
+
+def test_selected_attention_refuses_gradients_missing_sums_and_cpu_tensors():
+    for which in ("select", "attend", "both"):
+        with pytest.raises(ValueError, match="takes no gradient"):
+            _selected(which, q=_bf(2, 3, 8, 64).requires_grad_(True))
+        with pytest.raises(RuntimeError, match="ROCm GPU"):
+            _selected(which)
+    with pytest.raises(ValueError, match="keeps no k_block_sums"):
+        W.attend_selected(_bf(1, 1, 2, 64), {"k": _bf(1, 9, 2, 64), "v": _bf(1, 9, 2, 64)}, 9, topk=2)
+
+
+def test_selected_entry_points_refuse():
+    lib = _lib.lib()
+    assert lib.wa_select_blocks(None, None) == _lib.WA_ERR_ARG and lib.wa_selected_attn(None, None) == _lib.WA_ERR_ARG
+    a = _lib.SelectBlocksArgs()
+    a.q = a.k_sums = a.index = a.num = a.workspace = FAKE
+    a.B, a.n, a.H, a.Hk, a.D, a.block_size, a.n_blocks, a.topk, a.sink_blocks, a.local_blocks = 1, 1, 4, 3, 64, 64, 4, 4, 1, 1
+    for field, bad, match in (("Hk", 3, b"heads"), ("D", 80, b"head dim"), ("block_size", 16, b"block size"), ("topk", 0, b"topk"),
+                              ("n_blocks", 40000, b"blocks"), ("cap", 257, b"do not hold"), ("local_blocks", 4, b"local"),
+                              ("q", FAKE + 2, b"misaligned"), ("workspace", None, b"null")):
+        a.Hk = 2
+        keep = getattr(a, field)
+        setattr(a, field, bad)
+        assert lib.wa_select_blocks(ctypes.byref(a), None) == _lib.WA_ERR_ARG and match in lib.wa_last_error(), field
+        setattr(a, field, keep)
+    s = _lib.SelectedAttnArgs()
+    s.q = s.k = s.v = s.o = s.index = s.num = FAKE
+    s.B, s.n, s.cap, s.H, s.Hk, s.D, s.block_size, s.topk = 1, 1, 4096, 4, 2, 64, 64, 64
+    assert lib.wa_selected_attn_workspace_bytes(1, 1, 4, 2, 64, 64, 64) > 0
+    assert lib.wa_selected_attn(ctypes.byref(s), None) == _lib.WA_ERR_ARG and b"workspace" in lib.wa_last_error()
+    s.k_st = 3
+    assert lib.wa_selected_attn(ctypes.byref(s), None) == _lib.WA_ERR_ARG and b"aligned" in lib.wa_last_error()

@@ -389,6 +389,28 @@ DecayStepArgs = _struct("wa_decay_step_args", [
     ("log_decay", c_void_p), ("state", c_void_p), ("st_sb", c_int64), ("st_sh", c_int64), ("scale", c_float),
 ])
 
+SELECT_MAX_BLOCKS = 32768
+
+SelectBlocksArgs = _struct("wa_select_blocks_args", [
+    ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+    ("k_sums", c_void_p), ("n_blocks", c_int64),
+    ("kv_len", c_void_p), ("kv_len_all", c_int64), ("cap", c_int64),
+    ("B", c_int64), ("n", c_int64), ("H", c_int64), ("Hk", c_int64), ("D", c_int64),
+    ("block_size", c_int64), ("topk", c_int64), ("sink_blocks", c_int64), ("local_blocks", c_int64),
+    ("index", c_void_p), ("num", c_void_p), ("workspace", c_void_p),
+])
+
+SelectedAttnArgs = _struct("wa_selected_attn_args", [
+    ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+    ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
+    ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64), ("v_sh", c_int64),
+    ("o", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
+    ("lse", c_void_p), ("index", c_void_p), ("num", c_void_p), ("topk", c_int64),
+    ("kv_len", c_void_p), ("kv_len_all", c_int64),
+    ("B", c_int64), ("n", c_int64), ("cap", c_int64), ("H", c_int64), ("Hk", c_int64), ("D", c_int64),
+    ("block_size", c_int64), ("scale", c_float), ("workspace", c_void_p),
+])
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "wa_version": (c_int, []),
@@ -441,6 +463,10 @@ SIGNATURES = {
     "wa_decay_bwd_workspace_bytes": (c_int64, [c_int64] * 4),
     "wa_decay_bwd": (c_int, [POINTER(DecayBwdArgs), c_void_p]),
     "wa_decay_step": (c_int, [POINTER(DecayStepArgs), c_void_p]),
+    "wa_select_blocks_workspace_bytes": (c_int64, [c_int64] * 4),
+    "wa_select_blocks": (c_int, [POINTER(SelectBlocksArgs), c_void_p]),
+    "wa_selected_attn_workspace_bytes": (c_int64, [c_int64] * 7),
+    "wa_selected_attn": (c_int, [POINTER(SelectedAttnArgs), c_void_p]),
     "wa_hkv_gather_async": (c_int, [POINTER(HkvCopy), c_int64, c_void_p, c_void_p]),
     "wa_hkv_store_async": (c_int, [POINTER(HkvCopy), c_int64, c_void_p, c_void_p]),
 }

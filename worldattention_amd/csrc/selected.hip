@@ -1,0 +1,521 @@
+// Attention of single queries over key blocks that a score selects from a KV cache: the selection from
+// the cached key block sums (route.hip keeps its own for whole query blocks) and the attention over the
+// chosen blocks, for a decoding step, a few drafted tokens or a prompt chunk. No reference counterpart.
+#include <algorithm>
+
+#include "common.h"
+
+namespace {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+
+// Tokens query i of n sees: those up to its own, token length - n + i.
+__device__ __forceinline__ int64_t seen_tokens(const int32_t* kv_len, int64_t kv_len_all, int64_t cap, int n, int b, int i) {
+  const int64_t len = kv_len ? (int64_t)kv_len[b] : kv_len_all;
+  const int64_t in = len < 0 ? 0 : (len > cap ? cap : len);
+  const int64_t s = in - n + i + 1;
+  return s < 0 ? 0 : s;
+}
+
+// =============================================================================================
+// Scores: [B, n, Hk, n_blocks] fp64 = (sum of a group's queries) . (block's key sum). One wave takes 16
+// queries x 16 blocks at a time (v_mfma_f64_16x16x4): a query's sums and a key sum's products are
+// exact in fp64 to 2^-52 of the score, so the order of the products decides no choice. The sums are read
+// once; a decoding step fills one row of 16, which the fp64 matrix rate (one instruction per 256 bytes
+// read by a wave) still hides behind the read.
+// =============================================================================================
+struct ScoreParams {
+  const bf16_t* q; int64_t q_sb, q_st, q_sh;
+  const float* sums;
+  const int32_t* kv_len; int64_t kv_len_all, cap;
+  int n, H, Hk, nb, bs, sink, local;
+  int q_tiles, b_tiles, per;   // 16-query tiles; groups of `per` 16-block tiles
+  double* scores;
+};
+
+template <int D>
+__global__ void __launch_bounds__(64) score_kernel(ScoreParams p) {
+  const int lane = threadIdx.x, row = lane & 15, kg = lane >> 4;
+  int u = blockIdx.x;
+  const int bt = u % p.b_tiles;
+  u /= p.b_tiles;
+  const int qt = u % p.q_tiles, bh = u / p.q_tiles, b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk;
+  const int last = min(p.n, 16 * qt + 16) - 1;
+  // the blocks that the tile's last query scores: none from the first local one on
+  const int64_t seen = seen_tokens(p.kv_len, p.kv_len_all, p.cap, p.n, b, last);
+  const int end = (int)((seen + p.bs - 1) / p.bs) - p.local, begin = bt * p.per * 16;
+  if (begin >= end) return;
+  // slot (step 4 i + j, lane group kg) of the contraction is channel 16 i + 4 kg + j on both sides
+  double a[D / 4];
+  const int qi = 16 * qt + row;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    if (qi < p.n) {
+      const bf16_t* src = p.q + (int64_t)b * p.q_sb + (int64_t)qi * p.q_st + (int64_t)hk * G * p.q_sh + 16 * i + 4 * kg;
+      for (int g = 0; g < G; ++g) {
+        const bf16x4 x = *(const bf16x4*)(src + (int64_t)g * p.q_sh);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += (double)(float)x[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[4 * i + j] = s[j];
+  }
+  for (int t = 0; t < p.per; ++t) {
+    const int b0 = begin + 16 * t;
+    if (b0 >= end) break;
+    const int blk = min(b0 + row, p.nb - 1);
+    const float* src = p.sums + ((int64_t)bh * p.nb + blk) * D + 4 * kg;
+    f32x4 x[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) x[i] = *(const f32x4*)(src + 16 * i);
+    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[4 * i + j], (double)x[i][j], acc, 0, 0, 0);
+    // accumulator register r of lane (column block, kg) is query row kg + 4 r
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * qt + kg + 4 * r;
+      if (i < p.n && b0 + row < p.nb)
+        p.scores[(((int64_t)b * p.n + i) * p.Hk + hk) * p.nb + b0 + row] = acc[r];
+    }
+  }
+}
+
+// =============================================================================================
+// Choice: W waves hold a row's scores as order-preserving 64-bit keys, KPT a lane, and find the m-th
+// largest by bisection over the key's bits (counts by ballots), then write the chosen ids in
+// ascending order by prefix counts. W = 1: four rows a workgroup and no barrier.
+// =============================================================================================
+struct ChooseParams {
+  const double* scores;
+  const int32_t* kv_len; int64_t kv_len_all, cap;
+  int n, Hk, nb, bs, topk, sink, local;
+  int64_t rows;
+  int32_t* index; int32_t* num;
+};
+
+// Larger score, larger key; NaN above all, -0 as 0. Never 0, which stands for "not scored".
+__device__ __forceinline__ uint64_t score_key(double x) {
+  if (x != x) return ~0ull;
+  const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+
+template <int W, int KPT>
+__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(ChooseParams p) {
+  __shared__ int counts[2][W];
+  const int lane = threadIdx.x & 63, w = W == 1 ? 0 : threadIdx.x >> 6;
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  if (row >= p.rows) return;   // whole waves (W = 1), never a part of a workgroup with barriers
+  const int i = (int)(row / p.Hk % p.n), b = (int)(row / p.Hk / p.n);
+  const int64_t seen = seen_tokens(p.kv_len, p.kv_len_all, p.cap, p.n, b, i);
+  const int vis = (int)((seen + p.bs - 1) / p.bs), take = min(vis, p.topk);
+  const int lo = min(p.sink, vis), hi = max(lo, vis - p.local);   // scored: [lo, hi)
+  const int m = take - (vis - (hi - lo));                         // of them chosen
+  const bool all = take == vis;
+  const int first = w * 64 * KPT + lane;                          // this lane's blocks: first + 64 e
+  uint64_t key[KPT];
+#pragma unroll
+  for (int e = 0; e < KPT; ++e) {
+    const int j = first + 64 * e;
+    key[e] = 0;
+    if (!all && j >= lo && j < hi) key[e] = score_key(p.scores[row * p.nb + j]);
+  }
+  int flip = 0;
+  auto total = [&](int mine) {   // over the row's waves; mine is uniform in a wave
+    if (W == 1) return mine;
+    if (lane == 0) counts[flip][w] = mine;
+    __syncthreads();
+    int s = 0;
+    for (int x = 0; x < W; ++x) s += counts[flip][x];
+    flip ^= 1;                   // the next count's writes leave this one's slots alone until the barrier after it
+    return s;
+  };
+  // the m-th largest key: the largest T that at least m keys reach
+  uint64_t T = 0;
+  bool exact = false;            // exactly m keys reach T
+  if (!all && m > 0) {
+    for (int bit = 63; bit >= 0 && !exact; --bit) {
+      const uint64_t cand = T | (1ull << bit);
+      int c = 0;
+#pragma unroll
+      for (int e = 0; e < KPT; ++e) c += __popcll(__ballot(key[e] >= cand));
+      c = total(c);
+      if (c >= m) T = cand;
+      exact = c == m;
+    }
+  }
+  int ties = 0;                  // keys equal to T that are chosen, lowest ids first
+  if (!all && m > 0 && !exact) {
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < KPT; ++e) c += __popcll(__ballot(key[e] > T));
+    ties = m - total(c);
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  int tied = 0;                  // ties in the waves before this one
+  if (W > 1 && ties > 0) {
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < KPT; ++e) c += __popcll(__ballot(key[e] == T));
+    if (lane == 0) counts[flip][w] = c;
+    __syncthreads();
+    for (int x = 0; x < w; ++x) tied += counts[flip][x];
+    flip ^= 1;
+  }
+  // bit e of `mine`: this lane's block first + 64 e is chosen
+  uint64_t mine = 0;
+  int chosen = 0;
+#pragma unroll
+  for (int e = 0; e < KPT; ++e) {
+    const int j = first + 64 * e;
+    bool take_j = j < vis && (all || j < lo || j >= hi);
+    if (!all && m > 0 && j >= lo && j < hi) take_j = exact ? key[e] >= T : key[e] > T;
+    if (ties > 0) {
+      const bool tie = key[e] == T && j >= lo && j < hi;
+      const uint64_t t = __ballot(tie);
+      if (tie && tied + __popcll(t & below) < ties) take_j = true;
+      tied += __popcll(t);
+    }
+    chosen += __popcll(__ballot(take_j));
+    mine |= (uint64_t)take_j << e;
+  }
+  int at = 0;
+  if (W > 1) {
+    if (lane == 0) counts[flip][w] = chosen;
+    __syncthreads();
+    for (int x = 0; x < w; ++x) at += counts[flip][x];
+  }
+  int32_t* out = p.index + row * p.topk;
+#pragma unroll
+  for (int e = 0; e < KPT; ++e) {
+    const bool mine_e = (mine >> e) & 1;
+    const uint64_t t = __ballot(mine_e);
+    if (mine_e) out[at + __popcll(t & below)] = first + 64 * e;
+    at += __popcll(t);
+  }
+  const int threads = W == 1 ? 64 : 64 * W, tid = W == 1 ? lane : (int)threadIdx.x;
+  for (int s = take + tid; s < p.topk; s += threads) out[s] = -1;
+  if (tid == 0) p.num[row] = take;
+}
+
+// =============================================================================================
+// Attention. A workgroup takes up to 16 query heads of one (sequence, query, key head) over a part of
+// its block list; its four waves take 32-key tiles in turn, all in registers. Transposed products keep
+// every operand where it was loaded or computed:
+//   S^T (32 keys x 16 heads) = K Q^T: a lane holds 16 bytes of a key row;
+//   O^T (D x 16 heads) += V^T P^T: the accumulator's keys are the next product's contraction slots
+//   (lane group kg, element e: key 16 (e / 4) + 4 kg + e % 4), and lane m's 16 bytes of those eight value
+//   rows, regrouped by channel, are rows d = D / 16 m + j of V^T for product j.
+// So keys and values are read once, straight into registers, with no LDS until the waves' partial
+// results meet. Bound by that read.
+// =============================================================================================
+struct AttnParams {
+  const bf16_t* q; int64_t q_sb, q_st, q_sh;
+  const bf16_t* k; int64_t k_sb, k_st, k_sh;
+  const bf16_t* v; int64_t v_sb, v_st, v_sh;
+  bf16_t* o; int64_t o_sb, o_st, o_sh;
+  float* lse;
+  const int32_t* index; const int32_t* num;
+  const int32_t* kv_len; int64_t kv_len_all, cap;
+  int n, H, Hk, topk, bs, g_tiles, splits;
+  float scale2;      // scale / ln 2
+  float* part;       // [units][16][D + 2] fp32 of a split row
+};
+
+__device__ __forceinline__ f32x4 mma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+constexpr float kLowest = -1e30f;   // running maximum before the first key: finite, so that no difference of it is NaN
+
+template <int N> struct RowPart;     // N bf16 values of a value row
+template <> struct RowPart<8> { typedef bf16x8 type; };
+template <> struct RowPart<4> { typedef bf16x4 type; };
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
+  constexpr int KC = D / 32, VC = D / 16;   // 32-channel steps of a key row; channels of a value row a lane holds
+  typedef typename RowPart<VC>::type VRow;
+  __shared__ float sm[4][16], sl[4][16];
+  __shared__ float so[4][16][D + 4];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, kg = lane >> 4;
+  int64_t u = blockIdx.x;
+  const int split = (int)(u % p.splits);
+  u /= p.splits;
+  const int gt = (int)(u % p.g_tiles);
+  const int64_t row = u / p.g_tiles;        // (b, i, hk)
+  const int hk = (int)(row % p.Hk), i = (int)(row / p.Hk % p.n), b = (int)(row / p.Hk / p.n), G = p.H / p.Hk;
+  const int heads = min(16, G - 16 * gt);
+  const int64_t seen = seen_tokens(p.kv_len, p.kv_len_all, p.cap, p.n, b, i);
+  const int tpb = p.bs / 32;                // tiles of a block
+  const int tiles = max(0, min(p.num[row], p.topk)) * tpb;
+  const int per = (tiles + p.splits - 1) / p.splits;
+  const int t0 = split * per, t1 = min(tiles, t0 + per);
+  const int32_t* list = p.index + row * p.topk;
+
+  bf16x8 q[KC];
+#pragma unroll
+  for (int c = 0; c < KC; ++c) {
+    q[c] = bf16x8{};
+    if (l16 < heads)
+      q[c] = *(const bf16x8*)(p.q + (int64_t)b * p.q_sb + (int64_t)i * p.q_st + (int64_t)(hk * G + 16 * gt + l16) * p.q_sh + 32 * c + 8 * kg);
+  }
+  const bf16_t* kb = p.k + (int64_t)b * p.k_sb + (int64_t)hk * p.k_sh;
+  const bf16_t* vb = p.v + (int64_t)b * p.v_sb + (int64_t)hk * p.v_sh;
+  float m = kLowest, l = 0.f;
+  f32x4 o[VC];
+#pragma unroll
+  for (int j = 0; j < VC; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int t = t0 + w; t < t1; t += 4) {
+    const int id = list[t / tpb];
+    const int64_t key0 = (int64_t)id * p.bs + (t % tpb) * 32;
+    if (id < 0 || key0 >= seen) continue;
+    const int live = (int)min((int64_t)32, seen - key0);   // keys of the tile that are seen
+    bf16x8 k[2][KC];
+    VRow v[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bf16_t* src = kb + (key0 + min(16 * h + l16, live - 1)) * p.k_st + 8 * kg;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) k[h][c] = *(const bf16x8*)(src + 32 * c);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = *(const VRow*)(vb + (key0 + min(16 * (e >> 2) + 4 * kg + (e & 3), live - 1)) * p.v_st + VC * l16);
+    float s[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) acc = mma16(k[h][c], q[c], acc);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[4 * h + r] = acc[r] * p.scale2;
+    }
+    if (live < 32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (16 * (e >> 2) + 4 * kg + (e & 3) >= live) {
+          s[e] = -INFINITY;
+          v[e] = VRow{};    // a weight of 0 does not silence an infinity
+        }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e]);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any(top > m)) {
+      const float up = fmaxf(m, top), f = exp2f(m - up);
+      m = up;
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < VC; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[j][r] *= f;
+    }
+    // weights round to bf16 for their product with the values (2^-8 each, independent, so the sum over
+    // the keys gains from averaging); the sum that they are divided by, and that leaves as the log-sum-exp,
+    // is of the unrounded ones
+    bf16x8 pr;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = exp2f(s[e] - m);
+      pr[e] = (bf16_t)x;
+      l += x;
+    }
+#pragma unroll
+    for (int j = 0; j < VC; ++j) {
+      bf16x8 vt;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vt[e] = v[e][j];
+      o[j] = mma16(vt, pr, o[j]);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+
+  // the waves' parts: each to the common maximum, then summed in wave order
+  if (kg == 0) {
+    sm[w][l16] = m;
+    sl[w][l16] = l;
+  }
+  __syncthreads();
+  const float top = fmaxf(fmaxf(sm[0][l16], sm[1][l16]), fmaxf(sm[2][l16], sm[3][l16])), f = exp2f(m - top);
+#pragma unroll
+  for (int j = 0; j < VC; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) so[w][l16][VC * (4 * kg + r) + j] = o[j][r] * f;
+  __syncthreads();
+  for (int x = tid; x < heads * D; x += kThreads) {
+    const int g = x / D, d = x % D;
+    const float tm = fmaxf(fmaxf(sm[0][g], sm[1][g]), fmaxf(sm[2][g], sm[3][g]));
+    float sum = 0.f, tl = 0.f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      sum += so[y][g][d];
+      tl += sl[y][g] * exp2f(sm[y][g] - tm);
+    }
+    const int h = hk * G + 16 * gt + g;
+    if (p.splits == 1) {
+      p.o[(int64_t)b * p.o_sb + (int64_t)i * p.o_st + (int64_t)h * p.o_sh + d] = (bf16_t)(tl > 0.f ? sum / tl : (tl == 0.f ? 0.f : tl));
+      if (d == 0 && p.lse) p.lse[((int64_t)b * p.H + h) * p.n + i] = tl == 0.f ? -INFINITY : (tm + log2f(tl)) * WA_LN2;
+    } else {
+      float* at = p.part + (((row * p.g_tiles + gt) * p.splits + split) * 16 + g) * (D + 2);
+      at[2 + d] = sum;
+      if (d == 0) {
+        at[0] = tm;
+        at[1] = tl;
+      }
+    }
+  }
+}
+
+// The parts of split rows, in split order. One wave per (row, head).
+template <int D>
+__global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p, int64_t units) {
+  const int lane = threadIdx.x & 63;
+  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);   // (row, query head of the group)
+  if (u >= units) return;
+  const int G = p.H / p.Hk, g = (int)(u % G);
+  const int64_t row = u / G;
+  const int hk = (int)(row % p.Hk), i = (int)(row / p.Hk % p.n), b = (int)(row / p.Hk / p.n);
+  const float* at = p.part + (((row * p.g_tiles + g / 16) * p.splits) * 16 + g % 16) * (D + 2);
+  constexpr int64_t kSplit = 16 * (D + 2);
+  float top = kLowest;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, at[s * kSplit]);
+  float l = 0.f, o[D / 64];
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float f = exp2f(at[s * kSplit] - top);
+    l += at[s * kSplit + 1] * f;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] += at[s * kSplit + 2 + lane + 64 * e] * f;
+  }
+  const int h = hk * G + g;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e)
+    p.o[(int64_t)b * p.o_sb + (int64_t)i * p.o_st + (int64_t)h * p.o_sh + lane + 64 * e] = (bf16_t)(l > 0.f ? o[e] / l : (l == 0.f ? 0.f : l));
+  if (lane == 0 && p.lse) p.lse[((int64_t)b * p.H + h) * p.n + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * WA_LN2;
+}
+
+// Parts of a row: while the rows alone leave the GPU's 256 CUs short of two workgroups each, but not below
+// two tiles for each of a workgroup's waves.
+int64_t attn_splits(int64_t rows, int64_t tiles) {
+  const int64_t want = rows > 0 ? (512 + rows - 1) / rows : 1;
+  return std::max<int64_t>(1, std::min<int64_t>(want, tiles / 8));
+}
+
+int check_lists(const char* what, int64_t B, int64_t n, int64_t H, int64_t Hk, int64_t D, int64_t bs, int64_t topk) {
+  WA_CHECK_ARG(D == 64 || D == 128, "%s: head dim must be 64 or 128, got %lld", what, (long long)D);
+  WA_CHECK_ARG(bs == 64 || bs == 128, "%s: block size must be 64 or 128, got %lld", what, (long long)bs);
+  WA_CHECK_ARG(B >= 1 && n >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0, "%s: bad sizes B %lld n %lld heads %lld / %lld", what,
+               (long long)B, (long long)n, (long long)H, (long long)Hk);
+  WA_CHECK_ARG(topk >= 1 && topk <= WA_SELECT_MAX_BLOCKS, "%s: topk must be 1 .. %d, got %lld", what, WA_SELECT_MAX_BLOCKS, (long long)topk);
+  WA_CHECK_ARG(n <= INT32_MAX && B <= INT32_MAX && H <= 65536 && B * n <= (int64_t)1 << 31, "%s: too many queries", what);
+  return WA_OK;
+}
+
+template <int W, int KPT>
+void launch_choose(const ChooseParams& p, hipStream_t s) {
+  const int64_t grid = W == 1 ? (p.rows + 3) / 4 : p.rows;
+  hipLaunchKernelGGL((choose_kernel<W, KPT>), dim3((unsigned)grid), dim3(W == 1 ? 256 : 64 * W), 0, s, p);
+}
+
+}  // namespace
+
+extern "C" int64_t wa_select_blocks_workspace_bytes(int64_t B, int64_t n, int64_t Hk, int64_t n_blocks) {
+  return B * n * Hk * n_blocks * 8;
+}
+
+extern "C" int wa_select_blocks(const wa_select_blocks_args* a, void* stream) {
+  WA_CHECK_ARG(a, "select_blocks: null args");
+  const int rc = check_lists("select_blocks", a->B, a->n, a->H, a->Hk, a->D, a->block_size, a->topk);
+  if (rc != WA_OK) return rc;
+  WA_CHECK_ARG(a->n_blocks >= 1 && a->n_blocks <= WA_SELECT_MAX_BLOCKS, "select_blocks: 1 .. %d blocks, got %lld", WA_SELECT_MAX_BLOCKS,
+               (long long)a->n_blocks);
+  WA_CHECK_ARG(a->cap >= 0 && a->cap <= a->n_blocks * a->block_size, "select_blocks: %lld blocks do not hold %lld tokens",
+               (long long)a->n_blocks, (long long)a->cap);
+  WA_CHECK_ARG(a->sink_blocks >= 0 && a->local_blocks >= 1 && a->sink_blocks <= a->topk && a->local_blocks <= a->topk - a->sink_blocks,
+               "select_blocks: topk %lld must hold %lld sink and %lld (>= 1) local blocks", (long long)a->topk,
+               (long long)a->sink_blocks, (long long)a->local_blocks);
+  WA_CHECK_ARG(a->q && a->k_sums && a->index && a->num && a->workspace, "select_blocks: null tensor");
+  WA_CHECK_ARG(wa_aligned16(a->k_sums) && wa_aligned16(a->workspace) && ((uintptr_t)a->q & 7) == 0 && a->q_sb % 4 == 0 &&
+               a->q_st % 4 == 0 && a->q_sh % 4 == 0, "select_blocks: misaligned rows");
+  const int64_t cap = a->cap ? a->cap : a->n_blocks * a->block_size;
+  const int64_t rows = a->B * a->n * a->Hk;
+  hipStream_t s = (hipStream_t)stream;
+  ScoreParams p{};
+  p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.sums = a->k_sums; p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.cap = cap;
+  p.n = (int)a->n; p.H = (int)a->H; p.Hk = (int)a->Hk; p.nb = (int)a->n_blocks; p.bs = (int)a->block_size;
+  p.sink = (int)a->sink_blocks; p.local = (int)a->local_blocks;
+  p.scores = (double*)a->workspace;
+  p.q_tiles = (int)((a->n + 15) / 16);
+  // a wave keeps its queries for up to 8 block tiles where the tiles are many
+  const int64_t tiles = (a->n_blocks + 15) / 16, waves = a->B * a->Hk * p.q_tiles * tiles;
+  p.per = (int)std::max<int64_t>(1, std::min<int64_t>({8, tiles, waves / 2048}));
+  p.b_tiles = (int)((tiles + p.per - 1) / p.per);
+  const int64_t grid = a->B * a->Hk * p.q_tiles * p.b_tiles;
+  WA_CHECK_ARG(grid <= INT32_MAX && rows <= INT32_MAX, "select_blocks: too many queries");
+  if (a->n_blocks > a->topk) {   // otherwise every seen block is chosen
+    if (a->D == 128) hipLaunchKernelGGL((score_kernel<128>), dim3((unsigned)grid), dim3(64), 0, s, p);
+    else hipLaunchKernelGGL((score_kernel<64>), dim3((unsigned)grid), dim3(64), 0, s, p);
+  }
+  const ChooseParams c{p.scores, a->kv_len, a->kv_len_all, cap, p.n, p.Hk, p.nb, p.bs, (int)a->topk, p.sink, p.local, rows, a->index, a->num};
+  if (p.nb <= 256) launch_choose<1, 4>(c, s);
+  else if (p.nb <= 1024) launch_choose<1, 16>(c, s);
+  else if (p.nb <= 4096) launch_choose<4, 16>(c, s);
+  else if (p.nb <= 16384) launch_choose<16, 16>(c, s);
+  else launch_choose<16, 32>(c, s);
+  return wa_launch_status("select_blocks");
+}
+
+extern "C" int64_t wa_selected_attn_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t Hk, int64_t D, int64_t topk,
+                                                    int64_t block_size) {
+  if (Hk < 1 || H < Hk) return 0;
+  const int64_t units = B * n * Hk * ((H / Hk + 15) / 16), splits = attn_splits(units, topk * block_size / 32);
+  return splits > 1 ? units * splits * 16 * (D + 2) * 4 : 0;
+}
+
+extern "C" int wa_selected_attn(const wa_selected_attn_args* a, void* stream) {
+  WA_CHECK_ARG(a, "selected_attn: null args");
+  const int rc = check_lists("selected_attn", a->B, a->n, a->H, a->Hk, a->D, a->block_size, a->topk);
+  if (rc != WA_OK) return rc;
+  WA_CHECK_ARG(a->cap >= 1 && a->cap <= INT32_MAX, "selected_attn: bad cache of %lld tokens", (long long)a->cap);
+  WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->index && a->num, "selected_attn: null tensor");
+  auto rows16 = [](const void* x, int64_t sb, int64_t st, int64_t sh) { return wa_aligned16(x) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0; };
+  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->k, a->k_sb, a->k_st, a->k_sh) && rows16(a->v, a->v_sb, a->v_st, a->v_sh),
+               "selected_attn: rows must be 16-byte aligned");
+  AttnParams p{};
+  p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.k = (const bf16_t*)a->k; p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
+  p.v = (const bf16_t*)a->v; p.v_sb = a->v_sb; p.v_st = a->v_st; p.v_sh = a->v_sh;
+  p.o = (bf16_t*)a->o; p.o_sb = a->o_sb; p.o_st = a->o_st; p.o_sh = a->o_sh;
+  p.lse = a->lse; p.index = a->index; p.num = a->num; p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.cap = a->cap;
+  p.n = (int)a->n; p.H = (int)a->H; p.Hk = (int)a->Hk; p.topk = (int)a->topk; p.bs = (int)a->block_size;
+  p.g_tiles = (int)((a->H / a->Hk + 15) / 16);
+  p.scale2 = (a->scale == 0.f ? 1.f / sqrtf((float)a->D) : a->scale) * WA_LOG2E;
+  p.part = (float*)a->workspace;
+  const int64_t units = a->B * a->n * a->Hk * p.g_tiles;
+  p.splits = (int)attn_splits(units, a->topk * a->block_size / 32);
+  WA_CHECK_ARG(p.splits == 1 || p.part, "selected_attn: a launch of %lld rows needs a workspace", (long long)units);
+  WA_CHECK_ARG(units * p.splits <= INT32_MAX && a->B * a->n * a->H <= INT32_MAX, "selected_attn: too many queries");
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)(units * p.splits));
+  const int64_t heads = a->B * a->n * a->H;
+  if (a->D == 128) hipLaunchKernelGGL((attend_kernel<128>), grid, dim3(kThreads), 0, s, p);
+  else hipLaunchKernelGGL((attend_kernel<64>), grid, dim3(kThreads), 0, s, p);
+  if (p.splits > 1) {
+    if (a->D == 128) hipLaunchKernelGGL((join_kernel<128>), dim3((unsigned)((heads + 3) / 4)), dim3(kThreads), 0, s, p, heads);
+    else hipLaunchKernelGGL((join_kernel<64>), dim3((unsigned)((heads + 3) / 4)), dim3(kThreads), 0, s, p, heads);
+  }
+  return wa_launch_status("selected_attn");
+}

@@ -12,6 +12,7 @@ from .kvcache import kv_append, new_block_sums
 from .block_sparse import block_sparse_attention, block_sparse_attention_reference, map_to_index
 from .decay import decay_linear_attention, decay_linear_step
 from .rope import axis_frequencies, rope_axes
+from .selected import BlockSelection, attend_selected, select_key_blocks, selected_attention
 from .routing import (
     BlockRouting,
     block_attention_map,
@@ -41,4 +42,8 @@ __all__ = [
     "axis_frequencies",
     "decay_linear_attention",
     "decay_linear_step",
+    "BlockSelection",
+    "select_key_blocks",
+    "selected_attention",
+    "attend_selected",
 ]
