@@ -754,8 +754,11 @@ int wa_rope_axes(const wa_rope_axes_args* args, void* stream);
  * gradients) are 0 and the state ends at the last token before them.
  * The sequence is cut into wa_decay_segments(B, L, H) segments. `states` (device fp32
  * [B, H, segments, D, D]) receives the state before each, which the backward takes back;
+ * `derivs` (device fp32 [B, H, segments + 1, D, D], or NULL) receives the states' derivatives by
+ * log_decay, which a backward that computes dlog_decay takes back.
  * initial / final: fp32 [B, H, D, D] (key channel, value channel), contiguous; final may be NULL.
- * Rows must be 16-byte aligned. The state is kept and summed in fp32. */
+ * Rows must be 16-byte aligned and at most 2^23 elements apart. The state is kept and summed in
+ * fp32. */
 int64_t wa_decay_segments(int64_t B, int64_t L, int64_t H);
 typedef struct wa_decay_fwd_args {
   const void* q; int64_t q_sb, q_st, q_sh;
@@ -769,6 +772,7 @@ typedef struct wa_decay_fwd_args {
   const float* initial;
   float* final_state;
   float* states;
+  float* derivs;
   float scale;
 } wa_decay_fwd_args;
 int wa_decay_fwd(const wa_decay_fwd_args* args, void* stream);
@@ -790,6 +794,7 @@ typedef struct wa_decay_bwd_args {
   const float* log_decay;
   const int32_t* lengths;
   const float* states;
+  const float* derivs;
   const float* dfinal;
   float* dinitial;
   float* dlog_decay;

@@ -362,7 +362,7 @@ DecayFwdArgs = _struct("wa_decay_fwd_args", [
     ("dtype", c_int32),
     ("B", c_int64), ("L", c_int64), ("H", c_int64), ("D", c_int64),
     ("log_decay", c_void_p), ("lengths", c_void_p), ("initial", c_void_p), ("final_state", c_void_p),
-    ("states", c_void_p), ("scale", c_float),
+    ("states", c_void_p), ("derivs", c_void_p), ("scale", c_float),
 ])
 
 DecayBwdArgs = _struct("wa_decay_bwd_args", [
@@ -375,7 +375,7 @@ DecayBwdArgs = _struct("wa_decay_bwd_args", [
     ("dv", c_void_p), ("dv_sb", c_int64), ("dv_st", c_int64), ("dv_sh", c_int64),
     ("dtype", c_int32),
     ("B", c_int64), ("L", c_int64), ("H", c_int64), ("D", c_int64),
-    ("log_decay", c_void_p), ("lengths", c_void_p), ("states", c_void_p), ("dfinal", c_void_p),
+    ("log_decay", c_void_p), ("lengths", c_void_p), ("states", c_void_p), ("derivs", c_void_p), ("dfinal", c_void_p),
     ("dinitial", c_void_p), ("dlog_decay", c_void_p), ("workspace", c_void_p), ("scale", c_float),
 ])
 

@@ -8,13 +8,23 @@
 //   out: (a, b, c) = (q, k, v),   X = S,   lag 1;     dq: (dO, v, k), X = S^T, lag 1;
 //   dv:  (k, q, dO),  X = Y,      lag 0;              dk: (v, dO, q), X = Y^T, lag 0,
 // the last two with time running backwards, Y being the gradient of the state after the segment:
-// Y = lambda^n Y' + scale sum_j lambda^(n - j) q_j dO_j^T, which ends as the initial state's gradient.
+// Y = lambda^n Y' + scale sum_j lambda^(j + 1) q_j dO_j^T, which ends as the initial state's gradient.
 //
-// Three launches: every segment's own state (segment_state_kernel), the carried states (carry_kernel,
-// in place), the rows (rows_kernel, 64-token chunks in sequence with the running state on chip). The
-// states are fp32 everywhere; what enters a matrix product of bf16 tensors is rounded to bf16 except
-// where an fp32 result leaves the kernel (segment states, the decay's gradient): there the rounded
-// operand is split in two bf16 parts (2^-17 relative), so that a state is as exact as its sum.
+// Three launches: every segment's own state, the carried states (in place), the rows (64-token chunks in
+// sequence, the running state on chip).
+//
+// The decay's gradient, d/d log(lambda), counts the steps of every path from a token j to a token i. With
+// T = dS/d log(lambda), carried as T <- lambda^n (T + n S) + sum_j (n - 1 - j) lambda^(n - 1 - j) k_j v_j^T,
+// a segment adds
+//   scale sum_{j < i} (i - j) lambda^(i - j) (q_i . k_j)(dO_i . v_j)                    pairs inside it
+// + <S, scale sum_i (i + 1) lambda^(i + 1) q_i dO_i^T> + <T, scale sum_i lambda^(i + 1) q_i dO_i^T>,
+// and the sequence's end <T, dS>. The sums over i are the segment's own gradient state and its derivative,
+// so the state kernels, asked for derivatives, hold all but the pairs.
+//
+// Roundings. States, derivatives and all sums are fp32 (the decay's gradient is summed in fp64 across
+// workgroups). Operands of bf16 products whose results leave in fp32 (states, derivatives) enter cut in three
+// exact parts. In the rows of bf16 tensors, whose results leave in bf16, the decayed q.k and the running
+// state's weighted operand round to bf16 once; the state itself enters in two parts (2^-17).
 #include <algorithm>
 
 #include "tile.h"
@@ -24,66 +34,14 @@ namespace {
 constexpr int kChunk = 64;      // tokens a step of the running state takes
 constexpr int kThreads = 256;
 
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-
-template <typename T> struct Frag;
-template <> struct Frag<bf16_t> { typedef bf16x8 type; };
-template <> struct Frag<float> { typedef f32x8 type; };
-
-// 32 x 32 += (32 x 16) (16 x 32): lane (l32, g) holds 8 values of the contraction, 8 g .. 8 g + 7, of
-// operand row / column l32. fp32 runs as 8 products of depth 2 over the same slots.
-__device__ __forceinline__ f32x16 mma(const bf16x8& a, const bf16x8& b, const f32x16& c) { return wa_mfma32(a, b, c); }
-__device__ __forceinline__ f32x16 mma(const f32x8& a, const f32x8& b, f32x16 c) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-  return c;
-}
-
-// Accumulator register r of lane (l32, g) is row 8 (r / 4) + 4 g + r % 4, column l32.
+// Accumulator register r of lane (l32, g) of a 32 x 32 product is row 8 (r / 4) + 4 g + r % 4, column l32.
 __device__ __forceinline__ int acc_row(int r, int g) { return 8 * (r >> 2) + 4 * g + (r & 3); }
-
-// Row-major LDS tiles of W columns: bf16 swizzled (tile.h), fp32 padded by one 16-byte slot.
-template <typename T, int W> struct Tile;
-template <int W> struct Tile<bf16_t, W> {
-  static constexpr int kRow = W;
-  static __device__ __forceinline__ bf16x8 row8(const bf16_t* t, int row, int chunk) { return tile_row8<W>(t, row, chunk); }
-  static __device__ __forceinline__ bf16x8 col8(const bf16_t* t, int c, int col0, int lane) { return tile_tr8n<W>(t, c, col0, lane); }
-  static __device__ __forceinline__ void put8(bf16_t* t, int row, int chunk, const bf16x8& v) { tile_put8<W>(t, row, chunk, v); }
-  static __device__ __forceinline__ void put(bf16_t* t, int row, int col, float v) {
-    t[row * W + (((col >> 3) ^ dual_swizzle<W>(row)) * 8) + (col & 7)] = (bf16_t)v;
-  }
-};
-template <int W> struct Tile<float, W> {
-  static constexpr int kRow = W + 4;
-  static __device__ __forceinline__ f32x8 row8(const float* t, int row, int chunk) {
-    const f32x4 a = *(const f32x4*)(t + row * kRow + chunk * 8), b = *(const f32x4*)(t + row * kRow + chunk * 8 + 4);
-    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-  }
-  static __device__ __forceinline__ f32x8 col8(const float* t, int c, int col0, int lane) {
-    f32x8 v;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = t[(16 * c + 8 * (lane >> 5) + e) * kRow + col0 + (lane & 31)];
-    return v;
-  }
-  static __device__ __forceinline__ void put8(float* t, int row, int chunk, const f32x8& v) {
-    *(f32x4*)(t + row * kRow + chunk * 8) = f32x4{v[0], v[1], v[2], v[3]};
-    *(f32x4*)(t + row * kRow + chunk * 8 + 4) = f32x4{v[4], v[5], v[6], v[7]};
-  }
-  static __device__ __forceinline__ void put(float* t, int row, int col, float v) { t[row * kRow + col] = v; }
-};
-
-__device__ __forceinline__ bf16x8 load8(const bf16_t* p) { return *(const bf16x8*)p; }
-__device__ __forceinline__ f32x8 load8(const float* p) {
-  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-  return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
 
 struct View {
   const void* p; int64_t sb, st, sh;
 };
 
-// Geometry shared by all kernels. Segment c holds n = clamp(length - c seg, 0, seg) tokens; token i of
-// it, in the direction of time taken, is token seg c + i or (backwards) seg c + n - 1 - i.
+// Geometry shared by all kernels. Segment c holds n = clamp(length - c seg, 0, seg) tokens.
 struct Shape {
   int B, L, H, seg, n_seg;
   const float* log_decay;
@@ -103,140 +61,23 @@ __device__ __forceinline__ float log2_decay(const Shape& s, int h) {
 }
 __device__ __forceinline__ float power(float g2, int steps) { return exp2f(g2 * (float)steps); }
 
-// Rows [c0, c0 + 64) of a segment into a tile; rows from n on are zeros.
-template <typename T, int D>
-__device__ __forceinline__ void stage_rows(T* tile, const T* base, int64_t st, int c0, int n, bool rev) {
-  constexpr int CPR = D / 8;
-#pragma unroll
-  for (int i = 0; i < kChunk * CPR / kThreads; ++i) {
-    const int u = threadIdx.x + i * kThreads, row = u / CPR, ch = u % CPR, t = c0 + row;
-    typename Frag<T>::type v{};
-    if (t < n) v = load8(base + (int64_t)(rev ? n - 1 - t : t) * st + ch * 8);
-    Tile<T, D>::put8(tile, row, ch, v);
-  }
-}
-
-// The state's operand of 16 tokens with its weights lambda^(last - token), in one part or two.
-__device__ __forceinline__ void weigh(const bf16x8& b, const float (&w)[8], bf16x8& hi, bf16x8& lo) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = (float)b[e] * w[e];
-    hi[e] = (bf16_t)x;
-    lo[e] = (bf16_t)(x - (float)hi[e]);
-  }
-}
-__device__ __forceinline__ void weigh(const f32x8& b, const float (&w)[8], f32x8& hi, f32x8& lo) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    hi[e] = b[e] * w[e];
-    lo[e] = 0.f;
-  }
-}
-
-// acc (this wave's tiles of the state) = lambda^m acc + sum_j w_scale lambda^(m - 1 - j + ahead) b_j c_j^T over
-// the chunk's m tokens. D = 128: wave w holds state rows 32 w .. + 31 in four column tiles; D = 64: tile
-// (w / 2, w % 2). `split`: the weighted operand in two parts.
-template <typename T, int D, bool SPLIT>
-__device__ __forceinline__ void state_update(f32x16 (&acc)[D / 32 * D / 32 / 4], const T* tb, const T* tc, int m, float g2,
-                                             int ahead, float w_scale, int w, int lane) {
-  constexpr int TPW = D / 32 * D / 32 / 4;
-  const int g = lane >> 5, dt = D == 128 ? w : w >> 1;
-  const float keep = power(g2, m);
-#pragma unroll
-  for (int i = 0; i < TPW; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[i][r] *= keep;
-#pragma unroll
-  for (int jc = 0; jc < kChunk / 16; ++jc) {
-    float wt[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) wt[e] = w_scale * power(g2, max(0, m - 1 - (16 * jc + 8 * g + e) + ahead));
-    typename Frag<T>::type hi, lo;
-    weigh(Tile<T, D>::col8(tb, jc, 32 * dt, lane), wt, hi, lo);
-#pragma unroll
-    for (int i = 0; i < TPW; ++i) {
-      const int et = D == 128 ? i : w & 1;
-      const auto c = Tile<T, D>::col8(tc, jc, 32 * et, lane);
-      if (SPLIT && sizeof(T) == 2) acc[i] = mma(lo, c, acc[i]);
-      acc[i] = mma(hi, c, acc[i]);
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------------------------
-// Each segment's own state (or gradient state, backwards with lag 0).
-// ---------------------------------------------------------------------------------------------
+// A segment's own state, sum_j w_j b_j c_j^T with w_j = w_scale lambda^steps(j), forwards steps = n - 1 - j,
+// backwards (rev) j + 1. With derivatives (derivs not null) also sum_j steps w_j b_j c_j^T: forwards written
+// to derivs; backwards the segment's part of the decay's gradient instead, <S, that> + <T, the state>.
 struct StateParams {
   Shape s;
   View b, c;
-  float* states;   // [B, H, n_seg, D, D]
+  float* states;        // [B, H, n_seg, D, D]
+  float* derivs;        // forwards: [B, H, n_seg + 1, D, D]
+  const float* S;       // backwards: the carried states
+  const float* T;       //            and their derivatives [B, H, n_seg + 1, D, D]
+  double* part;         // [B, H, n_part], the segments' parts first
+  int n_part;
   int rev;
   float w_scale;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) segment_state_kernel(StateParams p) {
-  constexpr int TPW = D / 32 * D / 32 / 4;
-  __shared__ __attribute__((aligned(1024))) T tb[kChunk * Tile<T, D>::kRow];
-  __shared__ __attribute__((aligned(1024))) T tc[kChunk * Tile<T, D>::kRow];
-  const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 5, l32 = lane & 31;
-  const int n = tokens_of(p.s, b, seg);
-  const float g2 = log2_decay(p.s, h);
-  const int64_t first = (int64_t)seg * p.s.seg;
-  const T* bb = (const T*)p.b.p + (int64_t)b * p.b.sb + (int64_t)h * p.b.sh + first * p.b.st;
-  const T* cb = (const T*)p.c.p + (int64_t)b * p.c.sb + (int64_t)h * p.c.sh + first * p.c.st;
-  f32x16 acc[TPW];
-#pragma unroll
-  for (int i = 0; i < TPW; ++i) acc[i] = f32x16{};
-  for (int c0 = 0; c0 < n; c0 += kChunk) {
-    stage_rows<T, D>(tb, bb, p.b.st, c0, n, p.rev);
-    stage_rows<T, D>(tc, cb, p.c.st, c0, n, p.rev);
-    __syncthreads();
-    state_update<T, D, true>(acc, tb, tc, min(kChunk, n - c0), g2, p.rev, p.w_scale, w, lane);
-    __syncthreads();
-  }
-  float* out = p.states + ((int64_t)bh * p.s.n_seg + seg) * D * D;
-  const int dt = D == 128 ? w : w >> 1;
-#pragma unroll
-  for (int i = 0; i < TPW; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) out[(32 * dt + acc_row(r, g)) * D + 32 * (D == 128 ? i : w & 1) + l32] = acc[i][r];
-}
-
-// ---------------------------------------------------------------------------------------------
-// In place: each segment's own state becomes the state carried into it, and the last one leaves.
-// ---------------------------------------------------------------------------------------------
-struct CarryParams {
-  Shape s;
-  float* states;
-  const float* first;   // [B, H, D, D] or null
-  float* last;          // or null
-  int rev, dd;
-};
-
-__global__ void __launch_bounds__(kThreads) carry_kernel(CarryParams p) {
-  const int e = (blockIdx.x * kThreads + threadIdx.x) * 4, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
-  if (e >= p.dd) return;
-  const float g2 = log2_decay(p.s, h);
-  const int64_t own = (int64_t)bh * p.dd + e;
-  f32x4 x = p.first ? *(const f32x4*)(p.first + own) : f32x4{0.f, 0.f, 0.f, 0.f};
-  float* st = p.states + (int64_t)bh * p.s.n_seg * p.dd + e;
-  for (int i = 0; i < p.s.n_seg; ++i) {
-    const int c = p.rev ? p.s.n_seg - 1 - i : i;
-    float* at = st + (int64_t)c * p.dd;
-    const f32x4 local = *(const f32x4*)at;
-    *(f32x4*)at = x;
-    const float keep = power(g2, tokens_of(p.s, b, c));
-#pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = x[q] * keep + local[q];
-  }
-  if (p.last) *(f32x4*)(p.last + own) = x;
-}
-
-// ---------------------------------------------------------------------------------------------
 // Rows: one workgroup per (segment, batch and head, job).
-// ---------------------------------------------------------------------------------------------
 struct Job {
   View a, b, c;
   void* y; int64_t y_sb, y_st, y_sh;
@@ -249,60 +90,203 @@ struct RowsParams {
   Job job[3];
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
-  constexpr int TPW = D / 32 * D / 32 / 4;  // state tiles of a wave
+// Pairs inside the segments, for the decay's gradient.
+struct PairsParams {
+  Shape s;
+  View q, k, v, d;
+  double* part;         // [B, H, n_part] from part_at on
+  int n_part, part_at;
+  float scale;
+};
+
+// ---------------------------------------------------------------------------------------------
+// fp32 tensors: v_mfma_f32_32x32x2 on tiles staged through registers, four waves. Time runs backwards by
+// staging the rows in the other order.
+// ---------------------------------------------------------------------------------------------
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// 32 x 32 += (32 x 16) (16 x 32): lane (l32, g) holds slots 8 g .. 8 g + 7 of the contraction.
+__device__ __forceinline__ f32x16 mma(const f32x8& a, const f32x8& b, f32x16 c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+// Row-major LDS tiles of W columns, rows padded by one 16-byte slot.
+template <int W> struct Tile {
+  static constexpr int kRow = W + 4;
+  static __device__ __forceinline__ f32x8 row8(const float* t, int row, int chunk) {
+    const f32x4 a = *(const f32x4*)(t + row * kRow + chunk * 8), b = *(const f32x4*)(t + row * kRow + chunk * 8 + 4);
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+  static __device__ __forceinline__ f32x8 col8(const float* t, int c, int col0, int lane) {
+    f32x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = t[(16 * c + 8 * (lane >> 5) + e) * kRow + col0 + (lane & 31)];
+    return v;
+  }
+  static __device__ __forceinline__ void put8(float* t, int row, int chunk, const f32x8& v) {
+    *(f32x4*)(t + row * kRow + chunk * 8) = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4*)(t + row * kRow + chunk * 8 + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  }
+  static __device__ __forceinline__ void put(float* t, int row, int col, float v) { t[row * kRow + col] = v; }
+};
+
+__device__ __forceinline__ f32x8 load8(const float* p) {
+  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+  return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// Rows [c0, c0 + 64) of a segment's n, in time's direction, into a tile; rows from n on are zeros.
+template <int D>
+__device__ __forceinline__ void stage_rows(float* tile, const float* base, int64_t st, int c0, int n, bool rev) {
+  constexpr int CPR = D / 8;
+#pragma unroll
+  for (int i = 0; i < kChunk * CPR / kThreads; ++i) {
+    const int u = threadIdx.x + i * kThreads, row = u / CPR, ch = u % CPR, t = c0 + row;
+    f32x8 v{};
+    if (t < n) v = load8(base + (int64_t)(rev ? n - 1 - t : t) * st + ch * 8);
+    Tile<D>::put8(tile, row, ch, v);
+  }
+}
+
+// Tiles of the D x D state that a wave holds. D = 128: wave w rows 32 w .. + 31 in four column tiles; D = 64:
+// tile (w / 2, w % 2).
+template <int D> struct Held {
+  static constexpr int N = D / 32 * D / 32 / 4;
+  static __device__ __forceinline__ int row0(int w) { return 32 * (D == 128 ? w : w >> 1); }
+  static __device__ __forceinline__ int col0(int w, int i) { return 32 * (D == 128 ? i : w & 1); }
+};
+
+// The state after a chunk of m tokens (and its derivative): acc = lambda^m acc + sum_j w_j b_j c_j^T.
+template <int D, bool DERIV>
+__device__ __forceinline__ void state_update(f32x16 (&acc)[Held<D>::N], f32x16 (&dacc)[Held<D>::N], const float* tb,
+                                             const float* tc, int m, float g2, int ahead, float w_scale, int w, int lane) {
+  const int g = lane >> 5;
+  const float keep = power(g2, m);
+#pragma unroll
+  for (int i = 0; i < Held<D>::N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if (DERIV) dacc[i][r] = keep * (dacc[i][r] + (float)m * acc[i][r]);
+      acc[i][r] *= keep;
+    }
+#pragma unroll
+  for (int jc = 0; jc < kChunk / 16; ++jc) {
+    f32x8 bw = Tile<D>::col8(tb, jc, Held<D>::row0(w), lane), bd;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int steps = max(0, m - 1 - (16 * jc + 8 * g + e) + ahead);
+      bw[e] *= w_scale * power(g2, steps);
+      bd[e] = bw[e] * (float)steps;
+    }
+#pragma unroll
+    for (int i = 0; i < Held<D>::N; ++i) {
+      const f32x8 c = Tile<D>::col8(tc, jc, Held<D>::col0(w, i), lane);
+      acc[i] = mma(bw, c, acc[i]);
+      if (DERIV) dacc[i] = mma(bd, c, dacc[i]);
+    }
+  }
+}
+
+// The sum over a workgroup of NW waves, valid on thread 0. `red`: NW doubles of LDS, free of other use.
+template <int NW>
+__device__ __forceinline__ double workgroup_sum(double x, double* red) {
+  x = wa_wave_sum_d(x);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double s = 0.0;
+  if (threadIdx.x == 0)
+    for (int w = 0; w < NW; ++w) s += red[w];
+  return s;
+}
+
+template <int D, bool DERIV>
+__global__ void __launch_bounds__(kThreads) segment_state_f32_kernel(StateParams p) {
+  __shared__ __attribute__((aligned(16))) float tb[kChunk * Tile<D>::kRow];
+  __shared__ __attribute__((aligned(16))) float tc[kChunk * Tile<D>::kRow];
+  __shared__ double red[4];
+  const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 5, l32 = lane & 31;
+  const int n = tokens_of(p.s, b, seg);
+  const float g2 = log2_decay(p.s, h);
+  const int64_t first = (int64_t)seg * p.s.seg;
+  const float* bb = (const float*)p.b.p + (int64_t)b * p.b.sb + (int64_t)h * p.b.sh + first * p.b.st;
+  const float* cb = (const float*)p.c.p + (int64_t)b * p.c.sb + (int64_t)h * p.c.sh + first * p.c.st;
+  f32x16 acc[Held<D>::N], dacc[Held<D>::N];
+#pragma unroll
+  for (int i = 0; i < Held<D>::N; ++i) acc[i] = dacc[i] = f32x16{};
+  for (int c0 = 0; c0 < n; c0 += kChunk) {
+    stage_rows<D>(tb, bb, p.b.st, c0, n, p.rev);
+    stage_rows<D>(tc, cb, p.c.st, c0, n, p.rev);
+    __syncthreads();
+    state_update<D, DERIV>(acc, dacc, tb, tc, min(kChunk, n - c0), g2, p.rev, p.w_scale, w, lane);
+    __syncthreads();
+  }
+  const int64_t at = ((int64_t)bh * p.s.n_seg + seg) * D * D, dat = ((int64_t)bh * (p.s.n_seg + 1) + seg) * D * D;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < Held<D>::N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int e = (Held<D>::row0(w) + acc_row(r, g)) * D + Held<D>::col0(w, i) + l32;
+      p.states[at + e] = acc[i][r];
+      if (DERIV && !p.rev) p.derivs[dat + e] = dacc[i][r];
+      if (DERIV && p.rev) sum += (double)(p.S[at + e] * dacc[i][r] + p.T[dat + e] * acc[i][r]);
+    }
+  if (DERIV && p.rev) {
+    sum = workgroup_sum<4>(sum, red);
+    if (threadIdx.x == 0) p.part[(int64_t)bh * p.n_part + seg] = sum;
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) rows_f32_kernel(RowsParams p) {
   constexpr int YT = D / 64;                // output tiles of a wave: 32 rows x D / 2 columns
-  typedef typename Frag<T>::type F;
-  __shared__ __attribute__((aligned(1024))) T tb[kChunk * Tile<T, D>::kRow];
-  __shared__ __attribute__((aligned(1024))) T tc[kChunk * Tile<T, D>::kRow];
-  __shared__ __attribute__((aligned(1024))) T tp[kChunk * Tile<T, kChunk>::kRow];
-  __shared__ __attribute__((aligned(1024))) T tx[D * Tile<T, D>::kRow];
+  __shared__ __attribute__((aligned(16))) float tb[kChunk * Tile<D>::kRow];
+  __shared__ __attribute__((aligned(16))) float tc[kChunk * Tile<D>::kRow];
+  __shared__ __attribute__((aligned(16))) float tp[kChunk * Tile<kChunk>::kRow];
+  __shared__ __attribute__((aligned(16))) float tx[D * Tile<D>::kRow];
   const Job& jb = p.job[blockIdx.z];
   const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
-  const int rh = w >> 1, ch = w & 1, dt = D == 128 ? w : w >> 1;
+  const int rh = w >> 1, ch = w & 1;
   const int n = tokens_of(p.s, b, seg), lag = jb.rev ? 0 : 1;
   const float g2 = log2_decay(p.s, h), w_scale = jb.s_intra / jb.s_inter;
   const int64_t first = (int64_t)seg * p.s.seg;
-  const T* ab = (const T*)jb.a.p + (int64_t)b * jb.a.sb + (int64_t)h * jb.a.sh + first * jb.a.st;
-  const T* bb = (const T*)jb.b.p + (int64_t)b * jb.b.sb + (int64_t)h * jb.b.sh + first * jb.b.st;
-  const T* cb = (const T*)jb.c.p + (int64_t)b * jb.c.sb + (int64_t)h * jb.c.sh + first * jb.c.st;
-  T* yb = (T*)jb.y + (int64_t)b * jb.y_sb + (int64_t)h * jb.y_sh + first * jb.y_st;
+  const float* ab = (const float*)jb.a.p + (int64_t)b * jb.a.sb + (int64_t)h * jb.a.sh + first * jb.a.st;
+  const float* bb = (const float*)jb.b.p + (int64_t)b * jb.b.sb + (int64_t)h * jb.b.sh + first * jb.b.st;
+  const float* cb = (const float*)jb.c.p + (int64_t)b * jb.c.sb + (int64_t)h * jb.c.sh + first * jb.c.st;
+  float* yb = (float*)jb.y + (int64_t)b * jb.y_sb + (int64_t)h * jb.y_sh + first * jb.y_st;
 
   // tokens past the sequence's end
   const int rows = (int)min((int64_t)p.s.seg, p.s.L - first);
-  for (int u = tid; u < (rows - n) * (D / 8); u += kThreads) {
-    T* at = yb + (int64_t)(n + u / (D / 8)) * jb.y_st + (u % (D / 8)) * 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) at[e] = (T)0.f;
-  }
+  for (int u = tid; u < (rows - n) * (D / 4); u += kThreads)
+    *(f32x4*)(yb + (int64_t)(n + u / (D / 4)) * jb.y_st + (u % (D / 4)) * 4) = f32x4{0.f, 0.f, 0.f, 0.f};
   if (n == 0) return;
 
   const float* x0 = jb.x + ((int64_t)bh * p.s.n_seg + seg) * D * D;
-  f32x16 acc[TPW];
+  f32x16 acc[Held<D>::N], none[Held<D>::N];
 #pragma unroll
-  for (int i = 0; i < TPW; ++i)
+  for (int i = 0; i < Held<D>::N; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int row = 32 * dt + acc_row(r, g), col = 32 * (D == 128 ? i : w & 1) + l32;
+      const int row = Held<D>::row0(w) + acc_row(r, g), col = Held<D>::col0(w, i) + l32;
       acc[i][r] = jb.x_trans ? x0[col * D + row] : x0[row * D + col];
     }
 
   for (int c0 = 0; c0 < n; c0 += kChunk) {
-    const int m = min(kChunk, n - c0);
-    stage_rows<T, D>(tb, bb, jb.b.st, c0, n, jb.rev);
-    stage_rows<T, D>(tc, cb, jb.c.st, c0, n, jb.rev);
+    stage_rows<D>(tb, bb, jb.b.st, c0, n, jb.rev);
+    stage_rows<D>(tc, cb, jb.c.st, c0, n, jb.rev);
 #pragma unroll
-    for (int i = 0; i < TPW; ++i)
+    for (int i = 0; i < Held<D>::N; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        Tile<T, D>::put(tx, 32 * dt + acc_row(r, g), 32 * (D == 128 ? i : w & 1) + l32, acc[i][r]);
-    F a[D / 16];
+      for (int r = 0; r < 16; ++r) Tile<D>::put(tx, Held<D>::row0(w) + acc_row(r, g), Held<D>::col0(w, i) + l32, acc[i][r]);
+    f32x8 a[D / 16];
     const int ta = c0 + 32 * rh + l32;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      a[k] = F{};
+      a[k] = f32x8{};
       if (ta < n) a[k] = load8(ab + (int64_t)(jb.rev ? n - 1 - ta : ta) * jb.a.st + 16 * k + 8 * g);
     }
     __syncthreads();
@@ -310,12 +294,12 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
     f32x16 s{};
     if (ch <= rh) {
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) s = mma(a[k], Tile<T, D>::row8(tb, 32 * ch + l32, 2 * k + g), s);
+      for (int k = 0; k < D / 16; ++k) s = mma(a[k], Tile<D>::row8(tb, 32 * ch + l32, 2 * k + g), s);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int i = 32 * rh + acc_row(r, g), j = 32 * ch + l32;
-      Tile<T, kChunk>::put(tp, i, j, j <= i ? s[r] * power(g2, i - j) : 0.f);
+      Tile<kChunk>::put(tp, i, j, j <= i ? s[r] * power(g2, i - j) : 0.f);
     }
     __syncthreads();
 #pragma unroll
@@ -323,110 +307,43 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
       const int col0 = ch * (D / 2) + 32 * yt;
       f32x16 intra{}, inter{};
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) inter = mma(a[k], Tile<T, D>::col8(tx, k, col0, lane), inter);
+      for (int k = 0; k < D / 16; ++k) inter = mma(a[k], Tile<D>::col8(tx, k, col0, lane), inter);
 #pragma unroll
       for (int jc = 0; jc < kChunk / 16; ++jc)
-        intra = mma(Tile<T, kChunk>::row8(tp, 32 * rh + l32, 2 * jc + g), Tile<T, D>::col8(tc, jc, col0, lane), intra);
+        intra = mma(Tile<kChunk>::row8(tp, 32 * rh + l32, 2 * jc + g), Tile<D>::col8(tc, jc, col0, lane), intra);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int i = 32 * rh + acc_row(r, g), t = c0 + i;
         if (t < n)
-          yb[(int64_t)(jb.rev ? n - 1 - t : t) * jb.y_st + col0 + l32] =
-              (T)(jb.s_intra * intra[r] + jb.s_inter * power(g2, i + lag) * inter[r]);
+          yb[(int64_t)(jb.rev ? n - 1 - t : t) * jb.y_st + col0 + l32] = jb.s_intra * intra[r] + jb.s_inter * power(g2, i + lag) * inter[r];
       }
     }
-    // the running state enters products of bf16 tensors rounded to bf16, so one part does here
-    state_update<T, D, false>(acc, tb, tc, m, g2, 1 - lag, w_scale, w, lane);
+    state_update<D, false>(acc, none, tb, tc, min(kChunk, n - c0), g2, 1 - lag, w_scale, w, lane);
     __syncthreads();
   }
 }
 
-// ---------------------------------------------------------------------------------------------
-// The decay's gradient, d/d log(lambda). A path from token j to token i counts its i - j steps; those
-// inside a segment of n tokens are, with S the state before it and Y the gradient state after it,
-//   scale sum_{j < i} (i - j) lambda^(i - j) (q_i . k_j)(dO_i . v_j)          both ends inside
-// + scale sum_i (i + 1) lambda^(i + 1) q_i S dO_i                             only the end
-// + sum_j (n - 1 - j) lambda^(n - 1 - j) k_j Y v_j                            only the beginning
-// + n lambda^n <S, Y>                                                         neither.
-// All of it from unrounded products (fp32 accumulators; S and Y in two parts), summed in fp64.
-// ---------------------------------------------------------------------------------------------
-struct GammaParams {
-  Shape s;
-  View q, k, v, d;
-  const float* S; const float* Y;
-  double* part;   // [B, H, n_seg]
-  float scale;
-};
-
-// sum_i weight(i) x_i M z_i over a segment's rows, M fp32 [D, D] in global memory
-template <typename T, int D, typename W>
-__device__ double bilinear(const float* M, const T* xb, int64_t x_st, const T* zb, int64_t z_st, int n, T* mhi, T* mlo,
-                           const W& weight) {
-  typedef typename Frag<T>::type F;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31, rh = w >> 1, ch = w & 1;
-  __syncthreads();
-  for (int u = tid; u < D * D; u += kThreads) {
-    const float x = M[u];
-    const T hi = (T)x;
-    Tile<T, D>::put(mhi, u / D, u % D, (float)hi);
-    if (sizeof(T) == 2) Tile<T, D>::put(mlo, u / D, u % D, x - (float)hi);
-  }
-  __syncthreads();
-  double sum = 0.0;
-  for (int c0 = 0; c0 < n; c0 += kChunk) {
-    F a[D / 16];
-    const int ta = c0 + 32 * rh + l32;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      a[k] = F{};
-      if (ta < n) a[k] = load8(xb + (int64_t)ta * x_st + 16 * k + 8 * g);
-    }
-#pragma unroll
-    for (int yt = 0; yt < D / 64; ++yt) {
-      const int col0 = ch * (D / 2) + 32 * yt;
-      f32x16 s{};
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        if (sizeof(T) == 2) s = mma(a[k], Tile<T, D>::col8(mlo, k, col0, lane), s);
-        s = mma(a[k], Tile<T, D>::col8(mhi, k, col0, lane), s);
-      }
-      float part = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int t = c0 + 32 * rh + acc_row(r, g);
-        if (t < n) part += weight(t) * s[r] * (float)zb[(int64_t)t * z_st + col0 + l32];
-      }
-      sum += (double)part;
-    }
-  }
-  return sum;
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) gamma_kernel(GammaParams p) {
-  typedef typename Frag<T>::type F;
-  __shared__ __attribute__((aligned(1024))) T t0[D * Tile<T, D>::kRow];   // keys and values of a chunk, or a state
-  __shared__ __attribute__((aligned(1024))) T t1[sizeof(T) == 2 ? D * Tile<T, D>::kRow : kChunk * Tile<T, D>::kRow];
+template <int D>
+__global__ void __launch_bounds__(kThreads) pairs_f32_kernel(PairsParams p) {
+  __shared__ __attribute__((aligned(16))) float tk[kChunk * Tile<D>::kRow];
+  __shared__ __attribute__((aligned(16))) float tv[kChunk * Tile<D>::kRow];
   __shared__ double red[4];
   const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31, rh = w >> 1, ch = w & 1;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 5, l32 = lane & 31, rh = w >> 1, ch = w & 1;
   const int n = tokens_of(p.s, b, seg);
   const float g2 = log2_decay(p.s, h);
   const int64_t first = (int64_t)seg * p.s.seg;
-  const T* qb = (const T*)p.q.p + (int64_t)b * p.q.sb + (int64_t)h * p.q.sh + first * p.q.st;
-  const T* kb = (const T*)p.k.p + (int64_t)b * p.k.sb + (int64_t)h * p.k.sh + first * p.k.st;
-  const T* vb = (const T*)p.v.p + (int64_t)b * p.v.sb + (int64_t)h * p.v.sh + first * p.v.st;
-  const T* db = (const T*)p.d.p + (int64_t)b * p.d.sb + (int64_t)h * p.d.sh + first * p.d.st;
-  T* tk = t0;
-  T* tv = t1;
+  const float* qb = (const float*)p.q.p + (int64_t)b * p.q.sb + (int64_t)h * p.q.sh + first * p.q.st;
+  const float* kb = (const float*)p.k.p + (int64_t)b * p.k.sb + (int64_t)h * p.k.sh + first * p.k.st;
+  const float* vb = (const float*)p.v.p + (int64_t)b * p.v.sb + (int64_t)h * p.v.sh + first * p.v.st;
+  const float* db = (const float*)p.d.p + (int64_t)b * p.d.sb + (int64_t)h * p.d.sh + first * p.d.st;
   double sum = 0.0;
   for (int i0 = 0; i0 < n; i0 += kChunk) {
-    F aq[D / 16], ad[D / 16];
+    f32x8 aq[D / 16], ad[D / 16];
     const int ta = i0 + 32 * rh + l32;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      aq[k] = F{};
-      ad[k] = F{};
+      aq[k] = ad[k] = f32x8{};
       if (ta < n) {
         aq[k] = load8(qb + (int64_t)ta * p.q.st + 16 * k + 8 * g);
         ad[k] = load8(db + (int64_t)ta * p.d.st + 16 * k + 8 * g);
@@ -434,14 +351,14 @@ __global__ void __launch_bounds__(kThreads) gamma_kernel(GammaParams p) {
     }
     for (int j0 = 0; j0 <= i0; j0 += kChunk) {
       __syncthreads();
-      stage_rows<T, D>(tk, kb, p.k.st, j0, n, false);
-      stage_rows<T, D>(tv, vb, p.v.st, j0, n, false);
+      stage_rows<D>(tk, kb, p.k.st, j0, n, false);
+      stage_rows<D>(tv, vb, p.v.st, j0, n, false);
       __syncthreads();
       f32x16 a{}, e{};
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        a = mma(aq[k], Tile<T, D>::row8(tk, 32 * ch + l32, 2 * k + g), a);
-        e = mma(ad[k], Tile<T, D>::row8(tv, 32 * ch + l32, 2 * k + g), e);
+        a = mma(aq[k], Tile<D>::row8(tk, 32 * ch + l32, 2 * k + g), a);
+        e = mma(ad[k], Tile<D>::row8(tv, 32 * ch + l32, 2 * k + g), e);
       }
       float part = 0.f;
 #pragma unroll
@@ -452,30 +369,508 @@ __global__ void __launch_bounds__(kThreads) gamma_kernel(GammaParams p) {
       sum += (double)part;
     }
   }
-  sum *= (double)p.scale;
-  if (n > 0) {
-    const float* S = p.S + ((int64_t)bh * p.s.n_seg + seg) * D * D;
-    const float* Y = p.Y + ((int64_t)bh * p.s.n_seg + seg) * D * D;
-    sum += (double)p.scale * bilinear<T, D>(S, qb, p.q.st, db, p.d.st, n, t0, t1,
-                                            [&](int i) { return (float)(i + 1) * power(g2, i + 1); });
-    sum += bilinear<T, D>(Y, kb, p.k.st, vb, p.v.st, n, t0, t1,
-                          [&](int j) { return (float)(n - 1 - j) * power(g2, n - 1 - j); });
-    double dot = 0.0;
-    for (int u = tid; u < D * D; u += kThreads) dot += (double)(S[u] * Y[u]);
-    sum += dot * (double)((float)n * power(g2, n));
-  }
-  sum = wa_wave_sum_d(sum);
-  if (lane == 0) red[w] = sum;
-  __syncthreads();
-  if (tid == 0) p.part[(int64_t)bh * p.s.n_seg + seg] = (red[0] + red[1]) + (red[2] + red[3]);
+  sum = workgroup_sum<4>(sum * (double)p.scale, red);
+  if (threadIdx.x == 0) p.part[(int64_t)bh * p.n_part + p.part_at + seg] = sum;
 }
 
-__global__ void __launch_bounds__(64) gamma_sum_kernel(const double* part, int B, int H, int n_seg, float* out) {
-  const int h = blockIdx.x, lane = threadIdx.x;
+// ---------------------------------------------------------------------------------------------
+// bf16 forms. Tiles of 64 tokens stream into a ring of LDS stages by direct loads, two steps ahead; rows
+// past the segment's last token read as zeros. Time runs backwards by taking the chunks in the other
+// order, with weights and masks mirrored inside a chunk; memory order inside a tile stays.
+//
+// All products run transposed so that operands stay where they are. A column permutation of the
+// transpose reads makes it fit: the accumulator's row (register r, lane group g) is 8 (r / 4) + 4 g + r % 4;
+// feeding rows in the order pi (bits 2 and 3 swapped) leaves lane group g holding, in registers
+// 8 h .. 8 h + 7, rows 16 h + 8 g .. + 7: eight consecutive channels, which is both a 16-byte store and
+// the natural operand order of the next product.
+// ---------------------------------------------------------------------------------------------
+// tile_tr8 (contraction in accumulator order over the 16 tokens of chunk c) with lane l32 at column
+// col0 + pi(l32).
+template <int D>
+__device__ __forceinline__ bf16x8 tile_tr8_pi(const bf16_t* lds, int c, int col0, int lane) {
+  const int G = lane >> 4, r = (lane & 15) >> 2, q = ((lane & 1) << 1) | ((lane >> 1) & 1);
+  bf16x8 a;
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    const int row = 16 * c + 4 * (G >> 1) + 8 * hf + r;
+    const int col = col0 + 16 * (G & 1) + 4 * q;
+    const int slot = (col >> 3) ^ dual_swizzle<D>(row);
+    const wa_s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(WA_LDS_S16X4(lds + row * D + slot * 8 + (col & 7)));
+    const bf16x4 b = __builtin_bit_cast(bf16x4, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[4 * hf + e] = b[e];
+  }
+  return a;
+}
+__device__ __forceinline__ int pi32(int x) { return (x & 0x13) | ((x & 4) << 1) | ((x & 8) >> 1); }
+
+// TileStream (tile.h) over one segment, with the descriptor cut to the chunk's rows: any distance between the
+// segment's first and last token, up to kMaxTokenStride elements between two.
+constexpr int64_t kMaxTokenStride = (int64_t)1 << 23;
+template <int D, int NW>
+struct ChunkStream {
+  static constexpr int NI = TileStream<D, NW>::NI, RPI = TileStream<D, NW>::RPI;
+  const bf16_t* base;
+  int64_t st;
+  int off[NI];
+  __device__ __forceinline__ void init(const View& x, int b, int h, int64_t first, int w, int lane) {
+    base = (const bf16_t*)x.p + (int64_t)b * x.sb + (int64_t)h * x.sh + first * x.st;
+    st = x.st;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = (i * NW + w) * RPI + lane / (D / 8), pos = lane % (D / 8);
+      off[i] = (row * (int)st + (pos ^ dual_swizzle<D>(row)) * 8) * 2;
+    }
+  }
+  // rows row0 .. row0 + rows - 1 (at most 64) into `lds`, zeros behind them
+  __device__ __forceinline__ void issue(bf16_t* lds, int row0, int rows, int w) const {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(base + (int64_t)row0 * st), (short)0, ((rows - 1) * (int)st + D) * 2, WA_BUF_DWORD3);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) lds_dma16(rs, lds + (i * NW + w) * RPI * D, off[i]);
+  }
+};
+
+__device__ __forceinline__ bf16x8 pack8(const f32x16& a, int h) {
+  bf16x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (bf16_t)a[8 * h + e];
+  return v;
+}
+
+// x = hi + mid + lo exactly: three bf16 values cut off a float's 24 bits.
+__device__ __forceinline__ void cut3(const float (&x)[8], bf16x8& hi, bf16x8& mid, bf16x8& lo) {
+  u32x4 h, m, l;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t hb[2], mb[2], lb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float v = x[2 * q + i];
+      hb[i] = __float_as_uint(v);
+      const float r = v - __uint_as_float(hb[i] & 0xffff0000u);
+      mb[i] = __float_as_uint(r);
+      lb[i] = __float_as_uint(r - __uint_as_float(mb[i] & 0xffff0000u));
+    }
+    h[q] = __builtin_amdgcn_perm(hb[1], hb[0], 0x07060302);   // the high halves of two floats side by side
+    m[q] = __builtin_amdgcn_perm(mb[1], mb[0], 0x07060302);
+    l[q] = __builtin_amdgcn_perm(lb[1], lb[0], 0x07060302);
+  }
+  hi = __builtin_bit_cast(bf16x8, h);
+  mid = __builtin_bit_cast(bf16x8, m);
+  lo = __builtin_bit_cast(bf16x8, l);
+}
+
+// Weights of the tokens of a chunk in the running state after it, m tokens long: lambda^(m - 1 - j), backwards
+// lambda^(j + 1), times w_scale. Filled by the first wave.
+__device__ __forceinline__ void fill_weights(float* wt, float g2, int m, bool rev, float w_scale, int lane) {
+  wt[lane] = w_scale * power(g2, rev ? lane + 1 : max(0, m - 1 - lane));
+}
+// The 8 weights of a fragment's tokens (accumulator order).
+__device__ __forceinline__ void load_weights(const float* wt, int c, int g, float (&w)[8]) {
+  const f32x4 a = *(const f32x4*)(wt + 16 * c + 4 * g), b = *(const f32x4*)(wt + 16 * c + 8 + 4 * g);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    w[e] = a[e];
+    w[e + 4] = b[e];
+  }
+}
+
+// A segment's own state. Wave (ch, dh) of D / 16 waves: columns 32 ch .. + 31, half of the rows. The
+// weighted operand enters in three parts, so the state carries no rounding but its fp32 sums'.
+template <int D, bool DERIV>
+__global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(StateParams p) {
+  constexpr int NW = D / 16, CT = D / 32, DT = CT / 2, STAGES = 3, NI = ChunkStream<D, NW>::NI;
+  __shared__ __attribute__((aligned(1024))) bf16_t tb[STAGES][kChunk * D];
+  __shared__ __attribute__((aligned(1024))) bf16_t tc[STAGES][kChunk * D];
+  __shared__ __attribute__((aligned(16))) float wt[2][kChunk];
+  __shared__ double red[NW];
+  const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
+  const int ch = w % CT, dh = w / CT;
+  const int n = tokens_of(p.s, b, seg), chunks = (n + kChunk - 1) / kChunk, tail = n - (chunks - 1) * kChunk;
+  const float g2 = log2_decay(p.s, h);
+  const int64_t first = (int64_t)seg * p.s.seg;
+  ChunkStream<D, NW> sb, sc;
+  sb.init(p.b, b, h, first, w, lane);
+  sc.init(p.c, b, h, first, w, lane);
+  auto issue = [&](int it) {
+    const int row0 = (p.rev ? chunks - 1 - it : it) * kChunk, rows = min(kChunk, n - row0);
+    sb.issue(tb[it % STAGES], row0, rows, w);
+    sc.issue(tc[it % STAGES], row0, rows, w);
+  };
+  f32x16 acc[DT], dacc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) acc[i] = dacc[i] = f32x16{};
+  if (w == 0) {   // the whole chunks' weights, and those of the one cut off at the end
+    fill_weights(wt[0], g2, kChunk, p.rev, p.w_scale, lane);
+    fill_weights(wt[1], g2, tail, p.rev, p.w_scale, lane);
+  }
+  if (chunks > 0) issue(0);
+  if (chunks > 1) issue(1);
+  for (int it = 0; it < chunks; ++it) {
+    // tile it has landed (it + 1 may stream) and every wave is past tile it - 1, whose stage is refilled
+    if (it + 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (it + 2 < chunks) issue(it + 2);
+    const bool cut = (p.rev ? chunks - 1 - it : it) == chunks - 1;
+    const int m = cut ? tail : kChunk;
+    const float keep = power(g2, m);
+    const bf16_t* B = tb[it % STAGES];
+    const bf16_t* C = tc[it % STAGES];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (DERIV) dacc[i][r] = keep * (dacc[i][r] + (float)m * acc[i][r]);
+        acc[i][r] *= keep;
+      }
+#pragma unroll
+    for (int c = 0; c < kChunk / 16; ++c) {
+      float wv[8];
+      load_weights(wt[cut ? 1 : 0], c, g, wv);
+      const bf16x8 cv = tile_tr8<D>(C, c, 32 * ch, lane);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wv[e] *= (float)cv[e];
+      bf16x8 hi, mid, lo, bv[DT];
+#pragma unroll
+      for (int i = 0; i < DT; ++i) bv[i] = tile_tr8<D>(B, c, 32 * (DT * dh + i), lane);
+      cut3(wv, hi, mid, lo);
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        acc[i] = wa_mfma32(bv[i], lo, acc[i]);
+        acc[i] = wa_mfma32(bv[i], mid, acc[i]);
+        acc[i] = wa_mfma32(bv[i], hi, acc[i]);
+      }
+      if (DERIV) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = 16 * c + 4 * g + 8 * (e >> 2) + (e & 3);
+          wv[e] *= (float)(p.rev ? j + 1 : max(0, m - 1 - j));
+        }
+        cut3(wv, hi, mid, lo);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          dacc[i] = wa_mfma32(bv[i], lo, dacc[i]);
+          dacc[i] = wa_mfma32(bv[i], mid, dacc[i]);
+          dacc[i] = wa_mfma32(bv[i], hi, dacc[i]);
+        }
+      }
+    }
+  }
+  const int64_t at = ((int64_t)bh * p.s.n_seg + seg) * D * D, dat = ((int64_t)bh * (p.s.n_seg + 1) + seg) * D * D;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int e = (32 * (DT * dh + i) + acc_row(r, g)) * D + 32 * ch + l32;
+      p.states[at + e] = acc[i][r];
+      if (DERIV && !p.rev) p.derivs[dat + e] = dacc[i][r];
+      if (DERIV && p.rev) sum += (double)(p.S[at + e] * dacc[i][r] + p.T[dat + e] * acc[i][r]);
+    }
+  if (DERIV && p.rev) {
+    sum = workgroup_sum<NW>(sum, red);
+    if (tid == 0) p.part[(int64_t)bh * p.n_part + seg] = sum;
+  }
+}
+
+// Rows. Wave (ch, rh) of D / 16 waves: output channels 32 ch .. + 31 of the chunk's rows 32 rh .. + 31, and the
+// running state's columns 32 ch .. + 31 in accumulators (both halves keep a copy: the second update costs
+// less than passing it). Per chunk, with P^T = B A^T decayed and masked,
+//   Y^T = s_intra C^T P^T + s_inter lambda^.. X^T A^T,    X = lambda^m X + B^T (weighted C):
+// P^T's accumulators are the second product's operand in place, X's the third's.
+template <int D>
+__global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) {
+  constexpr int NW = D / 16, CT = D / 32, KS = D / 16, STAGES = 3, NI = ChunkStream<D, NW>::NI;
+  __shared__ __attribute__((aligned(1024))) bf16_t ta[STAGES][kChunk * D];
+  __shared__ __attribute__((aligned(1024))) bf16_t tb[STAGES][kChunk * D];
+  __shared__ __attribute__((aligned(1024))) bf16_t tc[STAGES][kChunk * D];
+  __shared__ __attribute__((aligned(16))) float wt[kChunk];
+  const Job& jb = p.job[blockIdx.z];
+  const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
+  const int ch = w % CT, rh = w / CT;
+  const bool rev = jb.rev;
+  const int n = tokens_of(p.s, b, seg), chunks = (n + kChunk - 1) / kChunk;
+  const float g2 = log2_decay(p.s, h);
+  const int64_t first = (int64_t)seg * p.s.seg;
+  bf16_t* yb = (bf16_t*)jb.y + (int64_t)b * jb.y_sb + (int64_t)h * jb.y_sh + first * jb.y_st;
+
+  // tokens past the sequence's end
+  const int rows = (int)min((int64_t)p.s.seg, p.s.L - first);
+  for (int u = tid; u < (rows - n) * (D / 8); u += 64 * NW)
+    *(u32x4*)(yb + (int64_t)(n + u / (D / 8)) * jb.y_st + (u % (D / 8)) * 8) = u32x4{0, 0, 0, 0};
+  if (n == 0) return;
+
+  ChunkStream<D, NW> sa, sb, sc;
+  sa.init(jb.a, b, h, first, w, lane);
+  sb.init(jb.b, b, h, first, w, lane);
+  sc.init(jb.c, b, h, first, w, lane);
+  auto issue = [&](int it) {
+    const int row0 = (rev ? chunks - 1 - it : it) * kChunk, m = min(kChunk, n - row0);
+    sa.issue(ta[it % STAGES], row0, m, w);
+    sb.issue(tb[it % STAGES], row0, m, w);
+    sc.issue(tc[it % STAGES], row0, m, w);
+  };
+  issue(0);
+  if (chunks > 1) issue(1);
+  if (w == 0) fill_weights(wt, g2, kChunk, rev, jb.s_intra / jb.s_inter, lane);
+
+  // X[d][e] of lane (l32, g): e = 32 ch + pi(l32), tile dt's register 8 h + x: d = 32 dt + 16 h + 8 g + x
+  f32x16 X[CT];
+  const float* x0 = jb.x + ((int64_t)bh * p.s.n_seg + seg) * D * D;
+  const int e0 = 32 * ch + pi32(l32);
+#pragma unroll
+  for (int dt = 0; dt < CT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int d = 32 * dt + 16 * (r >> 3) + 8 * g + (r & 7);
+      X[dt][r] = jb.x_trans ? x0[e0 * D + d] : x0[d * D + e0];
+    }
+  // decay from token j = 32 jh + acc_row to row i = 32 rh + l32 of the chunk, 0 against time's direction
+  float near[16], far[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int steps = rev ? acc_row(r, g) - l32 : l32 - acc_row(r, g);
+    near[r] = steps >= 0 ? power(g2, steps) : 0.f;
+    far[r] = power(g2, steps + 32);
+  }
+  const bool both = rev ? rh == 0 : rh == 1;   // this wave's rows also see the other half's tokens
+  const int i = 32 * rh + l32;
+
+  u32x4 y[2] = {};           // the chunk's finished outputs, stored in the next step ahead of its loads
+  int y_row = -1;
+  auto store = [&]() {
+    if (y_row >= 0 && y_row < n) {
+      bf16_t* at = yb + (int64_t)y_row * jb.y_st + 32 * ch + 8 * g;
+      *(u32x4*)at = y[0];
+      *(u32x4*)(at + 16) = y[1];
+    }
+  };
+  for (int it = 0; it < chunks; ++it) {
+    const int c0 = (rev ? chunks - 1 - it : it) * kChunk, m = min(kChunk, n - c0);
+    // Tile it has landed (only it + 1's loads were issued after it and the stores before them) and every
+    // wave is past tile it - 1, whose stage is refilled.
+    if (it + 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(3 * NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    store();
+    if (it + 2 < chunks) issue(it + 2);
+    const bf16_t* A = ta[it % STAGES];
+    const bf16_t* B = tb[it % STAGES];
+    const bf16_t* C = tc[it % STAGES];
+    bf16x8 a[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) a[k] = tile_row8<D>(A, i, 2 * k + g);
+    f32x16 y1{}, y2{};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      bf16x8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = X[k / 2][8 * (k % 2) + e];
+        hi[e] = (bf16_t)x;
+        lo[e] = (bf16_t)(x - (float)hi[e]);
+      }
+      y2 = wa_mfma32(lo, a[k], y2);
+      y2 = wa_mfma32(hi, a[k], y2);
+    }
+    bf16x8 cv[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) cv[c] = tile_tr8_pi<D>(C, c, 32 * ch, lane);
+#pragma unroll
+    for (int jh = 0; jh < 2; ++jh) {
+      if (jh != rh && !both) continue;
+      f32x16 s{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) s = wa_mfma32(tile_row8<D>(B, 32 * jh + l32, 2 * k + g), a[k], s);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= jh == rh ? near[r] : far[r];
+      y1 = wa_mfma32(cv[2 * jh], pack8(s, 0), y1);
+      y1 = wa_mfma32(cv[2 * jh + 1], pack8(s, 1), y1);
+    }
+    const float f = jb.s_inter * power(g2, rev ? max(0, m - 1 - i) : i + 1);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      bf16x8 o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = (bf16_t)(jb.s_intra * y1[8 * q + e] + f * y2[8 * q + e]);
+      y[q] = __builtin_bit_cast(u32x4, o);
+    }
+    y_row = c0 + i;
+    if (it + 1 < chunks) {   // forwards only whole chunks are followed by another
+      const float keep = power(g2, m);
+#pragma unroll
+      for (int dt = 0; dt < CT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) X[dt][r] *= keep;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float wv[8];
+        load_weights(wt, c, g, wv);
+        bf16x8 cw;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cw[e] = (bf16_t)(wv[e] * (float)cv[c][e]);
+#pragma unroll
+        for (int dt = 0; dt < CT; ++dt) X[dt] = wa_mfma32(tile_tr8_pi<D>(B, c, 32 * dt, lane), cw, X[dt]);
+      }
+    }
+  }
+  store();
+}
+
+// Pairs: a workgroup takes 256 rows i of a segment, 32 a wave, whose queries and output gradients stay in
+// registers as operands, against the segment's keys and values up to them (a ring of LDS stages). Tiles before
+// the diagonal separate: with e the tile's last token, (i - j) lambda^(i - j) = lambda^(i - e) [(i - e) + (e - j)]
+// lambda^(e - j), no power above 1, the column factors being the same for every tile.
+constexpr int kPairRows = 256;
+
+template <int D>
+__global__ void __launch_bounds__(512) pairs_bf16_kernel(PairsParams p) {
+  constexpr int NW = 8, KS = D / 16, STAGES = 3, NI = ChunkStream<D, NW>::NI;
+  __shared__ __attribute__((aligned(1024))) bf16_t tk[STAGES][kChunk * D];
+  __shared__ __attribute__((aligned(1024))) bf16_t tv[STAGES][kChunk * D];
+  __shared__ double red[NW];
+  const int groups = (p.s.seg + kPairRows - 1) / kPairRows;
+  const int seg = blockIdx.x / groups, ig = blockIdx.x % groups, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
+  const int n = tokens_of(p.s, b, seg), i0 = ig * kPairRows, iw = i0 + 32 * w, i = iw + l32;
+  double* out = p.part + (int64_t)bh * p.n_part + p.part_at + blockIdx.x;
+  if (i0 >= n) {
+    if (tid == 0) *out = 0.0;
+    return;
+  }
+  const int chunks = (min(n, i0 + kPairRows) + kChunk - 1) / kChunk;
+  const float g2 = log2_decay(p.s, h);
+  const int64_t first = (int64_t)seg * p.s.seg;
+  ChunkStream<D, NW> sk, sv;
+  sk.init(p.k, b, h, first, w, lane);
+  sv.init(p.v, b, h, first, w, lane);
+  auto issue = [&](int it) {
+    sk.issue(tk[it % STAGES], it * kChunk, min(kChunk, n - it * kChunk), w);
+    sv.issue(tv[it % STAGES], it * kChunk, min(kChunk, n - it * kChunk), w);
+  };
+  bf16x8 q[KS], d[KS];
+  const bf16_t* qb = (const bf16_t*)p.q.p + (int64_t)b * p.q.sb + (int64_t)h * p.q.sh + (first + i) * p.q.st + 8 * g;
+  const bf16_t* db = (const bf16_t*)p.d.p + (int64_t)b * p.d.sb + (int64_t)h * p.d.sh + (first + i) * p.d.st + 8 * g;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    q[k] = d[k] = bf16x8{};
+    if (i < n) {
+      q[k] = *(const bf16x8*)(qb + 16 * k);
+      d[k] = *(const bf16x8*)(db + 16 * k);
+    }
+  }
+  float cj[16];   // lambda^(e - j) of the tile's rows
+#pragma unroll
+  for (int r = 0; r < 16; ++r) cj[r] = power(g2, 31 - acc_row(r, g));
+  issue(0);
+  if (chunks > 1) issue(1);
+  double sum = 0.0;
+  for (int it = 0; it < chunks; ++it) {
+    if (it + 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (it + 2 < chunks) issue(it + 2);
+#pragma unroll
+    for (int jh = 0; jh < 2; ++jh) {
+      const int jt = it * kChunk + 32 * jh;
+      if (jt > iw || iw >= n) continue;
+      f32x16 s{}, t{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        s = wa_mfma32(tile_row8<D>(tk[it % STAGES], 32 * jh + l32, 2 * k + g), q[k], s);
+        t = wa_mfma32(tile_row8<D>(tv[it % STAGES], 32 * jh + l32, 2 * k + g), d[k], t);
+      }
+      if (jt < iw) {
+        float u = 0.f, v = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = cj[r] * (s[r] * t[r]);
+          u += x;
+          v += (float)(31 - acc_row(r, g)) * x;
+        }
+        const int steps = i - jt - 31;
+        sum += (double)(power(g2, steps) * ((float)steps * u + v));
+      } else {
+        float u = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int steps = l32 - acc_row(r, g);
+          u += steps > 0 ? (float)steps * power(g2, steps) * (s[r] * t[r]) : 0.f;
+        }
+        sum += (double)u;
+      }
+    }
+  }
+  sum = workgroup_sum<NW>(sum * (double)p.scale, red);
+  if (tid == 0) *out = sum;
+}
+
+// ---------------------------------------------------------------------------------------------
+// In place: each segment's own state becomes the state carried into it, and the last one leaves; forwards the
+// derivatives with them, backwards the sequence's end of the decay's gradient, <T, dS>.
+// ---------------------------------------------------------------------------------------------
+struct CarryParams {
+  Shape s;
+  float* states;
+  float* derivs;        // forwards, or null: [B, H, n_seg + 1, D, D], the last one the sequence's
+  const float* first;   // [B, H, D, D] or null
+  float* last;          // or null
+  const float* T;       // backwards, or null: the derivatives
+  double* part;
+  int n_part, part_at;
+  int rev, dd;
+};
+
+// One element a thread: only the multiply-adds are sequential, so the loads of eight segments go out together.
+__global__ void __launch_bounds__(kThreads) carry_kernel(CarryParams p) {
+  constexpr int AHEAD = 8;
+  __shared__ double red[kThreads / 64];
+  const int e = blockIdx.x * kThreads + threadIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
+  const float g2 = log2_decay(p.s, h);
+  const int64_t own = (int64_t)bh * p.dd + e;
+  float x = p.first ? p.first[own] : 0.f, dx = 0.f;
+  float* st = p.states + (int64_t)bh * p.s.n_seg * p.dd + e;
+  float* dt = p.derivs ? p.derivs + (int64_t)bh * (p.s.n_seg + 1) * p.dd + e : nullptr;
+  if (p.T) {
+    const double sum = workgroup_sum<kThreads / 64>((double)(x * p.T[((int64_t)bh * (p.s.n_seg + 1) + p.s.n_seg) * p.dd + e]), red);
+    if (threadIdx.x == 0) p.part[(int64_t)bh * p.n_part + p.part_at + blockIdx.x] = sum;
+  }
+  for (int i0 = 0; i0 < p.s.n_seg; i0 += AHEAD) {
+    float local[AHEAD], dlocal[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int c = p.rev ? p.s.n_seg - 1 - (i0 + i) : i0 + i;
+      if (i0 + i < p.s.n_seg) local[i] = st[(int64_t)c * p.dd];
+      if (i0 + i < p.s.n_seg && dt) dlocal[i] = dt[(int64_t)c * p.dd];
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int c = p.rev ? p.s.n_seg - 1 - (i0 + i) : i0 + i;
+      if (i0 + i < p.s.n_seg) {
+        const int n = tokens_of(p.s, b, c);
+        const float keep = power(g2, n);
+        st[(int64_t)c * p.dd] = x;
+        if (dt) {
+          dt[(int64_t)c * p.dd] = dx;
+          dx = keep * (dx + (float)n * x) + dlocal[i];
+        }
+        x = x * keep + local[i];
+      }
+    }
+  }
+  if (p.last) p.last[own] = x;
+  if (dt) dt[(int64_t)p.s.n_seg * p.dd] = dx;
+}
+
+// The decay's gradient of one head: all parts of its rows, in a fixed order.
+__global__ void __launch_bounds__(kThreads) decay_grad_kernel(const double* part, int B, int H, int n_part, float* out) {
+  __shared__ double red[kThreads / 64];
+  const int h = blockIdx.x;
   double s = 0.0;
-  for (int i = lane; i < B * n_seg; i += 64) s += part[((int64_t)(i / n_seg) * H + h) * n_seg + i % n_seg];
-  s = wa_wave_sum_d(s);
-  if (lane == 0) out[h] = (float)s;
+  for (int i = threadIdx.x; i < B * n_part; i += kThreads) s += part[((int64_t)(i / n_part) * H + h) * n_part + i % n_part];
+  s = workgroup_sum<kThreads / 64>(s, red);
+  if (threadIdx.x == 0) out[h] = (float)s;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -548,16 +943,26 @@ __global__ void __launch_bounds__(kThreads) step_kernel(StepParams p) {
   }
 }
 
-// Segments: enough workgroups for two on each of 256 CUs, a segment not below 128 tokens (its fp32 state,
-// read and written, then costs no more than its tokens) and a multiple of the chunk.
+// Segments: as many as give every CU work, in whole rounds of the 256 workgroups that run at once (the rows
+// kernel's LDS ring takes most of a CU), with the shortest time of rounds x segment length; a segment is a
+// multiple of the chunk and not below 128 tokens, where its fp32 state costs as much as its tokens.
 int64_t segment_length(int64_t B, int64_t L, int64_t H) {
-  const int64_t want = (L * B * H + 511) / 512;
-  return std::max<int64_t>(128, (want + kChunk - 1) / kChunk * kChunk);
+  const int64_t rows = B * H;
+  int64_t best = 0, best_cost = INT64_MAX;
+  for (int64_t k = 1; k <= std::min<int64_t>(256, (L + 127) / 128); ++k) {
+    const int64_t seg = std::max<int64_t>(128, ((L + k - 1) / k + kChunk - 1) / kChunk * kChunk);
+    const int64_t n = (L + seg - 1) / seg, cost = (rows * n + 255) / 256 * seg + 8 * n;
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = seg;
+    }
+  }
+  return best;
 }
 
 bool rows16(const void* p, int64_t sb, int64_t st, int64_t sh, int dtype) {
   const int v = dtype == WA_BF16 ? 8 : 4;
-  return wa_aligned16(p) && sb % v == 0 && st % v == 0 && sh % v == 0;
+  return wa_aligned16(p) && st >= 0 && st <= kMaxTokenStride && sb % v == 0 && st % v == 0 && sh % v == 0;
 }
 
 int check_shape(const char* what, int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
@@ -572,45 +977,74 @@ Shape shape_of(int64_t B, int64_t L, int64_t H, const float* g, const int32_t* l
   return Shape{(int)B, (int)L, (int)H, (int)segment_length(B, L, H), (int)wa_decay_segments(B, L, H), g, lengths};
 }
 
-template <typename T, int D>
-void launch_states(const Shape& s, const View& b, const View& c, float* states, const float* first, float* last, bool rev,
-                   float w_scale, hipStream_t st) {
-  hipLaunchKernelGGL((segment_state_kernel<T, D>), dim3(s.n_seg, s.B * s.H), dim3(kThreads), 0, st,
-                     StateParams{s, b, c, states, rev, w_scale});
-  hipLaunchKernelGGL(carry_kernel, dim3(D * D / 4 / kThreads, s.B * s.H), dim3(kThreads), 0, st,
-                     CarryParams{s, states, first, last, rev, D * D});
+// Workgroups of the pairs kernel along a head: one per segment in fp32, one per 256 rows in bf16.
+int64_t pair_groups(int dtype, const Shape& s) {
+  return dtype == WA_F32 ? s.n_seg : (int64_t)s.n_seg * ((s.seg + kPairRows - 1) / kPairRows);
 }
 
-template <typename T, int D>
+template <int D, bool DERIV>
+void segment_states(int dtype, const StateParams& p, hipStream_t st) {
+  const dim3 grid(p.s.n_seg, p.s.B * p.s.H);
+  if (dtype == WA_BF16) hipLaunchKernelGGL((segment_state_bf16_kernel<D, DERIV>), grid, dim3(64 * (D / 16)), 0, st, p);
+  else hipLaunchKernelGGL((segment_state_f32_kernel<D, DERIV>), grid, dim3(kThreads), 0, st, p);
+}
+
+template <int D>
+void all_rows(int dtype, const RowsParams& p, int jobs, hipStream_t st) {
+  const dim3 grid(p.s.n_seg, p.s.B * p.s.H, jobs);
+  if (dtype == WA_BF16) hipLaunchKernelGGL((rows_bf16_kernel<D>), grid, dim3(64 * (D / 16)), 0, st, p);
+  else hipLaunchKernelGGL((rows_f32_kernel<D>), grid, dim3(kThreads), 0, st, p);
+}
+
+template <int D>
 int run_fwd(const wa_decay_fwd_args* a, hipStream_t st) {
   const Shape s = shape_of(a->B, a->L, a->H, a->log_decay, a->lengths);
   const View q{a->q, a->q_sb, a->q_st, a->q_sh}, k{a->k, a->k_sb, a->k_st, a->k_sh}, v{a->v, a->v_sb, a->v_st, a->v_sh};
-  launch_states<T, D>(s, k, v, a->states, a->initial, a->final_state, false, 1.f, st);
+  StateParams sp{};
+  sp.s = s; sp.b = k; sp.c = v; sp.states = a->states; sp.derivs = a->derivs; sp.w_scale = 1.f;
+  if (a->derivs) segment_states<D, true>(a->dtype, sp, st);
+  else segment_states<D, false>(a->dtype, sp, st);
+  CarryParams cp{};
+  cp.s = s; cp.states = a->states; cp.derivs = a->derivs; cp.first = a->initial; cp.last = a->final_state; cp.dd = D * D;
+  hipLaunchKernelGGL(carry_kernel, dim3(D * D / kThreads, s.B * s.H), dim3(kThreads), 0, st, cp);
   RowsParams p{};
   p.s = s;
   p.job[0] = Job{q, k, v, a->o, a->o_sb, a->o_st, a->o_sh, a->states, 0, 0, a->scale, a->scale};
-  hipLaunchKernelGGL((rows_kernel<T, D>), dim3(s.n_seg, s.B * s.H, 1), dim3(kThreads), 0, st, p);
+  all_rows<D>(a->dtype, p, 1, st);
   return wa_launch_status("decay_fwd");
 }
 
-template <typename T, int D>
+template <int D>
 int run_bwd(const wa_decay_bwd_args* a, hipStream_t st) {
   const Shape s = shape_of(a->B, a->L, a->H, a->log_decay, a->lengths);
   const View q{a->q, a->q_sb, a->q_st, a->q_sh}, k{a->k, a->k_sb, a->k_st, a->k_sh}, v{a->v, a->v_sb, a->v_st, a->v_sh};
   const View d{a->dout, a->d_sb, a->d_st, a->d_sh};
   float* Y = (float*)a->workspace;
   double* part = (double*)(Y + (int64_t)s.B * s.H * s.n_seg * D * D);
-  launch_states<T, D>(s, q, d, Y, a->dfinal, a->dinitial, true, a->scale, st);
+  const int pairs = (int)pair_groups(a->dtype, s), n_part = s.n_seg + D * D / kThreads + pairs;
+  StateParams sp{};
+  sp.s = s; sp.b = q; sp.c = d; sp.states = Y; sp.S = a->states; sp.T = a->derivs; sp.part = part; sp.n_part = n_part;
+  sp.rev = 1; sp.w_scale = a->scale;
+  if (a->dlog_decay) segment_states<D, true>(a->dtype, sp, st);
+  else segment_states<D, false>(a->dtype, sp, st);
+  CarryParams cp{};
+  cp.s = s; cp.states = Y; cp.first = a->dfinal; cp.last = a->dinitial; cp.rev = 1; cp.dd = D * D;
+  if (a->dlog_decay) {
+    cp.T = a->derivs; cp.part = part; cp.n_part = n_part; cp.part_at = s.n_seg;
+  }
+  hipLaunchKernelGGL(carry_kernel, dim3(D * D / kThreads, s.B * s.H), dim3(kThreads), 0, st, cp);
   RowsParams p{};
   p.s = s;
   p.job[0] = Job{d, v, k, a->dq, a->dq_sb, a->dq_st, a->dq_sh, a->states, 1, 0, a->scale, a->scale};
   p.job[1] = Job{k, q, d, a->dv, a->dv_sb, a->dv_st, a->dv_sh, Y, 0, 1, a->scale, 1.f};
   p.job[2] = Job{v, d, q, a->dk, a->dk_sb, a->dk_st, a->dk_sh, Y, 1, 1, a->scale, 1.f};
-  hipLaunchKernelGGL((rows_kernel<T, D>), dim3(s.n_seg, s.B * s.H, 3), dim3(kThreads), 0, st, p);
+  all_rows<D>(a->dtype, p, 3, st);
   if (a->dlog_decay) {
-    hipLaunchKernelGGL((gamma_kernel<T, D>), dim3(s.n_seg, s.B * s.H), dim3(kThreads), 0, st,
-                       GammaParams{s, q, k, v, d, a->states, Y, part, a->scale});
-    hipLaunchKernelGGL(gamma_sum_kernel, dim3(s.H), dim3(64), 0, st, (const double*)part, s.B, s.H, s.n_seg, a->dlog_decay);
+    const PairsParams pp{s, q, k, v, d, part, n_part, s.n_seg + D * D / kThreads, a->scale};
+    const dim3 grid((unsigned)pairs, s.B * s.H);
+    if (a->dtype == WA_BF16) hipLaunchKernelGGL((pairs_bf16_kernel<D>), grid, dim3(512), 0, st, pp);
+    else hipLaunchKernelGGL((pairs_f32_kernel<D>), grid, dim3(kThreads), 0, st, pp);
+    hipLaunchKernelGGL(decay_grad_kernel, dim3(s.H), dim3(kThreads), 0, st, (const double*)part, s.B, s.H, n_part, a->dlog_decay);
   }
   return wa_launch_status("decay_bwd");
 }
@@ -624,7 +1058,10 @@ extern "C" int64_t wa_decay_segments(int64_t B, int64_t L, int64_t H) {
 }
 
 extern "C" int64_t wa_decay_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D) {
-  return B * H * wa_decay_segments(B, L, H) * (D * D * 4 + 8);
+  if (B <= 0 || L <= 0 || H <= 0) return 0;
+  const Shape s = shape_of(B, L, H, nullptr, nullptr);
+  const int64_t parts = s.n_seg + D * D / kThreads + std::max(pair_groups(WA_F32, s), pair_groups(WA_BF16, s));
+  return B * H * (s.n_seg * D * D * 4 + parts * 8);
 }
 
 extern "C" int wa_decay_fwd(const wa_decay_fwd_args* a, void* stream) {
@@ -635,10 +1072,9 @@ extern "C" int wa_decay_fwd(const wa_decay_fwd_args* a, void* stream) {
   WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->log_decay && a->states, "decay_fwd: null tensor");
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype) &&
                rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype) && wa_aligned16(a->states) && wa_aligned16(a->initial) &&
-               wa_aligned16(a->final_state), "decay_fwd: rows and states must be 16-byte aligned");
+               wa_aligned16(a->final_state), "decay_fwd: rows and states must be 16-byte aligned, tokens at most 2^23 elements apart");
   hipStream_t s = (hipStream_t)stream;
-  if (a->dtype == WA_BF16) return a->D == 128 ? run_fwd<bf16_t, 128>(a, s) : run_fwd<bf16_t, 64>(a, s);
-  return a->D == 128 ? run_fwd<float, 128>(a, s) : run_fwd<float, 64>(a, s);
+  return a->D == 128 ? run_fwd<128>(a, s) : run_fwd<64>(a, s);
 }
 
 extern "C" int wa_decay_bwd(const wa_decay_bwd_args* a, void* stream) {
@@ -648,13 +1084,13 @@ extern "C" int wa_decay_bwd(const wa_decay_bwd_args* a, void* stream) {
   WA_CHECK_ARG(a->B > 0 && a->L > 0 && a->H > 0, "decay_bwd: nothing to compute");
   WA_CHECK_ARG(a->q && a->k && a->v && a->dout && a->dq && a->dk && a->dv && a->log_decay && a->states && a->workspace,
                "decay_bwd: null tensor");
+  WA_CHECK_ARG(!a->dlog_decay || a->derivs, "decay_bwd: dlog_decay needs the forward's derivs");
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype) &&
                rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh, a->dtype) &&
                wa_aligned16(a->states) && wa_aligned16(a->workspace) && wa_aligned16(a->dfinal) && wa_aligned16(a->dinitial),
-               "decay_bwd: rows, states and workspace must be 16-byte aligned");
+               "decay_bwd: rows, states and workspace must be 16-byte aligned, tokens at most 2^23 elements apart");
   hipStream_t s = (hipStream_t)stream;
-  if (a->dtype == WA_BF16) return a->D == 128 ? run_bwd<bf16_t, 128>(a, s) : run_bwd<bf16_t, 64>(a, s);
-  return a->D == 128 ? run_bwd<float, 128>(a, s) : run_bwd<float, 64>(a, s);
+  return a->D == 128 ? run_bwd<128>(a, s) : run_bwd<64>(a, s);
 }
 
 extern "C" int wa_decay_step(const wa_decay_step_args* a, void* stream) {

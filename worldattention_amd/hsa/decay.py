@@ -19,36 +19,39 @@ __all__ = ["decay_linear_attention", "decay_linear_step"]
 
 
 def _ready(t: torch.Tensor) -> torch.Tensor:
-    return _lib.kernel_ready(t, t.dtype, 16 // t.element_size())
+    """``t`` in rows that the kernels take: 16-byte aligned, tokens at most 2^23 elements apart."""
+    return _lib.kernel_ready(t if t.stride(1) <= 1 << 23 else t.contiguous(), t.dtype, 16 // t.element_size())
 
 
-def _forward(q, k, v, log_decay, initial, lengths, scale, want_states):
+def _forward(q, k, v, log_decay, initial, lengths, scale, want_derivs=False):
     dev = q.device
     bsz, length, heads, d = q.shape
     f32 = dict(dtype=torch.float32, device=dev)
     out = torch.empty((bsz, length, heads, d), dtype=q.dtype, device=dev)
     final = torch.empty((bsz, heads, d, d), **f32)
-    states = torch.empty((bsz, heads, _lib.lib().wa_decay_segments(bsz, length, heads), d, d), **f32)
+    n_seg = _lib.lib().wa_decay_segments(bsz, length, heads)
+    states = torch.empty((bsz, heads, n_seg, d, d), **f32)
+    derivs = torch.empty((bsz, heads, n_seg + 1, d, d), **f32) if want_derivs else None
     args = _lib.DecayFwdArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), _lib.dtype_code(q), bsz, length,
                              heads, d, log_decay.data_ptr(), _lib.ptr(lengths), _lib.ptr(initial), final.data_ptr(),
-                             states.data_ptr(), scale)
+                             states.data_ptr(), _lib.ptr(derivs), scale)
     _lib.launch("wa_decay_fwd", args, dev)
-    return out, final, states if want_states else None
+    return out, final, states, derivs
 
 
 class _DecayLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial, lengths, scale):
         ctx.set_materialize_grads(False)
-        out, final, states = _forward(q, k, v, log_decay, initial, lengths, scale, True)
-        ctx.save_for_backward(q, k, v, log_decay, lengths, states)
+        out, final, states, derivs = _forward(q, k, v, log_decay, initial, lengths, scale, ctx.needs_input_grad[3])
+        ctx.save_for_backward(q, k, v, log_decay, lengths, states, derivs)
         ctx.scale = scale
         return out, final
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dfinal):
-        q, k, v, log_decay, lengths, states = ctx.saved_tensors
+        q, k, v, log_decay, lengths, states, derivs = ctx.saved_tensors
         if dout is None and dfinal is None:
             return None, None, None, None, None, None, None
         dev = q.device
@@ -62,7 +65,7 @@ class _DecayLinear(torch.autograd.Function):
         ws = torch.empty((_lib.lib().wa_decay_bwd_workspace_bytes(bsz, length, heads, d),), dtype=torch.uint8, device=dev)
         args = _lib.DecayBwdArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(dout), *_lib.blhd(dq),
                                  *_lib.blhd(dk), *_lib.blhd(dv), _lib.dtype_code(q), bsz, length, heads, d,
-                                 log_decay.data_ptr(), _lib.ptr(lengths), states.data_ptr(), _lib.ptr(dfinal),
+                                 log_decay.data_ptr(), _lib.ptr(lengths), states.data_ptr(), _lib.ptr(derivs), _lib.ptr(dfinal),
                                  _lib.ptr(dinitial), _lib.ptr(dlog), ws.data_ptr(), ctx.scale)
         _lib.launch("wa_decay_bwd", args, dev)
         return dq, dk, dv, dlog, dinitial, None, None
@@ -127,7 +130,7 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     if grad:
         out, final = _DecayLinear.apply(q, k, v, log_decay, initial_state, lengths, scale)
     else:
-        out, final, _ = _forward(q, k, v, log_decay, initial_state, lengths, scale, False)
+        out, final = _forward(q, k, v, log_decay, initial_state, lengths, scale)[:2]
     if d != dp or dv != dp:
         out, final = out[..., :dv].contiguous(), final[:, :, :d, :dv].contiguous()
     return out, final
