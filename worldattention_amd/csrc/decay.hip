@@ -59,7 +59,8 @@ __device__ __forceinline__ float log2_decay(const Shape& s, int h) {
   const float g = s.log_decay[h];
   return (g < -1e30f ? -1e30f : g) * WA_LOG2E;
 }
-__device__ __forceinline__ float power(float g2, int steps) { return exp2f(g2 * (float)steps); }
+// lambda^steps: the bare exponential instruction (1 ulp; what would be below 2^-126 is 0)
+__device__ __forceinline__ float power(float g2, int steps) { return __builtin_amdgcn_exp2f(g2 * (float)steps); }
 
 // A segment's own state, sum_j w_j b_j c_j^T with w_j = w_scale lambda^steps(j), forwards steps = n - 1 - j,
 // backwards (rev) j + 1. With derivatives (derivs not null) also sum_j steps w_j b_j c_j^T: forwards written
@@ -575,24 +576,29 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
   }
 }
 
-// Rows. Wave (ch, rh) of D / 16 waves: output channels 32 ch .. + 31 of the chunk's rows 32 rh .. + 31, and the
-// running state's columns 32 ch .. + 31 in accumulators (both halves keep a copy: the second update costs
-// less than passing it). Per chunk, with P^T = B A^T decayed and masked,
-//   Y^T = s_intra C^T P^T + s_inter lambda^.. X^T A^T,    X = lambda^m X + B^T (weighted C):
-// P^T's accumulators are the second product's operand in place, X's the third's.
+// Rows, in units of 32 tokens a wave (256 for D = 128, 128 for D = 64). A wave holds one 32-row tile of the
+// unit and, for the running state, two (one) of its D x D tiles. Per unit, with P^T = B A^T decayed and masked,
+//   Y^T = s_inter lambda^.. X^T A^T + s_intra C^T P^T,    X = lambda^m X + (weighted B)^T C:
+// X^T is read from LDS (two parts, written once a unit), P^T's accumulators are the next product's operand in
+// place, and the keys and values of the unit stream through a ring of two 64-token stages that serve the rows
+// behind them and the state at once. Work a unit, not a chunk, pays for the state: with a state read and
+// rewritten every 64 tokens (two waves a tile, no LDS copy) the vector instructions were 2,600 a wave and unit
+// and the launch took 235 us at 32,760 tokens of 12 x 128.
 template <int D>
 __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) {
-  constexpr int NW = D / 16, CT = D / 32, KS = D / 16, STAGES = 3, NI = ChunkStream<D, NW>::NI;
-  __shared__ __attribute__((aligned(1024))) bf16_t ta[STAGES][kChunk * D];
+  constexpr int NW = D / 16, CT = D / 32, KS = D / 16, STAGES = 2, UNIT = 32 * NW;
+  constexpr int XT = CT * CT / NW;          // state tiles of a wave: row tile w % CT, columns from (w / CT) XT on
   __shared__ __attribute__((aligned(1024))) bf16_t tb[STAGES][kChunk * D];
   __shared__ __attribute__((aligned(1024))) bf16_t tc[STAGES][kChunk * D];
-  __shared__ __attribute__((aligned(16))) float wt[kChunk];
+  __shared__ __attribute__((aligned(1024))) bf16_t xh[D * D], xl[D * D];   // X^T: row e, column d
+  __shared__ __attribute__((aligned(16))) float wt[UNIT], edge[32];
   const Job& jb = p.job[blockIdx.z];
   const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
-  const int ch = w % CT, rh = w / CT;
+  const int xd = w % CT, xe = w / CT * XT;
+  const int rt = w < NW / 2 ? w : 3 * NW / 2 - 1 - w;   // row tile: the two waves of a SIMD share the causal work evenly
   const bool rev = jb.rev;
-  const int n = tokens_of(p.s, b, seg), chunks = (n + kChunk - 1) / kChunk;
+  const int n = tokens_of(p.s, b, seg);
   const float g2 = log2_decay(p.s, h);
   const int64_t first = (int64_t)seg * p.s.seg;
   bf16_t* yb = (bf16_t*)jb.y + (int64_t)b * jb.y_sb + (int64_t)h * jb.y_sh + first * jb.y_st;
@@ -603,120 +609,174 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
     *(u32x4*)(yb + (int64_t)(n + u / (D / 8)) * jb.y_st + (u % (D / 8)) * 8) = u32x4{0, 0, 0, 0};
   if (n == 0) return;
 
-  ChunkStream<D, NW> sa, sb, sc;
-  sa.init(jb.a, b, h, first, w, lane);
+  const int units = (n + UNIT - 1) / UNIT, chunks = (n + kChunk - 1) / kChunk;
+  constexpr int CPU = UNIT / kChunk;        // chunks of a whole unit
+  ChunkStream<D, NW> sb, sc;
   sb.init(jb.b, b, h, first, w, lane);
   sc.init(jb.c, b, h, first, w, lane);
-  auto issue = [&](int it) {
-    const int row0 = (rev ? chunks - 1 - it : it) * kChunk, m = min(kChunk, n - row0);
-    sa.issue(ta[it % STAGES], row0, m, w);
-    sb.issue(tb[it % STAGES], row0, m, w);
-    sc.issue(tc[it % STAGES], row0, m, w);
+  // chunk `c` of the segment into the stage of the step that takes it
+  auto issue = [&](int c, int step) {
+    const int m = min(kChunk, n - c * kChunk);
+    sb.issue(tb[step % STAGES], c * kChunk, m, w);
+    sc.issue(tc[step % STAGES], c * kChunk, m, w);
   };
-  issue(0);
-  if (chunks > 1) issue(1);
-  if (w == 0) fill_weights(wt, g2, kChunk, rev, jb.s_intra / jb.s_inter, lane);
+  issue(rev ? (units - 1) * CPU : 0, 0);
 
-  // X[d][e] of lane (l32, g): e = 32 ch + pi(l32), tile dt's register 8 h + x: d = 32 dt + 16 h + 8 g + x
-  f32x16 X[CT];
+  // X[d][e] of lane (l32, g): e = 32 (xe + i) + pi(l32), register 8 hf + x: d = 32 xd + 16 hf + 8 g + x
+  f32x16 X[XT];
   const float* x0 = jb.x + ((int64_t)bh * p.s.n_seg + seg) * D * D;
-  const int e0 = 32 * ch + pi32(l32);
+  const int pl = pi32(l32);
 #pragma unroll
-  for (int dt = 0; dt < CT; ++dt)
+  for (int i = 0; i < XT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int d = 32 * dt + 16 * (r >> 3) + 8 * g + (r & 7);
-      X[dt][r] = jb.x_trans ? x0[e0 * D + d] : x0[d * D + e0];
+      const int d = 32 * xd + 16 * (r >> 3) + 8 * g + (r & 7), e = 32 * (xe + i) + pl;
+      X[i][r] = jb.x_trans ? x0[e * D + d] : x0[d * D + e];
     }
-  // decay from token j = 32 jh + acc_row to row i = 32 rh + l32 of the chunk, 0 against time's direction
-  float near[16], far[16];
+  auto put_state = [&]() {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int steps = rev ? acc_row(r, g) - l32 : l32 - acc_row(r, g);
-    near[r] = steps >= 0 ? power(g2, steps) : 0.f;
-    far[r] = power(g2, steps + 32);
-  }
-  const bool both = rev ? rh == 0 : rh == 1;   // this wave's rows also see the other half's tokens
-  const int i = 32 * rh + l32;
-
-  u32x4 y[2] = {};           // the chunk's finished outputs, stored in the next step ahead of its loads
-  int y_row = -1;
-  auto store = [&]() {
-    if (y_row >= 0 && y_row < n) {
-      bf16_t* at = yb + (int64_t)y_row * jb.y_st + 32 * ch + 8 * g;
-      *(u32x4*)at = y[0];
-      *(u32x4*)(at + 16) = y[1];
-    }
+    for (int i = 0; i < XT; ++i)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        bf16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = X[i][8 * hf + e];
+          hi[e] = (bf16_t)x;
+          lo[e] = (bf16_t)(x - (float)hi[e]);
+        }
+        tile_put8<D>(xh, 32 * (xe + i) + pl, 4 * xd + 2 * hf + g, hi);
+        tile_put8<D>(xl, 32 * (xe + i) + pl, 4 * xd + 2 * hf + g, lo);
+      }
   };
-  for (int it = 0; it < chunks; ++it) {
-    const int c0 = (rev ? chunks - 1 - it : it) * kChunk, m = min(kChunk, n - c0);
-    // Tile it has landed (only it + 1's loads were issued after it and the stores before them) and every
-    // wave is past tile it - 1, whose stage is refilled.
-    if (it + 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(3 * NI) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    store();
-    if (it + 2 < chunks) issue(it + 2);
-    const bf16_t* A = ta[it % STAGES];
-    const bf16_t* B = tb[it % STAGES];
-    const bf16_t* C = tc[it % STAGES];
+  put_state();
+  // weights of a unit's tokens in the state after it (backwards, before it): whole units
+  if (tid < UNIT) wt[tid] = jb.s_intra / jb.s_inter * power(g2, rev ? tid + 1 : UNIT - 1 - tid);
+  // decay between the tokens of a tile and its edge on the rows' side
+  if (tid < 32) edge[tid] = power(g2, rev ? tid : 31 - tid);
+
+  int step = 0;
+  for (int ui = 0; ui < units; ++ui) {
+    const int u = rev ? units - 1 - ui : ui, u0 = u * UNIT, m = min(UNIT, n - u0), t = u0 + 32 * rt + l32;
+    const int uc = (m + kChunk - 1) / kChunk;
     bf16x8 a[KS];
-#pragma unroll
-    for (int k = 0; k < KS; ++k) a[k] = tile_row8<D>(A, i, 2 * k + g);
-    f32x16 y1{}, y2{};
+    const bf16_t* ap = (const bf16_t*)jb.a.p + (int64_t)b * jb.a.sb + (int64_t)h * jb.a.sh + (first + t) * jb.a.st + 8 * g;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      bf16x8 hi, lo;
+      a[k] = bf16x8{};
+      if (t < n) a[k] = *(const bf16x8*)(ap + 16 * k);
+    }
+    f32x16 y[CT];
+    const float keep = power(g2, m);
+    for (int c = 0; c < uc; ++c, ++step) {
+      // this step's tiles have landed and every wave is past the step before, whose stage is refilled
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const int next = c + 1 < uc ? u * CPU + c + 1 : (rev ? u - 1 : u + 1) * CPU;
+      if (c + 1 < uc || ui + 1 < units) issue(next, step + 1);
+      if (c == 0) {
+        // the carried state's part, scaled so that the sums that follow share s_intra
+        const float f = jb.s_inter / jb.s_intra * power(g2, rev ? max(0, m - 1 - (32 * rt + l32)) : 32 * rt + l32 + 1);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = X[k / 2][8 * (k % 2) + e];
-        hi[e] = (bf16_t)x;
-        lo[e] = (bf16_t)(x - (float)hi[e]);
+        for (int et = 0; et < CT; ++et) {
+          f32x16 s{};
+          if (32 * rt < m) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              s = wa_mfma32(tile_row8<D>(xl, 32 * et + pl, 2 * k + g), a[k], s);
+              s = wa_mfma32(tile_row8<D>(xh, 32 * et + pl, 2 * k + g), a[k], s);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[et][r] = s[r] * f;
+        }
+#pragma unroll
+        for (int i = 0; i < XT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) X[i][r] *= keep;
       }
-      y2 = wa_mfma32(lo, a[k], y2);
-      y2 = wa_mfma32(hi, a[k], y2);
-    }
-    bf16x8 cv[4];
+      const bf16_t* B = tb[step % STAGES];
+      const bf16_t* C = tc[step % STAGES];
+      // decayed products with the chunk's two tiles of tokens, where the rows see them
+      bf16x8 pr[4];
+      bool seen[2];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) cv[c] = tile_tr8_pi<D>(C, c, 32 * ch, lane);
+      for (int jh = 0; jh < 2; ++jh) {
+        const int jt = 2 * c + jh;
+        seen[jh] = 32 * rt < m && (rev ? jt >= rt && 32 * jt < m : jt <= rt);
+        if (!seen[jh]) continue;
+        f32x16 s{};
 #pragma unroll
-    for (int jh = 0; jh < 2; ++jh) {
-      if (jh != rh && !both) continue;
-      f32x16 s{};
+        for (int k = 0; k < KS; ++k) s = wa_mfma32(tile_row8<D>(B, 32 * jh + l32, 2 * k + g), a[k], s);
+        if (jt == rt) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s = wa_mfma32(tile_row8<D>(B, 32 * jh + l32, 2 * k + g), a[k], s);
+          for (int r = 0; r < 16; ++r) {
+            const int steps = rev ? acc_row(r, g) - l32 : l32 - acc_row(r, g);
+            s[r] = steps >= 0 ? s[r] * power(g2, steps) : 0.f;
+          }
+        } else {
+          const float f = power(g2, rev ? 32 * (jt - rt) - l32 : 32 * (rt - jt) + l32 - 31);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= jh == rh ? near[r] : far[r];
-      y1 = wa_mfma32(cv[2 * jh], pack8(s, 0), y1);
-      y1 = wa_mfma32(cv[2 * jh + 1], pack8(s, 1), y1);
-    }
-    const float f = jb.s_inter * power(g2, rev ? max(0, m - 1 - i) : i + 1);
+          for (int r = 0; r < 4; ++r) {
+            const f32x4 e = *(const f32x4*)(edge + 8 * r + 4 * g);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      bf16x8 o;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = (bf16_t)(jb.s_intra * y1[8 * q + e] + f * y2[8 * q + e]);
-      y[q] = __builtin_bit_cast(u32x4, o);
-    }
-    y_row = c0 + i;
-    if (it + 1 < chunks) {   // forwards only whole chunks are followed by another
-      const float keep = power(g2, m);
-#pragma unroll
-      for (int dt = 0; dt < CT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) X[dt][r] *= keep;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float wv[8];
-        load_weights(wt, c, g, wv);
-        bf16x8 cw;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) cw[e] = (bf16_t)(wv[e] * (float)cv[c][e]);
-#pragma unroll
-        for (int dt = 0; dt < CT; ++dt) X[dt] = wa_mfma32(tile_tr8_pi<D>(B, c, 32 * dt, lane), cw, X[dt]);
+            for (int x = 0; x < 4; ++x) s[4 * r + x] *= e[x] * f;
+          }
+        }
+        pr[2 * jh] = pack8(s, 0);
+        pr[2 * jh + 1] = pack8(s, 1);
       }
+      // weighted keys of this wave's state rows
+      const bool more = ui + 1 < units;     // forwards only whole units are followed by another
+      bf16x8 bw[4];
+      if (more) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float wv[8];
+          load_weights(wt + c * kChunk, q, g, wv);
+          const bf16x8 bv = tile_tr8_pi<D>(B, q, 32 * xd, lane);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) bw[q][e] = (bf16_t)(wv[e] * (float)bv[e]);
+        }
+      }
+#pragma unroll
+      for (int et = 0; et < CT; ++et) {
+        const bool own = more && et >= xe && et < xe + XT;
+        if (!own && !seen[0] && !seen[1]) continue;
+        bf16x8 cv[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) cv[q] = tile_tr8_pi<D>(C, q, 32 * et, lane);
+#pragma unroll
+        for (int jh = 0; jh < 2; ++jh)
+          if (seen[jh]) {
+            y[et] = wa_mfma32(cv[2 * jh], pr[2 * jh], y[et]);
+            y[et] = wa_mfma32(cv[2 * jh + 1], pr[2 * jh + 1], y[et]);
+          }
+        if (own) {
+#pragma unroll
+          for (int i = 0; i < XT; ++i)
+            if (et == xe + i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) X[i] = wa_mfma32(bw[q], cv[q], X[i]);
+        }
+      }
+    }
+    if (t < n) {
+      bf16_t* at = yb + (int64_t)t * jb.y_st + 8 * g;
+#pragma unroll
+      for (int et = 0; et < CT; ++et)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          bf16x8 o;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = (bf16_t)(jb.s_intra * y[et][8 * hf + e]);
+          *(bf16x8*)(at + 32 * et + 16 * hf) = o;
+        }
+    }
+    if (ui + 1 < units) {
+      if (uc == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // every wave has read the old state
+      put_state();
     }
   }
-  store();
 }
 
 // Pairs: a workgroup takes 256 rows i of a segment, 32 a wave, whose queries and output gradients stay in
