@@ -625,15 +625,14 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
   // X[d][e] of lane (l32, g): e = 32 (xe + i) + pi(l32), register 8 hf + x: d = 32 xd + 16 hf + 8 g + x
   f32x16 X[XT];
   const float* x0 = jb.x + ((int64_t)bh * p.s.n_seg + seg) * D * D;
-  const int pl = pi32(l32);
 #pragma unroll
   for (int i = 0; i < XT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int d = 32 * xd + 16 * (r >> 3) + 8 * g + (r & 7), e = 32 * (xe + i) + pl;
+      const int d = 32 * xd + 16 * (r >> 3) + 8 * g + (r & 7), e = 32 * (xe + i) + pi32(l32);
       X[i][r] = jb.x_trans ? x0[e * D + d] : x0[d * D + e];
     }
-  auto put_state = [&]() {
+  auto put_state = [&](int row, int half) {   // the lane's pi(l32) and g
 #pragma unroll
     for (int i = 0; i < XT; ++i)
 #pragma unroll
@@ -645,123 +644,158 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
           hi[e] = (bf16_t)x;
           lo[e] = (bf16_t)(x - (float)hi[e]);
         }
-        tile_put8<D>(xh, 32 * (xe + i) + pl, 4 * xd + 2 * hf + g, hi);
-        tile_put8<D>(xl, 32 * (xe + i) + pl, 4 * xd + 2 * hf + g, lo);
+        tile_put8<D>(xh, 32 * (xe + i) + row, 4 * xd + 2 * hf + half, hi);
+        tile_put8<D>(xl, 32 * (xe + i) + row, 4 * xd + 2 * hf + half, lo);
       }
   };
-  put_state();
+  put_state(pi32(l32), g);
   // weights of a unit's tokens in the state after it (backwards, before it): whole units
   if (tid < UNIT) wt[tid] = jb.s_intra / jb.s_inter * power(g2, rev ? tid + 1 : UNIT - 1 - tid);
   // decay between the tokens of a tile and its edge on the rows' side
   if (tid < 32) edge[tid] = power(g2, rev ? tid : 31 - tid);
 
-  int step = 0;
-  for (int ui = 0; ui < units; ++ui) {
-    const int u = rev ? units - 1 - ui : ui, u0 = u * UNIT, m = min(UNIT, n - u0), t = u0 + 32 * rt + l32;
-    const int uc = (m + kChunk - 1) / kChunk;
-    bf16x8 a[KS];
-    const bf16_t* ap = (const bf16_t*)jb.a.p + (int64_t)b * jb.a.sb + (int64_t)h * jb.a.sh + (first + t) * jb.a.st + 8 * g;
+  // One step a chunk: the unit's first one starts its rows, its last one stores them and passes the state on.
+  bf16x8 a[KS];
+  auto load_rows = [&](int t, int half) {     // the operands of row t of the segment
+    const bf16_t* ap = (const bf16_t*)jb.a.p + (int64_t)b * jb.a.sb + (int64_t)h * jb.a.sh + (first + t) * jb.a.st + 8 * half;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       a[k] = bf16x8{};
       if (t < n) a[k] = *(const bf16x8*)(ap + 16 * k);
     }
-    f32x16 y[CT];
-    const float keep = power(g2, m);
-    for (int c = 0; c < uc; ++c, ++step) {
-      // this step's tiles have landed and every wave is past the step before, whose stage is refilled
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      const int next = c + 1 < uc ? u * CPU + c + 1 : (rev ? u - 1 : u + 1) * CPU;
-      if (c + 1 < uc || ui + 1 < units) issue(next, step + 1);
-      if (c == 0) {
-        // the carried state's part, scaled so that the sums that follow share s_intra
-        const float f = jb.s_inter / jb.s_intra * power(g2, rev ? max(0, m - 1 - (32 * rt + l32)) : 32 * rt + l32 + 1);
+  };
+  int u0 = rev ? (units - 1) * UNIT : 0, c = 0;   // the unit's first token, the chunk in it
+  load_rows(u0 + 32 * rt + l32, g);
+  f32x16 y[CT];
+  for (int step = 0; step < chunks; ++step) {
+    // this step's tiles have landed and every wave is past the step before, whose stage is refilled
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // the rows' operands have landed with them: named here, so that no wait for them follows the loads below
 #pragma unroll
-        for (int et = 0; et < CT; ++et) {
-          f32x16 s{};
-          if (32 * rt < m) {
+    for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(a[k]));
+    const int m = min(UNIT, n - u0), next_u0 = rev ? u0 - UNIT : u0 + UNIT;
+    const bool last = (c + 1) * kChunk >= m, more = rev ? u0 > 0 : u0 + UNIT < n;   // of the unit; units behind it
+    if (!last) issue(u0 / kChunk + c + 1, step + 1);
+    else if (more) issue(next_u0 / kChunk, step + 1);
+    // The lane in a form that the compiler cannot carry from step to step: kept, what is derived from it (LDS
+    // addresses, powers) takes the registers that hold operands ahead of their products.
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int lg = ln >> 5, lr = ln & 31, lp = pi32(lr);
+    const bf16_t* B = tb[step % STAGES];
+    const bf16_t* C = tc[step % STAGES];
+    const bool any = 32 * rt < m;
+    constexpr int Q = 4;      // operands are read four at a time, while the four products before them run
+    bf16x8 f[2][Q];
+    if (c == 0) {
+      // the carried state's part, scaled so that the sums that follow share s_intra
+      const float fs = jb.s_inter / jb.s_intra * power(g2, rev ? max(0, m - 1 - (32 * rt + lr)) : 32 * rt + lr + 1);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-              s = wa_mfma32(tile_row8<D>(xl, 32 * et + pl, 2 * k + g), a[k], s);
-              s = wa_mfma32(tile_row8<D>(xh, 32 * et + pl, 2 * k + g), a[k], s);
-            }
-          }
+      for (int x = 0; x < Q; ++x) f[0][x] = tile_row8<D>(xl, lp, 2 * x + lg);
+      constexpr int PER = 2 * KS / Q;       // groups of an output tile: the low parts, then the high ones
+      f32x16 s;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) y[et][r] = s[r] * f;
+      for (int q = 0; q < CT * PER; ++q) {
+        if (q + 1 < CT * PER) {
+          const int nq = q + 1, k0 = nq % PER * Q;
+#pragma unroll
+          for (int x = 0; x < Q; ++x)
+            f[nq % 2][x] = tile_row8<D>(k0 < KS ? xl : xh, 32 * (nq / PER) + lp, 2 * ((k0 + x) % KS) + lg);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (q % PER == 0) s = f32x16{};
 #pragma unroll
-        for (int i = 0; i < XT; ++i)
+        for (int x = 0; x < Q; ++x) s = wa_mfma32(f[q % 2][x], a[(q % PER * Q + x) % KS], s);
+        if (q % PER == PER - 1) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) X[i][r] *= keep;
-      }
-      const bf16_t* B = tb[step % STAGES];
-      const bf16_t* C = tc[step % STAGES];
-      // decayed products with the chunk's two tiles of tokens, where the rows see them
-      bf16x8 pr[4];
-      bool seen[2];
-#pragma unroll
-      for (int jh = 0; jh < 2; ++jh) {
-        const int jt = 2 * c + jh;
-        seen[jh] = 32 * rt < m && (rev ? jt >= rt && 32 * jt < m : jt <= rt);
-        if (!seen[jh]) continue;
-        f32x16 s{};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) s = wa_mfma32(tile_row8<D>(B, 32 * jh + l32, 2 * k + g), a[k], s);
-        if (jt == rt) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int steps = rev ? acc_row(r, g) - l32 : l32 - acc_row(r, g);
-            s[r] = steps >= 0 ? s[r] * power(g2, steps) : 0.f;
-          }
-        } else {
-          const float f = power(g2, rev ? 32 * (jt - rt) - l32 : 32 * (rt - jt) + l32 - 31);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const f32x4 e = *(const f32x4*)(edge + 8 * r + 4 * g);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) s[4 * r + x] *= e[x] * f;
-          }
-        }
-        pr[2 * jh] = pack8(s, 0);
-        pr[2 * jh + 1] = pack8(s, 1);
-      }
-      // weighted keys of this wave's state rows
-      const bool more = ui + 1 < units;     // forwards only whole units are followed by another
-      bf16x8 bw[4];
-      if (more) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float wv[8];
-          load_weights(wt + c * kChunk, q, g, wv);
-          const bf16x8 bv = tile_tr8_pi<D>(B, q, 32 * xd, lane);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) bw[q][e] = (bf16_t)(wv[e] * (float)bv[e]);
+          for (int r = 0; r < 16; ++r) y[q / PER][r] = s[r] * fs;
         }
       }
+      const float keep = power(g2, m);
+#pragma unroll
+      for (int i = 0; i < XT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) X[i][r] *= keep;
+    }
+    // decayed products with the chunk's two tiles of tokens, where the rows see them
+    bf16x8 pr[4];
+    bool seen[2];
+#pragma unroll
+    for (int jh = 0; jh < 2; ++jh) {
+      const int jt = 2 * c + jh;
+      seen[jh] = any && (rev ? jt >= rt && 32 * jt < m : jt <= rt);
+      if (!seen[jh]) continue;
+      f32x16 s{};
+#pragma unroll
+      for (int x = 0; x < Q; ++x) f[0][x] = tile_row8<D>(B, 32 * jh + lr, 2 * x + lg);
+#pragma unroll
+      for (int q = 0; q < KS / Q; ++q) {
+        if (q + 1 < KS / Q) {
+#pragma unroll
+          for (int x = 0; x < Q; ++x) f[(q + 1) % 2][x] = tile_row8<D>(B, 32 * jh + lr, 2 * (Q * (q + 1) + x) + lg);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < Q; ++x) s = wa_mfma32(f[q % 2][x], a[Q * q + x], s);
+      }
+      if (jt == rt) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int steps = rev ? acc_row(r, lg) - lr : lr - acc_row(r, lg);
+          s[r] = steps >= 0 ? s[r] * power(g2, steps) : 0.f;
+        }
+      } else {
+        const float fj = power(g2, rev ? 32 * (jt - rt) - lr : 32 * (rt - jt) + lr - 31);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 e = *(const f32x4*)(edge + 8 * r + 4 * lg);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[4 * r + x] *= e[x] * fj;
+        }
+      }
+      pr[2 * jh] = pack8(s, 0);
+      pr[2 * jh + 1] = pack8(s, 1);
+    }
+    // weighted keys of this wave's state rows; forwards only whole units are followed by another
+    bf16x8 bw[4];
+    if (more) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) bw[q] = tile_tr8_pi<D>(B, q, 32 * xd, ln);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float wv[8];
+        load_weights(wt + c * kChunk, q, lg, wv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bw[q][e] = (bf16_t)(wv[e] * (float)bw[q][e]);
+      }
+    }
+    if (more || seen[0] || seen[1]) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) f[0][q] = tile_tr8_pi<D>(C, q, 0, ln);
 #pragma unroll
       for (int et = 0; et < CT; ++et) {
-        const bool own = more && et >= xe && et < xe + XT;
-        if (!own && !seen[0] && !seen[1]) continue;
-        bf16x8 cv[4];
+        if (et + 1 < CT) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) cv[q] = tile_tr8_pi<D>(C, q, 32 * et, lane);
+          for (int q = 0; q < Q; ++q) f[(et + 1) % 2][q] = tile_tr8_pi<D>(C, q, 32 * (et + 1), ln);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int jh = 0; jh < 2; ++jh)
           if (seen[jh]) {
-            y[et] = wa_mfma32(cv[2 * jh], pr[2 * jh], y[et]);
-            y[et] = wa_mfma32(cv[2 * jh + 1], pr[2 * jh + 1], y[et]);
+            y[et] = wa_mfma32(f[et % 2][2 * jh], pr[2 * jh], y[et]);
+            y[et] = wa_mfma32(f[et % 2][2 * jh + 1], pr[2 * jh + 1], y[et]);
           }
-        if (own) {
+        if (more && et / XT == xe / XT) {
 #pragma unroll
-          for (int i = 0; i < XT; ++i)
-            if (et == xe + i)
-#pragma unroll
-              for (int q = 0; q < 4; ++q) X[i] = wa_mfma32(bw[q], cv[q], X[i]);
+          for (int q = 0; q < 4; ++q) X[et % XT] = wa_mfma32(bw[q], f[et % 2][q], X[et % XT]);
         }
       }
     }
+    ++c;
+    if (!last) continue;
+    const int t = u0 + 32 * rt + lr;
     if (t < n) {
-      bf16_t* at = yb + (int64_t)t * jb.y_st + 8 * g;
+      bf16_t* at = yb + (int64_t)t * jb.y_st + 8 * lg;
 #pragma unroll
       for (int et = 0; et < CT; ++et)
 #pragma unroll
@@ -772,9 +806,12 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
           *(bf16x8*)(at + 32 * et + 16 * hf) = o;
         }
     }
-    if (ui + 1 < units) {
-      if (uc == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // every wave has read the old state
-      put_state();
+    if (more) {
+      if (c == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // every wave has read the old state
+      put_state(lp, lg);
+      u0 = next_u0;
+      c = 0;
+      load_rows(u0 + 32 * rt + lr, lg);
     }
   }
 }
