@@ -385,24 +385,48 @@ __global__ void __launch_bounds__(kThreads) pairs_f32_kernel(PairsParams p) {
 // 8 h .. 8 h + 7, rows 16 h + 8 g .. + 7: eight consecutive channels, which is both a 16-byte store and
 // the natural operand order of the next product.
 // ---------------------------------------------------------------------------------------------
-// tile_tr8 (contraction in accumulator order over the 16 tokens of chunk c) with lane l32 at column
-// col0 + pi(l32).
+// A lane's byte offsets into swizzled tiles of D columns. The swizzle takes no bit of a row above the
+// fourth and turns a column step of 16 (a contraction step) or 32 (a tile) into one exclusive or, so four
+// offsets serve every read.
 template <int D>
-__device__ __forceinline__ bf16x8 tile_tr8_pi(const bf16_t* lds, int c, int col0, int lane) {
-  const int G = lane >> 4, r = (lane & 15) >> 2, q = ((lane & 1) << 1) | ((lane >> 1) & 1);
-  bf16x8 a;
+struct TileReads {
+  int row, rowpi;    // 128-bit reads: row l32 (pi(l32)), chunk g
+  int tr[2];         // transpose reads in order pi: tokens of the first 16, columns of the first 32
+  __device__ __forceinline__ void init(int lane) {
+    const int g = lane >> 5, l32 = lane & 31, lp = (l32 & 0x13) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);
+    row = (l32 * D + ((g ^ dual_swizzle<D>(l32)) * 8)) * 2;
+    rowpi = (lp * D + ((g ^ dual_swizzle<D>(lp)) * 8)) * 2;
+    const int G = lane >> 4, r = (lane & 15) >> 2, q = ((lane & 1) << 1) | ((lane >> 1) & 1);
 #pragma unroll
-  for (int hf = 0; hf < 2; ++hf) {
-    const int row = 16 * c + 4 * (G >> 1) + 8 * hf + r;
-    const int col = col0 + 16 * (G & 1) + 4 * q;
-    const int slot = (col >> 3) ^ dual_swizzle<D>(row);
-    const wa_s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(WA_LDS_S16X4(lds + row * D + slot * 8 + (col & 7)));
-    const bf16x4 b = __builtin_bit_cast(bf16x4, v);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) a[4 * hf + e] = b[e];
+    for (int hf = 0; hf < 2; ++hf) {
+      const int t = 4 * (G >> 1) + 8 * hf + r, col = 16 * (G & 1) + 4 * q;
+      tr[hf] = (t * D + (((col >> 3) ^ dual_swizzle<D>(t)) * 8) + (col & 7)) * 2;
+    }
   }
-  return a;
-}
+  // Hides from the compiler that the offsets stay the same from step to step: the sums it would keep of
+  // them take the registers that hold operands ahead of their products.
+  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(row), "+v"(rowpi), "+v"(tr[0]), "+v"(tr[1])); }
+  // rows 32 tile + l32, channels 16 k + 8 g .. + 7
+  __device__ __forceinline__ bf16x8 rows(const bf16_t* t, int tile, int k) const {
+    return *(const bf16x8*)((const char*)t + (row ^ (k << 5)) + tile * (32 * D * 2));
+  }
+  __device__ __forceinline__ bf16x8 rows_pi(const bf16_t* t, int tile, int k) const {
+    return *(const bf16x8*)((const char*)t + (rowpi ^ (k << 5)) + tile * (32 * D * 2));
+  }
+  // tile_tr8 of tokens 16 c .. with lane l32 at column 32 tile + pi(l32)
+  __device__ __forceinline__ bf16x8 cols_pi(const bf16_t* t, int c, int tile) const {
+    bf16x8 a;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const wa_s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          WA_LDS_S16X4((const char*)t + (tr[hf] ^ (tile << 6)) + c * (16 * D * 2)));
+      const bf16x4 b = __builtin_bit_cast(bf16x4, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[4 * hf + e] = b[e];
+    }
+    return a;
+  }
+};
 __device__ __forceinline__ int pi32(int x) { return (x & 0x13) | ((x & 4) << 1) | ((x & 8) >> 1); }
 
 // TileStream (tile.h) over one segment, with the descriptor cut to the chunk's rows: any distance between the
@@ -500,6 +524,8 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
     sb.issue(tb[it % STAGES], row0, rows, w);
     sc.issue(tc[it % STAGES], row0, rows, w);
   };
+  TileReads<D> rd;
+  rd.init(lane);
   f32x16 acc[DT], dacc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = dacc[i] = f32x16{};
@@ -526,22 +552,29 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
         if (DERIV) dacc[i][r] = keep * (dacc[i][r] + (float)m * acc[i][r]);
         acc[i][r] *= keep;
       }
+    rd.renew();
+    bf16x8 cv[2], bv[2][DT];   // the next 16 tokens' operands are read behind this ones' products
+    cv[0] = rd.cols_pi(C, 0, ch);
+#pragma unroll
+    for (int i = 0; i < DT; ++i) bv[0][i] = rd.cols_pi(B, 0, DT * dh + i);
 #pragma unroll
     for (int c = 0; c < kChunk / 16; ++c) {
       float wv[8];
       load_weights(wt[cut ? 1 : 0], c, g, wv);
-      const bf16x8 cv = tile_tr8<D>(C, c, 32 * ch, lane);
+      if (c + 1 < kChunk / 16) {
+        cv[(c + 1) % 2] = rd.cols_pi(C, c + 1, ch);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) wv[e] *= (float)cv[e];
-      bf16x8 hi, mid, lo, bv[DT];
+        for (int i = 0; i < DT; ++i) bv[(c + 1) % 2][i] = rd.cols_pi(B, c + 1, DT * dh + i);
+      }
 #pragma unroll
-      for (int i = 0; i < DT; ++i) bv[i] = tile_tr8<D>(B, c, 32 * (DT * dh + i), lane);
+      for (int e = 0; e < 8; ++e) wv[e] *= (float)cv[c % 2][e];
+      bf16x8 hi, mid, lo;
       cut3(wv, hi, mid, lo);
 #pragma unroll
       for (int i = 0; i < DT; ++i) {
-        acc[i] = wa_mfma32(bv[i], lo, acc[i]);
-        acc[i] = wa_mfma32(bv[i], mid, acc[i]);
-        acc[i] = wa_mfma32(bv[i], hi, acc[i]);
+        acc[i] = wa_mfma32(bv[c % 2][i], lo, acc[i]);
+        acc[i] = wa_mfma32(bv[c % 2][i], mid, acc[i]);
+        acc[i] = wa_mfma32(bv[c % 2][i], hi, acc[i]);
       }
       if (DERIV) {
 #pragma unroll
@@ -552,9 +585,9 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
         cut3(wv, hi, mid, lo);
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
-          dacc[i] = wa_mfma32(bv[i], lo, dacc[i]);
-          dacc[i] = wa_mfma32(bv[i], mid, dacc[i]);
-          dacc[i] = wa_mfma32(bv[i], hi, dacc[i]);
+          dacc[i] = wa_mfma32(bv[c % 2][i], lo, dacc[i]);
+          dacc[i] = wa_mfma32(bv[c % 2][i], mid, dacc[i]);
+          dacc[i] = wa_mfma32(bv[c % 2][i], hi, dacc[i]);
         }
       }
     }
@@ -565,7 +598,7 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int e = (32 * (DT * dh + i) + acc_row(r, g)) * D + 32 * ch + l32;
+      const int e = (32 * (DT * dh + i) + 16 * (r >> 3) + 8 * g + (r & 7)) * D + 32 * ch + pi32(l32);
       p.states[at + e] = acc[i][r];
       if (DERIV && !p.rev) p.derivs[dat + e] = dacc[i][r];
       if (DERIV && p.rev) sum += (double)(p.S[at + e] * dacc[i][r] + p.T[dat + e] * acc[i][r]);
@@ -667,6 +700,8 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
   int u0 = rev ? (units - 1) * UNIT : 0, c = 0;   // the unit's first token, the chunk in it
   load_rows(u0 + 32 * rt + l32, g);
   f32x16 y[CT];
+  TileReads<D> rd;
+  rd.init(lane);
   for (int step = 0; step < chunks; ++step) {
     // this step's tiles have landed and every wave is past the step before, whose stage is refilled
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -677,122 +712,128 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
     const bool last = (c + 1) * kChunk >= m, more = rev ? u0 > 0 : u0 + UNIT < n;   // of the unit; units behind it
     if (!last) issue(u0 / kChunk + c + 1, step + 1);
     else if (more) issue(next_u0 / kChunk, step + 1);
-    // The lane in a form that the compiler cannot carry from step to step: kept, what is derived from it (LDS
-    // addresses, powers) takes the registers that hold operands ahead of their products.
-    int ln = lane;
-    asm volatile("" : "+v"(ln));
-    const int lg = ln >> 5, lr = ln & 31, lp = pi32(lr);
     const bf16_t* B = tb[step % STAGES];
     const bf16_t* C = tc[step % STAGES];
+    if (c == 0) {
+#pragma unroll
+      for (int et = 0; et < CT; ++et) y[et] = f32x16{};
+    }
     const bool any = 32 * rt < m;
+    // tiles of the chunk that the rows see: [lo, hi) of 0, 1 (the diagonal one among them)
+    const int at = rt - 2 * c, lo = rev ? max(0, at) : 0, hi = rev ? 2 : min(2, at + 1);
+    const bool sees = any && lo < hi;
     constexpr int Q = 4;      // operands are read four at a time, while the four products before them run
     bf16x8 f[2][Q];
+    rd.renew();
+    int ln = lane;     // renewed likewise, for what is derived from it
+    asm volatile("" : "+v"(ln));
+    const int lg = ln >> 5, lr = ln & 31;
     if (c == 0) {
-      // the carried state's part, scaled so that the sums that follow share s_intra
+      // the carried state's part
       const float fs = jb.s_inter / jb.s_intra * power(g2, rev ? max(0, m - 1 - (32 * rt + lr)) : 32 * rt + lr + 1);
+      if (any) {
 #pragma unroll
-      for (int x = 0; x < Q; ++x) f[0][x] = tile_row8<D>(xl, lp, 2 * x + lg);
-      constexpr int PER = 2 * KS / Q;       // groups of an output tile: the low parts, then the high ones
-      f32x16 s;
+        for (int x = 0; x < Q; ++x) f[0][x] = rd.rows_pi(xl, 0, x);
+        constexpr int PER = 2 * KS / Q;       // groups of an output tile: the low parts, then the high ones
+        f32x16 s;
 #pragma unroll
-      for (int q = 0; q < CT * PER; ++q) {
-        if (q + 1 < CT * PER) {
-          const int nq = q + 1, k0 = nq % PER * Q;
+        for (int q = 0; q < CT * PER; ++q) {
+          if (q + 1 < CT * PER) {
+            const int nq = q + 1, k0 = nq % PER * Q;
 #pragma unroll
-          for (int x = 0; x < Q; ++x)
-            f[nq % 2][x] = tile_row8<D>(k0 < KS ? xl : xh, 32 * (nq / PER) + lp, 2 * ((k0 + x) % KS) + lg);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (q % PER == 0) s = f32x16{};
+            for (int x = 0; x < Q; ++x)
+              f[nq % 2][x] = rd.rows_pi(k0 < KS ? xl : xh, nq / PER, (k0 + x) % KS);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if (q % PER == 0) s = f32x16{};
 #pragma unroll
-        for (int x = 0; x < Q; ++x) s = wa_mfma32(f[q % 2][x], a[(q % PER * Q + x) % KS], s);
-        if (q % PER == PER - 1) {
+          for (int x = 0; x < Q; ++x) s = wa_mfma32(f[q % 2][x], a[(q % PER * Q + x) % KS], s);
+          if (q % PER == PER - 1) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) y[q / PER][r] = s[r] * fs;
+            for (int r = 0; r < 16; ++r) y[q / PER][r] += s[r] * fs;
+          }
         }
       }
+    }
+    // decayed products with the chunk's two tiles of tokens, zero where the rows do not see them
+    bf16x8 pr[4];
+    if (sees) {
+      f32x16 s[2] = {};
+#pragma unroll
+      for (int x = 0; x < Q; ++x) f[0][x] = rd.rows(B, 0, x);
+#pragma unroll
+      for (int q = 0; q < 2 * KS / Q; ++q) {
+        if (q + 1 < 2 * KS / Q) {
+#pragma unroll
+          for (int x = 0; x < Q; ++x)
+            f[(q + 1) % 2][x] = rd.rows(B, (q + 1) * Q / KS, (Q * (q + 1) + x) % KS);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < Q; ++x) s[q * Q / KS] = wa_mfma32(f[q % 2][x], a[(Q * q + x) % KS], s[q * Q / KS]);
+      }
+#pragma unroll
+      for (int jh = 0; jh < 2; ++jh) {
+        if (jh == at) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int steps = rev ? acc_row(r, lg) - lr : lr - acc_row(r, lg);
+            s[jh][r] = steps >= 0 ? s[jh][r] * power(g2, steps) : 0.f;
+          }
+        } else if (jh >= lo && jh < hi) {
+          const float fj = power(g2, rev ? 32 * (jh - at) - lr : 32 * (at - jh) + lr - 31);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const f32x4 e = *(const f32x4*)(edge + 8 * r + 4 * lg);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[jh][4 * r + x] *= e[x] * fj;
+          }
+        } else {
+          s[jh] = f32x16{};
+        }
+        pr[2 * jh] = pack8(s[jh], 0);
+        pr[2 * jh + 1] = pack8(s[jh], 1);
+      }
+    }
+    // weighted keys of this wave's state rows (past the last unit the state is not used again)
+    if (c == 0) {
       const float keep = power(g2, m);
 #pragma unroll
       for (int i = 0; i < XT; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) X[i][r] *= keep;
     }
-    // decayed products with the chunk's two tiles of tokens, where the rows see them
-    bf16x8 pr[4];
-    bool seen[2];
-#pragma unroll
-    for (int jh = 0; jh < 2; ++jh) {
-      const int jt = 2 * c + jh;
-      seen[jh] = any && (rev ? jt >= rt && 32 * jt < m : jt <= rt);
-      if (!seen[jh]) continue;
-      f32x16 s{};
-#pragma unroll
-      for (int x = 0; x < Q; ++x) f[0][x] = tile_row8<D>(B, 32 * jh + lr, 2 * x + lg);
-#pragma unroll
-      for (int q = 0; q < KS / Q; ++q) {
-        if (q + 1 < KS / Q) {
-#pragma unroll
-          for (int x = 0; x < Q; ++x) f[(q + 1) % 2][x] = tile_row8<D>(B, 32 * jh + lr, 2 * (Q * (q + 1) + x) + lg);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int x = 0; x < Q; ++x) s = wa_mfma32(f[q % 2][x], a[Q * q + x], s);
-      }
-      if (jt == rt) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int steps = rev ? acc_row(r, lg) - lr : lr - acc_row(r, lg);
-          s[r] = steps >= 0 ? s[r] * power(g2, steps) : 0.f;
-        }
-      } else {
-        const float fj = power(g2, rev ? 32 * (jt - rt) - lr : 32 * (rt - jt) + lr - 31);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const f32x4 e = *(const f32x4*)(edge + 8 * r + 4 * lg);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) s[4 * r + x] *= e[x] * fj;
-        }
-      }
-      pr[2 * jh] = pack8(s, 0);
-      pr[2 * jh + 1] = pack8(s, 1);
-    }
-    // weighted keys of this wave's state rows; forwards only whole units are followed by another
     bf16x8 bw[4];
-    if (more) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) bw[q] = tile_tr8_pi<D>(B, q, 32 * xd, ln);
+    for (int q = 0; q < 4; ++q) bw[q] = rd.cols_pi(B, q, xd);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float wv[8];
-        load_weights(wt + c * kChunk, q, lg, wv);
+    for (int q = 0; q < Q; ++q) f[0][q] = rd.cols_pi(C, q, 0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) bw[q][e] = (bf16_t)(wv[e] * (float)bw[q][e]);
-      }
+    for (int q = 0; q < 4; ++q) {
+      float wv[8];
+      load_weights(wt + c * kChunk, q, lg, wv);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bw[q][e] = (bf16_t)(wv[e] * (float)bw[q][e]);
     }
-    if (more || seen[0] || seen[1]) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) f[0][q] = tile_tr8_pi<D>(C, q, 0, ln);
+    for (int et = 0; et < CT; ++et) {
+      if (et + 1 < CT) {
 #pragma unroll
-      for (int et = 0; et < CT; ++et) {
-        if (et + 1 < CT) {
+        for (int q = 0; q < Q; ++q) f[(et + 1) % 2][q] = rd.cols_pi(C, q, et + 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (sees) {
 #pragma unroll
-          for (int q = 0; q < Q; ++q) f[(et + 1) % 2][q] = tile_tr8_pi<D>(C, q, 32 * (et + 1), ln);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int q = 0; q < 4; ++q) y[et] = wa_mfma32(f[et % 2][q], pr[q], y[et]);
+      }
+      if (et / XT == xe / XT) {
 #pragma unroll
-        for (int jh = 0; jh < 2; ++jh)
-          if (seen[jh]) {
-            y[et] = wa_mfma32(f[et % 2][2 * jh], pr[2 * jh], y[et]);
-            y[et] = wa_mfma32(f[et % 2][2 * jh + 1], pr[2 * jh + 1], y[et]);
-          }
-        if (more && et / XT == xe / XT) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) X[et % XT] = wa_mfma32(bw[q], f[et % 2][q], X[et % XT]);
-        }
+        for (int q = 0; q < 4; ++q) X[et % XT] = wa_mfma32(bw[q], f[et % 2][q], X[et % XT]);
       }
     }
     ++c;
     if (!last) continue;
+    const int lp = pi32(lr);
     const int t = u0 + 32 * rt + lr;
     if (t < n) {
       bf16_t* at = yb + (int64_t)t * jb.y_st + 8 * lg;
@@ -831,7 +872,8 @@ __global__ void __launch_bounds__(512) pairs_bf16_kernel(PairsParams p) {
   const int groups = (p.s.seg + kPairRows - 1) / kPairRows;
   const int seg = blockIdx.x / groups, ig = blockIdx.x % groups, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
-  const int n = tokens_of(p.s, b, seg), i0 = ig * kPairRows, iw = i0 + 32 * w, i = iw + l32;
+  const int rt = w < NW / 2 ? w : 3 * NW / 2 - 1 - w;   // the two waves of a SIMD share the causal work evenly
+  const int n = tokens_of(p.s, b, seg), i0 = ig * kPairRows, iw = i0 + 32 * rt, i = iw + l32;
   double* out = p.part + (int64_t)bh * p.n_part + p.part_at + blockIdx.x;
   if (i0 >= n) {
     if (tid == 0) *out = 0.0;
@@ -861,39 +903,62 @@ __global__ void __launch_bounds__(512) pairs_bf16_kernel(PairsParams p) {
   float cj[16];   // lambda^(e - j) of the tile's rows
 #pragma unroll
   for (int r = 0; r < 16; ++r) cj[r] = power(g2, 31 - acc_row(r, g));
+  TileReads<D> rd;
+  rd.init(lane);
   issue(0);
   if (chunks > 1) issue(1);
   double sum = 0.0;
   for (int it = 0; it < chunks; ++it) {
     if (it + 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (it == 0) {   // this wave's rows have landed too: no wait for them behind the loads below
+#pragma unroll
+      for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]), "+v"(d[k]));
+    }
     if (it + 2 < chunks) issue(it + 2);
+    const int before = iw - it * kChunk, at = before / 32;   // the tile of the chunk on the diagonal; those before it separate
+    if (iw >= n || before < 0) continue;
+    rd.renew();
+    const bf16_t* K = tk[it % STAGES];
+    const bf16_t* V = tv[it % STAGES];
+    // operands are read four at a time, while the four products before them run: keys, then values of a tile
+    constexpr int Q = 4, PER = KS / Q;
+    bf16x8 f[2][Q];
+    f32x16 s[2] = {}, t[2] = {};
+#pragma unroll
+    for (int x = 0; x < Q; ++x) f[0][x] = rd.rows(K, 0, x);
+#pragma unroll
+    for (int u = 0; u < 4 * PER; ++u) {
+      if (u + 1 < 4 * PER) {
+        const int nu = u + 1;
+#pragma unroll
+        for (int x = 0; x < Q; ++x) f[nu % 2][x] = rd.rows(nu / PER % 2 ? V : K, nu / (2 * PER), nu % PER * Q + x);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < Q; ++x) {
+        f32x16& acc = u / PER % 2 ? t[u / (2 * PER)] : s[u / (2 * PER)];
+        acc = wa_mfma32(f[u % 2][x], (u / PER % 2 ? d : q)[u % PER * Q + x], acc);
+      }
+    }
 #pragma unroll
     for (int jh = 0; jh < 2; ++jh) {
-      const int jt = it * kChunk + 32 * jh;
-      if (jt > iw || iw >= n) continue;
-      f32x16 s{}, t{};
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        s = wa_mfma32(tile_row8<D>(tk[it % STAGES], 32 * jh + l32, 2 * k + g), q[k], s);
-        t = wa_mfma32(tile_row8<D>(tv[it % STAGES], 32 * jh + l32, 2 * k + g), d[k], t);
-      }
-      if (jt < iw) {
+      if (jh < at) {
         float u = 0.f, v = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float x = cj[r] * (s[r] * t[r]);
+          const float x = cj[r] * (s[jh][r] * t[jh][r]);
           u += x;
           v += (float)(31 - acc_row(r, g)) * x;
         }
-        const int steps = i - jt - 31;
+        const int steps = i - (it * kChunk + 32 * jh) - 31;
         sum += (double)(power(g2, steps) * ((float)steps * u + v));
-      } else {
+      } else if (jh == at) {
         float u = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int steps = l32 - acc_row(r, g);
-          u += steps > 0 ? (float)steps * power(g2, steps) * (s[r] * t[r]) : 0.f;
+          u += steps > 0 ? (float)steps * power(g2, steps) * (s[jh][r] * t[jh][r]) : 0.f;
         }
         sum += (double)u;
       }
