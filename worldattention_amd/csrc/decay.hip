@@ -405,7 +405,13 @@ struct TileReads {
   }
   // Hides from the compiler that the offsets stay the same from step to step: the sums it would keep of
   // them take the registers that hold operands ahead of their products.
-  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(row), "+v"(rowpi), "+v"(tr[0]), "+v"(tr[1])); }
+  __device__ __forceinline__ void renew_rows() { asm volatile("" : "+v"(row)); }
+  __device__ __forceinline__ void renew_cols() { asm volatile("" : "+v"(tr[0]), "+v"(tr[1])); }
+  __device__ __forceinline__ void renew() {
+    asm volatile("" : "+v"(rowpi));
+    renew_rows();
+    renew_cols();
+  }
   // rows 32 tile + l32, channels 16 k + 8 g .. + 7
   __device__ __forceinline__ bf16x8 rows(const bf16_t* t, int tile, int k) const {
     return *(const bf16x8*)((const char*)t + (row ^ (k << 5)) + tile * (32 * D * 2));
@@ -435,24 +441,25 @@ constexpr int64_t kMaxTokenStride = (int64_t)1 << 23;
 template <int D, int NW>
 struct ChunkStream {
   static constexpr int NI = TileStream<D, NW>::NI, RPI = TileStream<D, NW>::RPI;
+  static_assert(NW * RPI % 16 == 0, "the swizzle repeats every 16 rows, so one lane offset serves all instructions");
   const bf16_t* base;
   int64_t st;
-  int off[NI];
+  int off;
   __device__ __forceinline__ void init(const View& x, int b, int h, int64_t first, int w, int lane) {
     base = (const bf16_t*)x.p + (int64_t)b * x.sb + (int64_t)h * x.sh + first * x.st;
     st = x.st;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int row = (i * NW + w) * RPI + lane / (D / 8), pos = lane % (D / 8);
-      off[i] = (row * (int)st + (pos ^ dual_swizzle<D>(row)) * 8) * 2;
-    }
+    const int row = w * RPI + lane / (D / 8), pos = lane % (D / 8);
+    off = (row * (int)st + (pos ^ dual_swizzle<D>(row)) * 8) * 2;
   }
   // rows row0 .. row0 + rows - 1 (at most 64) into `lds`, zeros behind them
   __device__ __forceinline__ void issue(bf16_t* lds, int row0, int rows, int w) const {
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)(base + (int64_t)row0 * st), (short)0, ((rows - 1) * (int)st + D) * 2, WA_BUF_DWORD3);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) lds_dma16(rs, lds + (i * NW + w) * RPI * D, off[i]);
+    for (int i = 0; i < NI; ++i) {
+      const int skip = i * NW * RPI;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(base + (int64_t)(row0 + skip) * st), (short)0, rows > skip ? ((rows - skip - 1) * (int)st + D) * 2 : 0, WA_BUF_DWORD3);
+      lds_dma16(rs, lds + (i * NW + w) * RPI * D, off);
+    }
   }
 };
 
@@ -552,7 +559,7 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
         if (DERIV) dacc[i][r] = keep * (dacc[i][r] + (float)m * acc[i][r]);
         acc[i][r] *= keep;
       }
-    rd.renew();
+    rd.renew_cols();
     bf16x8 cv[2], bv[2][DT];   // the next 16 tokens' operands are read behind this ones' products
     cv[0] = rd.cols_pi(C, 0, ch);
 #pragma unroll
@@ -857,28 +864,32 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
   }
 }
 
-// Pairs: a workgroup takes 256 rows i of a segment, 32 a wave, whose queries and output gradients stay in
-// registers as operands, against the segment's keys and values up to them (a ring of LDS stages). Tiles before
-// the diagonal separate: with e the tile's last token, (i - j) lambda^(i - j) = lambda^(i - e) [(i - e) + (e - j)]
-// lambda^(e - j), no power above 1, the column factors being the same for every tile.
+// Pairs: a workgroup takes 256 rows i of a segment, its four waves two 32-row tiles each (w and 7 - w, which
+// share the causal work evenly), whose queries and output gradients stay in registers as operands; the
+// segment's keys and values up to the rows pass through a ring of two LDS stages, each operand read
+// serving both tiles (with one tile a wave the LDS reads took as long as the products: 256 us against 168 at
+// 32,760 tokens of 12 x 128). Tiles before the diagonal separate: with e the tile's last token,
+// (i - j) lambda^(i - j) = lambda^(i - e) [(i - e) + (e - j)] lambda^(e - j), no power above 1.
 constexpr int kPairRows = 256;
 
 template <int D>
-__global__ void __launch_bounds__(512) pairs_bf16_kernel(PairsParams p) {
-  constexpr int NW = 8, KS = D / 16, STAGES = 3, NI = ChunkStream<D, NW>::NI;
+__global__ void __launch_bounds__(256, 2) pairs_bf16_kernel(PairsParams p) {
+  constexpr int NW = 4, KS = D / 16, STAGES = 2, Q = 2, PER = KS / Q;
   __shared__ __attribute__((aligned(1024))) bf16_t tk[STAGES][kChunk * D];
   __shared__ __attribute__((aligned(1024))) bf16_t tv[STAGES][kChunk * D];
+  __shared__ __attribute__((aligned(16))) float edge[2][32];   // lambda^(e - j) of a tile's tokens, and (e - j) times it
   __shared__ double red[NW];
   const int groups = (p.s.seg + kPairRows - 1) / kPairRows;
-  const int seg = blockIdx.x / groups, ig = blockIdx.x % groups, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
+  // the groups with the most keys first, so that the short ones fill the end of the launch
+  const int seg = blockIdx.x / groups, ig = groups - 1 - (int)blockIdx.x % groups, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
-  const int rt = w < NW / 2 ? w : 3 * NW / 2 - 1 - w;   // the two waves of a SIMD share the causal work evenly
-  const int n = tokens_of(p.s, b, seg), i0 = ig * kPairRows, iw = i0 + 32 * rt, i = iw + l32;
+  const int n = tokens_of(p.s, b, seg), i0 = ig * kPairRows;
   double* out = p.part + (int64_t)bh * p.n_part + p.part_at + blockIdx.x;
   if (i0 >= n) {
     if (tid == 0) *out = 0.0;
     return;
   }
+  const int row0[2] = {i0 + 32 * w, i0 + 32 * (7 - w)};
   const int chunks = (min(n, i0 + kPairRows) + kChunk - 1) / kChunk;
   const float g2 = log2_decay(p.s, h);
   const int64_t first = (int64_t)seg * p.s.seg;
@@ -889,79 +900,95 @@ __global__ void __launch_bounds__(512) pairs_bf16_kernel(PairsParams p) {
     sk.issue(tk[it % STAGES], it * kChunk, min(kChunk, n - it * kChunk), w);
     sv.issue(tv[it % STAGES], it * kChunk, min(kChunk, n - it * kChunk), w);
   };
-  bf16x8 q[KS], d[KS];
-  const bf16_t* qb = (const bf16_t*)p.q.p + (int64_t)b * p.q.sb + (int64_t)h * p.q.sh + (first + i) * p.q.st + 8 * g;
-  const bf16_t* db = (const bf16_t*)p.d.p + (int64_t)b * p.d.sb + (int64_t)h * p.d.sh + (first + i) * p.d.st + 8 * g;
-#pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    q[k] = d[k] = bf16x8{};
-    if (i < n) {
-      q[k] = *(const bf16x8*)(qb + 16 * k);
-      d[k] = *(const bf16x8*)(db + 16 * k);
-    }
-  }
-  float cj[16];   // lambda^(e - j) of the tile's rows
-#pragma unroll
-  for (int r = 0; r < 16; ++r) cj[r] = power(g2, 31 - acc_row(r, g));
   TileReads<D> rd;
   rd.init(lane);
-  issue(0);
-  if (chunks > 1) issue(1);
-  double sum = 0.0;
-  for (int it = 0; it < chunks; ++it) {
-    if (it + 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (it == 0) {   // this wave's rows have landed too: no wait for them behind the loads below
+  // The rows' operands come through the stages too (the four hold 256 rows), in whole lines: read straight
+  // into registers, 32 bytes of 32 rows at a time, they took 14 us of a workgroup's 60.
+  bf16x8 q[2][KS], d[2][KS];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]), "+v"(d[k]));
+  for (int x = 0; x < 2; ++x) {
+    ChunkStream<D, NW> sr;
+    sr.init(x ? p.d : p.q, b, h, first, w, lane);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) sr.issue(y < 2 ? tk[y] : tv[y - 2], i0 + kChunk * y, min(kChunk, n - (i0 + kChunk * y)), w);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int rt = y ? 7 - w : w;
+      const bf16_t* T = rt < 4 ? tk[rt / 2] : tv[rt / 2 - 2];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) (x ? d : q)[y][k] = rd.rows(T, rt % 2, k);
     }
-    if (it + 2 < chunks) issue(it + 2);
-    const int before = iw - it * kChunk, at = before / 32;   // the tile of the chunk on the diagonal; those before it separate
-    if (iw >= n || before < 0) continue;
-    rd.renew();
-    const bf16_t* K = tk[it % STAGES];
-    const bf16_t* V = tv[it % STAGES];
-    // operands are read four at a time, while the four products before them run: keys, then values of a tile
-    constexpr int Q = 4, PER = KS / Q;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+  if (tid < 32) {
+    edge[0][tid] = power(g2, 31 - tid);
+    edge[1][tid] = (float)(31 - tid) * edge[0][tid];
+  }
+  issue(0);
+  double sum = 0.0;
+  // One tile of 32 tokens from jt on against both row tiles (the upper one may not see it).
+  auto tile = [&](const bf16_t* K, const bf16_t* V, int jh, int jt) {
     bf16x8 f[2][Q];
     f32x16 s[2] = {}, t[2] = {};
 #pragma unroll
-    for (int x = 0; x < Q; ++x) f[0][x] = rd.rows(K, 0, x);
+    for (int x = 0; x < Q; ++x) f[0][x] = rd.rows(K, jh, x);
 #pragma unroll
-    for (int u = 0; u < 4 * PER; ++u) {
-      if (u + 1 < 4 * PER) {
-        const int nu = u + 1;
+    for (int u = 0; u < 2 * PER; ++u) {   // keys, then values: two operands read behind the products before them
+      if (u + 1 < 2 * PER) {
 #pragma unroll
-        for (int x = 0; x < Q; ++x) f[nu % 2][x] = rd.rows(nu / PER % 2 ? V : K, nu / (2 * PER), nu % PER * Q + x);
+        for (int x = 0; x < Q; ++x) f[(u + 1) % 2][x] = rd.rows((u + 1) / PER ? V : K, jh, (u + 1) % PER * Q + x);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < Q; ++x) {
-        f32x16& acc = u / PER % 2 ? t[u / (2 * PER)] : s[u / (2 * PER)];
-        acc = wa_mfma32(f[u % 2][x], (u / PER % 2 ? d : q)[u % PER * Q + x], acc);
-      }
+      for (int x = 0; x < Q; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          if (u / PER) t[y] = wa_mfma32(f[u % 2][x], d[y][u % PER * Q + x], t[y]);
+          else s[y] = wa_mfma32(f[u % 2][x], q[y][u % PER * Q + x], s[y]);
+        }
+    }
+    int ln = lane;     // the lane renewed, so that the powers below are not kept in registers
+    asm volatile("" : "+v"(ln));
+    const int lg = ln >> 5, lr = ln & 31;
+    float u[2] = {0.f, 0.f}, v[2] = {0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const f32x4 e0 = *(const f32x4*)(edge[0] + 8 * r + 4 * lg), e1 = *(const f32x4*)(edge[1] + 8 * r + 4 * lg);
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float x = s[y][4 * r + z] * t[y][4 * r + z];
+          u[y] += e0[z] * x;
+          v[y] += e1[z] * x;
+        }
     }
 #pragma unroll
-    for (int jh = 0; jh < 2; ++jh) {
-      if (jh < at) {
-        float u = 0.f, v = 0.f;
+    for (int y = 0; y < 2; ++y) {
+      if (jt < row0[y]) {
+        const int steps = row0[y] + lr - jt - 31;
+        sum += (double)(power(g2, steps) * ((float)steps * u[y] + v[y]));
+      } else if (jt == row0[y]) {
+        float x = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float x = cj[r] * (s[jh][r] * t[jh][r]);
-          u += x;
-          v += (float)(31 - acc_row(r, g)) * x;
+          const int steps = lr - acc_row(r, lg);
+          x += steps > 0 ? (float)steps * power(g2, steps) * (s[y][r] * t[y][r]) : 0.f;
         }
-        const int steps = i - (it * kChunk + 32 * jh) - 31;
-        sum += (double)(power(g2, steps) * ((float)steps * u + v));
-      } else if (jh == at) {
-        float u = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int steps = l32 - acc_row(r, g);
-          u += steps > 0 ? (float)steps * power(g2, steps) * (s[jh][r] * t[jh][r]) : 0.f;
-        }
-        sum += (double)u;
+        sum += (double)x;
       }
+    }
+  };
+  for (int it = 0; it < chunks; ++it) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (it + 1 < chunks) issue(it + 1);
+#pragma unroll 1
+    for (int jh = 0; jh < 2; ++jh) {
+      const int jt = it * kChunk + 32 * jh;
+      if (jt > row0[1] || jt >= n) break;
+      rd.renew_rows();
+      tile(tk[it % STAGES], tv[it % STAGES], jh, jt);
     }
   }
   sum = workgroup_sum<NW>(sum * (double)p.scale, red);
@@ -1204,7 +1231,7 @@ int run_bwd(const wa_decay_bwd_args* a, hipStream_t st) {
   if (a->dlog_decay) {
     const PairsParams pp{s, q, k, v, d, part, n_part, s.n_seg + D * D / kThreads, a->scale};
     const dim3 grid((unsigned)pairs, s.B * s.H);
-    if (a->dtype == WA_BF16) hipLaunchKernelGGL((pairs_bf16_kernel<D>), grid, dim3(512), 0, st, pp);
+    if (a->dtype == WA_BF16) hipLaunchKernelGGL((pairs_bf16_kernel<D>), grid, dim3(256), 0, st, pp);
     else hipLaunchKernelGGL((pairs_f32_kernel<D>), grid, dim3(kThreads), 0, st, pp);
     hipLaunchKernelGGL(decay_grad_kernel, dim3(s.H), dim3(kThreads), 0, st, (const double*)part, s.B, s.H, n_part, a->dlog_decay);
   }
