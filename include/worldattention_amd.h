@@ -752,14 +752,14 @@ int wa_rope_axes(const wa_rope_axes_args* args, void* stream);
  * log_decay: device fp32 [H], meant to be <= 0 (-inf: a head without memory). lengths (optional):
  * device int32 [B], clamped to [0, L]: tokens from lengths[b] on are not read, their outputs (and
  * gradients) are 0 and the state ends at the last token before them.
- * The sequence is cut into wa_decay_segments(B, L, H) segments. `states` (device fp32
+ * The sequence is cut into wa_decay_segments(B, L, H, derivs) segments. `states` (device fp32
  * [B, H, segments, D, D]) receives the state before each, which the backward takes back;
- * `derivs` (device fp32 [B, H, segments + 1, D, D], or NULL) receives the states' derivatives by
- * log_decay, which a backward that computes dlog_decay takes back.
+ * `derivs` (device fp32 [B, H, segments + 1, D, D], or NULL with derivs = 0 above) receives the states'
+ * derivatives by log_decay, which a backward that computes dlog_decay takes back (others get NULL).
  * initial / final: fp32 [B, H, D, D] (key channel, value channel), contiguous; final may be NULL.
  * Rows must be 16-byte aligned and at most 2^23 elements apart. The state is kept and summed in
  * fp32. */
-int64_t wa_decay_segments(int64_t B, int64_t L, int64_t H);
+int64_t wa_decay_segments(int64_t B, int64_t L, int64_t H, int32_t derivs);
 typedef struct wa_decay_fwd_args {
   const void* q; int64_t q_sb, q_st, q_sh;
   const void* k; int64_t k_sb, k_st, k_sh;
@@ -780,7 +780,7 @@ int wa_decay_fwd(const wa_decay_fwd_args* args, void* stream);
 /* Gradients of wa_decay_fwd. dfinal (NULL: 0): the gradient of the final state. dq, dk, dv are
  * written in the inputs' dtype; dinitial (fp32) and dlog_decay (fp32 [H], summed in a fixed order)
  * are optional. The workspace (device, wa_decay_bwd_workspace_bytes) holds the gradient states. */
-int64_t wa_decay_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D);
+int64_t wa_decay_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D, int32_t derivs);
 typedef struct wa_decay_bwd_args {
   const void* q; int64_t q_sb, q_st, q_sh;
   const void* k; int64_t k_sb, k_st, k_sh;

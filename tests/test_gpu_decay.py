@@ -229,4 +229,4 @@ def test_long_sequences_address_past_32_bits():
     want = W.decay_linear_attention(x["q"], x["k"], x["v"], x["log_decay"])
     got = W.decay_linear_attention(x["q"], view, x["v"], x["log_decay"])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
-    assert _lib.lib().wa_decay_segments(1, n, 1) > 1
+    assert _lib.lib().wa_decay_segments(1, n, 1, 0) > 1

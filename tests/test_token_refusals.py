@@ -99,7 +99,7 @@ def test_decay_entry_points_refuse():
     lib = _lib.lib()
     for fn in (lib.wa_decay_fwd, lib.wa_decay_bwd, lib.wa_decay_step):
         assert fn(None, None) == _lib.WA_ERR_ARG
-    assert lib.wa_decay_segments(1, 0, 4) == 0 and lib.wa_decay_segments(1, 1, 1) == 1
+    assert lib.wa_decay_segments(1, 0, 4, 0) == 0 and lib.wa_decay_segments(1, 1, 1, 1) == 1
     f = _lib.DecayFwdArgs()
     f.q = f.k = f.v = f.o = f.log_decay = f.states = FAKE
     f.B, f.L, f.H, f.D, f.dtype = 1, 4, 2, 96, _lib.WA_BF16

@@ -458,9 +458,9 @@ SIGNATURES = {
     "wa_hkv_score_topk": (c_int, [POINTER(HkvTopkArgs), c_void_p]),
     "wa_rerope": (c_int, [POINTER(RopeArgs), c_void_p]),
     "wa_rope_axes": (c_int, [POINTER(RopeAxesArgs), c_void_p]),
-    "wa_decay_segments": (c_int64, [c_int64] * 3),
+    "wa_decay_segments": (c_int64, [c_int64] * 3 + [c_int32]),
     "wa_decay_fwd": (c_int, [POINTER(DecayFwdArgs), c_void_p]),
-    "wa_decay_bwd_workspace_bytes": (c_int64, [c_int64] * 4),
+    "wa_decay_bwd_workspace_bytes": (c_int64, [c_int64] * 4 + [c_int32]),
     "wa_decay_bwd": (c_int, [POINTER(DecayBwdArgs), c_void_p]),
     "wa_decay_step": (c_int, [POINTER(DecayStepArgs), c_void_p]),
     "wa_select_blocks_workspace_bytes": (c_int64, [c_int64] * 4),

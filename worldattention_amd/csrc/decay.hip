@@ -493,11 +493,6 @@ __device__ __forceinline__ void cut3(const float (&x)[8], bf16x8& hi, bf16x8& mi
   lo = __builtin_bit_cast(bf16x8, l);
 }
 
-// Weights of the tokens of a chunk in the running state after it, m tokens long: lambda^(m - 1 - j), backwards
-// lambda^(j + 1), times w_scale. Filled by the first wave.
-__device__ __forceinline__ void fill_weights(float* wt, float g2, int m, bool rev, float w_scale, int lane) {
-  wt[lane] = w_scale * power(g2, rev ? lane + 1 : max(0, m - 1 - lane));
-}
 // The 8 weights of a fragment's tokens (accumulator order).
 __device__ __forceinline__ void load_weights(const float* wt, int c, int g, float (&w)[8]) {
   const f32x4 a = *(const f32x4*)(wt + 16 * c + 4 * g), b = *(const f32x4*)(wt + 16 * c + 8 + 4 * g);
@@ -508,37 +503,51 @@ __device__ __forceinline__ void load_weights(const float* wt, int c, int g, floa
   }
 }
 
-// A segment's own state. Wave (ch, dh) of D / 16 waves: columns 32 ch .. + 31, half of the rows. The
-// weighted operand enters in three parts, so the state carries no rounding but its fp32 sums'.
+// A segment's own state. Wave (ch, half) of D / 16 waves: columns 32 ch .. + 31 over all rows, from half of each
+// chunk's tokens (the two halves meet in LDS at the end): every weighted operand is then cut once a workgroup.
+// It enters in three parts, so the state carries no rounding but its fp32 sums'. The state decays once in two
+// chunks, whose tokens' weights run to the end of the two. 32,760 tokens of 12 x 128: 53 us, with derivatives
+// 75 (a wave a half of the rows, cutting twice, decaying every chunk: 99); 200 MB at a copy's rate are 41.
+constexpr int kSpan = 2 * kChunk;
+
 template <int D, bool DERIV>
 __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(StateParams p) {
-  constexpr int NW = D / 16, CT = D / 32, DT = CT / 2, STAGES = 3, NI = ChunkStream<D, NW>::NI;
-  __shared__ __attribute__((aligned(1024))) bf16_t tb[STAGES][kChunk * D];
-  __shared__ __attribute__((aligned(1024))) bf16_t tc[STAGES][kChunk * D];
-  __shared__ __attribute__((aligned(16))) float wt[2][kChunk];
+  constexpr int NW = D / 16, CT = D / 32, STAGES = 3, NI = ChunkStream<D, NW>::NI;
+  __shared__ __attribute__((aligned(1024))) bf16_t tiles[2 * STAGES * kChunk * D];
+  __shared__ __attribute__((aligned(16))) float wt[2][kSpan];
   __shared__ double red[NW];
+  static_assert(sizeof(float) * D * D <= sizeof(tiles), "one half's state passes through the stages");
   const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
-  const int ch = w % CT, dh = w / CT;
-  const int n = tokens_of(p.s, b, seg), chunks = (n + kChunk - 1) / kChunk, tail = n - (chunks - 1) * kChunk;
+  const int ch = w % CT, half = w / CT;
+  const int n = tokens_of(p.s, b, seg), chunks = (n + kChunk - 1) / kChunk, spans = (n + kSpan - 1) / kSpan;
+  const int tail = n - (spans - 1) * kSpan;   // tokens of the span cut off at the end
   const float g2 = log2_decay(p.s, h);
   const int64_t first = (int64_t)seg * p.s.seg;
   ChunkStream<D, NW> sb, sc;
   sb.init(p.b, b, h, first, w, lane);
   sc.init(p.c, b, h, first, w, lane);
+  auto stage_b = [&](int it) { return tiles + (it % STAGES) * 2 * kChunk * D; };
+  auto stage_c = [&](int it) { return tiles + (it % STAGES) * 2 * kChunk * D + kChunk * D; };
+  // step `it` takes chunk `it`, backwards the spans from the last one with their chunks in order
+  auto chunk_of = [&](int it) {
+    if (!p.rev) return it;
+    const int of_last = chunks - 2 * (spans - 1);
+    return it < of_last ? 2 * (spans - 1) + it : 2 * (spans - 2 - (it - of_last) / 2) + (it - of_last) % 2;
+  };
   auto issue = [&](int it) {
-    const int row0 = (p.rev ? chunks - 1 - it : it) * kChunk, rows = min(kChunk, n - row0);
-    sb.issue(tb[it % STAGES], row0, rows, w);
-    sc.issue(tc[it % STAGES], row0, rows, w);
+    const int row0 = chunk_of(it) * kChunk, rows = min(kChunk, n - row0);
+    sb.issue(stage_b(it), row0, rows, w);
+    sc.issue(stage_c(it), row0, rows, w);
   };
   TileReads<D> rd;
   rd.init(lane);
-  f32x16 acc[DT], dacc[DT];
+  f32x16 acc[CT], dacc[CT];
 #pragma unroll
-  for (int i = 0; i < DT; ++i) acc[i] = dacc[i] = f32x16{};
-  if (w == 0) {   // the whole chunks' weights, and those of the one cut off at the end
-    fill_weights(wt[0], g2, kChunk, p.rev, p.w_scale, lane);
-    fill_weights(wt[1], g2, tail, p.rev, p.w_scale, lane);
+  for (int i = 0; i < CT; ++i) acc[i] = dacc[i] = f32x16{};
+  if (tid < kSpan) {   // weights of whole spans' tokens, and of the one cut off
+    wt[0][tid] = p.w_scale * power(g2, p.rev ? tid + 1 : kSpan - 1 - tid);
+    wt[1][tid] = p.w_scale * power(g2, p.rev ? tid + 1 : max(0, tail - 1 - tid));
   }
   if (chunks > 0) issue(0);
   if (chunks > 1) issue(1);
@@ -547,69 +556,106 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
     if (it + 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (it + 2 < chunks) issue(it + 2);
-    const bool cut = (p.rev ? chunks - 1 - it : it) == chunks - 1;
-    const int m = cut ? tail : kChunk;
-    const float keep = power(g2, m);
-    const bf16_t* B = tb[it % STAGES];
-    const bf16_t* C = tc[it % STAGES];
+    const int c = chunk_of(it), at = c % 2 * kChunk;   // the chunk's place in its span
+    const bool cut = c / 2 == spans - 1;
+    const int m = cut ? tail : kSpan;
+    if (c % 2 == 0) {
+      const float keep = power(g2, m);
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
+      for (int i = 0; i < CT; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        if (DERIV) dacc[i][r] = keep * (dacc[i][r] + (float)m * acc[i][r]);
-        acc[i][r] *= keep;
-      }
+        for (int r = 0; r < 16; ++r) {
+          if (DERIV) dacc[i][r] = keep * (dacc[i][r] + (float)m * acc[i][r]);
+          acc[i][r] *= keep;
+        }
+    }
+    const bf16_t* B = stage_b(it);
+    const bf16_t* C = stage_c(it);
     rd.renew_cols();
-    bf16x8 cv[2], bv[2][DT];   // the next 16 tokens' operands are read behind this ones' products
-    cv[0] = rd.cols_pi(C, 0, ch);
+    bf16x8 cv[2], bv[2][CT];
 #pragma unroll
-    for (int i = 0; i < DT; ++i) bv[0][i] = rd.cols_pi(B, 0, DT * dh + i);
+    for (int x = 0; x < 2; ++x) {
+      cv[x] = rd.cols_pi(C, 2 * half + x, ch);
 #pragma unroll
-    for (int c = 0; c < kChunk / 16; ++c) {
+      for (int i = 0; i < CT; ++i) bv[x][i] = rd.cols_pi(B, 2 * half + x, i);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
       float wv[8];
-      load_weights(wt[cut ? 1 : 0], c, g, wv);
-      if (c + 1 < kChunk / 16) {
-        cv[(c + 1) % 2] = rd.cols_pi(C, c + 1, ch);
+      load_weights(wt[cut ? 1 : 0] + at, 2 * half + x, g, wv);
 #pragma unroll
-        for (int i = 0; i < DT; ++i) bv[(c + 1) % 2][i] = rd.cols_pi(B, c + 1, DT * dh + i);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) wv[e] *= (float)cv[c % 2][e];
+      for (int e = 0; e < 8; ++e) wv[e] *= (float)cv[x][e];
       bf16x8 hi, mid, lo;
       cut3(wv, hi, mid, lo);
 #pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        acc[i] = wa_mfma32(bv[c % 2][i], lo, acc[i]);
-        acc[i] = wa_mfma32(bv[c % 2][i], mid, acc[i]);
-        acc[i] = wa_mfma32(bv[c % 2][i], hi, acc[i]);
-      }
+      for (int i = 0; i < CT; ++i) acc[i] = wa_mfma32(bv[x][i], lo, acc[i]);
+#pragma unroll
+      for (int i = 0; i < CT; ++i) acc[i] = wa_mfma32(bv[x][i], mid, acc[i]);
+#pragma unroll
+      for (int i = 0; i < CT; ++i) acc[i] = wa_mfma32(bv[x][i], hi, acc[i]);
       if (DERIV) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int j = 16 * c + 4 * g + 8 * (e >> 2) + (e & 3);
+          const int j = at + 16 * (2 * half + x) + 4 * g + 8 * (e >> 2) + (e & 3);
           wv[e] *= (float)(p.rev ? j + 1 : max(0, m - 1 - j));
         }
         cut3(wv, hi, mid, lo);
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          dacc[i] = wa_mfma32(bv[c % 2][i], lo, dacc[i]);
-          dacc[i] = wa_mfma32(bv[c % 2][i], mid, dacc[i]);
-          dacc[i] = wa_mfma32(bv[c % 2][i], hi, dacc[i]);
-        }
+        for (int i = 0; i < CT; ++i) dacc[i] = wa_mfma32(bv[x][i], lo, dacc[i]);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) dacc[i] = wa_mfma32(bv[x][i], mid, dacc[i]);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) dacc[i] = wa_mfma32(bv[x][i], hi, dacc[i]);
       }
     }
   }
+  // The halves meet: the first takes the states, the second the derivatives.
+  float* meet = (float*)tiles;
+  auto join = [&](f32x16 (&x)[CT], int to) {
+    __syncthreads();
+    if (half != to) {
+#pragma unroll
+      for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) meet[((ch * CT + i) * 16 + r) * 64 + lane] = x[i][r];
+    }
+    __syncthreads();
+    if (half == to) {
+#pragma unroll
+      for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[i][r] += meet[((ch * CT + i) * 16 + r) * 64 + lane];
+    }
+  };
+  join(acc, 0);
+  if (DERIV) join(dacc, 1);
   const int64_t at = ((int64_t)bh * p.s.n_seg + seg) * D * D, dat = ((int64_t)bh * (p.s.n_seg + 1) + seg) * D * D;
   double sum = 0.0;
+  auto element = [&](int i, int r) { return (32 * i + 16 * (r >> 3) + 8 * g + (r & 7)) * D + 32 * ch + pi32(l32); };
+  auto write = [&](const f32x16 (&x)[CT], float* out) {
 #pragma unroll
-  for (int i = 0; i < DT; ++i)
+    for (int i = 0; i < CT; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int e = (32 * (DT * dh + i) + 16 * (r >> 3) + 8 * g + (r & 7)) * D + 32 * ch + pi32(l32);
-      p.states[at + e] = acc[i][r];
-      if (DERIV && !p.rev) p.derivs[dat + e] = dacc[i][r];
-      if (DERIV && p.rev) sum += (double)(p.S[at + e] * dacc[i][r] + p.T[dat + e] * acc[i][r]);
+      for (int r = 0; r < 16; ++r) out[element(i, r)] = x[i][r];
+  };
+  auto dot = [&](const f32x16 (&x)[CT], const float* other) {
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      float o[16], part = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[r] = other[element(i, r)];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) part += o[r] * x[i][r];
+      sum += (double)part;
     }
+  };
+  if (half == 0) {
+    write(acc, p.states + at);
+    if (DERIV && p.rev) dot(acc, p.T + dat);
+  } else if (DERIV) {
+    if (p.rev) dot(dacc, p.S + at);
+    else write(dacc, p.derivs + dat);
+  }
   if (DERIV && p.rev) {
     sum = workgroup_sum<NW>(sum, red);
     if (tid == 0) p.part[(int64_t)bh * p.n_part + seg] = sum;
@@ -1132,16 +1178,22 @@ __global__ void __launch_bounds__(kThreads) step_kernel(StepParams p) {
   }
 }
 
-// Segments: as many as give every CU work, in whole rounds of the 256 workgroups that run at once (the rows
-// kernel's LDS ring takes most of a CU), with the shortest time of rounds x segment length; a segment is a
-// multiple of the chunk and not below 128 tokens, where its fp32 state costs as much as its tokens.
-int64_t segment_length(int64_t B, int64_t L, int64_t H) {
-  const int64_t rows = B * H;
-  int64_t best = 0, best_cost = INT64_MAX;
-  for (int64_t k = 1; k <= std::min<int64_t>(256, (L + 127) / 128); ++k) {
+// Segments. The rows kernel's LDS ring takes most of a CU, so its workgroups run in rounds of 256, as long as a
+// segment; each segment costs its states' writing, carrying and reading; with derivatives (training) the pairs
+// inside a segment grow with its length. Weights in us, fitted at 32,760 tokens of 12 x 128: 0.08 a token of a
+// round and rows launch (5 launches' worth in training, 1.4 with the state pass alone), 0.05 (0.2 with
+// derivatives) a segment, 2.8e-7 a token and token of segment. That call takes 21 segments of 1,600 tokens for its
+// output alone and 64 of 512 in training (kernels 918 us; in 21 segments 937, the pairs 237 of it instead of 117).
+int64_t segment_length(int64_t B, int64_t L, int64_t H, bool derivs) {
+  const double rows = (double)(B * H);
+  int64_t best = 0;
+  double best_cost = 0.0;
+  for (int64_t k = 1; k <= std::min<int64_t>(512, (L + 127) / 128); ++k) {
     const int64_t seg = std::max<int64_t>(128, ((L + k - 1) / k + kChunk - 1) / kChunk * kChunk);
-    const int64_t n = (L + seg - 1) / seg, cost = (rows * n + 255) / 256 * seg + 8 * n;
-    if (cost < best_cost) {
+    const int64_t n = (L + seg - 1) / seg, rounds = (B * H * n + 255) / 256;
+    const double cost = (derivs ? 0.4 : 0.11) * (double)(rounds * seg) + rows * ((derivs ? 0.2 : 0.05) * (double)n +
+                        (derivs ? 2.8e-7 * (double)L * (double)seg : 0.0));
+    if (best == 0 || cost < best_cost) {
       best_cost = cost;
       best = seg;
     }
@@ -1162,8 +1214,9 @@ int check_shape(const char* what, int dtype, int64_t B, int64_t L, int64_t H, in
   return WA_OK;
 }
 
-Shape shape_of(int64_t B, int64_t L, int64_t H, const float* g, const int32_t* lengths) {
-  return Shape{(int)B, (int)L, (int)H, (int)segment_length(B, L, H), (int)wa_decay_segments(B, L, H), g, lengths};
+Shape shape_of(int64_t B, int64_t L, int64_t H, bool derivs, const float* g, const int32_t* lengths) {
+  const int64_t seg = segment_length(B, L, H, derivs);
+  return Shape{(int)B, (int)L, (int)H, (int)seg, (int)((L + seg - 1) / seg), g, lengths};
 }
 
 // Workgroups of the pairs kernel along a head: one per segment in fp32, one per 256 rows in bf16.
@@ -1187,7 +1240,7 @@ void all_rows(int dtype, const RowsParams& p, int jobs, hipStream_t st) {
 
 template <int D>
 int run_fwd(const wa_decay_fwd_args* a, hipStream_t st) {
-  const Shape s = shape_of(a->B, a->L, a->H, a->log_decay, a->lengths);
+  const Shape s = shape_of(a->B, a->L, a->H, a->derivs != nullptr, a->log_decay, a->lengths);
   const View q{a->q, a->q_sb, a->q_st, a->q_sh}, k{a->k, a->k_sb, a->k_st, a->k_sh}, v{a->v, a->v_sb, a->v_st, a->v_sh};
   StateParams sp{};
   sp.s = s; sp.b = k; sp.c = v; sp.states = a->states; sp.derivs = a->derivs; sp.w_scale = 1.f;
@@ -1205,7 +1258,7 @@ int run_fwd(const wa_decay_fwd_args* a, hipStream_t st) {
 
 template <int D>
 int run_bwd(const wa_decay_bwd_args* a, hipStream_t st) {
-  const Shape s = shape_of(a->B, a->L, a->H, a->log_decay, a->lengths);
+  const Shape s = shape_of(a->B, a->L, a->H, a->derivs != nullptr, a->log_decay, a->lengths);
   const View q{a->q, a->q_sb, a->q_st, a->q_sh}, k{a->k, a->k_sb, a->k_st, a->k_sh}, v{a->v, a->v_sb, a->v_st, a->v_sh};
   const View d{a->dout, a->d_sb, a->d_st, a->d_sh};
   float* Y = (float*)a->workspace;
@@ -1240,15 +1293,14 @@ int run_bwd(const wa_decay_bwd_args* a, hipStream_t st) {
 
 }  // namespace
 
-extern "C" int64_t wa_decay_segments(int64_t B, int64_t L, int64_t H) {
+extern "C" int64_t wa_decay_segments(int64_t B, int64_t L, int64_t H, int32_t derivs) {
   if (B <= 0 || L <= 0 || H <= 0) return 0;
-  const int64_t seg = segment_length(B, L, H);
-  return (L + seg - 1) / seg;
+  return shape_of(B, L, H, derivs != 0, nullptr, nullptr).n_seg;
 }
 
-extern "C" int64_t wa_decay_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D) {
+extern "C" int64_t wa_decay_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D, int32_t derivs) {
   if (B <= 0 || L <= 0 || H <= 0) return 0;
-  const Shape s = shape_of(B, L, H, nullptr, nullptr);
+  const Shape s = shape_of(B, L, H, derivs != 0, nullptr, nullptr);
   const int64_t parts = s.n_seg + D * D / kThreads + std::max(pair_groups(WA_F32, s), pair_groups(WA_BF16, s));
   return B * H * (s.n_seg * D * D * 4 + parts * 8);
 }
@@ -1273,7 +1325,7 @@ extern "C" int wa_decay_bwd(const wa_decay_bwd_args* a, void* stream) {
   WA_CHECK_ARG(a->B > 0 && a->L > 0 && a->H > 0, "decay_bwd: nothing to compute");
   WA_CHECK_ARG(a->q && a->k && a->v && a->dout && a->dq && a->dk && a->dv && a->log_decay && a->states && a->workspace,
                "decay_bwd: null tensor");
-  WA_CHECK_ARG(!a->dlog_decay || a->derivs, "decay_bwd: dlog_decay needs the forward's derivs");
+  WA_CHECK_ARG(!a->dlog_decay == !a->derivs, "decay_bwd: dlog_decay goes with the forward's derivs");
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype) &&
                rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh, a->dtype) &&
                wa_aligned16(a->states) && wa_aligned16(a->workspace) && wa_aligned16(a->dfinal) && wa_aligned16(a->dinitial),

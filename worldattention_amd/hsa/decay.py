@@ -29,7 +29,7 @@ def _forward(q, k, v, log_decay, initial, lengths, scale, want_derivs=False):
     f32 = dict(dtype=torch.float32, device=dev)
     out = torch.empty((bsz, length, heads, d), dtype=q.dtype, device=dev)
     final = torch.empty((bsz, heads, d, d), **f32)
-    n_seg = _lib.lib().wa_decay_segments(bsz, length, heads)
+    n_seg = _lib.lib().wa_decay_segments(bsz, length, heads, int(want_derivs))
     states = torch.empty((bsz, heads, n_seg, d, d), **f32)
     derivs = torch.empty((bsz, heads, n_seg + 1, d, d), **f32) if want_derivs else None
     args = _lib.DecayFwdArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), _lib.dtype_code(q), bsz, length,
@@ -62,7 +62,8 @@ class _DecayLinear(torch.autograd.Function):
         dq, dk, dv = (torch.empty((bsz, length, heads, d), dtype=q.dtype, device=dev) for _ in range(3))
         dinitial = torch.empty((bsz, heads, d, d), **f32) if ctx.needs_input_grad[4] else None
         dlog = torch.empty((heads,), **f32) if ctx.needs_input_grad[3] else None
-        ws = torch.empty((_lib.lib().wa_decay_bwd_workspace_bytes(bsz, length, heads, d),), dtype=torch.uint8, device=dev)
+        size = _lib.lib().wa_decay_bwd_workspace_bytes(bsz, length, heads, d, int(derivs is not None))
+        ws = torch.empty((size,), dtype=torch.uint8, device=dev)
         args = _lib.DecayBwdArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(dout), *_lib.blhd(dq),
                                  *_lib.blhd(dk), *_lib.blhd(dv), _lib.dtype_code(q), bsz, length, heads, d,
                                  log_decay.data_ptr(), _lib.ptr(lengths), states.data_ptr(), _lib.ptr(derivs), _lib.ptr(dfinal),
