@@ -82,6 +82,19 @@ def test_every_cache_length_the_choice_is_cut_for(nb):
         assert torch.equal(got.num.cpu(), num) and torch.equal(got.index.cpu(), index)
 
 
+@pytest.mark.parametrize("n,nb", [(1, 1024), (1, 1025), (8, 1024), (9, 1024), (15, 512), (16, 512), (17, 512), (16, 513), (40, 100)])
+def test_every_number_of_queries_the_choice_is_cut_for(n, nb):
+    """One launch or two, one query tile or several; the first queries before the sequence's first token."""
+    g = torch.Generator().manual_seed(n * nb)
+    sums = torch.randn(2, 2, nb, 128, generator=g).to(DEV)
+    q = torch.randn(2, n, 6, 128, generator=g).bfloat16().to(DEV)
+    for lens in ((nb * 64, nb * 32 + 7), (n - 1, 64 * 20), (0, 64 * 9 + 1)):
+        kv_len = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        got = W.select_key_blocks(q, sums, kv_len, block_size=64, topk=7, sink_blocks=2, local_blocks=2)
+        index, num = OT.select_key_blocks(q, sums, lens, block_size=64, topk=7, sink_blocks=2, local_blocks=2)
+        assert torch.equal(got.num.cpu(), num) and torch.equal(got.index.cpu(), index)
+
+
 @pytest.mark.parametrize("nb", [200, 800, 3000, 9000])
 def test_ties_infinities_and_nan_in_the_scores(nb):
     """Equal scores (few distinct values, zeros of both signs), infinite and NaN sums, long runs of ties."""

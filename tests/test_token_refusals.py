@@ -172,12 +172,15 @@ def test_selected_entry_points_refuse():
     a.B, a.n, a.H, a.Hk, a.D, a.block_size, a.n_blocks, a.topk, a.sink_blocks, a.local_blocks = 1, 1, 4, 3, 64, 64, 4, 4, 1, 1
     for field, bad, match in (("Hk", 3, b"heads"), ("D", 80, b"head dim"), ("block_size", 16, b"block size"), ("topk", 0, b"topk"),
                               ("n_blocks", 40000, b"blocks"), ("cap", 257, b"do not hold"), ("local_blocks", 4, b"local"),
-                              ("q", FAKE + 2, b"misaligned"), ("workspace", None, b"null")):
+                              ("q", FAKE + 2, b"misaligned"), ("index", None, b"null")):
         a.Hk = 2
         keep = getattr(a, field)
         setattr(a, field, bad)
         assert lib.wa_select_blocks(ctypes.byref(a), None) == _lib.WA_ERR_ARG and match in lib.wa_last_error(), field
         setattr(a, field, keep)
+    a.n, a.workspace = 17, None                              # more queries than one launch scores
+    assert lib.wa_select_blocks_workspace_bytes(1, 17, 2, 4) > 0
+    assert lib.wa_select_blocks(ctypes.byref(a), None) == _lib.WA_ERR_ARG and b"null" in lib.wa_last_error()
     s = _lib.SelectedAttnArgs()
     s.q = s.k = s.v = s.o = s.index = s.num = FAKE
     s.B, s.n, s.cap, s.H, s.Hk, s.D, s.block_size, s.topk = 1, 1, 4096, 4, 2, 64, 64, 64

@@ -20,86 +20,99 @@ __device__ __forceinline__ int64_t seen_tokens(const int32_t* kv_len, int64_t kv
 }
 
 // =============================================================================================
-// Scores: [B, n, Hk, n_blocks] fp64 = (sum of a group's queries) . (block's key sum). One wave takes 16
-// queries x 16 blocks at a time (v_mfma_f64_16x16x4): a query's sums and a key sum's products are
-// exact in fp64 to 2^-52 of the score, so the order of the products decides no choice. The sums are read
-// once; a decoding step fills one row of 16, which the fp64 matrix rate (one instruction per 256 bytes
-// read by a wave) still hides behind the read.
+// Scores: (sum of a group's queries) . (block's key sum) in fp64, 16 queries x 16 blocks at a time
+// (v_mfma_f64_16x16x4): a query's sums and a key sum's products are exact in fp64 to 2^-52 of the score,
+// so the order of the products decides no choice. The sums are read once; a decoding step fills one
+// row of 16, which the fp64 matrix rate still hides behind the read.
 // =============================================================================================
-struct ScoreParams {
+struct SelectParams {
   const bf16_t* q; int64_t q_sb, q_st, q_sh;
   const float* sums;
   const int32_t* kv_len; int64_t kv_len_all, cap;
-  int n, H, Hk, nb, bs, sink, local;
+  int n, H, Hk, nb, bs, topk, sink, local;
   int q_tiles, b_tiles, per;   // 16-query tiles; groups of `per` 16-block tiles
-  double* scores;
+  int64_t rows;
+  double* scores;              // [B, n, Hk, n_blocks]
+  int32_t* index; int32_t* num;
 };
 
+// The group's queries of 16-query tile `qt`, in contraction order: slot (step 4 i + j, lane group kg) is channel
+// 16 i + 4 kg + j on both sides.
 template <int D>
-__global__ void __launch_bounds__(64) score_kernel(ScoreParams p) {
+__device__ __forceinline__ void group_queries(const SelectParams& p, int b, int hk, int qt, int lane, double (&a)[D / 4]) {
+  const int qi = 16 * qt + (lane & 15), kg = lane >> 4, G = p.H / p.Hk;
+#pragma unroll
+  for (int i = 0; i < D / 4; ++i) a[i] = 0.0;
+  if (qi >= p.n) return;
+  const bf16_t* src = p.q + (int64_t)b * p.q_sb + (int64_t)qi * p.q_st + (int64_t)hk * G * p.q_sh + 4 * kg;
+  for (int g = 0; g < G; ++g) {
+    bf16x4 x[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) x[i] = *(const bf16x4*)(src + (int64_t)g * p.q_sh + 16 * i);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[4 * i + j] += (double)(float)x[i][j];
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void load_sums(const SelectParams& p, int64_t bh, int b0, int lane, f32x4 (&x)[D / 16]) {
+  const float* src = p.sums + (bh * p.nb + min(b0 + (lane & 15), p.nb - 1)) * D + 4 * (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) x[i] = *(const f32x4*)(src + 16 * i);
+}
+
+// Accumulator register r of lane (column block, kg) is query row kg + 4 r. Two chains, so that a product need
+// not wait for the one before it.
+template <int D>
+__device__ __forceinline__ f64x4 score_tile(const double (&a)[D / 4], const f32x4 (&x)[D / 16]) {
+  f64x4 acc[2] = {{0.0, 0.0, 0.0, 0.0}, {0.0, 0.0, 0.0, 0.0}};
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[4 * i + j], (double)x[i][j], acc[j & 1], 0, 0, 0);
+  return acc[0] + acc[1];
+}
+
+// Blocks that query i scores end here: from the first local one on they are chosen anyway.
+__device__ __forceinline__ int score_end(const SelectParams& p, int b, int i) {
+  return (int)((seen_tokens(p.kv_len, p.kv_len_all, p.cap, p.n, b, i) + p.bs - 1) / p.bs) - p.local;
+}
+
+template <int D>
+__global__ void __launch_bounds__(64) score_kernel(SelectParams p) {
   const int lane = threadIdx.x, row = lane & 15, kg = lane >> 4;
   int u = blockIdx.x;
   const int bt = u % p.b_tiles;
   u /= p.b_tiles;
-  const int qt = u % p.q_tiles, bh = u / p.q_tiles, b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk;
-  const int last = min(p.n, 16 * qt + 16) - 1;
-  // the blocks that the tile's last query scores: none from the first local one on
-  const int64_t seen = seen_tokens(p.kv_len, p.kv_len_all, p.cap, p.n, b, last);
-  const int end = (int)((seen + p.bs - 1) / p.bs) - p.local, begin = bt * p.per * 16;
+  const int qt = u % p.q_tiles, bh = u / p.q_tiles, b = bh / p.Hk, hk = bh % p.Hk;
+  const int end = score_end(p, b, min(p.n, 16 * qt + 16) - 1), begin = bt * p.per * 16;
   if (begin >= end) return;
-  // slot (step 4 i + j, lane group kg) of the contraction is channel 16 i + 4 kg + j on both sides
   double a[D / 4];
-  const int qi = 16 * qt + row;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    double s[4] = {0.0, 0.0, 0.0, 0.0};
-    if (qi < p.n) {
-      const bf16_t* src = p.q + (int64_t)b * p.q_sb + (int64_t)qi * p.q_st + (int64_t)hk * G * p.q_sh + 16 * i + 4 * kg;
-      for (int g = 0; g < G; ++g) {
-        const bf16x4 x = *(const bf16x4*)(src + (int64_t)g * p.q_sh);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] += (double)(float)x[j];
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) a[4 * i + j] = s[j];
-  }
-  for (int t = 0; t < p.per; ++t) {
-    const int b0 = begin + 16 * t;
-    if (b0 >= end) break;
-    const int blk = min(b0 + row, p.nb - 1);
-    const float* src = p.sums + ((int64_t)bh * p.nb + blk) * D + 4 * kg;
-    f32x4 x[D / 16];
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) x[i] = *(const f32x4*)(src + 16 * i);
-    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[4 * i + j], (double)x[i][j], acc, 0, 0, 0);
-    // accumulator register r of lane (column block, kg) is query row kg + 4 r
+  group_queries<D>(p, b, hk, qt, lane, a);
+  f32x4 x[2][D / 16];
+  load_sums<D>(p, bh, begin, lane, x[0]);
+  auto tile = [&](int b0, const f32x4 (&now)[D / 16], f32x4 (&next)[D / 16]) {
+    if (b0 + 16 < end) load_sums<D>(p, bh, b0 + 16, lane, next);
+    const f64x4 acc = score_tile<D>(a, now);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * qt + kg + 4 * r;
-      if (i < p.n && b0 + row < p.nb)
-        p.scores[(((int64_t)b * p.n + i) * p.Hk + hk) * p.nb + b0 + row] = acc[r];
+      if (i < p.n && b0 + row < p.nb) p.scores[(((int64_t)b * p.n + i) * p.Hk + hk) * p.nb + b0 + row] = acc[r];
     }
+  };
+  for (int t = 0; t < p.per && begin + 16 * t < end; t += 2) {
+    tile(begin + 16 * t, x[0], x[1]);
+    if (t + 1 < p.per && begin + 16 * (t + 1) < end) tile(begin + 16 * (t + 1), x[1], x[0]);
   }
 }
 
 // =============================================================================================
 // Choice: W waves hold a row's scores as order-preserving 64-bit keys, KPT a lane, and find the m-th
 // largest by bisection over the key's bits (counts by ballots), then write the chosen ids in
-// ascending order by prefix counts. W = 1: four rows a workgroup and no barrier.
+// ascending order by prefix counts.
 // =============================================================================================
-struct ChooseParams {
-  const double* scores;
-  const int32_t* kv_len; int64_t kv_len_all, cap;
-  int n, Hk, nb, bs, topk, sink, local;
-  int64_t rows;
-  int32_t* index; int32_t* num;
-};
-
 // Larger score, larger key; NaN above all, -0 as 0. Never 0, which stands for "not scored".
 __device__ __forceinline__ uint64_t score_key(double x) {
   if (x != x) return ~0ull;
@@ -107,13 +120,11 @@ __device__ __forceinline__ uint64_t score_key(double x) {
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-template <int W, int KPT>
-__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(ChooseParams p) {
-  __shared__ int counts[2][W];
-  const int lane = threadIdx.x & 63, w = W == 1 ? 0 : threadIdx.x >> 6;
-  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
-  if (row >= p.rows) return;   // whole waves (W = 1), never a part of a workgroup with barriers
-  const int i = (int)(row / p.Hk % p.n), b = (int)(row / p.Hk / p.n);
+// One row (query i of sequence b, key head hk) by waves 0 .. W - 1 of a workgroup, all of which call it; this is
+// wave w. score(j): the row's score of block j.
+template <int W, int KPT, typename Score>
+__device__ __forceinline__ void choose_row(const SelectParams& p, int b, int i, int hk, int w, int lane, int (*counts)[W], const Score& score) {
+  const int64_t row = ((int64_t)b * p.n + i) * p.Hk + hk;
   const int64_t seen = seen_tokens(p.kv_len, p.kv_len_all, p.cap, p.n, b, i);
   const int vis = (int)((seen + p.bs - 1) / p.bs), take = min(vis, p.topk);
   const int lo = min(p.sink, vis), hi = max(lo, vis - p.local);   // scored: [lo, hi)
@@ -125,7 +136,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(ChoosePar
   for (int e = 0; e < KPT; ++e) {
     const int j = first + 64 * e;
     key[e] = 0;
-    if (!all && j >= lo && j < hi) key[e] = score_key(p.scores[row * p.nb + j]);
+    if (!all && j >= lo && j < hi) key[e] = score_key(score(j));
   }
   int flip = 0;
   auto total = [&](int mine) {   // over the row's waves; mine is uniform in a wave
@@ -170,7 +181,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(ChoosePar
     flip ^= 1;
   }
   // bit e of `mine`: this lane's block first + 64 e is chosen
-  uint64_t mine = 0;
+  uint32_t mine = 0;
   int chosen = 0;
 #pragma unroll
   for (int e = 0; e < KPT; ++e) {
@@ -184,7 +195,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(ChoosePar
       tied += __popcll(t);
     }
     chosen += __popcll(__ballot(take_j));
-    mine |= (uint64_t)take_j << e;
+    mine |= (uint32_t)take_j << e;
   }
   int at = 0;
   if (W > 1) {
@@ -200,14 +211,63 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(ChoosePar
     if (mine_e) out[at + __popcll(t & below)] = first + 64 * e;
     at += __popcll(t);
   }
-  const int threads = W == 1 ? 64 : 64 * W, tid = W == 1 ? lane : (int)threadIdx.x;
-  for (int s = take + tid; s < p.topk; s += threads) out[s] = -1;
+  const int tid = 64 * w + lane;
+  for (int s = take + tid; s < p.topk; s += 64 * W) out[s] = -1;
   if (tid == 0) p.num[row] = take;
+}
+
+// W = 1: four rows a workgroup and no barrier.
+template <int W, int KPT>
+__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(SelectParams p) {
+  __shared__ int counts[2][W];
+  const int lane = threadIdx.x & 63;
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  if (row >= p.rows) return;   // whole waves (W = 1), never a part of a workgroup with barriers
+  const int hk = (int)(row % p.Hk), i = (int)(row / p.Hk % p.n), b = (int)(row / p.Hk / p.n);
+  choose_row<W, KPT>(p, b, i, hk, W == 1 ? 0 : threadIdx.x >> 6, lane, counts, [&](int j) { return p.scores[row * p.nb + j]; });
+}
+
+// Scores and choice of a few queries over a short cache in one launch: a workgroup per sequence and key head,
+// the scores in LDS. One launch and 8 bytes a score less; its CU reads the sums alone, so at most kFusedBlocks
+// blocks, and the queries' scores must fit. 32 sequences of up to 512 blocks x 8 key heads: FUSED us against SPLIT in
+// two launches; one sequence of 64 blocks: FUSED1 against SPLIT1.
+constexpr int kFusedBlocks = 1024, kFusedScores = 8192;
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) select_few_kernel(SelectParams p) {
+  __shared__ double sc[kFusedScores];
+  __shared__ int counts[2][4], one[2][1];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = lane & 15, kg = lane >> 4;
+  const int bh = blockIdx.x, b = bh / p.Hk, hk = bh % p.Hk;
+  const int end = score_end(p, b, p.n - 1);
+  if (p.nb > p.topk && 16 * w < end) {
+    double a[D / 4];
+    f32x4 x[2][D / 16];
+    load_sums<D>(p, bh, 16 * w, lane, x[0]);
+    group_queries<D>(p, b, hk, 0, lane, a);
+    auto tile = [&](int b0, const f32x4 (&now)[D / 16], f32x4 (&next)[D / 16]) {
+      if (b0 + 64 < end) load_sums<D>(p, bh, b0 + 64, lane, next);
+      const f64x4 acc = score_tile<D>(a, now);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (kg + 4 * r < p.n && b0 + row < p.nb) sc[(kg + 4 * r) * p.nb + b0 + row] = acc[r];
+    };
+    for (int b0 = 16 * w; b0 < end; b0 += 128) {
+      tile(b0, x[0], x[1]);
+      if (b0 + 64 < end) tile(b0 + 64, x[1], x[0]);
+    }
+  }
+  __syncthreads();
+  if (p.n == 1) {
+    choose_row<4, kFusedBlocks / 256>(p, b, 0, hk, w, lane, counts, [&](int j) { return sc[j]; });
+  } else {
+    for (int i = w; i < p.n; i += 4) choose_row<1, kFusedBlocks / 64>(p, b, i, hk, 0, lane, one, [&](int j) { return sc[i * p.nb + j]; });
+  }
 }
 
 // =============================================================================================
 // Attention. A workgroup takes up to 16 query heads of one (sequence, query, key head) over a part of
-// its block list; its four waves take 32-key tiles in turn, all in registers. Transposed products keep
+// its block list; its waves take 32-key tiles in turn, all in registers. Transposed products keep
 // every operand where it was loaded or computed:
 //   S^T (32 keys x 16 heads) = K Q^T: a lane holds 16 bytes of a key row;
 //   O^T (D x 16 heads) += V^T P^T: the accumulator's keys are the next product's contraction slots
@@ -239,12 +299,12 @@ template <int N> struct RowPart;     // N bf16 values of a value row
 template <> struct RowPart<8> { typedef bf16x8 type; };
 template <> struct RowPart<4> { typedef bf16x4 type; };
 
-template <int D>
-__global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
+template <int D, int NW>
+__global__ void __launch_bounds__(64 * NW) attend_kernel(AttnParams p) {
   constexpr int KC = D / 32, VC = D / 16;   // 32-channel steps of a key row; channels of a value row a lane holds
   typedef typename RowPart<VC>::type VRow;
-  __shared__ float sm[4][16], sl[4][16];
-  __shared__ float so[4][16][D + 4];
+  __shared__ float sm[NW][16], sl[NW][16];
+  __shared__ float so[NW][16][D + 4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, kg = lane >> 4;
   int64_t u = blockIdx.x;
   const int split = (int)(u % p.splits);
@@ -274,7 +334,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
 #pragma unroll
   for (int j = 0; j < VC; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int t = t0 + w; t < t1; t += 4) {
+  for (int t = t0 + w; t < t1; t += NW) {
     const int id = list[t / tpb];
     const int64_t key0 = (int64_t)id * p.bs + (t % tpb) * 32;
     if (id < 0 || key0 >= seen) continue;
@@ -312,7 +372,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     if (__any(top > m)) {
-      const float up = fmaxf(m, top), f = exp2f(m - up);
+      const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
       m = up;
       l *= f;
 #pragma unroll
@@ -326,7 +386,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
     bf16x8 pr;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = exp2f(s[e] - m);
+      const float x = __builtin_amdgcn_exp2f(s[e] - m);
       pr[e] = (bf16_t)x;
       l += x;
     }
@@ -347,18 +407,24 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(AttnParams p) {
     sl[w][l16] = l;
   }
   __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0][l16], sm[1][l16]), fmaxf(sm[2][l16], sm[3][l16])), f = exp2f(m - top);
+  auto highest = [&](int g) {
+    float x = sm[0][g];
+#pragma unroll
+    for (int y = 1; y < NW; ++y) x = fmaxf(x, sm[y][g]);
+    return x;
+  };
+  const float f = exp2f(m - highest(l16));
 #pragma unroll
   for (int j = 0; j < VC; ++j)
 #pragma unroll
     for (int r = 0; r < 4; ++r) so[w][l16][VC * (4 * kg + r) + j] = o[j][r] * f;
   __syncthreads();
-  for (int x = tid; x < heads * D; x += kThreads) {
+  for (int x = tid; x < heads * D; x += 64 * NW) {
     const int g = x / D, d = x % D;
-    const float tm = fmaxf(fmaxf(sm[0][g], sm[1][g]), fmaxf(sm[2][g], sm[3][g]));
+    const float tm = highest(g);
     float sum = 0.f, tl = 0.f;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+    for (int y = 0; y < NW; ++y) {
       sum += so[y][g][d];
       tl += sl[y][g] * exp2f(sm[y][g] - tm);
     }
@@ -406,11 +472,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p, int64_t un
   if (lane == 0 && p.lse) p.lse[((int64_t)b * p.H + h) * p.n + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * WA_LN2;
 }
 
-// Parts of a row: while the rows alone leave the GPU's 256 CUs short of two workgroups each, but not below
-// two tiles for each of a workgroup's waves.
+// Waves of an attention workgroup: eight where the rows are too few to give every SIMD two with four.
+int attn_waves(int64_t rows) { return rows < 512 ? 8 : 4; }
+
+// Parts of a row: while the rows alone leave CUs without a workgroup, but not below four tiles for each wave, since
+// the parts cost a second launch.
 int64_t attn_splits(int64_t rows, int64_t tiles) {
-  const int64_t want = rows > 0 ? (512 + rows - 1) / rows : 1;
-  return std::max<int64_t>(1, std::min<int64_t>(want, tiles / 8));
+  const int64_t want = rows > 0 ? 256 / rows : 1;
+  return std::max<int64_t>(1, std::min<int64_t>(want, tiles / (4 * attn_waves(rows))));
 }
 
 int check_lists(const char* what, int64_t B, int64_t n, int64_t H, int64_t Hk, int64_t D, int64_t bs, int64_t topk) {
@@ -423,8 +492,11 @@ int check_lists(const char* what, int64_t B, int64_t n, int64_t H, int64_t Hk, i
   return WA_OK;
 }
 
+// Whether one launch scores and chooses: at most 16 queries (one product tile) whose scores fit.
+bool fused(int64_t n, int64_t n_blocks) { return n <= 16 && n_blocks <= kFusedBlocks && n * n_blocks <= kFusedScores; }
+
 template <int W, int KPT>
-void launch_choose(const ChooseParams& p, hipStream_t s) {
+void launch_choose(const SelectParams& p, hipStream_t s) {
   const int64_t grid = W == 1 ? (p.rows + 3) / 4 : p.rows;
   hipLaunchKernelGGL((choose_kernel<W, KPT>), dim3((unsigned)grid), dim3(W == 1 ? 256 : 64 * W), 0, s, p);
 }
@@ -432,7 +504,7 @@ void launch_choose(const ChooseParams& p, hipStream_t s) {
 }  // namespace
 
 extern "C" int64_t wa_select_blocks_workspace_bytes(int64_t B, int64_t n, int64_t Hk, int64_t n_blocks) {
-  return B * n * Hk * n_blocks * 8;
+  return fused(n, n_blocks) ? 0 : B * n * Hk * n_blocks * 8;
 }
 
 extern "C" int wa_select_blocks(const wa_select_blocks_args* a, void* stream) {
@@ -446,35 +518,42 @@ extern "C" int wa_select_blocks(const wa_select_blocks_args* a, void* stream) {
   WA_CHECK_ARG(a->sink_blocks >= 0 && a->local_blocks >= 1 && a->sink_blocks <= a->topk && a->local_blocks <= a->topk - a->sink_blocks,
                "select_blocks: topk %lld must hold %lld sink and %lld (>= 1) local blocks", (long long)a->topk,
                (long long)a->sink_blocks, (long long)a->local_blocks);
-  WA_CHECK_ARG(a->q && a->k_sums && a->index && a->num && a->workspace, "select_blocks: null tensor");
+  WA_CHECK_ARG(a->q && a->k_sums && a->index && a->num && (a->workspace || fused(a->n, a->n_blocks)), "select_blocks: null tensor");
+  WA_CHECK_ARG(a->B * a->n * a->Hk <= INT32_MAX, "select_blocks: too many queries");
   WA_CHECK_ARG(wa_aligned16(a->k_sums) && wa_aligned16(a->workspace) && ((uintptr_t)a->q & 7) == 0 && a->q_sb % 4 == 0 &&
                a->q_st % 4 == 0 && a->q_sh % 4 == 0, "select_blocks: misaligned rows");
   const int64_t cap = a->cap ? a->cap : a->n_blocks * a->block_size;
   const int64_t rows = a->B * a->n * a->Hk;
   hipStream_t s = (hipStream_t)stream;
-  ScoreParams p{};
+  SelectParams p{};
   p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.sums = a->k_sums; p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.cap = cap;
   p.n = (int)a->n; p.H = (int)a->H; p.Hk = (int)a->Hk; p.nb = (int)a->n_blocks; p.bs = (int)a->block_size;
-  p.sink = (int)a->sink_blocks; p.local = (int)a->local_blocks;
+  p.topk = (int)a->topk; p.sink = (int)a->sink_blocks; p.local = (int)a->local_blocks;
+  p.rows = rows; p.index = a->index; p.num = a->num;
+  if (fused(a->n, a->n_blocks)) {
+    const dim3 grid((unsigned)(a->B * a->Hk));
+    if (a->D == 128) hipLaunchKernelGGL((select_few_kernel<128>), grid, dim3(kThreads), 0, s, p);
+    else hipLaunchKernelGGL((select_few_kernel<64>), grid, dim3(kThreads), 0, s, p);
+    return wa_launch_status("select_blocks");
+  }
   p.scores = (double*)a->workspace;
   p.q_tiles = (int)((a->n + 15) / 16);
   // a wave keeps its queries for up to 8 block tiles where the tiles are many
   const int64_t tiles = (a->n_blocks + 15) / 16, waves = a->B * a->Hk * p.q_tiles * tiles;
-  p.per = (int)std::max<int64_t>(1, std::min<int64_t>({8, tiles, waves / 2048}));
+  p.per = (int)std::max<int64_t>(1, std::min<int64_t>({8, tiles, waves / 4096}));
   p.b_tiles = (int)((tiles + p.per - 1) / p.per);
   const int64_t grid = a->B * a->Hk * p.q_tiles * p.b_tiles;
-  WA_CHECK_ARG(grid <= INT32_MAX && rows <= INT32_MAX, "select_blocks: too many queries");
+  WA_CHECK_ARG(grid <= INT32_MAX, "select_blocks: too many queries");
   if (a->n_blocks > a->topk) {   // otherwise every seen block is chosen
     if (a->D == 128) hipLaunchKernelGGL((score_kernel<128>), dim3((unsigned)grid), dim3(64), 0, s, p);
     else hipLaunchKernelGGL((score_kernel<64>), dim3((unsigned)grid), dim3(64), 0, s, p);
   }
-  const ChooseParams c{p.scores, a->kv_len, a->kv_len_all, cap, p.n, p.Hk, p.nb, p.bs, (int)a->topk, p.sink, p.local, rows, a->index, a->num};
-  if (p.nb <= 256) launch_choose<1, 4>(c, s);
-  else if (p.nb <= 1024) launch_choose<1, 16>(c, s);
-  else if (p.nb <= 4096) launch_choose<4, 16>(c, s);
-  else if (p.nb <= 16384) launch_choose<16, 16>(c, s);
-  else launch_choose<16, 32>(c, s);
+  if (p.nb <= 256) launch_choose<1, 4>(p, s);
+  else if (p.nb <= 1024) launch_choose<1, 16>(p, s);
+  else if (p.nb <= 4096) launch_choose<4, 16>(p, s);
+  else if (p.nb <= 16384) launch_choose<16, 16>(p, s);
+  else launch_choose<16, 32>(p, s);
   return wa_launch_status("select_blocks");
 }
 
@@ -511,8 +590,13 @@ extern "C" int wa_selected_attn(const wa_selected_attn_args* a, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(units * p.splits));
   const int64_t heads = a->B * a->n * a->H;
-  if (a->D == 128) hipLaunchKernelGGL((attend_kernel<128>), grid, dim3(kThreads), 0, s, p);
-  else hipLaunchKernelGGL((attend_kernel<64>), grid, dim3(kThreads), 0, s, p);
+  if (attn_waves(units) == 8) {
+    if (a->D == 128) hipLaunchKernelGGL((attend_kernel<128, 8>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((attend_kernel<64, 8>), grid, dim3(512), 0, s, p);
+  } else {
+    if (a->D == 128) hipLaunchKernelGGL((attend_kernel<128, 4>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attend_kernel<64, 4>), grid, dim3(256), 0, s, p);
+  }
   if (p.splits > 1) {
     if (a->D == 128) hipLaunchKernelGGL((join_kernel<128>), dim3((unsigned)((heads + 3) / 4)), dim3(kThreads), 0, s, p, heads);
     else hipLaunchKernelGGL((join_kernel<64>), dim3((unsigned)((heads + 3) / 4)), dim3(kThreads), 0, s, p, heads);

@@ -68,10 +68,11 @@ def _select(q, sums, kv_len, bs, topk, sink, local, cap) -> BlockSelection:
     num = torch.empty((bsz, n, hk), dtype=torch.int32, device=dev)
     if num.numel() == 0:
         return BlockSelection(index, num)
-    ws = torch.empty((_lib.lib().wa_select_blocks_workspace_bytes(bsz, n, hk, nb),), dtype=torch.uint8, device=dev)
+    size = _lib.lib().wa_select_blocks_workspace_bytes(bsz, n, hk, nb)
+    ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
     keep, len_ptr, len_all = _lengths(kv_len)
     args = _lib.SelectBlocksArgs(*_lib.blhd(q), sums.data_ptr(), nb, len_ptr, len_all, cap, bsz, n, heads, hk, d, bs, topk,
-                                 sink, local, index.data_ptr(), num.data_ptr(), ws.data_ptr())
+                                 sink, local, index.data_ptr(), num.data_ptr(), _lib.ptr(ws))
     _lib.launch("wa_select_blocks", args, dev)
     return BlockSelection(index, num)
 
