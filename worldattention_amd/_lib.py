@@ -340,6 +340,7 @@ HkvCopy = _struct("wa_hkv_copy", [
 ])
 
 ROPE_MAX_AXES, ROPE_MAX_DIM = 4, 1024
+RopeSections = c_int64 * ROPE_MAX_AXES
 
 RopeAxesArgs = _struct("wa_rope_axes_args", [
     ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
@@ -350,7 +351,7 @@ RopeAxesArgs = _struct("wa_rope_axes_args", [
     ("B", c_int64), ("L", c_int64), ("Hq", c_int64), ("Hk", c_int64), ("D", c_int64),
     ("positions", c_void_p), ("p_sb", c_int64), ("p_st", c_int64), ("p_sa", c_int64), ("pos_int64", c_int32),
     ("inv_freq", c_void_p),
-    ("n_axes", c_int64), ("sections", c_int64 * ROPE_MAX_AXES),
+    ("n_axes", c_int64), ("sections", RopeSections),
     ("interleaved", c_int32), ("inverse", c_int32),
 ])
 
@@ -487,25 +488,39 @@ def lib() -> ctypes.CDLL:
     return handle
 
 
+def _raise(name: str, rc: int) -> None:
+    msg = lib().wa_last_error().decode(errors="replace")
+    if rc == WA_ERR_IO:
+        raise OSError(f"{name}: {msg}")
+    if rc < 0:
+        raise ValueError(f"{name}: {msg}")
+    raise RuntimeError(f"{name} failed (hip error {rc}): {msg}")
+
+
 def call(name: str, *args) -> None:
     rc = getattr(lib(), name)(*args)
     if rc != 0:
-        msg = lib().wa_last_error().decode(errors="replace")
-        if rc == WA_ERR_IO:
-            raise OSError(f"{name}: {msg}")
-        if rc < 0:
-            raise ValueError(f"{name}: {msg}")
-        raise RuntimeError(f"{name} failed (hip error {rc}): {msg}")
+        _raise(name, rc)
+
+
+_BOUND: dict = {}
 
 
 def launch(name: str, args, dev: torch.device) -> None:
     """:func:`call` on ``dev``'s current stream, with ``dev`` made the current device around it (a kernel
-    launch takes the current device's)."""
-    if dev.index == torch.cuda.current_device():
-        call(name, args, torch.cuda.current_stream(dev).cuda_stream)
+    launch takes the current device's). The entry point is looked up once and the stream's handle taken
+    without a stream object: a single-token call's host time is mostly such things."""
+    fn = _BOUND.get(name)
+    if fn is None:
+        fn = _BOUND[name] = getattr(lib(), name)
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            call(name, args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _raise(name, rc)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -557,9 +572,10 @@ def heads_arg(t):
 
 def blhd(t: torch.Tensor):
     """(ptr, sb, st, sh) of a [B, L, H, C] tensor whose channel dim is contiguous."""
-    if t.stride(-1) != 1:
+    sb, st, sh, sc = t.stride()
+    if sc != 1:
         raise ValueError("channel dimension must be contiguous")
-    return t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
+    return t.data_ptr(), sb, st, sh
 
 
 def bhld(t: torch.Tensor):
@@ -573,7 +589,7 @@ def kernel_ready(t: torch.Tensor, dtype=torch.bfloat16, align_elems: int = 8) ->
     """Cast to ``dtype`` and make the channel dim contiguous with 16-byte aligned rows."""
     if t.dtype != dtype:
         t = t.to(dtype)
-    if t.stride(-1) != 1 or any(s % align_elems for s in t.stride()[:-1]) or t.data_ptr() % 16:
+    if not is_kernel_ready(t, dtype, align_elems):
         t = t.contiguous()
         if t.data_ptr() % 16 or any(s % align_elems for s in t.stride()[:-1]):
             t = t.clone(memory_format=torch.contiguous_format)
@@ -582,8 +598,13 @@ def kernel_ready(t: torch.Tensor, dtype=torch.bfloat16, align_elems: int = 8) ->
 
 def is_kernel_ready(t: torch.Tensor, dtype=torch.bfloat16, align_elems: int = 8) -> bool:
     """Whether :func:`kernel_ready` would return ``t`` itself (no cast, no copy)."""
-    return (t.dtype == dtype and t.stride(-1) == 1 and not any(s % align_elems for s in t.stride()[:-1])
-            and t.data_ptr() % 16 == 0)
+    *outer, inner = t.stride()
+    if t.dtype != dtype or inner != 1 or t.data_ptr() % 16:
+        return False
+    for s in outer:
+        if s % align_elems:
+            return False
+    return True
 
 
 _HEAD_CACHE: dict = {}

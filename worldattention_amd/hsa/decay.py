@@ -147,21 +147,22 @@ def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_dec
     dv = v.shape[-1]
     if d > 256 or dv > 256:
         raise ValueError(f"head dims must be at most 256, got {d} and {dv}")
-    if state.stride(-1) != 1 or (d > 1 and state.stride(-2) != dv):
+    s_sb, s_sh, s_row, s_col = state.stride()
+    if s_col != 1 or (d > 1 and s_row != dv):
         raise ValueError("the state's [D, Dv] matrices must be contiguous")
-    if (bsz > 1 and state.stride(0) == 0) or (heads > 1 and state.stride(1) == 0):
+    if (bsz > 1 and s_sb == 0) or (heads > 1 and s_sh == 0):
         raise ValueError("the state is updated in place: every sequence and head needs memory of its own")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or state.requires_grad):
         raise ValueError("decay_linear_step takes no gradient (decay_linear_attention does): call it under torch.no_grad()")
     dev = _lib.require_gpu(q, k, v, log_decay, state)
-    _lib.dtype_code(q)
+    dtype = _lib.dtype_code(q)
     out = torch.empty((bsz, length, heads, dv), dtype=q.dtype, device=dev)
     if out.numel() == 0 or d == 0:
         return out.zero_()
     q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
     log_decay = log_decay.contiguous()
-    args = _lib.DecayStepArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), _lib.dtype_code(q), bsz, length,
-                              heads, d, dv, log_decay.data_ptr(), state.data_ptr(), state.stride(0), state.stride(1),
-                              d ** -0.5 if scale is None else float(scale))
+    args = _lib.DecayStepArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), dtype, bsz, length, heads, d, dv,
+                              log_decay.data_ptr(), state.data_ptr(), s_sb, s_sh, d ** -0.5 if scale is None else float(scale))
     _lib.launch("wa_decay_step", args, dev)
     return out

@@ -34,7 +34,7 @@ def axis_frequencies(head_dim: int, axes: int = 3, theta: float = 10000.0, devic
 
 def _launch(q, k, positions, inv_freq, sections, interleaved, inverse):
     """Rotated copies of the tensors given (either may be None)."""
-    dev = _lib.require_gpu(q, k, positions, inv_freq)
+    dev = positions.device
     outs, fields = [], []
     for t in (q, k):
         if t is None:
@@ -47,11 +47,11 @@ def _launch(q, k, positions, inv_freq, sections, interleaved, inverse):
         fields += [src.data_ptr(), *src.stride()[:3], out.data_ptr(), *out.stride()[:3]]
     some = q if q is not None else k
     bsz, length, _, d = some.shape
+    places = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
     args = _lib.RopeAxesArgs(*fields, _lib.dtype_code(some), bsz, length, q.shape[2] if q is not None else 0,
-                             k.shape[2] if k is not None else 0, d, positions.data_ptr(),
-                             positions.stride(0) if positions.dim() == 3 else 0, positions.stride(-2),
-                             positions.stride(-1), int(positions.dtype == torch.int64), inv_freq.data_ptr(),
-                             len(sections), (_lib.c_int64 * _lib.ROPE_MAX_AXES)(*sections), int(interleaved), int(inverse))
+                             k.shape[2] if k is not None else 0, d, positions.data_ptr(), *places,
+                             positions.dtype == torch.int64, inv_freq.data_ptr(), len(sections),
+                             _lib.RopeSections(*sections), interleaved, inverse)
     _lib.launch("wa_rope_axes", args, dev)
     return outs
 
@@ -112,7 +112,8 @@ def rope_axes(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, 
     _lib.require_gpu(q, k, positions, inv_freq)
     _lib.dtype_code(q)
     inv_freq = inv_freq.double().contiguous()
+    interleaved = bool(interleaved)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RopeAxes.apply(q, k, positions, inv_freq, sections, bool(interleaved))
+        return _RopeAxes.apply(q, k, positions, inv_freq, sections, interleaved)
     out, k_out = _launch(q, k, positions, inv_freq, sections, interleaved, False)
     return out if k is None else (out, k_out)

@@ -47,7 +47,9 @@ def _check_query(q, kv_heads: int, bsz: int, d: int, block_size: int, kv_len: Kv
 
 
 def _no_gradient(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    if any([t.requires_grad for t in tensors]):
         raise ValueError("attention over selected cache blocks takes no gradient: call it under torch.no_grad(), or train "
                          "with block_sparse_attention(block_map=...)")
 
