@@ -847,7 +847,8 @@ int wa_select_blocks(const wa_select_blocks_args* args, void* stream);
  * tensors, fp32 statistics. index / num as above (any int32 lists: an id that names no seen block adds
  * nothing, one listed twice counts twice). A query that sees nothing gets 0 and a log-sum-exp of
  * -inf. Keys and values behind a sequence's end are not used, whatever they hold. k, v: BLHD
- * [B, cap, Hk, D] with 16-byte aligned rows; lse: fp32 [B, H, n] or NULL; block_size 64 or 128. */
+ * [B, cap, Hk, D] with 16-byte aligned rows at most 2^24 elements apart; lse: fp32 [B, H, n] or NULL;
+ * block_size 64 or 128. The workspace may be NULL where its size is 0 (in both calls). */
 int64_t wa_selected_attn_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t Hk, int64_t D, int64_t topk,
                                          int64_t block_size);
 typedef struct wa_selected_attn_args {

@@ -58,7 +58,8 @@ def _check_attention(out, lse, q, k, v, index, num, host, bs, scale=None):
 @pytest.mark.parametrize("b,n,h,hk,d,cap,topk,sink,local", [
     (1, 1, 1, 1, 64, 1, 1, 0, 1), (1, 1, 8, 2, 128, 1000, 4, 1, 2), (3, 1, 12, 12, 128, 2000, 6, 0, 1),
     (2, 5, 8, 1, 64, 1500, 5, 2, 1), (1, 33, 4, 2, 128, 700, 3, 1, 1), (2, 2, 20, 1, 64, 900, 8, 1, 1),
-    (1, 1, 48, 1, 128, 3000, 40, 1, 1), (4, 3, 6, 3, 128, 1300, 64, 3, 4), (1, 2, 5, 5, 64, 6000, 16, 1, 2)])
+    (1, 1, 48, 1, 128, 3000, 40, 1, 1), (4, 3, 6, 3, 128, 1300, 64, 3, 4), (1, 2, 5, 5, 64, 6000, 16, 1, 2),
+    (1, 130, 4, 4, 64, 500, 4, 1, 1), (2, 523, 4, 4, 128, 900, 4, 1, 1), (1, 1101, 8, 4, 64, 1200, 4, 1, 1)])
 def test_against_the_oracle(bs, b, n, h, hk, d, cap, topk, sink, local):
     """Ragged lengths: the whole cache, one token, none, around block ends, below the number of queries, past the cache."""
     cache, g = _cache(b, cap, hk, d, bs, seed=cap)

@@ -3,7 +3,7 @@
 // chosen blocks, for a decoding step, a few drafted tokens or a prompt chunk. No reference counterpart.
 #include <algorithm>
 
-#include "common.h"
+#include "tile.h"
 
 namespace {
 
@@ -233,48 +233,57 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(SelectPar
 // two launches; one sequence of 64 blocks: FUSED1 against SPLIT1.
 constexpr int kFusedBlocks = 1024, kFusedScores = 8192;
 
+constexpr int kFewWaves = 8;
+
 template <int D>
-__global__ void __launch_bounds__(kThreads) select_few_kernel(SelectParams p) {
+__global__ void __launch_bounds__(64 * kFewWaves) select_few_kernel(SelectParams p) {
   __shared__ double sc[kFusedScores];
-  __shared__ int counts[2][4], one[2][1];
+  __shared__ int counts[2][kFewWaves], one[2][1];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = lane & 15, kg = lane >> 4;
   const int bh = blockIdx.x, b = bh / p.Hk, hk = bh % p.Hk;
   const int end = score_end(p, b, p.n - 1);
   if (p.nb > p.topk && 16 * w < end) {
+    constexpr int STEP = 16 * kFewWaves;
     double a[D / 4];
     f32x4 x[2][D / 16];
     load_sums<D>(p, bh, 16 * w, lane, x[0]);
     group_queries<D>(p, b, hk, 0, lane, a);
     auto tile = [&](int b0, const f32x4 (&now)[D / 16], f32x4 (&next)[D / 16]) {
-      if (b0 + 64 < end) load_sums<D>(p, bh, b0 + 64, lane, next);
+      if (b0 + STEP < end) load_sums<D>(p, bh, b0 + STEP, lane, next);
       const f64x4 acc = score_tile<D>(a, now);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (kg + 4 * r < p.n && b0 + row < p.nb) sc[(kg + 4 * r) * p.nb + b0 + row] = acc[r];
     };
-    for (int b0 = 16 * w; b0 < end; b0 += 128) {
+    for (int b0 = 16 * w; b0 < end; b0 += 2 * STEP) {
       tile(b0, x[0], x[1]);
-      if (b0 + 64 < end) tile(b0 + 64, x[1], x[0]);
+      if (b0 + STEP < end) tile(b0 + STEP, x[1], x[0]);
     }
   }
   __syncthreads();
-  if (p.n == 1) {
-    choose_row<4, kFusedBlocks / 256>(p, b, 0, hk, w, lane, counts, [&](int j) { return sc[j]; });
+  // A wave a query; a single query with many blocks takes all waves.
+  if (p.n == 1 && p.nb > 256) {
+    choose_row<kFewWaves, kFusedBlocks / (64 * kFewWaves)>(p, b, 0, hk, w, lane, counts, [&](int j) { return sc[j]; });
   } else {
-    for (int i = w; i < p.n; i += 4) choose_row<1, kFusedBlocks / 64>(p, b, i, hk, 0, lane, one, [&](int j) { return sc[i * p.nb + j]; });
+    for (int i = w; i < p.n; i += kFewWaves) {
+      if (p.nb <= 256) choose_row<1, 4>(p, b, i, hk, 0, lane, one, [&](int j) { return sc[i * p.nb + j]; });
+      else choose_row<1, kFusedBlocks / 64>(p, b, i, hk, 0, lane, one, [&](int j) { return sc[i * p.nb + j]; });
+    }
   }
 }
 
 // =============================================================================================
-// Attention. A workgroup takes up to 16 query heads of one (sequence, query, key head) over a part of
-// its block list; its waves take 32-key tiles in turn, all in registers. Transposed products keep
-// every operand where it was loaded or computed:
+// Attention. WPR waves take up to 16 query heads of one (sequence, query, key head) over a part of its block
+// list, 32-key tiles in turn. Transposed products keep every operand where it was loaded or computed:
 //   S^T (32 keys x 16 heads) = K Q^T: a lane holds 16 bytes of a key row;
 //   O^T (D x 16 heads) += V^T P^T: the accumulator's keys are the next product's contraction slots
 //   (lane group kg, element e: key 16 (e / 4) + 4 kg + e % 4), and lane m's 16 bytes of those eight value
 //   rows, regrouped by channel, are rows d = D / 16 m + j of V^T for product j.
-// So keys and values are read once, straight into registers, with no LDS until the waves' partial
-// results meet. Bound by that read.
+// Values go straight into registers, whole rows at a time; keys pass through 8 KiB of LDS of the wave's own
+// by direct loads, whole rows too (loaded as operands, 64 bytes of 16 rows at a time, they took more than
+// twice the values' time: 1,024 queries x 8 key heads of 16 blocks 322 us against PROMPT). A tile's registers
+// are not doubled: with a second tile loaded ahead a SIMD holds fewer waves, and less is in flight.
+// Bound by reading the chosen keys and values: from HBM for a decoding step, from the caches for a prompt.
 // =============================================================================================
 struct AttnParams {
   const bf16_t* q; int64_t q_sb, q_st, q_sh;
@@ -286,7 +295,7 @@ struct AttnParams {
   const int32_t* kv_len; int64_t kv_len_all, cap;
   int n, H, Hk, topk, bs, g_tiles, splits;
   float scale2;      // scale / ln 2
-  float* part;       // [units][16][D + 2] fp32 of a split row
+  float* part;       // [rows][g_tiles][splits][16][D + 2] fp32 of split rows
 };
 
 __device__ __forceinline__ f32x4 mma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
@@ -295,23 +304,46 @@ __device__ __forceinline__ f32x4 mma16(const bf16x8& a, const bf16x8& b, const f
 
 constexpr float kLowest = -1e30f;   // running maximum before the first key: finite, so that no difference of it is NaN
 
+constexpr float kSlack = 8.f;
+
+// A lane's value combined over the four 16-lane groups (lanes of equal number in their group).
+template <typename Op>
+__device__ __forceinline__ float over_groups(float x, const Op& op) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float y = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ uint32_t half_word(const bf16x8& v, int i) { return __builtin_bit_cast(u32x4, v)[i]; }
+__device__ __forceinline__ uint32_t half_word(const bf16x4& v, int i) { return __builtin_bit_cast(u32x2, v)[i]; }
+
 template <int N> struct RowPart;     // N bf16 values of a value row
 template <> struct RowPart<8> { typedef bf16x8 type; };
 template <> struct RowPart<4> { typedef bf16x4 type; };
 
-template <int D, int NW>
-__global__ void __launch_bounds__(64 * NW) attend_kernel(AttnParams p) {
+template <int D, int WPR>
+__global__ void __launch_bounds__(WPR == 8 ? 512 : 256) attend_kernel(AttnParams p) {
+  constexpr int NW = WPR == 8 ? 8 : 4, ROWS = NW / WPR;   // waves and query rows of a workgroup
   constexpr int KC = D / 32, VC = D / 16;   // 32-channel steps of a key row; channels of a value row a lane holds
+  constexpr int CPR = D / 8, RPI = 64 / CPR, KI = 32 / RPI;   // 16-byte chunks of a row; rows and direct loads of a tile
+  constexpr int KBYTES = NW * 32 * D * 2, OBYTES = WPR == 1 ? 0 : NW * 16 * (D + 4) * 4;
   typedef typename RowPart<VC>::type VRow;
+  __shared__ __attribute__((aligned(1024))) char lds[KBYTES > OBYTES ? KBYTES : OBYTES];   // keys, then the waves' outputs
   __shared__ float sm[NW][16], sl[NW][16];
-  __shared__ float so[NW][16][D + 4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, kg = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, kg = lane >> 4;
+  const int wr = w % WPR;                   // the wave's number in its row
   int64_t u = blockIdx.x;
   const int split = (int)(u % p.splits);
   u /= p.splits;
   const int gt = (int)(u % p.g_tiles);
-  const int64_t row = u / p.g_tiles;        // (b, i, hk)
-  const int hk = (int)(row % p.Hk), i = (int)(row / p.Hk % p.n), b = (int)(row / p.Hk / p.n), G = p.H / p.Hk;
+  u /= p.g_tiles;
+  // neighbouring workgroups take the key heads in turn: with eight of them each XCD's L2 sees one head's cache
+  const int hk = (int)(u % p.Hk), groups = (p.n + ROWS - 1) / ROWS;
+  u /= p.Hk;
+  const int i = (int)(u % groups) * ROWS + w / WPR, b = (int)(u / groups), G = p.H / p.Hk;
+  if (i >= p.n) return;                     // a whole wave, where waves share nothing
+  const int64_t row = ((int64_t)b * p.n + i) * p.Hk + hk;
   const int heads = min(16, G - 16 * gt);
   const int64_t seen = seen_tokens(p.kv_len, p.kv_len_all, p.cap, p.n, b, i);
   const int tpb = p.bs / 32;                // tiles of a block
@@ -334,27 +366,60 @@ __global__ void __launch_bounds__(64 * NW) attend_kernel(AttnParams p) {
 #pragma unroll
   for (int j = 0; j < VC; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int t = t0 + w; t < t1; t += NW) {
-    const int id = list[t / tpb];
-    const int64_t key0 = (int64_t)id * p.bs + (t % tpb) * 32;
-    if (id < 0 || key0 >= seen) continue;
-    const int live = (int)min((int64_t)32, seen - key0);   // keys of the tile that are seen
-    bf16x8 k[2][KC];
-    VRow v[8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bf16_t* src = kb + (key0 + min(16 * h + l16, live - 1)) * p.k_st + 8 * kg;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) k[h][c] = *(const bf16x8*)(src + 32 * c);
+  // The ids of this wave's next 64 tiles sit in its lanes; a tile without seen tokens is passed over before its
+  // loads.
+  int ids = 0, ids_at = t1;     // first tile whose id is held
+  auto key_of = [&](int t) -> int64_t {   // the tile's first key, -1 if none of its tokens is seen
+    if (t >= ids_at + 64 * WPR || t < ids_at) {
+      ids_at = t;
+      const int mine = t + lane * WPR;
+      ids = mine < t1 ? list[mine / tpb] : -1;
     }
+    const int id = __builtin_amdgcn_readlane(ids, (t - ids_at) / WPR);
+    const int64_t key0 = (int64_t)id * p.bs + (t % tpb) * 32;
+    return id < 0 || key0 >= seen ? -1 : key0;
+  };
+  // Keys in LDS: 16-byte chunk c of row r in slot c ^ swizzle(r), so that 16 rows' chunks fall in all banks.
+  bf16_t* kt = (bf16_t*)lds + w * 32 * D;
+  auto swizzle = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+  int k_off[D == 128 ? 4 : 2];  // the lane's row and chunk in direct load i: the swizzle repeats every 16 rows
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = *(const VRow*)(vb + (key0 + min(16 * (e >> 2) + 4 * kg + (e & 3), live - 1)) * p.v_st + VC * l16);
+  for (int x = 0; x < (D == 128 ? 4 : 2); ++x) {
+    const int r = lane / CPR;
+    k_off[x] = (r * (int)p.k_st + ((lane % CPR) ^ swizzle(x * RPI + r)) * 8) * 2;
+  }
+  const uint32_t v_off = (uint32_t)(4 * kg * (int)p.v_st + VC * l16) * 2;
+
+  for (int t = t0 + wr; t < t1; t += WPR) {
+    const int64_t key0 = key_of(t);
+    if (key0 < 0) continue;
+    const int live = (int)min((int64_t)32, seen - key0);   // keys of the tile that are seen
+    VRow v[8];
+    const bf16_t* kr = kb + key0 * p.k_st;
+    const bf16_t* vr = vb + key0 * p.v_st;
+#pragma unroll
+    for (int x = 0; x < KI; ++x) {
+      const int r0 = x * RPI;   // rows from `live` on read as zeros
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(kr + (int64_t)r0 * p.k_st), (short)0, live > r0 ? ((live - r0 - 1) * (int)p.k_st + D) * 2 : 0, WA_BUF_DWORD3);
+      lds_dma16(rs, kt + r0 * D, k_off[x % (D == 128 ? 4 : 2)]);
+    }
+    if (live == 32) {           // rows at scalar addresses plus one lane offset
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = *(const VRow*)((const char*)(vr + (16 * (e >> 2) + (e & 3)) * p.v_st) + v_off);
+    } else {                    // past the last seen token its row again
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = *(const VRow*)(vr + min(16 * (e >> 2) + 4 * kg + (e & 3), live - 1) * p.v_st + VC * l16);
+    }
+    // the keys have landed (only the eight value loads were issued after theirs)
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     float s[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < KC; ++c) acc = mma16(k[h][c], q[c], acc);
+      for (int c = 0; c < KC; ++c)
+        acc = mma16(*(const bf16x8*)(kt + (16 * h + l16) * D + ((4 * c + kg) ^ swizzle(l16)) * 8), q[c], acc);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[4 * h + r] = acc[r] * p.scale2;
     }
@@ -366,12 +431,10 @@ __global__ void __launch_bounds__(64 * NW) attend_kernel(AttnParams p) {
           v[e] = VRow{};    // a weight of 0 does not silence an infinity
         }
     }
-    float top = s[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e]);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > m)) {
+    const float top = over_groups(fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))),
+                                  [](float a, float b) { return fmaxf(a, b); });
+    // the running maximum follows only when a score is 2^kSlack above it: weights of up to 2^kSlack are as exact
+    if (__any(top > m + kSlack)) {
       const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
       m = up;
       l *= f;
@@ -392,42 +455,17 @@ __global__ void __launch_bounds__(64 * NW) attend_kernel(AttnParams p) {
     }
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
-      bf16x8 vt;
+      u32x4 vt;     // channel j of the eight rows: halves of two rows side by side
 #pragma unroll
-      for (int e = 0; e < 8; ++e) vt[e] = v[e][j];
-      o[j] = mma16(vt, pr, o[j]);
+      for (int e = 0; e < 4; ++e)
+        vt[e] = __builtin_amdgcn_perm(half_word(v[2 * e + 1], j / 2), half_word(v[2 * e], j / 2), j % 2 ? 0x07060302 : 0x05040100);
+      o[j] = mma16(__builtin_bit_cast(bf16x8, vt), pr, o[j]);
     }
   }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  l = over_groups(l, [](float a, float b) { return a + b; });
 
-  // the waves' parts: each to the common maximum, then summed in wave order
-  if (kg == 0) {
-    sm[w][l16] = m;
-    sl[w][l16] = l;
-  }
-  __syncthreads();
-  auto highest = [&](int g) {
-    float x = sm[0][g];
-#pragma unroll
-    for (int y = 1; y < NW; ++y) x = fmaxf(x, sm[y][g]);
-    return x;
-  };
-  const float f = exp2f(m - highest(l16));
-#pragma unroll
-  for (int j = 0; j < VC; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) so[w][l16][VC * (4 * kg + r) + j] = o[j][r] * f;
-  __syncthreads();
-  for (int x = tid; x < heads * D; x += 64 * NW) {
-    const int g = x / D, d = x % D;
-    const float tm = highest(g);
-    float sum = 0.f, tl = 0.f;
-#pragma unroll
-    for (int y = 0; y < NW; ++y) {
-      sum += so[y][g][d];
-      tl += sl[y][g] * exp2f(sm[y][g] - tm);
-    }
+  // Channel VC (4 kg + r) + j of head l16 is register r of accumulator j.
+  auto finish = [&](int g, int d, float sum, float tm, float tl) {
     const int h = hk * G + 16 * gt + g;
     if (p.splits == 1) {
       p.o[(int64_t)b * p.o_sb + (int64_t)i * p.o_st + (int64_t)h * p.o_sh + d] = (bf16_t)(tl > 0.f ? sum / tl : (tl == 0.f ? 0.f : tl));
@@ -439,6 +477,52 @@ __global__ void __launch_bounds__(64 * NW) attend_kernel(AttnParams p) {
         at[0] = tm;
         at[1] = tl;
       }
+    }
+  };
+  if constexpr (WPR == 1) {
+    if (l16 < heads) {
+      const int h = hk * G + 16 * gt + l16;
+      const float inv = l > 0.f ? 1.f / l : l;   // 0 for a row without keys, NaN where the scores were
+      bf16_t* at = p.o + (int64_t)b * p.o_sb + (int64_t)i * p.o_st + (int64_t)h * p.o_sh;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        VRow x;
+#pragma unroll
+        for (int j = 0; j < VC; ++j) x[j] = (bf16_t)(o[j][r] * inv);
+        *(VRow*)(at + VC * (4 * kg + r)) = x;
+      }
+      if (kg == 0 && p.lse) p.lse[((int64_t)b * p.H + h) * p.n + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * WA_LN2;
+    }
+  } else {
+    // the waves' parts: each to the common maximum, then summed in wave order
+    float(*so)[16][D + 4] = (float(*)[16][D + 4])lds;
+    if (kg == 0) {
+      sm[w][l16] = m;
+      sl[w][l16] = l;
+    }
+    __syncthreads();
+    auto highest = [&](int g) {
+      float x = sm[0][g];
+#pragma unroll
+      for (int y = 1; y < NW; ++y) x = fmaxf(x, sm[y][g]);
+      return x;
+    };
+    const float f = exp2f(m - highest(l16));
+#pragma unroll
+    for (int j = 0; j < VC; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) so[w][l16][VC * (4 * kg + r) + j] = o[j][r] * f;
+    __syncthreads();
+    for (int x = tid; x < heads * D; x += 64 * NW) {
+      const int g = x / D, d = x % D;
+      const float tm = highest(g);
+      float sum = 0.f, tl = 0.f;
+#pragma unroll
+      for (int y = 0; y < NW; ++y) {
+        sum += so[y][g][d];
+        tl += sl[y][g] * exp2f(sm[y][g] - tm);
+      }
+      finish(g, d, sum, tm, tl);
     }
   }
 }
@@ -472,14 +556,15 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p, int64_t un
   if (lane == 0 && p.lse) p.lse[((int64_t)b * p.H + h) * p.n + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * WA_LN2;
 }
 
-// Waves of an attention workgroup: eight where the rows are too few to give every SIMD two with four.
-int attn_waves(int64_t rows) { return rows < 512 ? 8 : 4; }
+// Waves of a row: one where the rows alone fill the GPU (its list's ids and its ends are then paid once), else
+// four, and eight where the rows leave CUs empty.
+int waves_per_row(int64_t rows) { return rows >= 4096 ? 1 : rows >= 512 ? 4 : 8; }
 
 // Parts of a row: while the rows alone leave CUs without a workgroup, but not below four tiles for each wave, since
 // the parts cost a second launch.
 int64_t attn_splits(int64_t rows, int64_t tiles) {
   const int64_t want = rows > 0 ? 256 / rows : 1;
-  return std::max<int64_t>(1, std::min<int64_t>(want, tiles / (4 * attn_waves(rows))));
+  return std::max<int64_t>(1, std::min<int64_t>(want, tiles / (4 * waves_per_row(rows))));
 }
 
 int check_lists(const char* what, int64_t B, int64_t n, int64_t H, int64_t Hk, int64_t D, int64_t bs, int64_t topk) {
@@ -533,15 +618,15 @@ extern "C" int wa_select_blocks(const wa_select_blocks_args* a, void* stream) {
   p.rows = rows; p.index = a->index; p.num = a->num;
   if (fused(a->n, a->n_blocks)) {
     const dim3 grid((unsigned)(a->B * a->Hk));
-    if (a->D == 128) hipLaunchKernelGGL((select_few_kernel<128>), grid, dim3(kThreads), 0, s, p);
-    else hipLaunchKernelGGL((select_few_kernel<64>), grid, dim3(kThreads), 0, s, p);
+    if (a->D == 128) hipLaunchKernelGGL((select_few_kernel<128>), grid, dim3(64 * kFewWaves), 0, s, p);
+    else hipLaunchKernelGGL((select_few_kernel<64>), grid, dim3(64 * kFewWaves), 0, s, p);
     return wa_launch_status("select_blocks");
   }
   p.scores = (double*)a->workspace;
   p.q_tiles = (int)((a->n + 15) / 16);
   // a wave keeps its queries for up to 8 block tiles where the tiles are many
   const int64_t tiles = (a->n_blocks + 15) / 16, waves = a->B * a->Hk * p.q_tiles * tiles;
-  p.per = (int)std::max<int64_t>(1, std::min<int64_t>({8, tiles, waves / 4096}));
+  p.per = (int)std::max<int64_t>(1, std::min<int64_t>({8, tiles, waves / 2048}));
   p.b_tiles = (int)((tiles + p.per - 1) / p.per);
   const int64_t grid = a->B * a->Hk * p.q_tiles * p.b_tiles;
   WA_CHECK_ARG(grid <= INT32_MAX, "select_blocks: too many queries");
@@ -570,9 +655,12 @@ extern "C" int wa_selected_attn(const wa_selected_attn_args* a, void* stream) {
   if (rc != WA_OK) return rc;
   WA_CHECK_ARG(a->cap >= 1 && a->cap <= INT32_MAX, "selected_attn: bad cache of %lld tokens", (long long)a->cap);
   WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->index && a->num, "selected_attn: null tensor");
-  auto rows16 = [](const void* x, int64_t sb, int64_t st, int64_t sh) { return wa_aligned16(x) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0; };
-  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->k, a->k_sb, a->k_st, a->k_sh) && rows16(a->v, a->v_sb, a->v_st, a->v_sh),
-               "selected_attn: rows must be 16-byte aligned");
+  auto rows16 = [](const void* x, int64_t sb, int64_t st, int64_t sh) {
+    return wa_aligned16(x) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0 && st >= 0 && st <= (int64_t)1 << 24;
+  };
+  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->k, a->k_sb, a->k_st, a->k_sh) && rows16(a->v, a->v_sb, a->v_st, a->v_sh) &&
+               rows16(a->o, a->o_sb, a->o_st, a->o_sh),
+               "selected_attn: rows must be 16-byte aligned, tokens at most 2^24 elements apart");
   AttnParams p{};
   p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.k = (const bf16_t*)a->k; p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
@@ -588,14 +676,17 @@ extern "C" int wa_selected_attn(const wa_selected_attn_args* a, void* stream) {
   WA_CHECK_ARG(p.splits == 1 || p.part, "selected_attn: a launch of %lld rows needs a workspace", (long long)units);
   WA_CHECK_ARG(units * p.splits <= INT32_MAX && a->B * a->n * a->H <= INT32_MAX, "selected_attn: too many queries");
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)(units * p.splits));
+  const int wpr = waves_per_row(units), rows = wpr == 1 ? 4 : 1;   // waves of a row, rows of a workgroup
+  const dim3 grid((unsigned)(a->B * ((a->n + rows - 1) / rows) * a->Hk * p.g_tiles * p.splits));
   const int64_t heads = a->B * a->n * a->H;
-  if (attn_waves(units) == 8) {
-    if (a->D == 128) hipLaunchKernelGGL((attend_kernel<128, 8>), grid, dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((attend_kernel<64, 8>), grid, dim3(512), 0, s, p);
+  if (a->D == 128) {
+    if (wpr == 1) hipLaunchKernelGGL((attend_kernel<128, 1>), grid, dim3(256), 0, s, p);
+    else if (wpr == 4) hipLaunchKernelGGL((attend_kernel<128, 4>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attend_kernel<128, 8>), grid, dim3(512), 0, s, p);
   } else {
-    if (a->D == 128) hipLaunchKernelGGL((attend_kernel<128, 4>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((attend_kernel<64, 4>), grid, dim3(256), 0, s, p);
+    if (wpr == 1) hipLaunchKernelGGL((attend_kernel<64, 1>), grid, dim3(256), 0, s, p);
+    else if (wpr == 4) hipLaunchKernelGGL((attend_kernel<64, 4>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attend_kernel<64, 8>), grid, dim3(512), 0, s, p);
   }
   if (p.splits > 1) {
     if (a->D == 128) hipLaunchKernelGGL((join_kernel<128>), dim3((unsigned)((heads + 3) / 4)), dim3(kThreads), 0, s, p, heads);

@@ -116,9 +116,10 @@ def _check_cache(q, k, v) -> None:
         raise ValueError(f"cache k / v must be matching [B, cap, Hk, D] tensors, got {tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError(f"cache k / v must be bf16, got {k.dtype} and {v.dtype}")
-    if k.shape[1] < 1 or not (_lib.is_kernel_ready(k) and _lib.is_kernel_ready(v)):
-        raise ValueError("cache k / v must hold tokens, with contiguous channels in 16-byte aligned rows (a cache is read in "
-                         "place)")
+    if (k.shape[1] < 1 or not (_lib.is_kernel_ready(k) and _lib.is_kernel_ready(v))
+            or max(k.stride(1), v.stride(1)) > 1 << 24):
+        raise ValueError("cache k / v must hold tokens, with contiguous channels in 16-byte aligned rows at most 2^24 elements "
+                         "apart (a cache is read in place)")
 
 
 def select_key_blocks(q: torch.Tensor, k_block_sums: torch.Tensor, kv_len: KvLen, *, block_size: int, topk: int,
