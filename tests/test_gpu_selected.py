@@ -69,6 +69,15 @@ def test_against_the_oracle(bs, b, n, h, hk, d, cap, topk, sink, local):
     _check(q, cache, cap, topk, sink, local, scale=0.3)
 
 
+@pytest.mark.parametrize("b,hk,d", [(130, 4, 64), (128, 8, 64), (1024, 1, 128), (514, 8, 64)])
+def test_many_sequences_of_single_tokens(b, hk, d):
+    """Enough key heads that a row, and a choice, gets fewer waves."""
+    cache, g = _cache(b, 400, hk, d, 64, seed=b)
+    q = torch.randn(b, 1, 2 * hk, d, generator=g).bfloat16().to(DEV)
+    lens = torch.randint(0, 420, (b,), generator=g, dtype=torch.int32)
+    _check(q, cache, lens.to(DEV), 4, 1, 1)
+
+
 @pytest.mark.parametrize("nb", [1, 255, 256, 257, 1024, 1025, 4096, 4097, 16384, 16385, 32768])
 def test_every_cache_length_the_choice_is_cut_for(nb):
     """The choice alone, at the block counts where its launch changes."""
@@ -83,7 +92,8 @@ def test_every_cache_length_the_choice_is_cut_for(nb):
         assert torch.equal(got.num.cpu(), num) and torch.equal(got.index.cpu(), index)
 
 
-@pytest.mark.parametrize("n,nb", [(1, 1024), (1, 1025), (8, 1024), (9, 1024), (15, 512), (16, 512), (17, 512), (16, 513), (40, 100)])
+@pytest.mark.parametrize("n,nb", [(1, 1024), (1, 1025), (8, 1024), (9, 1024), (15, 512), (16, 512), (17, 512), (16, 513), (40, 100),
+                                  (8, 1000), (8, 1001)])
 def test_every_number_of_queries_the_choice_is_cut_for(n, nb):
     """One launch or two, one query tile or several; the first queries before the sequence's first token."""
     g = torch.Generator().manual_seed(n * nb)
@@ -164,6 +174,32 @@ def test_extreme_scores():
     mag, _ = OT.selected_attention(q, cache["k"], cache["v"].abs(), index, num, [cap], block_size=bs)
     assert ((out.cpu().double() - want).abs() <= U * mag + U * want.abs() + 2.0 ** -7 * mag).all()
     assert ((lse.cpu().double() - want_lse).abs() <= 2.0 ** -7).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 4200])
+def test_scores_far_below_zero_are_no_empty_rows(n):
+    """All of a row's scores near -10^33 (bf16 reaches 10^38): the largest still gets the weight, whatever number of waves
+    and parts a row has."""
+    cap, bs = 2048, 64
+    g = torch.Generator().manual_seed(12)
+    k = torch.zeros(1, cap, 1, 64)
+    k[..., 0] = -1e32 * (2 + torch.randperm(cap, generator=g).view(1, cap, 1) / cap)
+    k = k.bfloat16()
+    v = torch.randn(1, cap, 1, 64, generator=g).bfloat16()
+    best = k[0, :, 0, 0].argmax().item()
+    k[0, best, 0, 0] = -1e32       # the only one of its value
+    q = torch.zeros(1, n, 2, 64, dtype=torch.bfloat16)
+    q[..., 0] = 80
+    index = torch.arange(32, dtype=torch.int32).expand(1, n, 1, 32).contiguous()
+    num = torch.full((1, n, 1), 32, dtype=torch.int32)
+    num[0, n // 2:] = best // bs + 1
+    # every query's own token lies behind the best one's
+    lens = cap + n - 1
+    out, lse = W.selected_attention(q.to(DEV), torch.cat((k, k[:, :0].new_full((1, n - 1, 1, 64), -3e38)), 1).to(DEV),
+                                    torch.cat((v, v.new_zeros(1, n - 1, 1, 64)), 1).to(DEV), index.to(DEV), num.to(DEV), lens, block_size=bs)
+    assert torch.equal(out.cpu(), v[:, best].view(1, 1, 1, 64).expand_as(out))
+    want = 80 * k[0, best, 0, 0].double() / 8
+    assert ((lse.cpu().double() - want).abs() <= 2.0 ** -20 * want.abs()).all()
 
 
 def test_long_cache_addresses_past_32_bits():

@@ -229,21 +229,22 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(SelectPar
 
 // Scores and choice of a few queries over a short cache in one launch: a workgroup per sequence and key head,
 // the scores in LDS. One launch and 8 bytes a score less; its CU reads the sums alone, so at most kFusedBlocks
-// blocks, and the queries' scores must fit. 32 sequences of up to 512 blocks x 8 key heads: FUSED us against SPLIT in
-// two launches; one sequence of 64 blocks: FUSED1 against SPLIT1.
-constexpr int kFusedBlocks = 1024, kFusedScores = 8192;
+// blocks. 32 sequences of up to 512 blocks x 8 key heads: 22.7 us against 19.8 + 13.6 in two launches; one sequence of
+// 64 blocks: 9.9 against 5.8 + 4.4, and a launch less for the host. The time of few workgroups is a wave's, so
+// eight share the blocks; two where workgroups wait for CUs (8 key heads, 8 waves against 2: 32 sequences 23 us
+// against 36, 64 of 128 blocks 18 against 18, 128 of them 31 against 22, 512 of 32 blocks 80 against 39).
+constexpr int kFusedBlocks = 1024, kFusedScores = 8000;   // the scores within 64 KiB
+constexpr int64_t kManyHeads = 1024;
 
-constexpr int kFewWaves = 8;
-
-template <int D>
-__global__ void __launch_bounds__(64 * kFewWaves) select_few_kernel(SelectParams p) {
-  __shared__ double sc[kFusedScores];
-  __shared__ int counts[2][kFewWaves], one[2][1];
+template <int D, int W>
+__global__ void __launch_bounds__(64 * W) select_few_kernel(SelectParams p) {
+  extern __shared__ double sc[];   // [n, n_blocks]
+  __shared__ int counts[2][W], one[2][1];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = lane & 15, kg = lane >> 4;
   const int bh = blockIdx.x, b = bh / p.Hk, hk = bh % p.Hk;
   const int end = score_end(p, b, p.n - 1);
   if (p.nb > p.topk && 16 * w < end) {
-    constexpr int STEP = 16 * kFewWaves;
+    constexpr int STEP = 16 * W;
     double a[D / 4];
     f32x4 x[2][D / 16];
     load_sums<D>(p, bh, 16 * w, lane, x[0]);
@@ -263,9 +264,9 @@ __global__ void __launch_bounds__(64 * kFewWaves) select_few_kernel(SelectParams
   __syncthreads();
   // A wave a query; a single query with many blocks takes all waves.
   if (p.n == 1 && p.nb > 256) {
-    choose_row<kFewWaves, kFusedBlocks / (64 * kFewWaves)>(p, b, 0, hk, w, lane, counts, [&](int j) { return sc[j]; });
+    choose_row<W, kFusedBlocks / (64 * W)>(p, b, 0, hk, w, lane, counts, [&](int j) { return sc[j]; });
   } else {
-    for (int i = w; i < p.n; i += kFewWaves) {
+    for (int i = w; i < p.n; i += W) {
       if (p.nb <= 256) choose_row<1, 4>(p, b, i, hk, 0, lane, one, [&](int j) { return sc[i * p.nb + j]; });
       else choose_row<1, kFusedBlocks / 64>(p, b, i, hk, 0, lane, one, [&](int j) { return sc[i * p.nb + j]; });
     }
@@ -281,9 +282,11 @@ __global__ void __launch_bounds__(64 * kFewWaves) select_few_kernel(SelectParams
 //   rows, regrouped by channel, are rows d = D / 16 m + j of V^T for product j.
 // Values go straight into registers, whole rows at a time; keys pass through 8 KiB of LDS of the wave's own
 // by direct loads, whole rows too (loaded as operands, 64 bytes of 16 rows at a time, they took more than
-// twice the values' time: 1,024 queries x 8 key heads of 16 blocks 322 us against PROMPT). A tile's registers
-// are not doubled: with a second tile loaded ahead a SIMD holds fewer waves, and less is in flight.
-// Bound by reading the chosen keys and values: from HBM for a decoding step, from the caches for a prompt.
+// twice the values' time: 1,024 queries x 8 key heads of 16 blocks 322 us against 245, both with WPR 4). A
+// tile's registers are not doubled: with a second tile loaded ahead a SIMD holds fewer waves, and less is in
+// flight (503 us). Bound by reading the chosen keys and values from HBM for a decoding step (32 ragged
+// sequences x 32 blocks 43 us), and by a tile's instructions for a prompt, whose blocks the caches hold (190 us
+// with WPR 1, 170 with no loads at all).
 // =============================================================================================
 struct AttnParams {
   const bf16_t* q; int64_t q_sb, q_st, q_sh;
@@ -302,9 +305,9 @@ __device__ __forceinline__ f32x4 mma16(const bf16x8& a, const bf16x8& b, const f
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-constexpr float kLowest = -1e30f;   // running maximum before the first key: finite, so that no difference of it is NaN
+constexpr float kLowest = -3.4028234e38f;   // running maximum before the first key: below every score, and no difference of it is NaN
 
-constexpr float kSlack = 8.f;
+constexpr float kSlack = 8.f;       // log2 of the growth that the running maximum lets pass
 
 // A lane's value combined over the four 16-lane groups (lanes of equal number in their group).
 template <typename Op>
@@ -556,15 +559,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p, int64_t un
   if (lane == 0 && p.lse) p.lse[((int64_t)b * p.H + h) * p.n + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * WA_LN2;
 }
 
-// Waves of a row: one where the rows alone fill the GPU (its list's ids and its ends are then paid once), else
-// four, and eight where the rows leave CUs empty.
-int waves_per_row(int64_t rows) { return rows >= 4096 ? 1 : rows >= 512 ? 4 : 8; }
+// Waves of a row: one where the rows alone fill the GPU (a list's ids and a row's ends are then paid once, and no
+// barrier), else four, and eight where the rows leave CUs empty. One wave against four against eight, us: 8,192 rows of
+// 16 blocks 194 / 246 / 339, 2,048 98 / 72 / 92, 1,024 46 / 38 / 48; 512 of 32 108 / 87 / 88, 256 - / 43 / 43,
+// 8 of 16 (with parts) - / 14.8 / 10.3. One-wave rows share a workgroup by query, so single queries take four (4,096
+// rows 282 / 288).
+int waves_per_row(int64_t rows, int64_t n) { return rows >= 4096 && n >= 4 ? 1 : rows >= 512 ? 4 : 8; }
 
 // Parts of a row: while the rows alone leave CUs without a workgroup, but not below four tiles for each wave, since
 // the parts cost a second launch.
 int64_t attn_splits(int64_t rows, int64_t tiles) {
   const int64_t want = rows > 0 ? 256 / rows : 1;
-  return std::max<int64_t>(1, std::min<int64_t>(want, tiles / (4 * waves_per_row(rows))));
+  return std::max<int64_t>(1, std::min<int64_t>(want, tiles / (4 * 8)));
 }
 
 int check_lists(const char* what, int64_t B, int64_t n, int64_t H, int64_t Hk, int64_t D, int64_t bs, int64_t topk) {
@@ -618,13 +624,20 @@ extern "C" int wa_select_blocks(const wa_select_blocks_args* a, void* stream) {
   p.rows = rows; p.index = a->index; p.num = a->num;
   if (fused(a->n, a->n_blocks)) {
     const dim3 grid((unsigned)(a->B * a->Hk));
-    if (a->D == 128) hipLaunchKernelGGL((select_few_kernel<128>), grid, dim3(64 * kFewWaves), 0, s, p);
-    else hipLaunchKernelGGL((select_few_kernel<64>), grid, dim3(64 * kFewWaves), 0, s, p);
+    const size_t scores = (size_t)(a->n * a->n_blocks * 8);
+    if (a->B * a->Hk >= kManyHeads) {
+      if (a->D == 128) hipLaunchKernelGGL((select_few_kernel<128, 2>), grid, dim3(128), scores, s, p);
+      else hipLaunchKernelGGL((select_few_kernel<64, 2>), grid, dim3(128), scores, s, p);
+    } else {
+      if (a->D == 128) hipLaunchKernelGGL((select_few_kernel<128, 8>), grid, dim3(512), scores, s, p);
+      else hipLaunchKernelGGL((select_few_kernel<64, 8>), grid, dim3(512), scores, s, p);
+    }
     return wa_launch_status("select_blocks");
   }
   p.scores = (double*)a->workspace;
   p.q_tiles = (int)((a->n + 15) / 16);
-  // a wave keeps its queries for up to 8 block tiles where the tiles are many
+  // A wave keeps its queries for up to 8 block tiles where the tiles are many, and takes one while waves are few
+  // (one against eight: 1,024 queries x 8 heads x 256 blocks 54 us against 30, 128 queries 10 against 18).
   const int64_t tiles = (a->n_blocks + 15) / 16, waves = a->B * a->Hk * p.q_tiles * tiles;
   p.per = (int)std::max<int64_t>(1, std::min<int64_t>({8, tiles, waves / 2048}));
   p.b_tiles = (int)((tiles + p.per - 1) / p.per);
@@ -676,7 +689,7 @@ extern "C" int wa_selected_attn(const wa_selected_attn_args* a, void* stream) {
   WA_CHECK_ARG(p.splits == 1 || p.part, "selected_attn: a launch of %lld rows needs a workspace", (long long)units);
   WA_CHECK_ARG(units * p.splits <= INT32_MAX && a->B * a->n * a->H <= INT32_MAX, "selected_attn: too many queries");
   hipStream_t s = (hipStream_t)stream;
-  const int wpr = waves_per_row(units), rows = wpr == 1 ? 4 : 1;   // waves of a row, rows of a workgroup
+  const int wpr = waves_per_row(units, a->n), rows = wpr == 1 ? 4 : 1;   // waves of a row, rows of a workgroup
   const dim3 grid((unsigned)(a->B * ((a->n + rows - 1) / rows) * a->Hk * p.g_tiles * p.splits));
   const int64_t heads = a->B * a->n * a->H;
   if (a->D == 128) {
