@@ -106,11 +106,16 @@ def test_decay_entry_points_refuse():
     assert lib.wa_decay_fwd(ctypes.byref(f), None) == _lib.WA_ERR_ARG and b"head dim" in lib.wa_last_error()
     f.D, f.q = 64, FAKE + 2
     assert lib.wa_decay_fwd(ctypes.byref(f), None) == _lib.WA_ERR_ARG and b"aligned" in lib.wa_last_error()
-    f.q, f.L = FAKE, 0
+    f.q, f.o_st = FAKE, 3
+    assert lib.wa_decay_fwd(ctypes.byref(f), None) == _lib.WA_ERR_ARG and b"aligned" in lib.wa_last_error()
+    f.o_st, f.L = 0, 0
     assert lib.wa_decay_fwd(ctypes.byref(f), None) == _lib.WA_ERR_ARG and b"nothing" in lib.wa_last_error()
     b = _lib.DecayBwdArgs()
     b.B, b.L, b.H, b.D, b.dtype = 1, 4, 2, 64, _lib.WA_F32
     assert lib.wa_decay_bwd(ctypes.byref(b), None) == _lib.WA_ERR_ARG and b"null" in lib.wa_last_error()
+    b.q = b.k = b.v = b.dout = b.dk = b.dv = b.log_decay = b.states = b.workspace = FAKE
+    b.dq = FAKE + 4
+    assert lib.wa_decay_bwd(ctypes.byref(b), None) == _lib.WA_ERR_ARG and b"aligned" in lib.wa_last_error()
     s = _lib.DecayStepArgs()
     s.B, s.L, s.H, s.D, s.Dv, s.dtype = 1, 1, 2, 300, 64, _lib.WA_F32
     assert lib.wa_decay_step(ctypes.byref(s), None) == _lib.WA_ERR_ARG and b"1 .. 256" in lib.wa_last_error()

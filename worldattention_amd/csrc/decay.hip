@@ -506,8 +506,10 @@ __device__ __forceinline__ void load_weights(const float* wt, int c, int g, floa
 // A segment's own state. Wave (ch, half) of D / 16 waves: columns 32 ch .. + 31 over all rows, from half of each
 // chunk's tokens (the two halves meet in LDS at the end): every weighted operand is then cut once a workgroup.
 // It enters in three parts, so the state carries no rounding but its fp32 sums'. The state decays once in two
-// chunks, whose tokens' weights run to the end of the two. 32,760 tokens of 12 x 128: 53 us, with derivatives
-// 75 (a wave a half of the rows, cutting twice, decaying every chunk: 99); 200 MB at a copy's rate are 41.
+// chunks, whose tokens' weights run to the end of the two. 32,760 tokens of 12 x 128: 51 us in 21 segments, 41 of
+// them what its 200 MB take at a copy's rate; with derivatives in 64 segments 101, and 117 in the backward pass,
+// which multiplies them with the forward's. A wave a half of the rows, cutting twice, decaying every chunk: 99
+// without derivatives.
 constexpr int kSpan = 2 * kChunk;
 
 template <int D, bool DERIV>
@@ -669,7 +671,8 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
 // place, and the keys and values of the unit stream through a ring of two 64-token stages that serve the rows
 // behind them and the state at once. Work a unit, not a chunk, pays for the state: with a state read and
 // rewritten every 64 tokens (two waves a tile, no LDS copy) the vector instructions were 2,600 a wave and unit
-// and the launch took 235 us at 32,760 tokens of 12 x 128.
+// and the launch took 235 us at 32,760 tokens of 12 x 128; it takes 127, the three gradients in one launch
+// 398. Bound by its instructions: the ring and X^T fill a CU's LDS, so one workgroup runs at a time.
 template <int D>
 __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) {
   constexpr int NW = D / 16, CT = D / 32, KS = D / 16, STAGES = 2, UNIT = 32 * NW;
@@ -913,9 +916,10 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
 // Pairs: a workgroup takes 256 rows i of a segment, its four waves two 32-row tiles each (w and 7 - w, which
 // share the causal work evenly), whose queries and output gradients stay in registers as operands; the
 // segment's keys and values up to the rows pass through a ring of two LDS stages, each operand read
-// serving both tiles (with one tile a wave the LDS reads took as long as the products: 256 us against 168 at
-// 32,760 tokens of 12 x 128). Tiles before the diagonal separate: with e the tile's last token,
-// (i - j) lambda^(i - j) = lambda^(i - e) [(i - e) + (e - j)] lambda^(e - j), no power above 1.
+// serving both tiles. 32,760 tokens of 12 x 128 in 64 segments: 117 us, 0.44 PFLOP/s of the products' causal
+// half; bound by the instructions that decay, mask and multiply the two score tiles. Tiles before the diagonal
+// separate: with e the tile's last token, (i - j) lambda^(i - j) = lambda^(i - e) [(i - e) + (e - j)] lambda^(e - j),
+// no power above 1.
 constexpr int kPairRows = 256;
 
 template <int D>
@@ -949,7 +953,8 @@ __global__ void __launch_bounds__(256, 2) pairs_bf16_kernel(PairsParams p) {
   TileReads<D> rd;
   rd.init(lane);
   // The rows' operands come through the stages too (the four hold 256 rows), in whole lines: read straight
-  // into registers, 32 bytes of 32 rows at a time, they took 14 us of a workgroup's 60.
+  // into registers, 32 bytes of 32 rows at a time, they took 14 us of a workgroup's 60 (260 us against 231 in 21
+  // segments of the size above).
   bf16x8 q[2][KS], d[2][KS];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
@@ -1312,8 +1317,8 @@ extern "C" int wa_decay_fwd(const wa_decay_fwd_args* a, void* stream) {
   WA_CHECK_ARG(a->B > 0 && a->L > 0 && a->H > 0, "decay_fwd: nothing to compute");
   WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->log_decay && a->states, "decay_fwd: null tensor");
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype) &&
-               rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype) && wa_aligned16(a->states) && wa_aligned16(a->initial) &&
-               wa_aligned16(a->final_state), "decay_fwd: rows and states must be 16-byte aligned, tokens at most 2^23 elements apart");
+               rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype) && rows16(a->o, a->o_sb, a->o_st, a->o_sh, a->dtype) &&
+               wa_aligned16(a->states) && wa_aligned16(a->initial) && wa_aligned16(a->final_state), "decay_fwd: rows and states must be 16-byte aligned, tokens at most 2^23 elements apart");
   hipStream_t s = (hipStream_t)stream;
   return a->D == 128 ? run_fwd<128>(a, s) : run_fwd<64>(a, s);
 }
@@ -1328,6 +1333,8 @@ extern "C" int wa_decay_bwd(const wa_decay_bwd_args* a, void* stream) {
   WA_CHECK_ARG(!a->dlog_decay == !a->derivs, "decay_bwd: dlog_decay goes with the forward's derivs");
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype) &&
                rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh, a->dtype) &&
+               rows16(a->dq, a->dq_sb, a->dq_st, a->dq_sh, a->dtype) && rows16(a->dk, a->dk_sb, a->dk_st, a->dk_sh, a->dtype) &&
+               rows16(a->dv, a->dv_sb, a->dv_st, a->dv_sh, a->dtype) &&
                wa_aligned16(a->states) && wa_aligned16(a->workspace) && wa_aligned16(a->dfinal) && wa_aligned16(a->dinitial),
                "decay_bwd: rows, states and workspace must be 16-byte aligned, tokens at most 2^23 elements apart");
   hipStream_t s = (hipStream_t)stream;

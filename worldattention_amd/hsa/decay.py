@@ -101,7 +101,8 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
 
     Outputs have the inputs' dtype; the state is summed in fp32. Differentiable once, through both results, in
     ``q``, ``k``, ``v``, ``log_decay`` and ``initial_state``. A value that is not finite in ``v`` (or, backwards,
-    in the gradient) reaches its 64-token neighbourhood, as it reaches a tile of softmax attention.
+    in the gradient) reaches its 64-token neighbourhood, as it reaches a tile of softmax attention. To capture a
+    backward pass in a graph, capture its forward pass too, and let no eager graph of the same leaves live then.
     """
     _check(q, k, v, log_decay, initial_state, "initial_state")
     bsz, length, heads, d = q.shape
@@ -111,11 +112,11 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
         raise ValueError(f"lengths must be int32 [{bsz}], got {lengths.dtype} {tuple(lengths.shape)}")
     dev = _lib.require_gpu(q, k, v, log_decay, initial_state, lengths)
     _lib.dtype_code(q)
-    scale = d ** -0.5 if scale is None else float(scale)
+    scale = max(d, 1) ** -0.5 if scale is None else float(scale)
     if q.numel() == 0 or v.numel() == 0:
         state = (torch.zeros((bsz, heads, d, dv), dtype=torch.float32, device=dev) if initial_state is None
                  else initial_state.clone())
-        return v.new_zeros(v.shape), state
+        return v.clone() if v.numel() == 0 else v.new_zeros(v.shape), state
     if d != dp:
         q, k = (torch.nn.functional.pad(t, (0, dp - d)) for t in (q, k))
     if dv != dp:
@@ -140,8 +141,9 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
 def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, *,
                       scale: Optional[float] = None) -> torch.Tensor:
     """The recurrence for single tokens: ``[B, L, H, D]`` with ``L`` 1 (or a few, one after the other), ``state``
-    ``[B, H, D, Dv]`` fp32 updated in place, outputs ``[B, L, H, Dv]`` returned. Head dims up to 256. Not
-    differentiable: inputs that ask for a gradient are refused while gradients are enabled."""
+    ``[B, H, D, Dv]`` fp32 updated in place (sequences and heads in memory of their own), outputs ``[B, L, H, Dv]``
+    returned. Head dims up to 256. Not differentiable: inputs that ask for a gradient are refused while gradients
+    are enabled."""
     _check(q, k, v, log_decay, state, "state")
     bsz, length, heads, d = q.shape
     dv = v.shape[-1]

@@ -86,7 +86,8 @@ def rope_axes(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, 
       ``(p, p + P)``.
 
     bf16 or fp32; angles in fp64, rotation in fp32, one rounding. Returns new contiguous tensors (``q``'s,
-    or ``(q, k)``'s). Differentiable once in ``q`` and ``k``.
+    or ``(q, k)``'s). Differentiable once in ``q`` and ``k``. To capture a backward pass in a graph, capture its
+    forward pass too, and let no eager graph of the same leaves live then.
     """
     sections = tuple(int(s) for s in sections)
     for name, t in (("q", q), ("k", k)):
