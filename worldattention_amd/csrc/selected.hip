@@ -284,9 +284,9 @@ __global__ void __launch_bounds__(64 * W) select_few_kernel(SelectParams p) {
 // by direct loads, whole rows too (loaded as operands, 64 bytes of 16 rows at a time, they took more than
 // twice the values' time: 1,024 queries x 8 key heads of 16 blocks 322 us against 245, both with WPR 4). A
 // tile's registers are not doubled: with a second tile loaded ahead a SIMD holds fewer waves, and less is in
-// flight (503 us). Bound by reading the chosen keys and values from HBM for a decoding step (32 ragged
-// sequences x 32 blocks 43 us), and by a tile's instructions for a prompt, whose blocks the caches hold (190 us
-// with WPR 1, 170 with no loads at all).
+// flight (503 us). Bound by reading the chosen keys and values: from HBM for a decoding step (32 ragged
+// sequences x 32 blocks 42 us), from the L2s for a prompt, whose queries share blocks (190 us with WPR 1: 4.3 GB,
+// 22 TB/s; a fourth wave a SIMD makes it 208).
 // =============================================================================================
 struct AttnParams {
   const bf16_t* q; int64_t q_sb, q_st, q_sh;
@@ -325,8 +325,10 @@ template <int N> struct RowPart;     // N bf16 values of a value row
 template <> struct RowPart<8> { typedef bf16x8 type; };
 template <> struct RowPart<4> { typedef bf16x4 type; };
 
+// Two waves a SIMD promised keep the outputs out of the accumulation registers, whose moves cost 1,024 rows 38 us
+// against 34; one-wave rows, bound by the caches, do not gain.
 template <int D, int WPR>
-__global__ void __launch_bounds__(WPR == 8 ? 512 : 256) attend_kernel(AttnParams p) {
+__global__ void __launch_bounds__(WPR == 8 ? 512 : 256, WPR == 1 ? 1 : 2) attend_kernel(AttnParams p) {
   constexpr int NW = WPR == 8 ? 8 : 4, ROWS = NW / WPR;   // waves and query rows of a workgroup
   constexpr int KC = D / 32, VC = D / 16;   // 32-channel steps of a key row; channels of a value row a lane holds
   constexpr int CPR = D / 8, RPI = 64 / CPR, KI = 32 / RPI;   // 16-byte chunks of a row; rows and direct loads of a tile
@@ -349,8 +351,8 @@ __global__ void __launch_bounds__(WPR == 8 ? 512 : 256) attend_kernel(AttnParams
   const int64_t row = ((int64_t)b * p.n + i) * p.Hk + hk;
   const int heads = min(16, G - 16 * gt);
   const int64_t seen = seen_tokens(p.kv_len, p.kv_len_all, p.cap, p.n, b, i);
-  const int tpb = p.bs / 32;                // tiles of a block
-  const int tiles = max(0, min(p.num[row], p.topk)) * tpb;
+  const int shift = p.bs == 64 ? 1 : 2;     // log2 of a block's tiles
+  const int tiles = max(0, min(p.num[row], p.topk)) << shift;
   const int per = (tiles + p.splits - 1) / p.splits;
   const int t0 = split * per, t1 = min(tiles, t0 + per);
   const int32_t* list = p.index + row * p.topk;
@@ -376,10 +378,10 @@ __global__ void __launch_bounds__(WPR == 8 ? 512 : 256) attend_kernel(AttnParams
     if (t >= ids_at + 64 * WPR || t < ids_at) {
       ids_at = t;
       const int mine = t + lane * WPR;
-      ids = mine < t1 ? list[mine / tpb] : -1;
+      ids = mine < t1 ? list[mine >> shift] : -1;
     }
     const int id = __builtin_amdgcn_readlane(ids, (t - ids_at) / WPR);
-    const int64_t key0 = (int64_t)id * p.bs + (t % tpb) * 32;
+    const int64_t key0 = ((int64_t)id << (shift + 5)) + (t & ((1 << shift) - 1)) * 32;
     return id < 0 || key0 >= seen ? -1 : key0;
   };
   // Keys in LDS: 16-byte chunk c of row r in slot c ^ swizzle(r), so that 16 rows' chunks fall in all banks.
@@ -417,14 +419,21 @@ __global__ void __launch_bounds__(WPR == 8 ? 512 : 256) attend_kernel(AttnParams
     // the keys have landed (only the eight value loads were issued after theirs)
     asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     float s[8];
+    {
+      bf16x8 ka[2][KC];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) ka[h][c] = *(const bf16x8*)(kt + (16 * h + l16) * D + ((4 * c + kg) ^ swizzle(l16)) * 8);
+      f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int c = 0; c < KC; ++c)
-        acc = mma16(*(const bf16x8*)(kt + (16 * h + l16) * D + ((4 * c + kg) ^ swizzle(l16)) * 8), q[c], acc);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[4 * h + r] = acc[r] * p.scale2;
+        for (int h = 0; h < 2; ++h) acc[h] = mma16(ka[h][c], q[c], acc[h]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[4 * h + r] = acc[h][r] * p.scale2;
     }
     if (live < 32) {
 #pragma unroll
@@ -561,7 +570,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p, int64_t un
 
 // Waves of a row: one where the rows alone fill the GPU (a list's ids and a row's ends are then paid once, and no
 // barrier), else four, and eight where the rows leave CUs empty. One wave against four against eight, us: 8,192 rows of
-// 16 blocks 194 / 246 / 339, 2,048 98 / 72 / 92, 1,024 46 / 38 / 48; 512 of 32 108 / 87 / 88, 256 - / 43 / 43,
+// 16 blocks 194 / 246 / 339, 2,048 98 / 70 / 92, 1,024 46 / 34 / 48; 512 of 32 108 / 87 / 88, 256 - / 43 / 43,
 // 8 of 16 (with parts) - / 14.8 / 10.3. One-wave rows share a workgroup by query, so single queries take four (4,096
 // rows 282 / 288).
 int waves_per_row(int64_t rows, int64_t n) { return rows >= 4096 && n >= 4 ? 1 : rows >= 512 ? 4 : 8; }
