@@ -36,11 +36,11 @@ struct SelectParams {
   int32_t* index; int32_t* num;
 };
 
-// The group's queries of 16-query tile `qt`, in contraction order: slot (step 4 i + j, lane group kg) is channel
+// The group's queries of token qi, in contraction order: slot (step 4 i + j, lane group kg) is channel
 // 16 i + 4 kg + j on both sides.
 template <int D>
-__device__ __forceinline__ void group_queries(const SelectParams& p, int b, int hk, int qt, int lane, double (&a)[D / 4]) {
-  const int qi = 16 * qt + (lane & 15), kg = lane >> 4, G = p.H / p.Hk;
+__device__ __forceinline__ void group_queries(const SelectParams& p, int b, int hk, int qi, int kg, double (&a)[D / 4]) {
+  const int G = p.H / p.Hk;
 #pragma unroll
   for (int i = 0; i < D / 4; ++i) a[i] = 0.0;
   if (qi >= p.n) return;
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(64) score_kernel(SelectParams p) {
   const int end = score_end(p, b, min(p.n, 16 * qt + 16) - 1), begin = bt * p.per * 16;
   if (begin >= end) return;
   double a[D / 4];
-  group_queries<D>(p, b, hk, qt, lane, a);
+  group_queries<D>(p, b, hk, 16 * qt + row, kg, a);
   f32x4 x[2][D / 16];
   load_sums<D>(p, bh, begin, lane, x[0]);
   auto tile = [&](int b0, const f32x4 (&now)[D / 16], f32x4 (&next)[D / 16]) {
@@ -229,41 +229,87 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) choose_kernel(SelectPar
 
 // Scores and choice of a few queries over a short cache in one launch: a workgroup per sequence and key head,
 // the scores in LDS. One launch and 8 bytes a score less; its CU reads the sums alone, so at most kFusedBlocks
-// blocks. 32 sequences of up to 512 blocks x 8 key heads: 22.7 us against 19.8 + 13.6 in two launches; one sequence of
-// 64 blocks: 9.9 against 5.8 + 4.4, and a launch less for the host. The time of few workgroups is a wave's, so
-// eight share the blocks; two where workgroups wait for CUs (8 key heads, 8 waves against 2: 32 sequences 23 us
-// against 36, 64 of 128 blocks 18 against 18, 128 of them 31 against 22, 512 of 32 blocks 80 against 39).
+// blocks. A single query multiplies on the vector units: of a matrix product it would fill one row of 16, at a
+// sixteenth of the rate a CU then has alone (23 us against 16 below). 32 sequences of up to 512 blocks x 8 key heads:
+// 16 us against 19.8 + 13.6 in two launches; one sequence of 64 blocks: 6.3 against 5.8 + 4.4, and a launch less
+// for the host. The time of few workgroups is a wave's, so eight share the blocks; two where workgroups wait for
+// CUs (8 key heads, 8 waves against 2: 32 sequences 15.9 us against 20.4, 64 of 128 blocks 10.2 against 11.6, 128 of
+// them 17.3 against 14.5, 512 of 32 blocks 47 against 19).
 constexpr int kFusedBlocks = 1024, kFusedScores = 8000;   // the scores within 64 KiB
 constexpr int64_t kManyHeads = 1024;
 
-template <int D, int W>
+template <int D, int W, bool SINGLE>
 __global__ void __launch_bounds__(64 * W) select_few_kernel(SelectParams p) {
   extern __shared__ double sc[];   // [n, n_blocks]
   __shared__ int counts[2][W], one[2][1];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = lane & 15, kg = lane >> 4;
   const int bh = blockIdx.x, b = bh / p.Hk, hk = bh % p.Hk;
   const int end = score_end(p, b, p.n - 1);
+  constexpr int STEP = 16 * W;
   if (p.nb > p.topk && 16 * w < end) {
-    constexpr int STEP = 16 * W;
-    double a[D / 4];
-    f32x4 x[2][D / 16];
-    load_sums<D>(p, bh, 16 * w, lane, x[0]);
-    group_queries<D>(p, b, hk, 0, lane, a);
-    auto tile = [&](int b0, const f32x4 (&now)[D / 16], f32x4 (&next)[D / 16]) {
-      if (b0 + STEP < end) load_sums<D>(p, bh, b0 + STEP, lane, next);
-      const f64x4 acc = score_tile<D>(a, now);
+    if constexpr (SINGLE) {
+      // eight lanes a block, two blocks a lane: channels 32 i + 4 c + j of block b0 + 8 x + r
+      const int r = lane >> 3, c = lane & 7;
+      double a[D / 8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (kg + 4 * r < p.n && b0 + row < p.nb) sc[(kg + 4 * r) * p.nb + b0 + row] = acc[r];
-    };
-    for (int b0 = 16 * w; b0 < end; b0 += 2 * STEP) {
-      tile(b0, x[0], x[1]);
-      if (b0 + STEP < end) tile(b0 + STEP, x[1], x[0]);
+      for (int i = 0; i < D / 8; ++i) a[i] = 0.0;
+      const bf16_t* q = p.q + (int64_t)b * p.q_sb + (int64_t)hk * (p.H / p.Hk) * p.q_sh + 4 * c;
+      for (int g = 0; g < p.H / p.Hk; ++g)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const bf16x4 v = *(const bf16x4*)(q + (int64_t)g * p.q_sh + 32 * i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[4 * i + j] += (double)(float)v[j];
+        }
+      f32x4 x[2][2][D / 32];
+      auto load = [&](int b0, f32x4 (&to)[2][D / 32]) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+            to[y][i] = *(const f32x4*)(p.sums + ((int64_t)bh * p.nb + min(b0 + 8 * y + r, p.nb - 1)) * D + 32 * i + 4 * c);
+      };
+      auto tile = [&](int b0, const f32x4 (&now)[2][D / 32], f32x4 (&next)[2][D / 32]) {
+        if (b0 + STEP < end) load(b0 + STEP, next);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          double s[2] = {0.0, 0.0};
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j & 1] += a[4 * i + j] * (double)now[y][i][j];
+          double sum = s[0] + s[1];
+#pragma unroll
+          for (int m = 1; m < 8; m *= 2) sum += __shfl_xor(sum, m);
+          if (c == 0 && b0 + 8 * y + r < p.nb) sc[b0 + 8 * y + r] = sum;
+        }
+      };
+      load(16 * w, x[0]);
+      for (int b0 = 16 * w; b0 < end; b0 += 2 * STEP) {
+        tile(b0, x[0], x[1]);
+        if (b0 + STEP < end) tile(b0 + STEP, x[1], x[0]);
+      }
+    } else {
+      double a[D / 4];
+      f32x4 x[2][D / 16];
+      load_sums<D>(p, bh, 16 * w, lane, x[0]);
+      group_queries<D>(p, b, hk, row, kg, a);
+      auto tile = [&](int b0, const f32x4 (&now)[D / 16], f32x4 (&next)[D / 16]) {
+        if (b0 + STEP < end) load_sums<D>(p, bh, b0 + STEP, lane, next);
+        const f64x4 acc = score_tile<D>(a, now);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (kg + 4 * r < p.n && b0 + row < p.nb) sc[(kg + 4 * r) * p.nb + b0 + row] = acc[r];
+      };
+      for (int b0 = 16 * w; b0 < end; b0 += 2 * STEP) {
+        tile(b0, x[0], x[1]);
+        if (b0 + STEP < end) tile(b0 + STEP, x[1], x[0]);
+      }
     }
   }
   __syncthreads();
   // A wave a query; a single query with many blocks takes all waves.
-  if (p.n == 1 && p.nb > 256) {
+  if (SINGLE && p.nb > 256) {
     choose_row<W, kFusedBlocks / (64 * W)>(p, b, 0, hk, w, lane, counts, [&](int j) { return sc[j]; });
   } else {
     for (int i = w; i < p.n; i += W) {
@@ -601,6 +647,17 @@ void launch_choose(const SelectParams& p, hipStream_t s) {
   hipLaunchKernelGGL((choose_kernel<W, KPT>), dim3((unsigned)grid), dim3(W == 1 ? 256 : 64 * W), 0, s, p);
 }
 
+template <int D, int W>
+void launch_few(const SelectParams& p, dim3 grid, size_t lds, hipStream_t s) {
+  if (p.n == 1) hipLaunchKernelGGL((select_few_kernel<D, W, true>), grid, dim3(64 * W), lds, s, p);
+  else hipLaunchKernelGGL((select_few_kernel<D, W, false>), grid, dim3(64 * W), lds, s, p);
+}
+template <int D>
+void launch_few(const SelectParams& p, bool many, dim3 grid, size_t lds, hipStream_t s) {
+  if (many) launch_few<D, 2>(p, grid, lds, s);
+  else launch_few<D, 8>(p, grid, lds, s);
+}
+
 }  // namespace
 
 extern "C" int64_t wa_select_blocks_workspace_bytes(int64_t B, int64_t n, int64_t Hk, int64_t n_blocks) {
@@ -634,13 +691,9 @@ extern "C" int wa_select_blocks(const wa_select_blocks_args* a, void* stream) {
   if (fused(a->n, a->n_blocks)) {
     const dim3 grid((unsigned)(a->B * a->Hk));
     const size_t scores = (size_t)(a->n * a->n_blocks * 8);
-    if (a->B * a->Hk >= kManyHeads) {
-      if (a->D == 128) hipLaunchKernelGGL((select_few_kernel<128, 2>), grid, dim3(128), scores, s, p);
-      else hipLaunchKernelGGL((select_few_kernel<64, 2>), grid, dim3(128), scores, s, p);
-    } else {
-      if (a->D == 128) hipLaunchKernelGGL((select_few_kernel<128, 8>), grid, dim3(512), scores, s, p);
-      else hipLaunchKernelGGL((select_few_kernel<64, 8>), grid, dim3(512), scores, s, p);
-    }
+    const bool many = a->B * a->Hk >= kManyHeads;
+    if (a->D == 128) launch_few<128>(p, many, grid, scores, s);
+    else launch_few<64>(p, many, grid, scores, s);
     return wa_launch_status("select_blocks");
   }
   p.scores = (double*)a->workspace;
