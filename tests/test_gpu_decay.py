@@ -181,6 +181,19 @@ def test_step(dtype, b, n, h, d, dv):
     assert (pool[0] == 7).all() and (pool[:, 0] == 7).all() and (pool[:, -1] == 7).all()
 
 
+def test_step_with_channels_that_are_not_contiguous():
+    """A transposed view, and a single channel whose stride says nothing."""
+    for d in (1, 6):
+        g = torch.Generator().manual_seed(d)
+        q, k, v = (torch.randn(2, 1, d, 5, generator=g).to(DEV).transpose(2, 3) for _ in range(3))
+        log_decay = -torch.rand(5, generator=g).to(DEV)
+        state = torch.randn(2, 5, d, d, generator=g).to(DEV)
+        want, want_s = OT.decay_linear_attention(q, k, v, log_decay, initial_state=state)
+        out = W.decay_linear_step(q, k, v, log_decay, state)
+        # sums of at most 7 terms below 2^5 in fp32
+        assert ((out.double() - want).abs() <= 2.0 ** -15).all() and ((state.double() - want_s).abs() <= 2.0 ** -15).all()
+
+
 def test_steps_continue_a_prompt():
     x, _ = _inputs(2, 201, 3, 128, 128, torch.bfloat16, seed=21, initial=False)
     want, want_s = OT.decay_linear_attention(x["q"], x["k"], x["v"], x["log_decay"])

@@ -506,6 +506,12 @@ def call(name: str, *args) -> None:
 _BOUND: dict = {}
 
 
+@functools.lru_cache(maxsize=1024)
+def sizes(name: str, *args: int) -> int:
+    """What the entry point ``name`` answers for these sizes: workspace bytes, segments; it depends on nothing else."""
+    return getattr(lib(), name)(*args)
+
+
 def launch(name: str, args, dev: torch.device) -> None:
     """:func:`call` on ``dev``'s current stream, with ``dev`` made the current device around it (a kernel
     launch takes the current device's). The entry point is looked up once and the stream's handle taken

@@ -29,7 +29,7 @@ def _forward(q, k, v, log_decay, initial, lengths, scale, want_derivs=False):
     f32 = dict(dtype=torch.float32, device=dev)
     out = torch.empty((bsz, length, heads, d), dtype=q.dtype, device=dev)
     final = torch.empty((bsz, heads, d, d), **f32)
-    n_seg = _lib.lib().wa_decay_segments(bsz, length, heads, int(want_derivs))
+    n_seg = _lib.sizes("wa_decay_segments", bsz, length, heads, int(want_derivs))
     states = torch.empty((bsz, heads, n_seg, d, d), **f32)
     derivs = torch.empty((bsz, heads, n_seg + 1, d, d), **f32) if want_derivs else None
     args = _lib.DecayFwdArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), _lib.dtype_code(q), bsz, length,
@@ -62,7 +62,7 @@ class _DecayLinear(torch.autograd.Function):
         dq, dk, dv = (torch.empty((bsz, length, heads, d), dtype=q.dtype, device=dev) for _ in range(3))
         dinitial = torch.empty((bsz, heads, d, d), **f32) if ctx.needs_input_grad[4] else None
         dlog = torch.empty((heads,), **f32) if ctx.needs_input_grad[3] else None
-        size = _lib.lib().wa_decay_bwd_workspace_bytes(bsz, length, heads, d, int(derivs is not None))
+        size = _lib.sizes("wa_decay_bwd_workspace_bytes", bsz, length, heads, d, int(derivs is not None))
         ws = torch.empty((size,), dtype=torch.uint8, device=dev)
         args = _lib.DecayBwdArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(dout), *_lib.blhd(dq),
                                  *_lib.blhd(dk), *_lib.blhd(dv), _lib.dtype_code(q), bsz, length, heads, d,
@@ -99,7 +99,7 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
       ``[0, L]``); the tokens behind are not read, their outputs and gradients are 0.
     * ``scale``: default ``D ** -0.5``.
 
-    Outputs have the inputs' dtype; the state is summed in fp32. Differentiable once, through both results, in
+    At most 65,535 sequences times heads. Outputs have the inputs' dtype; the state is summed in fp32. Differentiable once, through both results, in
     ``q``, ``k``, ``v``, ``log_decay`` and ``initial_state``. A value that is not finite in ``v`` (or, backwards,
     in the gradient) reaches its 64-token neighbourhood, as it reaches a tile of softmax attention. To capture a
     backward pass in a graph, capture its forward pass too, and let no eager graph of the same leaves live then.
@@ -162,7 +162,7 @@ def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_dec
     out = torch.empty((bsz, length, heads, dv), dtype=q.dtype, device=dev)
     if out.numel() == 0 or d == 0:
         return out.zero_()
-    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    q, k, v = (t if t.stride(-1) == 1 else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
     log_decay = log_decay.contiguous()
     args = _lib.DecayStepArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), dtype, bsz, length, heads, d, dv,
                               log_decay.data_ptr(), state.data_ptr(), s_sb, s_sh, d ** -0.5 if scale is None else float(scale))

@@ -70,7 +70,7 @@ def _select(q, sums, kv_len, bs, topk, sink, local, cap) -> BlockSelection:
     num = torch.empty((bsz, n, hk), dtype=torch.int32, device=dev)
     if num.numel() == 0:
         return BlockSelection(index, num)
-    size = _lib.lib().wa_select_blocks_workspace_bytes(bsz, n, hk, nb)
+    size = _lib.sizes("wa_select_blocks_workspace_bytes", bsz, n, hk, nb)
     ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
     keep, len_ptr, len_all = _lengths(kv_len)
     args = _lib.SelectBlocksArgs(*_lib.blhd(q), sums.data_ptr(), nb, len_ptr, len_all, cap, bsz, n, heads, hk, d, bs, topk,
@@ -88,7 +88,7 @@ def _attend(q, k, v, index, num, kv_len, bs, scale):
     if lse.numel() == 0:
         return out, lse
     topk = index.shape[-1]
-    size = _lib.lib().wa_selected_attn_workspace_bytes(bsz, n, heads, hk, d, topk, bs)
+    size = _lib.sizes("wa_selected_attn_workspace_bytes", bsz, n, heads, hk, d, topk, bs)
     ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
     keep, len_ptr, len_all = _lengths(kv_len)
     args = _lib.SelectedAttnArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), lse.data_ptr(),
