@@ -73,6 +73,19 @@ def test_shared_positions_int32_strides_and_one_tensor():
            "fp32 frequencies")
 
 
+def test_queries_and_keys_both_copied_for_the_kernel():
+    """Both tensors with strided channels, all of one size: neither copy's memory serves the other's output."""
+    g = torch.Generator().manual_seed(8)
+    pos = torch.randint(0, 1000, (700, 1), generator=g).to(DEV)
+    inv, sections = W.axis_frequencies(64, axes=1, device=DEV)
+    q, k = (torch.randn(3, 700, 64, 8, generator=g).to(DEV).transpose(2, 3) for _ in range(2))
+    for _ in range(3):
+        got = W.rope_axes(q, pos, inv, sections, k=k)
+        for out, x in zip(got, (q, k)):
+            # sine, cosine and two rounded products of fp32
+            assert ((out.double() - OT.rope_axes(x, pos, inv, sections)).abs() <= 2.0 ** -20 * x.abs().max()).all()
+
+
 def test_matches_the_models_own_grid_rope():
     """On a frame x height x width grid with the framework's frequencies it is the 3-D RoPE of its workloads."""
     f, hh, ww, d = 3, 5, 7, 128

@@ -34,26 +34,30 @@ def axis_frequencies(head_dim: int, axes: int = 3, theta: float = 10000.0, devic
 
 def _launch(q, k, positions, inv_freq, sections, interleaved, inverse):
     """Rotated copies of the tensors given (either may be None)."""
-    dev = positions.device
-    outs, fields = [], []
-    for t in (q, k):
-        if t is None:
-            outs.append(None)
-            fields += [None, 0, 0, 0, None, 0, 0, 0]
-            continue
-        src = t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-        out = torch.empty(t.shape, dtype=t.dtype, device=dev)
-        outs.append(out)
-        fields += [src.data_ptr(), *src.stride()[:3], out.data_ptr(), *out.stride()[:3]]
+    q_src, q_out, q_fields, q_heads = _side(q)     # the sources are held until the launch: one may be a copy
+    k_src, k_out, k_fields, k_heads = _side(k)
     some = q if q is not None else k
     bsz, length, _, d = some.shape
-    places = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
-    args = _lib.RopeAxesArgs(*fields, _lib.dtype_code(some), bsz, length, q.shape[2] if q is not None else 0,
-                             k.shape[2] if k is not None else 0, d, positions.data_ptr(), *places,
-                             positions.dtype == torch.int64, inv_freq.data_ptr(), len(sections),
-                             _lib.RopeSections(*sections), interleaved, inverse)
-    _lib.launch("wa_rope_axes", args, dev)
-    return outs
+    places = positions.stride()
+    args = _lib.RopeAxesArgs(*q_fields, *k_fields, _lib.dtype_code(some), bsz, length, q_heads, k_heads, d, positions.data_ptr(),
+                             *(places if len(places) == 3 else (0, *places)), positions.dtype is torch.int64,
+                             inv_freq.data_ptr(), len(sections), _lib.RopeSections(*sections), interleaved, inverse)
+    _lib.launch("wa_rope_axes", args, positions.device)
+    return q_out, k_out
+
+
+def _side(t):
+    """What the kernel reads for a tensor, its output, their argument fields and the heads."""
+    if t is None:
+        return None, None, (None, 0, 0, 0, None, 0, 0, 0), 0
+    bsz, length, heads, d = t.shape
+    out = torch.empty(bsz, length, heads, d, dtype=t.dtype, device=t.device)
+    sb, st, sh, sc = t.stride()
+    if sc != 1 and d != 1:
+        t = t.contiguous()
+        sb, st, sh, _ = t.stride()
+    ob, ot, oh, _ = out.stride()
+    return t, out, (t.data_ptr(), sb, st, sh, out.data_ptr(), ob, ot, oh), heads
 
 
 class _RopeAxes(torch.autograd.Function):
@@ -89,25 +93,27 @@ def rope_axes(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, 
     or ``(q, k)``'s). Differentiable once in ``q`` and ``k``. To capture a backward pass in a graph, capture its
     forward pass too, and let no eager graph of the same leaves live then.
     """
-    sections = tuple(int(s) for s in sections)
-    for name, t in (("q", q), ("k", k)):
-        if t is not None and t.dim() != 4:
-            raise ValueError(f"{name} must be [B, L, H, D], got {tuple(t.shape)}")
+    sections = tuple(map(int, sections))
+    if q.dim() != 4:
+        raise ValueError(f"q must be [B, L, H, D], got {tuple(q.shape)}")
+    if k is not None and k.dim() != 4:
+        raise ValueError(f"k must be [B, L, H, D], got {tuple(k.shape)}")
     bsz, length, _, d = q.shape
     if k is not None and (k.shape[0] != bsz or k.shape[1] != length or k.shape[3] != d or k.dtype != q.dtype):
         raise ValueError(f"k must hold q's tokens and head dim in its dtype, got {tuple(k.shape)} {k.dtype} for "
                          f"{tuple(q.shape)} {q.dtype}")
-    if not 1 <= len(sections) <= _lib.ROPE_MAX_AXES or min(sections) < 0 or sum(sections) < 1:
+    axes, pairs = len(sections), sum(sections)
+    if not 1 <= axes <= _lib.ROPE_MAX_AXES or min(sections) < 0 or pairs < 1:
         raise ValueError(f"sections must be 1 to {_lib.ROPE_MAX_AXES} pair counts, got {sections}")
-    if d > _lib.ROPE_MAX_DIM or 2 * sum(sections) > d:
-        raise ValueError(f"{sum(sections)} pairs do not fit a head dim of {d} (at most {_lib.ROPE_MAX_DIM})")
-    if tuple(positions.shape) not in ((length, len(sections)), (bsz, length, len(sections))):
-        raise ValueError(f"positions must be [{length}, {len(sections)}] or [{bsz}, {length}, {len(sections)}], got "
+    if d > _lib.ROPE_MAX_DIM or 2 * pairs > d:
+        raise ValueError(f"{pairs} pairs do not fit a head dim of {d} (at most {_lib.ROPE_MAX_DIM})")
+    if positions.shape != (bsz, length, axes) and positions.shape != (length, axes):
+        raise ValueError(f"positions must be [{length}, {axes}] or [{bsz}, {length}, {axes}], got "
                          f"{tuple(positions.shape)}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-    if tuple(inv_freq.shape) != (sum(sections),) or inv_freq.dtype not in (torch.float32, torch.float64):
-        raise ValueError(f"inv_freq must be [{sum(sections)}] in fp64 or fp32, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
+    if inv_freq.shape != (pairs,) or inv_freq.dtype not in (torch.float32, torch.float64):
+        raise ValueError(f"inv_freq must be [{pairs}] in fp64 or fp32, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
     if inv_freq.requires_grad and torch.is_grad_enabled():
         raise ValueError("inv_freq takes no gradient: detach it")
     _lib.require_gpu(q, k, positions, inv_freq)
