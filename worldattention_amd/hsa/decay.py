@@ -73,16 +73,16 @@ class _DecayLinear(torch.autograd.Function):
 
 
 def _check(q, k, v, log_decay, state, what):
-    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:3] != q.shape[:3]:
+    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or (v.shape != q.shape and v.shape[:3] != q.shape[:3]):
         raise ValueError(f"q and k must be [B, L, H, D] and v [B, L, H, Dv], got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
-    if not q.dtype == k.dtype == v.dtype:
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError(f"q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
     bsz, _, heads, d = q.shape
-    if tuple(log_decay.shape) != (heads,) or log_decay.dtype != torch.float32:
+    if log_decay.shape != (heads,) or log_decay.dtype is not torch.float32:
         raise ValueError(f"log_decay must be fp32 [{heads}], got {log_decay.dtype} {tuple(log_decay.shape)}")
     shape = (bsz, heads, d, v.shape[-1])
-    if state is not None and (tuple(state.shape) != shape or state.dtype != torch.float32):
+    if state is not None and (state.shape != shape or state.dtype is not torch.float32):
         raise ValueError(f"{what} must be fp32 {shape}, got {state.dtype} {tuple(state.shape)}")
 
 
@@ -159,10 +159,10 @@ def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_dec
         raise ValueError("decay_linear_step takes no gradient (decay_linear_attention does): call it under torch.no_grad()")
     dev = _lib.require_gpu(q, k, v, log_decay, state)
     dtype = _lib.dtype_code(q)
-    out = torch.empty((bsz, length, heads, dv), dtype=q.dtype, device=dev)
+    out = torch.empty(bsz, length, heads, dv, dtype=q.dtype, device=dev)
     if out.numel() == 0 or d == 0:
         return out.zero_()
-    q, k, v = (t if t.stride(-1) == 1 else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    q, k, v = [t if t.stride(-1) == 1 else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v)]
     log_decay = log_decay.contiguous()
     args = _lib.DecayStepArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), dtype, bsz, length, heads, d, dv,
                               log_decay.data_ptr(), state.data_ptr(), s_sb, s_sh, d ** -0.5 if scale is None else float(scale))

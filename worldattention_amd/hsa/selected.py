@@ -34,10 +34,11 @@ KvLen = Union[int, torch.Tensor]
 def _check_query(q, kv_heads: int, bsz: int, d: int, block_size: int, kv_len: KvLen) -> None:
     if q.dim() != 4 or q.shape[0] != bsz or q.shape[3] != d:
         raise ValueError(f"q must be [B={bsz}, n, H, D={d}], got {tuple(q.shape)}")
+    heads = q.shape[2]
     if d not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {d}")
-    if kv_heads < 1 or q.shape[2] % kv_heads or q.shape[2] < kv_heads:
-        raise ValueError(f"{q.shape[2]} query heads do not share {kv_heads} key heads")
+    if kv_heads < 1 or heads % kv_heads or heads < kv_heads:
+        raise ValueError(f"{heads} query heads do not share {kv_heads} key heads")
     if block_size not in (64, 128):
         raise ValueError(f"block_size must be 64 or 128, got {block_size}")
     if q.dtype != torch.bfloat16:
@@ -49,7 +50,9 @@ def _check_query(q, kv_heads: int, bsz: int, d: int, block_size: int, kv_len: Kv
 def _no_gradient(*tensors) -> None:
     if not torch.is_grad_enabled():
         return
-    if any([t.requires_grad for t in tensors]):
+    for t in tensors:
+        if not t.requires_grad:
+            continue
         raise ValueError("attention over selected cache blocks takes no gradient: call it under torch.no_grad(), or train "
                          "with block_sparse_attention(block_map=...)")
 
@@ -66,12 +69,12 @@ def _select(q, sums, kv_len, bs, topk, sink, local, cap) -> BlockSelection:
     dev = q.device
     bsz, n, heads, d = q.shape
     hk, nb = sums.shape[1:3]
-    index = torch.empty((bsz, n, hk, topk), dtype=torch.int32, device=dev)
-    num = torch.empty((bsz, n, hk), dtype=torch.int32, device=dev)
-    if num.numel() == 0:
+    index = torch.empty(bsz, n, hk, topk, dtype=torch.int32, device=dev)
+    num = torch.empty(bsz, n, hk, dtype=torch.int32, device=dev)
+    if bsz == 0 or n == 0:
         return BlockSelection(index, num)
     size = _lib.sizes("wa_select_blocks_workspace_bytes", bsz, n, hk, nb)
-    ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     keep, len_ptr, len_all = _lengths(kv_len)
     args = _lib.SelectBlocksArgs(*_lib.blhd(q), sums.data_ptr(), nb, len_ptr, len_all, cap, bsz, n, heads, hk, d, bs, topk,
                                  sink, local, index.data_ptr(), num.data_ptr(), _lib.ptr(ws))
@@ -83,13 +86,13 @@ def _attend(q, k, v, index, num, kv_len, bs, scale):
     dev = q.device
     bsz, n, heads, d = q.shape
     cap, hk = k.shape[1:3]
-    out = torch.empty((bsz, n, heads, d), dtype=torch.bfloat16, device=dev)
-    lse = torch.empty((bsz, heads, n), dtype=torch.float32, device=dev)
-    if lse.numel() == 0:
+    out = torch.empty(bsz, n, heads, d, dtype=torch.bfloat16, device=dev)
+    lse = torch.empty(bsz, heads, n, dtype=torch.float32, device=dev)
+    if bsz == 0 or n == 0:
         return out, lse
     topk = index.shape[-1]
     size = _lib.sizes("wa_selected_attn_workspace_bytes", bsz, n, heads, hk, d, topk, bs)
-    ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     keep, len_ptr, len_all = _lengths(kv_len)
     args = _lib.SelectedAttnArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), lse.data_ptr(),
                                  index.data_ptr(), num.data_ptr(), topk, len_ptr, len_all, bsz, n, cap, heads, hk, d, bs,
@@ -105,19 +108,25 @@ def _check_budget(topk: int, sink: int, local: int) -> None:
 
 
 def _check_sums(sums, what: str) -> None:
-    if sums.dim() != 4 or sums.dtype != torch.float32 or not sums.is_contiguous():
+    if sums.dim() != 4 or sums.dtype is not torch.float32 or not sums.is_contiguous():
         raise ValueError(f"{what} must be contiguous fp32 [B, Hk, blocks, D], got {sums.dtype} {tuple(sums.shape)}")
     if not 1 <= sums.shape[2] <= _lib.SELECT_MAX_BLOCKS:
         raise ValueError(f"{what} must hold 1 to {_lib.SELECT_MAX_BLOCKS} blocks, got {sums.shape[2]}")
 
 
-def _check_cache(q, k, v) -> None:
+def _readable(strides) -> bool:
+    sb, st, sh, sc = strides
+    return sc == 1 and sb % 8 == 0 and st % 8 == 0 and sh % 8 == 0 and st <= 1 << 24
+
+
+def _check_cache(k, v) -> None:
     if k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"cache k / v must be matching [B, cap, Hk, D] tensors, got {tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError(f"cache k / v must be bf16, got {k.dtype} and {v.dtype}")
-    if (k.shape[1] < 1 or not (_lib.is_kernel_ready(k) and _lib.is_kernel_ready(v))
-            or max(k.stride(1), v.stride(1)) > 1 << 24):
+    strides = k.stride()
+    if (k.shape[1] < 1 or not _readable(strides) or (v.stride() != strides and not _readable(v.stride()))
+            or k.data_ptr() % 16 or v.data_ptr() % 16):
         raise ValueError("cache k / v must hold tokens, with contiguous channels in 16-byte aligned rows at most 2^24 elements "
                          "apart (a cache is read in place)")
 
@@ -154,7 +163,7 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
     nothing, a repeated one counts again). A query that sees nothing gets 0 and ``lse = -inf``; what the cache
     holds behind a sequence's end is not used. ``scale``: default ``D ** -0.5``.
     """
-    _check_cache(q, k, v)
+    _check_cache(k, v)
     bsz, _, hk, d = k.shape
     _check_query(q, hk, bsz, d, block_size, kv_len)
     if index.dim() != 4 or tuple(index.shape[:3]) != (bsz, q.shape[1], hk) or tuple(num.shape) != (bsz, q.shape[1], hk):
@@ -179,11 +188,11 @@ def attend_selected(q: torch.Tensor, kv_cache: dict, kv_len: KvLen, *, topk: int
         raise ValueError("kv_cache keeps no k_block_sums: write it with kv_append(..., block_size=...)")
     k, v, sums = kv_cache["k"], kv_cache["v"], kv_cache["k_block_sums"]
     bs = int(kv_cache["k_block_sums_block_size"])
-    _check_cache(q, k, v)
+    _check_cache(k, v)
     bsz, cap, hk, d = k.shape
     _check_query(q, hk, bsz, d, bs, kv_len)
     _check_sums(sums, "k_block_sums")
-    if tuple(sums.shape) != (bsz, hk, -(-cap // bs), d):
+    if sums.shape != (bsz, hk, -(-cap // bs), d):
         raise ValueError(f"k_block_sums must be [{bsz}, {hk}, {-(-cap // bs)}, {d}], got {tuple(sums.shape)}")
     _check_budget(topk, sink_blocks, local_blocks)
     if scale is not None and float(scale) == 0.0:
