@@ -78,7 +78,9 @@ struct StateParams {
   float w_scale;
 };
 
-// Rows: one workgroup per (segment, batch and head, job).
+// Rows: one workgroup per (segment, batch and head, job). The jobs of a segment read the same tensors: they are dealt
+// eight workgroups apart, to one XCD at about one time, so that its L2 serves the second and third (three gradients
+// of 32,760 tokens of 12 x 128: 387 us; one job after the other over all segments 403).
 struct Job {
   View a, b, c;
   void* y; int64_t y_sb, y_st, y_sh;
@@ -90,6 +92,19 @@ struct RowsParams {
   Shape s;
   Job job[3];
 };
+
+__device__ __forceinline__ void place_of(const RowsParams& p, int& seg, int& job) {
+  const int n = p.s.n_seg, jobs = gridDim.x / n, whole = n / 8 * 8;
+  int u = blockIdx.x;
+  if (u < jobs * whole) {
+    job = u % (8 * jobs) / 8;
+    seg = u / (8 * jobs) * 8 + u % 8;
+  } else {
+    u -= jobs * whole;
+    job = u / (n - whole);
+    seg = whole + u % (n - whole);
+  }
+}
 
 // Pairs inside the segments, for the decay's gradient.
 struct PairsParams {
@@ -248,8 +263,10 @@ __global__ void __launch_bounds__(kThreads) rows_f32_kernel(RowsParams p) {
   __shared__ __attribute__((aligned(16))) float tc[kChunk * Tile<D>::kRow];
   __shared__ __attribute__((aligned(16))) float tp[kChunk * Tile<kChunk>::kRow];
   __shared__ __attribute__((aligned(16))) float tx[D * Tile<D>::kRow];
-  const Job& jb = p.job[blockIdx.z];
-  const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
+  int seg, job;
+  place_of(p, seg, job);
+  const Job& jb = p.job[job];
+  const int bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
   const int rh = w >> 1, ch = w & 1;
   const int n = tokens_of(p.s, b, seg), lag = jb.rev ? 0 : 1;
@@ -672,7 +689,7 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
 // behind them and the state at once. Work a unit, not a chunk, pays for the state: with a state read and
 // rewritten every 64 tokens (two waves a tile, no LDS copy) the vector instructions were 2,600 a wave and unit
 // and the launch took 235 us at 32,760 tokens of 12 x 128; it takes 127, the three gradients in one launch
-// 398. Bound by its instructions: the ring and X^T fill a CU's LDS, so one workgroup runs at a time.
+// 387. Bound by its instructions: the ring and X^T fill a CU's LDS, so one workgroup runs at a time.
 template <int D>
 __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) {
   constexpr int NW = D / 16, CT = D / 32, KS = D / 16, STAGES = 2, UNIT = 32 * NW;
@@ -681,8 +698,10 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
   __shared__ __attribute__((aligned(1024))) bf16_t tc[STAGES][kChunk * D];
   __shared__ __attribute__((aligned(1024))) bf16_t xh[D * D], xl[D * D];   // X^T: row e, column d
   __shared__ __attribute__((aligned(16))) float wt[UNIT], edge[32];
-  const Job& jb = p.job[blockIdx.z];
-  const int seg = blockIdx.x, bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
+  int seg, job;
+  place_of(p, seg, job);
+  const Job& jb = p.job[job];
+  const int bh = blockIdx.y, b = bh / p.s.H, h = bh % p.s.H;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
   const int xd = w % CT, xe = w / CT * XT;
   const int rt = w < NW / 2 ? w : 3 * NW / 2 - 1 - w;   // row tile: the two waves of a SIMD share the causal work evenly
@@ -1239,7 +1258,7 @@ void segment_states(int dtype, const StateParams& p, hipStream_t st) {
 
 template <int D>
 void all_rows(int dtype, const RowsParams& p, int jobs, hipStream_t st) {
-  const dim3 grid(p.s.n_seg, p.s.B * p.s.H, jobs);
+  const dim3 grid(p.s.n_seg * jobs, p.s.B * p.s.H);
   if (dtype == WA_BF16) hipLaunchKernelGGL((rows_bf16_kernel<D>), grid, dim3(64 * (D / 16)), 0, st, p);
   else hipLaunchKernelGGL((rows_f32_kernel<D>), grid, dim3(kThreads), 0, st, p);
 }
