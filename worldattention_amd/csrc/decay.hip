@@ -80,7 +80,7 @@ struct StateParams {
 
 // Rows: one workgroup per (segment, batch and head, job). The jobs of a segment read the same tensors: they are dealt
 // eight workgroups apart, to one XCD at about one time, so that its L2 serves the second and third (three gradients
-// of 32,760 tokens of 12 x 128: 370 us; one job after the other over all segments 398).
+// of 32,760 tokens of 12 x 128: 387 us; one job after the other over all segments 403).
 struct Job {
   View a, b, c;
   void* y; int64_t y_sb, y_st, y_sh;
@@ -527,7 +527,7 @@ __device__ __forceinline__ void load_weights(const float* wt, int c, int g, floa
 // chunk's tokens (the two halves meet in LDS at the end): every weighted operand is then cut once a workgroup.
 // It enters in three parts, so the state carries no rounding but its fp32 sums'. The state decays once in two
 // chunks, whose tokens' weights run to the end of the two. 32,760 tokens of 12 x 128: 51 us in 21 segments, 41 of
-// them what its 200 MB take at a copy's rate; with derivatives in 64 segments 100, and 112 in the backward pass,
+// them what its 200 MB take at a copy's rate; with derivatives in 64 segments 100, and 112-117 in the backward pass,
 // which multiplies them with the forward's. A wave a half of the rows, cutting twice, decaying every chunk: 99
 // without derivatives.
 constexpr int kSpan = 2 * kChunk;
@@ -691,8 +691,8 @@ __global__ void __launch_bounds__(64 * (D / 16)) segment_state_bf16_kernel(State
 // place, and the keys and values of the unit stream through a ring of two 64-token stages that serve the rows
 // behind them and the state at once. Work a unit, not a chunk, pays for the state: with a state read and
 // rewritten every 64 tokens (two waves a tile, no LDS copy) the vector instructions were 2,600 a wave and unit
-// and the launch took 235 us at 32,760 tokens of 12 x 128; it takes 127, the three gradients in one launch
-// 370. Bound by its instructions: the ring and X^T fill a CU's LDS, so one workgroup runs at a time.
+// and the launch took 235 us at 32,760 tokens of 12 x 128; it takes 127-131, the three gradients in one launch
+// 370-387. Bound by its instructions: the ring and X^T fill a CU's LDS, so one workgroup runs at a time.
 template <int D>
 __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) {
   constexpr int NW = D / 16, CT = D / 32, KS = D / 16, STAGES = 2, UNIT = 32 * NW;
@@ -938,7 +938,7 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
 // Pairs: a workgroup takes 256 rows i of a segment, its four waves two 32-row tiles each (w and 7 - w, which
 // share the causal work evenly), whose queries and output gradients stay in registers as operands; the
 // segment's keys and values up to the rows pass through a ring of two LDS stages, each operand read
-// serving both tiles. 32,760 tokens of 12 x 128 in 64 segments: 111 us, 0.46 PFLOP/s of the products' causal
+// serving both tiles. 32,760 tokens of 12 x 128 in 64 segments: 111-117 us, 0.45 PFLOP/s of the products' causal
 // half; bound by the instructions that decay, mask and multiply the two score tiles. Tiles before the diagonal
 // separate: with e the tile's last token, (i - j) lambda^(i - j) = lambda^(i - e) [(i - e) + (e - j)] lambda^(e - j),
 // no power above 1.
