@@ -757,8 +757,8 @@ int wa_rope_axes(const wa_rope_axes_args* args, void* stream);
  * `derivs` (device fp32 [B, H, segments + 1, D, D], or NULL with derivs = 0 above) receives the states'
  * derivatives by log_decay, which a backward that computes dlog_decay takes back (others get NULL).
  * initial / final: fp32 [B, H, D, D] (key channel, value channel), contiguous; final may be NULL.
- * Rows must be 16-byte aligned and at most 2^23 elements apart. The state is kept and summed in
- * fp32. */
+ * Rows must be 16-byte aligned, at most 2^23 elements apart and, in bf16 and in every output, at least D
+ * (tokens may not share memory). The state is kept and summed in fp32. */
 int64_t wa_decay_segments(int64_t B, int64_t L, int64_t H, int32_t derivs);
 typedef struct wa_decay_fwd_args {
   const void* q; int64_t q_sb, q_st, q_sh;

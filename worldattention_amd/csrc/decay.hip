@@ -456,7 +456,7 @@ struct TileReads {
 __device__ __forceinline__ int pi32(int x) { return (x & 0x13) | ((x & 4) << 1) | ((x & 8) >> 1); }
 
 // TileStream (tile.h) over one segment, with the descriptor cut to the chunk's rows: any distance between the
-// segment's first and last token, up to kMaxTokenStride elements between two.
+// segment's first and last token, D (so that the cut falls between rows) to kMaxTokenStride elements between two.
 constexpr int64_t kMaxTokenStride = (int64_t)1 << 23;
 template <int D, int NW>
 struct ChunkStream {
@@ -1229,10 +1229,15 @@ int64_t segment_length(int64_t B, int64_t L, int64_t H, bool derivs) {
   return best;
 }
 
-bool rows16(const void* p, int64_t sb, int64_t st, int64_t sh, int dtype) {
+// Rows that the kernels read or write: 16-byte aligned, at most kMaxTokenStride elements apart and at least `apart`.
+bool rows16(const void* p, int64_t sb, int64_t st, int64_t sh, int dtype, int64_t apart) {
   const int v = dtype == WA_BF16 ? 8 : 4;
-  return wa_aligned16(p) && st >= 0 && st <= kMaxTokenStride && sb % v == 0 && st % v == 0 && sh % v == 0;
+  return wa_aligned16(p) && st >= apart && st <= kMaxTokenStride && sb % v == 0 && st % v == 0 && sh % v == 0;
 }
+// Outputs are written once, and ChunkStream cuts rows off by a byte range, which holds parts of them all where they
+// overlap: there each row must lie behind the one before it.
+int64_t apart_written(int64_t L, int64_t D) { return L > 1 ? D : 0; }
+int64_t apart_read(int dtype, int64_t L, int64_t D) { return dtype == WA_BF16 ? apart_written(L, D) : 0; }
 
 int check_shape(const char* what, int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
   WA_CHECK_ARG(dtype == WA_F32 || dtype == WA_BF16, "%s: unsupported dtype %d", what, dtype);
@@ -1339,9 +1344,10 @@ extern "C" int wa_decay_fwd(const wa_decay_fwd_args* a, void* stream) {
   if (rc != WA_OK) return rc;
   WA_CHECK_ARG(a->B > 0 && a->L > 0 && a->H > 0, "decay_fwd: nothing to compute");
   WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->log_decay && a->states, "decay_fwd: null tensor");
-  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype) &&
-               rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype) && rows16(a->o, a->o_sb, a->o_st, a->o_sh, a->dtype) &&
-               wa_aligned16(a->states) && wa_aligned16(a->initial) && wa_aligned16(a->final_state), "decay_fwd: rows and states must be 16-byte aligned, tokens at most 2^23 elements apart");
+  const int64_t wr = apart_written(a->L, a->D), rd = apart_read(a->dtype, a->L, a->D);
+  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype, rd) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype, rd) &&
+               rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype, rd) && rows16(a->o, a->o_sb, a->o_st, a->o_sh, a->dtype, wr) &&
+               wa_aligned16(a->states) && wa_aligned16(a->initial) && wa_aligned16(a->final_state), "decay_fwd: rows and states must be 16-byte aligned, tokens at most 2^23 elements apart and, written or in bf16, not overlapping");
   hipStream_t s = (hipStream_t)stream;
   return a->D == 128 ? run_fwd<128>(a, s) : run_fwd<64>(a, s);
 }
@@ -1354,12 +1360,13 @@ extern "C" int wa_decay_bwd(const wa_decay_bwd_args* a, void* stream) {
   WA_CHECK_ARG(a->q && a->k && a->v && a->dout && a->dq && a->dk && a->dv && a->log_decay && a->states && a->workspace,
                "decay_bwd: null tensor");
   WA_CHECK_ARG(!a->dlog_decay == !a->derivs, "decay_bwd: dlog_decay goes with the forward's derivs");
-  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype) &&
-               rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh, a->dtype) &&
-               rows16(a->dq, a->dq_sb, a->dq_st, a->dq_sh, a->dtype) && rows16(a->dk, a->dk_sb, a->dk_st, a->dk_sh, a->dtype) &&
-               rows16(a->dv, a->dv_sb, a->dv_st, a->dv_sh, a->dtype) &&
+  const int64_t wr = apart_written(a->L, a->D), rd = apart_read(a->dtype, a->L, a->D);
+  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype, rd) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype, rd) &&
+               rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype, rd) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh, a->dtype, rd) &&
+               rows16(a->dq, a->dq_sb, a->dq_st, a->dq_sh, a->dtype, wr) && rows16(a->dk, a->dk_sb, a->dk_st, a->dk_sh, a->dtype, wr) &&
+               rows16(a->dv, a->dv_sb, a->dv_st, a->dv_sh, a->dtype, wr) &&
                wa_aligned16(a->states) && wa_aligned16(a->workspace) && wa_aligned16(a->dfinal) && wa_aligned16(a->dinitial),
-               "decay_bwd: rows, states and workspace must be 16-byte aligned, tokens at most 2^23 elements apart");
+               "decay_bwd: rows, states and workspace must be 16-byte aligned, tokens at most 2^23 elements apart and, written or in bf16, not overlapping");
   hipStream_t s = (hipStream_t)stream;
   return a->D == 128 ? run_bwd<128>(a, s) : run_bwd<64>(a, s);
 }

@@ -19,8 +19,10 @@ __all__ = ["decay_linear_attention", "decay_linear_step"]
 
 
 def _ready(t: torch.Tensor) -> torch.Tensor:
-    """``t`` in rows that the kernels take: 16-byte aligned, tokens at most 2^23 elements apart."""
-    return _lib.kernel_ready(t if t.stride(1) <= 1 << 23 else t.contiguous(), t.dtype, 16 // t.element_size())
+    """``t`` in rows that the kernels take: 16-byte aligned, tokens at most 2^23 elements apart and, in bf16 (whose kernels
+    cut rows off by a byte range), each behind the one before it: expanded and overlapping tokens are copied."""
+    shared = t.dtype is torch.bfloat16 and t.shape[1] > 1 and t.stride(1) < t.shape[3]
+    return _lib.kernel_ready(t.contiguous() if shared or t.stride(1) > 1 << 23 else t, t.dtype, 16 // t.element_size())
 
 
 def _forward(q, k, v, log_decay, initial, lengths, scale, want_derivs=False):
