@@ -85,9 +85,20 @@ struct Job {
   View a, b, c;
   void* y; int64_t y_sb, y_st, y_sh;
   const float* x;     // carried states
-  int x_trans, rev;
+  bool x_trans, rev;
   float s_intra, s_inter;
+  float w_scale;                  // of the state's own tokens: s_inter X sums s_intra b c^T
+  float unit, in_unit, x_in_unit; // bf16 rows sum y / unit: s_intra and s_inter in it
 };
+// time forwards, the carried state holds bare sums: both parts take the scale; backwards it holds scaled ones.
+// The unit is the scale, which then stays out of the products. One of 0, or so small or large that its
+// reciprocal times a row of the state could leave fp32, cannot be divided by: the unit is then 1.
+Job rows_job(const View& a, const View& b, const View& c, void* y, int64_t y_sb, int64_t y_st, int64_t y_sh, const float* x, bool x_trans,
+             bool rev, float scale) {
+  const float s_inter = rev ? 1.f : scale, size = scale < 0.f ? -scale : scale;
+  const float unit = size >= 0x1p-32f && size <= 0x1p32f ? scale : 1.f;
+  return Job{a, b, c, y, y_sb, y_st, y_sh, x, x_trans, rev, scale, s_inter, rev ? scale : 1.f, unit, scale / unit, s_inter / unit};
+}
 struct RowsParams {
   Shape s;
   Job job[3];
@@ -273,7 +284,7 @@ __global__ void __launch_bounds__(kThreads) rows_f32_kernel(RowsParams p) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
   const int rh = w >> 1, ch = w & 1;
   const int n = tokens_of(p.s, b, seg), lag = jb.rev ? 0 : 1;
-  const float g2 = log2_decay(p.s, h), w_scale = jb.s_intra / jb.s_inter;
+  const float g2 = log2_decay(p.s, h);
   const int64_t first = (int64_t)seg * p.s.seg;
   const float* ab = (const float*)jb.a.p + (int64_t)b * jb.a.sb + (int64_t)h * jb.a.sh + first * jb.a.st;
   const float* bb = (const float*)jb.b.p + (int64_t)b * jb.b.sb + (int64_t)h * jb.b.sh + first * jb.b.st;
@@ -339,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) rows_f32_kernel(RowsParams p) {
           yb[(int64_t)(jb.rev ? n - 1 - t : t) * jb.y_st + col0 + l32] = jb.s_intra * intra[r] + jb.s_inter * power(g2, i + lag) * inter[r];
       }
     }
-    state_update<D, false>(acc, none, tb, tc, min(kChunk, n - c0), g2, 1 - lag, w_scale, w, lane);
+    state_update<D, false>(acc, none, tb, tc, min(kChunk, n - c0), g2, 1 - lag, jb.w_scale, w, lane);
     __syncthreads();
   }
 }
@@ -761,9 +772,9 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
   };
   put_state(pi32(l32), g);
   // weights of a unit's tokens in the state after it (backwards, before it): whole units
-  if (tid < UNIT) wt[tid] = jb.s_intra / jb.s_inter * power(g2, rev ? tid + 1 : UNIT - 1 - tid);
+  if (tid < UNIT) wt[tid] = jb.w_scale * power(g2, rev ? tid + 1 : UNIT - 1 - tid);
   // decay between the tokens of a tile and its edge on the rows' side
-  if (tid < 32) edge[tid] = power(g2, rev ? tid : 31 - tid);
+  if (tid < 32) edge[tid] = jb.in_unit * power(g2, rev ? tid : 31 - tid);
 
   // One step a chunk: the unit's first one starts its rows, its last one stores them and passes the state on.
   bf16x8 a[KS];
@@ -808,7 +819,7 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
     const int lg = ln >> 5, lr = ln & 31;
     if (c == 0) {
       // the carried state's part
-      const float fs = jb.s_inter / jb.s_intra * power(g2, rev ? max(0, m - 1 - (32 * rt + lr)) : 32 * rt + lr + 1);
+      const float fs = jb.x_in_unit * power(g2, rev ? max(0, m - 1 - (32 * rt + lr)) : 32 * rt + lr + 1);
       if (any) {
 #pragma unroll
         for (int x = 0; x < Q; ++x) f[0][x] = rd.rows_pi(xl, 0, x);
@@ -856,7 +867,7 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int steps = rev ? acc_row(r, lg) - lr : lr - acc_row(r, lg);
-            s[jh][r] = steps >= 0 ? s[jh][r] * power(g2, steps) : 0.f;
+            s[jh][r] = steps >= 0 ? s[jh][r] * (jb.in_unit * power(g2, steps)) : 0.f;
           }
         } else if (jh >= lo && jh < hi) {
           const float fj = power(g2, rev ? 32 * (jh - at) - lr : 32 * (at - jh) + lr - 31);
@@ -921,7 +932,7 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
         for (int hf = 0; hf < 2; ++hf) {
           bf16x8 o;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = (bf16_t)(jb.s_intra * y[et][8 * hf + e]);
+          for (int e = 0; e < 8; ++e) o[e] = (bf16_t)(jb.unit * y[et][8 * hf + e]);
           *(bf16x8*)(at + 32 * et + 16 * hf) = o;
         }
     }
@@ -1284,7 +1295,7 @@ int run_fwd(const wa_decay_fwd_args* a, hipStream_t st) {
   hipLaunchKernelGGL(carry_kernel, dim3(D * D / kThreads, s.B * s.H), dim3(kThreads), 0, st, cp);
   RowsParams p{};
   p.s = s;
-  p.job[0] = Job{q, k, v, a->o, a->o_sb, a->o_st, a->o_sh, a->states, 0, 0, a->scale, a->scale};
+  p.job[0] = rows_job(q, k, v, a->o, a->o_sb, a->o_st, a->o_sh, a->states, false, false, a->scale);
   all_rows<D>(a->dtype, p, 1, st);
   return wa_launch_status("decay_fwd");
 }
@@ -1310,9 +1321,9 @@ int run_bwd(const wa_decay_bwd_args* a, hipStream_t st) {
   hipLaunchKernelGGL(carry_kernel, dim3(D * D / kThreads, s.B * s.H), dim3(kThreads), 0, st, cp);
   RowsParams p{};
   p.s = s;
-  p.job[0] = Job{d, v, k, a->dq, a->dq_sb, a->dq_st, a->dq_sh, a->states, 1, 0, a->scale, a->scale};
-  p.job[1] = Job{k, q, d, a->dv, a->dv_sb, a->dv_st, a->dv_sh, Y, 0, 1, a->scale, 1.f};
-  p.job[2] = Job{v, d, q, a->dk, a->dk_sb, a->dk_st, a->dk_sh, Y, 1, 1, a->scale, 1.f};
+  p.job[0] = rows_job(d, v, k, a->dq, a->dq_sb, a->dq_st, a->dq_sh, a->states, true, false, a->scale);
+  p.job[1] = rows_job(k, q, d, a->dv, a->dv_sb, a->dv_st, a->dv_sh, Y, false, true, a->scale);
+  p.job[2] = rows_job(v, d, q, a->dk, a->dk_sb, a->dk_st, a->dk_sh, Y, true, true, a->scale);
   all_rows<D>(a->dtype, p, 3, st);
   if (a->dlog_decay) {
     const PairsParams pp{s, q, k, v, d, part, n_part, s.n_seg + D * D / kThreads, a->scale};
