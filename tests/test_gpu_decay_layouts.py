@@ -61,3 +61,17 @@ def test_tokens_that_share_memory(dtype, d, n, lengths, kinds):
     _, size = OT.decay_linear_attention(copies["q"], copies["k"].abs(), copies["v"].abs(), log_decay, initial_state=initial.abs(),
                                         lengths=lengths)
     assert ((got[1].double() - exact).abs() <= 2.0 ** -16 * size).all()
+
+
+def test_a_single_token_of_any_stride():
+    """One token says nothing about the distance between two: 2^24 elements of it are no reason to refuse."""
+    g = torch.Generator().manual_seed(1)
+    x = [_normal(g, 1, 1, H, 64) for _ in range(3)]
+    pool = torch.zeros(1 << 10, dtype=torch.bfloat16, device=DEV)
+    far = []
+    for i, t in enumerate(x):
+        far.append(pool[i * 256:].as_strided((1, 1, H, 64), (1 << 25, 1 << 24, 64, 1)))
+        far[-1].copy_(t)
+    log_decay = torch.tensor([-0.5, -0.1], device=DEV)
+    got, want = W.decay_linear_attention(*far, log_decay), W.decay_linear_attention(*x, log_decay)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

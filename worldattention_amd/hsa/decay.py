@@ -22,7 +22,9 @@ def _ready(t: torch.Tensor) -> torch.Tensor:
     """``t`` in rows that the kernels take: 16-byte aligned, tokens at most 2^23 elements apart and, in bf16 (whose kernels
     cut rows off by a byte range), each behind the one before it: expanded and overlapping tokens are copied."""
     shared = t.dtype is torch.bfloat16 and t.shape[1] > 1 and t.stride(1) < t.shape[3]
-    return _lib.kernel_ready(t.contiguous() if shared or t.stride(1) > 1 << 23 else t, t.dtype, 16 // t.element_size())
+    if shared or t.stride(1) > 1 << 23:
+        t = t.clone(memory_format=torch.contiguous_format)   # contiguous() leaves a single token's stride as it is
+    return _lib.kernel_ready(t, t.dtype, 16 // t.element_size())
 
 
 def _forward(q, k, v, log_decay, initial, lengths, scale, want_derivs=False):
