@@ -75,3 +75,23 @@ def test_a_single_token_of_any_stride():
     log_decay = torch.tensor([-0.5, -0.1], device=DEV)
     got, want = W.decay_linear_attention(*far, log_decay), W.decay_linear_attention(*x, log_decay)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_states_on_any_address():
+    """An initial state and a final state's gradient that begin on no 16-byte boundary."""
+    g = torch.Generator().manual_seed(2)
+    x = {name: _normal(g, 1, 70, H, 64) for name in "qkv"}
+    dout = _normal(g, 1, 70, H, 64)
+    log_decay = torch.tensor([-0.5, -0.1], device=DEV)
+    initial, dfinal = (_normal(g, 1, H, 64, 64, dtype=torch.float32) for _ in range(2))
+    odd = []
+    for t in (initial, dfinal):
+        pool = torch.zeros(t.numel() + 1, device=DEV)
+        odd.append(pool[1:].view(t.shape))
+        odd[-1].copy_(t)
+    want = _run(x, log_decay, initial, None, dout, dfinal)
+    leaves = {name: t.detach().clone().requires_grad_(True) for name, t in x.items()}
+    decay, state = log_decay.clone().requires_grad_(True), odd[0].requires_grad_(True)
+    out, final = W.decay_linear_attention(leaves["q"], leaves["k"], leaves["v"], decay, initial_state=state)
+    got = (out.detach(), final.detach(), *torch.autograd.grad((out, final), (*leaves.values(), decay, state), (dout, odd[1])))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1357,8 +1357,8 @@ extern "C" int wa_decay_fwd(const wa_decay_fwd_args* a, void* stream) {
   WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->log_decay && a->states, "decay_fwd: null tensor");
   const int64_t wr = apart_written(a->L, a->D), rd = apart_read(a->dtype, a->L, a->D);
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh, a->dtype, rd) && rows16(a->k, a->k_sb, a->k_st, a->k_sh, a->dtype, rd) &&
-               rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype, rd) && rows16(a->o, a->o_sb, a->o_st, a->o_sh, a->dtype, wr) &&
-               wa_aligned16(a->states) && wa_aligned16(a->initial) && wa_aligned16(a->final_state), "decay_fwd: rows and states must be 16-byte aligned, tokens at most 2^23 elements apart and, written or in bf16, not overlapping");
+               rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype, rd) && rows16(a->o, a->o_sb, a->o_st, a->o_sh, a->dtype, wr),
+               "decay_fwd: rows must be 16-byte aligned, tokens at most 2^23 elements apart and, written or in bf16, not overlapping");
   hipStream_t s = (hipStream_t)stream;
   return a->D == 128 ? run_fwd<128>(a, s) : run_fwd<64>(a, s);
 }
@@ -1376,8 +1376,7 @@ extern "C" int wa_decay_bwd(const wa_decay_bwd_args* a, void* stream) {
                rows16(a->v, a->v_sb, a->v_st, a->v_sh, a->dtype, rd) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh, a->dtype, rd) &&
                rows16(a->dq, a->dq_sb, a->dq_st, a->dq_sh, a->dtype, wr) && rows16(a->dk, a->dk_sb, a->dk_st, a->dk_sh, a->dtype, wr) &&
                rows16(a->dv, a->dv_sb, a->dv_st, a->dv_sh, a->dtype, wr) &&
-               wa_aligned16(a->states) && wa_aligned16(a->workspace) && wa_aligned16(a->dfinal) && wa_aligned16(a->dinitial),
-               "decay_bwd: rows, states and workspace must be 16-byte aligned, tokens at most 2^23 elements apart and, written or in bf16, not overlapping");
+               wa_aligned16(a->workspace), "decay_bwd: rows and workspace must be 16-byte aligned, tokens at most 2^23 elements apart and, written or in bf16, not overlapping");
   hipStream_t s = (hipStream_t)stream;
   return a->D == 128 ? run_bwd<128>(a, s) : run_bwd<64>(a, s);
 }
