@@ -171,4 +171,6 @@ def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_dec
     args = _lib.DecayStepArgs(*_lib.blhd(q), *_lib.blhd(k), *_lib.blhd(v), *_lib.blhd(out), dtype, bsz, length, heads, d, dv,
                               log_decay.data_ptr(), state.data_ptr(), s_sb, s_sh, d ** -0.5 if scale is None else float(scale))
     _lib.launch("wa_decay_step", args, dev)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)   # a graph that saved the state must not use what it has become
     return out
