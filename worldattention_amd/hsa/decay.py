@@ -32,6 +32,9 @@ def _forward(q, k, v, log_decay, initial, lengths, scale, want_derivs=False):
     bsz, length, heads, d = q.shape
     f32 = dict(dtype=torch.float32, device=dev)
     out = torch.empty((bsz, length, heads, d), dtype=q.dtype, device=dev)
+    if out.numel() == 0:      # no tokens: the state passes through
+        final = torch.zeros((bsz, heads, d, d), **f32) if initial is None else initial.clone()
+        return out, final, None, None
     final = torch.empty((bsz, heads, d, d), **f32)
     n_seg = _lib.sizes("wa_decay_segments", bsz, length, heads, int(want_derivs))
     states = torch.empty((bsz, heads, n_seg, d, d), **f32)
@@ -61,6 +64,12 @@ class _DecayLinear(torch.autograd.Function):
         dev = q.device
         bsz, length, heads, d = q.shape
         f32 = dict(dtype=torch.float32, device=dev)
+        if q.numel() == 0:
+            dlog = torch.zeros((heads,), **f32) if ctx.needs_input_grad[3] else None
+            dinitial = None
+            if ctx.needs_input_grad[4]:
+                dinitial = torch.zeros((bsz, heads, d, d), **f32) if dfinal is None else dfinal.clone()
+            return *(torch.zeros_like(t) for t in (q, k, v)), dlog, dinitial, None, None
         dout = torch.zeros_like(q, memory_format=torch.contiguous_format) if dout is None else _ready(dout)
         dfinal = None if dfinal is None else dfinal.contiguous()
         dq, dk, dv = (torch.empty((bsz, length, heads, d), dtype=q.dtype, device=dev) for _ in range(3))
@@ -117,10 +126,6 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     dev = _lib.require_gpu(q, k, v, log_decay, initial_state, lengths)
     _lib.dtype_code(q)
     scale = max(d, 1) ** -0.5 if scale is None else float(scale)
-    if q.numel() == 0 or v.numel() == 0:
-        state = (torch.zeros((bsz, heads, d, dv), dtype=torch.float32, device=dev) if initial_state is None
-                 else initial_state.clone())
-        return v.clone() if v.numel() == 0 else v.new_zeros(v.shape), state
     if d != dp:
         q, k = (torch.nn.functional.pad(t, (0, dp - d)) for t in (q, k))
     if dv != dp:
