@@ -726,8 +726,9 @@ int wa_hkv_gather_rotate(const wa_hkv_gather_rotate_args* args, void* stream);
  * positions[b, t, axis(p)] * inv_freq[p] (its negative with `inverse`: the gradient); the pairs are
  * dealt to the axes in runs of sections[0], sections[1], ... pairs (n_axes of them, 4 at most).
  * Pair p holds channels (2p, 2p + 1) with `interleaved`, else (p, p + P) of P pairs; channels from
- * 2P on are copied. The angle is formed and reduced in fp64, its sine and cosine and the rotation
- * are fp32, the result is rounded once to the tensors' dtype. positions: device int64 (pos_int64)
+ * 2P on are copied. The angle is formed and reduced in two doubles (its fraction of a revolution is off by
+ * less than 2^-40 at any position, frequencies up to 1), its sine and cosine and the rotation are fp32,
+ * the result is rounded once to the tensors' dtype. positions: device int64 (pos_int64)
  * or int32 with element strides (p_sb = 0: shared by the batch). q_out / k_out must not overlap
  * the inputs. */
 #define WA_ROPE_MAX_AXES 4

@@ -3,8 +3,9 @@
 // of the QKV epilogue (cache.hip): positions are given per token and axis, so text, action and image
 // tokens mix freely and lie as far out as an integer reaches.
 //
-// Angle: position * inv_freq in fp64, taken to revolutions and reduced there (at position 10^6 and
-// frequency 1 an fp32 angle is off by 0.03 rad; the fp64 one's error stays below 10^-9), then one
+// Angle: position * inv_freq in revolutions, reduced from a product of two doubles that keeps the bits of
+// its fraction: off by less than 2^-40 of a revolution at any 64-bit position and frequencies up to 1 (at
+// position 10^6 and frequency 1 an fp32 angle is off by 0.03 rad; an fp64 one is at 2^40 by 10^-4). Then one
 // fp32 sine and cosine of the reduced angle. A workgroup forms them once per (token, pair) in LDS and
 // uses them for its heads, so the fp64 part is 1 / heads of the work.
 #include <algorithm>
@@ -35,6 +36,19 @@ struct RopeAxesParams {
 
 // u / n by n's constant floor(2^32 / n) + 1 (0 for n = 1), exact for u n < 2^32.
 __device__ __forceinline__ uint32_t div_by(uint32_t u, uint32_t magic) { return magic ? __umulhi(u, magic) : u; }
+
+// The fraction, -1/2 to 1/2, of position * freq / (2 pi). 1 / (2 pi) and the revolutions of a step (freq / (2 pi)) are
+// sums of two doubles, 2^-105 relative; the position is cut into 53 bits, a double, and the 11 behind them.
+__device__ __forceinline__ double revolutions(int64_t position, double freq) {
+#pragma clang fp contract(off)   // a product fused into the difference below would count its rounding twice
+  constexpr double kInv = 0.15915494309189535, kInvLow = -9.839338337591243e-18;
+  const double step = freq * kInv, low = fma(freq, kInv, -step) + freq * kInvLow;
+  const int64_t tail = position & 2047;
+  const double head = (double)(position - tail), whole = head * step;
+  // whole - rint(whole) is exact, as the product's rounding is; the other two terms stay below 2^12
+  const double x = (whole - rint(whole)) + (fma(head, step, -whole) + fma(head, low, (double)tail * step));
+  return x - rint(x);
+}
 
 template <typename T, int VEC>
 struct Chunk {
@@ -84,10 +98,9 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(RopeAxesParams p) {
 #pragma unroll
     for (int a = 0; a < WA_ROPE_MAX_AXES - 1; ++a) axis += pr >= p.sec_end[a];
     const int64_t at = (int64_t)b * p.p_sb + (int64_t)(t0 + r) * p.p_st + (int64_t)axis * p.p_sa;
-    const double pos = p.pos64 ? (double)((const int64_t*)p.pos)[at] : (double)((const int32_t*)p.pos)[at];
-    const double rev = pos * p.inv_freq[pr] * 0.15915494309189533577;  // 1 / (2 pi)
+    const int64_t pos = p.pos64 ? ((const int64_t*)p.pos)[at] : (int64_t)((const int32_t*)p.pos)[at];
     float s, c;
-    sincospif(2.f * (float)(rev - rint(rev)), &s, &c);
+    sincospif(2.f * (float)revolutions(pos, p.inv_freq[pr]), &s, &c);
     turn[i] = float2{c, p.inverse ? -s : s};
   }
   __syncthreads();

@@ -89,7 +89,8 @@ def rope_axes(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, 
     * ``interleaved``: pair ``p`` is channels ``(2p, 2p + 1)`` (the model's own layout); otherwise
       ``(p, p + P)``.
 
-    bf16 or fp32; angles in fp64, rotation in fp32, one rounding. Returns new contiguous tensors (``q``'s,
+    bf16 or fp32; the angle's fraction of a revolution is exact to 2^-40 at any position (frequencies up to 1), the
+    rotation is fp32, one rounding. Returns new contiguous tensors (``q``'s,
     or ``(q, k)``'s). Differentiable once in ``q`` and ``k``. To capture a backward pass in a graph, capture its
     forward pass too, and let no eager graph of the same leaves live then.
     """
