@@ -26,6 +26,7 @@
 // exact parts. In the rows of bf16 tensors, whose results leave in bf16, the decayed q.k and the running
 // state's weighted operand round to bf16 once; the state itself enters in two parts (2^-17).
 #include <algorithm>
+#include <cmath>
 
 #include "tile.h"
 
@@ -89,15 +90,16 @@ struct Job {
   float s_intra, s_inter;
   float w_scale;                  // of the state's own tokens: s_inter X sums s_intra b c^T
   float unit, in_unit, x_in_unit; // bf16 rows sum y / unit: s_intra and s_inter in it
+  float in_log2;                  // log2 of s_intra in the unit, for weights formed as one exponential
 };
 // time forwards, the carried state holds bare sums: both parts take the scale; backwards it holds scaled ones.
 // The unit is the scale, which then stays out of the products. One of 0, or so small or large that its
-// reciprocal times a row of the state could leave fp32, cannot be divided by: the unit is then 1.
+// reciprocal times a row of the state could leave fp32, cannot be divided by: the unit is then 1 with its sign.
 Job rows_job(const View& a, const View& b, const View& c, void* y, int64_t y_sb, int64_t y_st, int64_t y_sh, const float* x, bool x_trans,
              bool rev, float scale) {
   const float s_inter = rev ? 1.f : scale, size = scale < 0.f ? -scale : scale;
-  const float unit = size >= 0x1p-32f && size <= 0x1p32f ? scale : 1.f;
-  return Job{a, b, c, y, y_sb, y_st, y_sh, x, x_trans, rev, scale, s_inter, rev ? scale : 1.f, unit, scale / unit, s_inter / unit};
+  const float unit = size >= 0x1p-32f && size <= 0x1p32f ? scale : scale < 0.f ? -1.f : 1.f;
+  return Job{a, b, c, y, y_sb, y_st, y_sh, x, x_trans, rev, scale, s_inter, rev ? scale : 1.f, unit, scale / unit, s_inter / unit, std::log2(scale / unit)};
 }
 struct RowsParams {
   Shape s;
@@ -776,6 +778,8 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
   // decay between the tokens of a tile and its edge on the rows' side
   if (tid < 32) edge[tid] = jb.in_unit * power(g2, rev ? tid : 31 - tid);
 
+  float in_log2 = jb.in_log2;     // a register: read where it is used, it would come from memory there
+  asm volatile("" : "+s"(in_log2));
   // One step a chunk: the unit's first one starts its rows, its last one stores them and passes the state on.
   bf16x8 a[KS];
   auto load_rows = [&](int t, int half) {     // the operands of row t of the segment
@@ -867,7 +871,7 @@ __global__ void __launch_bounds__(64 * (D / 16)) rows_bf16_kernel(RowsParams p) 
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int steps = rev ? acc_row(r, lg) - lr : lr - acc_row(r, lg);
-            s[jh][r] = steps >= 0 ? s[jh][r] * (jb.in_unit * power(g2, steps)) : 0.f;
+            s[jh][r] = steps >= 0 ? s[jh][r] * __builtin_amdgcn_exp2f(__builtin_fmaf(g2, (float)steps, in_log2)) : 0.f;
           }
         } else if (jh >= lo && jh < hi) {
           const float fj = power(g2, rev ? 32 * (jh - at) - lr : 32 * (at - jh) + lr - 31);
