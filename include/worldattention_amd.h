@@ -805,7 +805,8 @@ typedef struct wa_decay_bwd_args {
 int wa_decay_bwd(const wa_decay_bwd_args* args, void* stream);
 
 /* The same recurrence for L tokens (one, as a decoding step makes it, or a few), one after the other,
- * with the fp32 state [B, H, D, Dv] (strides st_sb, st_sh; rows contiguous) updated in place. Any
+ * with the fp32 state [B, H, D, Dv] (strides st_sb, st_sh; rows contiguous; no two states may share
+ * memory) updated in place. Any
  * head dims 1 .. 256; bf16 or fp32 tensors of any strides with contiguous channels. */
 typedef struct wa_decay_step_args {
   const void* q; int64_t q_sb, q_st, q_sh;

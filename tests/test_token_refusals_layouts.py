@@ -2,8 +2,10 @@
 import ctypes
 
 import pytest
+import torch
 
 from worldattention_amd import _lib
+from worldattention_amd import hsa as W
 
 FAKE = 1 << 20
 
@@ -32,3 +34,38 @@ def test_decay_refuses_tokens_that_share_memory(fn, cls, read, written, dtype):
             setattr(a, field, st)
             assert getattr(_lib.lib(), fn)(ctypes.byref(a), None) == _lib.WA_ERR_ARG, (field, st)
             assert b"overlapping" in _lib.lib().wa_last_error()
+
+
+def _state(b, h, sb, sh):
+    return torch.zeros(4096).as_strided((b, h, 4, 8), (sb, sh, 8, 1))
+
+
+def _step(state):
+    b, h = state.shape[:2]
+    x = [torch.zeros(b, 1, h, d) for d in (4, 4, 8)]
+    return W.decay_linear_step(*x, torch.zeros(h), state)
+
+
+@pytest.mark.parametrize("b,h,sb,sh", [(2, 1, 31, 32), (1, 2, 64, 16), (2, 3, 64, 32), (2, 2, 32, 32), (3, 2, 32, 64), (2, 2, 70, 100),
+                                       (2, 2, 0, 32), (4, 1, 1, 0), (3, 3, 33, 49)])
+def test_decay_step_refuses_states_that_share_memory(b, h, sb, sh):
+    """Two workgroups would update the same elements."""
+    with pytest.raises(ValueError, match="memory of its own"):
+        _step(_state(b, h, sb, sh))
+
+
+@pytest.mark.parametrize("b,h,sb,sh", [(2, 3, 96, 32), (2, 3, 32, 64), (1, 1, 0, 0), (1, 3, 0, 32), (3, 1, 40, 7), (2, 3, 48, 32 + 64), (2, 2, 40, 72),
+                                       (2, 3, 100, 66)])
+def test_decay_step_takes_states_apart(b, h, sb, sh):
+    """Past the layouts' check, to the one for a GPU."""
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        _step(_state(b, h, sb, sh))
+
+
+def test_decay_step_entry_point_refuses_one_state_for_two():
+    a = _lib.DecayStepArgs()
+    a.q = a.k = a.v = a.o = a.log_decay = a.state = FAKE
+    a.B, a.L, a.H, a.D, a.Dv, a.dtype = 2, 1, 3, 64, 64, _lib.WA_F32
+    for sb, sh in ((0, 4096), (4096, 0), (4096, 4096)):
+        a.st_sb, a.st_sh = sb, sh
+        assert _lib.lib().wa_decay_step(ctypes.byref(a), None) == _lib.WA_ERR_ARG and b"share memory" in _lib.lib().wa_last_error()

@@ -1394,6 +1394,8 @@ extern "C" int wa_decay_step(const wa_decay_step_args* a, void* stream) {
                (long long)a->B, (long long)a->L, (long long)a->H);
   if (a->B == 0 || a->L == 0 || a->H == 0) return WA_OK;
   WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->log_decay && a->state, "decay_step: null tensor");
+  WA_CHECK_ARG((a->B == 1 || a->st_sb != 0) && (a->H == 1 || a->st_sh != 0) && (a->B == 1 || a->H == 1 || a->st_sb != a->st_sh),
+               "decay_step: states must not share memory");
   const StepParams p{View{a->q, a->q_sb, a->q_st, a->q_sh}, View{a->k, a->k_sb, a->k_st, a->k_sh}, View{a->v, a->v_sb, a->v_st, a->v_sh},
                      a->o, a->o_sb, a->o_st, a->o_sh, (int)a->L, (int)a->H, (int)a->D, (int)a->Dv, (int)a->dtype,
                      a->log_decay, a->state, a->st_sb, a->st_sh, a->scale};

@@ -147,6 +147,16 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     return out, final
 
 
+def _apart(n: int, sn: int, m: int, sm: int, size: int) -> bool:
+    """Whether ``n`` times ``m`` runs of ``size`` elements, strides ``sn`` and ``sm``, lie in memory of their own."""
+    if (m == 1 or sm >= size) and (n == 1 or sn >= (m - 1) * sm + size):
+        return True
+    if (n == 1 or sn >= size) and (m == 1 or sm >= (n - 1) * sn + size):
+        return True
+    starts = sorted(i * sn + j * sm for i in range(n) for j in range(m))   # neither within the other: one by one
+    return all(y - x >= size for x, y in zip(starts, starts[1:]))
+
+
 def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, *,
                       scale: Optional[float] = None) -> torch.Tensor:
     """The recurrence for single tokens: ``[B, L, H, D]`` with ``L`` 1 (or a few, one after the other), ``state``
@@ -161,7 +171,7 @@ def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_dec
     s_sb, s_sh, s_row, s_col = state.stride()
     if s_col != 1 or (d > 1 and s_row != dv):
         raise ValueError("the state's [D, Dv] matrices must be contiguous")
-    if (bsz > 1 and s_sb == 0) or (heads > 1 and s_sh == 0):
+    if not _apart(bsz, s_sb, heads, s_sh, d * dv):
         raise ValueError("the state is updated in place: every sequence and head needs memory of its own")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or state.requires_grad):
