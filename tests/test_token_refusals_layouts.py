@@ -69,3 +69,17 @@ def test_decay_step_entry_point_refuses_one_state_for_two():
     for sb, sh in ((0, 4096), (4096, 0), (4096, 4096)):
         a.st_sb, a.st_sh = sb, sh
         assert _lib.lib().wa_decay_step(ctypes.byref(a), None) == _lib.WA_ERR_ARG and b"share memory" in _lib.lib().wa_last_error()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-50, -1e-46, 7e-46])
+def test_selected_attention_refuses_a_scale_of_zero_in_fp32(scale):
+    """The library reads 0 as the default, so a scale that rounds to 0 would have been taken for D ** -0.5."""
+    q, k = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 64, 2, 64, dtype=torch.bfloat16)
+    index, num = torch.zeros(1, 1, 2, 1, dtype=torch.int32), torch.ones(1, 1, 2, dtype=torch.int32)
+    cache = {"k": k, "v": k, "k_block_sums": torch.zeros(1, 2, 1, 64), "k_block_sums_block_size": 64}
+    with pytest.raises(ValueError, match="scale"):
+        W.selected_attention(q, k, k, index, num, 64, block_size=64, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        W.attend_selected(q, cache, 64, topk=2, scale=scale)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):     # the smallest that fp32 holds
+        W.selected_attention(q, k, k, index, num, 64, block_size=64, scale=2.0 ** -149)

@@ -11,6 +11,7 @@ There is no gradient: training at this granularity runs
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -101,6 +102,16 @@ def _attend(q, k, v, index, num, kv_len, bs, scale):
     return out, lse
 
 
+def _scale_arg(scale: Optional[float]) -> float:
+    """The kernel's fp32 scale, whose 0 stands for the default."""
+    if scale is None:
+        return 0.0
+    scale = float(scale)
+    if ctypes.c_float(scale).value == 0.0:
+        raise ValueError(f"scale must not be 0 in fp32, got {scale}")
+    return scale
+
+
 def _check_budget(topk: int, sink: int, local: int) -> None:
     if sink < 0 or local < 1 or sink + local > topk or topk > _lib.SELECT_MAX_BLOCKS:
         raise ValueError(f"topk {topk} (at most {_lib.SELECT_MAX_BLOCKS}) must hold {sink} sink and {local} (at least 1) local "
@@ -172,12 +183,10 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
     if index.dtype != torch.int32 or num.dtype != torch.int32 or not 1 <= index.shape[3] <= _lib.SELECT_MAX_BLOCKS:
         raise ValueError(f"index / num must be int32 with 1 to {_lib.SELECT_MAX_BLOCKS} ids a row, got {index.dtype}, {num.dtype} "
                          f"and {index.shape[3]}")
-    if scale is not None and float(scale) == 0.0:
-        raise ValueError("scale must not be 0")
+    scale = _scale_arg(scale)
     _no_gradient(q, k, v)
     _lib.require_gpu(q, k, v, index, num, kv_len if isinstance(kv_len, torch.Tensor) else None)
-    return _attend(_lib.kernel_ready(q), k, v, index.contiguous(), num.contiguous(), kv_len, block_size,
-                   0.0 if scale is None else float(scale))
+    return _attend(_lib.kernel_ready(q), k, v, index.contiguous(), num.contiguous(), kv_len, block_size, scale)
 
 
 def attend_selected(q: torch.Tensor, kv_cache: dict, kv_len: KvLen, *, topk: int, sink_blocks: int = 1,
@@ -195,11 +204,10 @@ def attend_selected(q: torch.Tensor, kv_cache: dict, kv_len: KvLen, *, topk: int
     if sums.shape != (bsz, hk, -(-cap // bs), d):
         raise ValueError(f"k_block_sums must be [{bsz}, {hk}, {-(-cap // bs)}, {d}], got {tuple(sums.shape)}")
     _check_budget(topk, sink_blocks, local_blocks)
-    if scale is not None and float(scale) == 0.0:
-        raise ValueError("scale must not be 0")
+    scale = _scale_arg(scale)
     _no_gradient(q, k, v, sums)
     _lib.require_gpu(q, k, v, sums, kv_len if isinstance(kv_len, torch.Tensor) else None)
     q = _lib.kernel_ready(q)
     chosen = _select(q, sums, kv_len, bs, int(topk), int(sink_blocks), int(local_blocks), cap)
-    out, lse = _attend(q, k, v, chosen.index, chosen.num, kv_len, bs, 0.0 if scale is None else float(scale))
+    out, lse = _attend(q, k, v, chosen.index, chosen.num, kv_len, bs, scale)
     return out, lse, chosen
