@@ -731,11 +731,13 @@ extern "C" int wa_selected_attn(const wa_selected_attn_args* a, void* stream) {
   WA_CHECK_ARG(a->cap >= 1 && a->cap <= INT32_MAX, "selected_attn: bad cache of %lld tokens", (long long)a->cap);
   WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->index && a->num, "selected_attn: null tensor");
   auto rows16 = [](const void* x, int64_t sb, int64_t st, int64_t sh) {
-    return wa_aligned16(x) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0 && st >= 0 && st <= (int64_t)1 << 24;
+    return wa_aligned16(x) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0;
   };
+  // a tile's keys and values at 32-bit offsets from its first one
+  auto near = [](int64_t st) { return st >= 0 && st <= (int64_t)1 << 24; };
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->k, a->k_sb, a->k_st, a->k_sh) && rows16(a->v, a->v_sb, a->v_st, a->v_sh) &&
-               rows16(a->o, a->o_sb, a->o_st, a->o_sh),
-               "selected_attn: rows must be 16-byte aligned, tokens at most 2^24 elements apart");
+               rows16(a->o, a->o_sb, a->o_st, a->o_sh) && near(a->k_st) && near(a->v_st),
+               "selected_attn: rows must be 16-byte aligned, a cache's tokens at most 2^24 elements apart");
   AttnParams p{};
   p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.k = (const bf16_t*)a->k; p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
