@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from worldattention_amd import _lib
 from worldattention_amd import hsa as W
@@ -83,3 +84,40 @@ def test_selected_attention_refuses_a_scale_of_zero_in_fp32(scale):
         W.attend_selected(q, cache, 64, topk=2, scale=scale)
     with pytest.raises(RuntimeError, match="ROCm GPU"):     # the smallest that fp32 holds
         W.selected_attention(q, k, k, index, num, 64, block_size=64, scale=2.0 ** -149)
+
+
+def _calls():
+    """Each operator on CPU tensors, by the argument that a tangent rides on."""
+    def f(*shape):
+        return torch.zeros(*shape)
+
+    def b(*shape):
+        return torch.zeros(*shape, dtype=torch.bfloat16)
+
+    pos, inv = torch.zeros(5, 1, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
+    x, state, g = f(1, 5, 2, 64), f(1, 2, 64, 64), f(2)
+    index, num = torch.zeros(1, 1, 2, 1, dtype=torch.int32), torch.ones(1, 1, 2, dtype=torch.int32)
+    kv, sums = b(1, 64, 2, 64), f(1, 2, 1, 64)
+    cache = {"k": kv, "v": kv, "k_block_sums": sums, "k_block_sums_block_size": 64}
+    yield "rope_axes", x, lambda t: W.rope_axes(t, pos, inv, (32,))
+    yield "rope_axes k", x, lambda t: W.rope_axes(x, pos, inv, (32,), k=t)
+    yield "rope_axes inv_freq", inv, lambda t: W.rope_axes(x, pos, t, (32,))
+    yield "decay v", x, lambda t: W.decay_linear_attention(x, x, t, g)
+    yield "decay log_decay", g, lambda t: W.decay_linear_attention(x, x, x, t)
+    yield "decay initial_state", state, lambda t: W.decay_linear_attention(x, x, x, g, initial_state=t)
+    yield "step q", x, lambda t: W.decay_linear_step(t, x, x, g, state)
+    yield "step state", state, lambda t: W.decay_linear_step(x, x, x, g, t)
+    yield "select q", b(1, 1, 2, 64), lambda t: W.select_key_blocks(t, sums, 64, block_size=64, topk=2)
+    yield "selected_attention v", kv, lambda t: W.selected_attention(b(1, 1, 2, 64), kv, t, index, num, 64, block_size=64)
+    yield "attend_selected sums", sums, lambda t: W.attend_selected(b(1, 1, 2, 64), dict(cache, k_block_sums=t), 64, topk=2)
+
+
+@pytest.mark.parametrize("name,t,call", list(_calls()), ids=[c[0] for c in _calls()])
+def test_tangents_are_refused(name, t, call):
+    """A dual tensor would lose its tangent: the kernels read the primal values alone."""
+    with forward_ad.dual_level():
+        for enabled in (True, False):
+            with torch.set_grad_enabled(enabled), pytest.raises(ValueError, match="forward-mode"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
+            with torch.set_grad_enabled(enabled), pytest.raises(RuntimeError, match="ROCm GPU"):
+                call(t)

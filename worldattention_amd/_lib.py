@@ -11,6 +11,7 @@ import os
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 
 # WORLDATTENTION_AMD_LIB selects another build of the library (e.g. to compare two builds); the
 # default is the in-tree build next to this file
@@ -547,6 +548,15 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
         elif t.device != dev:
             raise ValueError(f"tensors on different devices: {dev} and {t.device}")
     return dev
+
+
+def refuse_tangents(*tensors) -> None:
+    """Kernels read primal values alone: a forward-mode tangent would be dropped without a word."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("forward-mode differentiation (a dual tensor) is not supported")
 
 
 def dtype_code(t: torch.Tensor) -> int:

@@ -123,6 +123,7 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     dp = padded_head_dim(max(d, dv))
     if lengths is not None and (tuple(lengths.shape) != (bsz,) or lengths.dtype != torch.int32):
         raise ValueError(f"lengths must be int32 [{bsz}], got {lengths.dtype} {tuple(lengths.shape)}")
+    _lib.refuse_tangents(q, k, v, log_decay, initial_state)
     dev = _lib.require_gpu(q, k, v, log_decay, initial_state, lengths)
     _lib.dtype_code(q)
     scale = max(d, 1) ** -0.5 if scale is None else float(scale)
@@ -176,6 +177,7 @@ def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_dec
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or state.requires_grad):
         raise ValueError("decay_linear_step takes no gradient (decay_linear_attention does): call it under torch.no_grad()")
+    _lib.refuse_tangents(q, k, v, log_decay, state)
     dev = _lib.require_gpu(q, k, v, log_decay, state)
     dtype = _lib.dtype_code(q)
     out = torch.empty(bsz, length, heads, dv, dtype=q.dtype, device=dev)

@@ -117,6 +117,7 @@ def rope_axes(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, 
         raise ValueError(f"inv_freq must be [{pairs}] in fp64 or fp32, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
     if inv_freq.requires_grad and torch.is_grad_enabled():
         raise ValueError("inv_freq takes no gradient: detach it")
+    _lib.refuse_tangents(q, k, inv_freq)
     _lib.require_gpu(q, k, positions, inv_freq)
     _lib.dtype_code(q)
     inv_freq = inv_freq.double().contiguous()

@@ -49,6 +49,7 @@ def _check_query(q, kv_heads: int, bsz: int, d: int, block_size: int, kv_len: Kv
 
 
 def _no_gradient(*tensors) -> None:
+    _lib.refuse_tangents(*tensors)
     if not torch.is_grad_enabled():
         return
     for t in tensors:
