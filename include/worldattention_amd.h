@@ -827,8 +827,10 @@ int wa_decay_step(const wa_decay_step_args* args, void* stream);
  * hk (H / Hk) .. (hk + 1)(H / Hk) - 1 read key head hk and share its choice. Chosen are the first
  * sink_blocks and the last local_blocks (>= 1) seen blocks and, up to topk in all, those whose
  *   score_j = (sum of the group's queries) . k_sums[b, hk, j]
- * is largest (formed in fp64, so neither the launch's shape nor the batch moves a border; ties take
- * the lowest id, NaN counts as the largest). Every scored block is whole, so the sums need no division.
+ * is largest (ties take the lowest id, NaN counts as the largest). Every scored block is whole, so the
+ * sums need no division. Scores are sums of D products in fp64, off by at most D 2^-52 of the sum of their
+ * magnitudes. Equal key sums tie exactly in every launch; other scores that are closer to each other than
+ * that can rank differently in a launch of one query and in one of several, which sum in another order.
  * k_sums: fp32 [B, Hk, n_blocks, D] as wa_kv_append keeps them. kv_len: device int32 [B] (NULL:
  * kv_len_all), clamped to [0, cap]; cap <= n_blocks * block_size (0: that).
  * index: int32 [B, n, Hk, topk], ascending, -1 behind; num: int32 [B, n, Hk]. D = 64 or 128. */

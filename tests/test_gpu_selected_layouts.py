@@ -58,3 +58,24 @@ def test_caches_whose_tokens_share_memory(n):
         for kv_len in (300, 257, 33, n):
             got, want = (W.attend_selected(q, c, kv_len, topk=5) for c in (shared, copies))
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,nb", [(1, 60), (1, 700), (1, 1500), (4, 60), (9, 700), (40, 700)])
+def test_equal_key_sums_tie_in_every_launch(d, n, nb):
+    """Blocks with one of five key sums: whole runs are chosen, and of the last one the lowest ids, for one query (either of
+    its forms), a few and many."""
+    g = torch.Generator().manual_seed(nb + n)
+    kinds = torch.randn(2, 5, d, generator=g) * 30
+    kind = torch.randint(0, 5, (2, nb), generator=g)
+    sums = torch.stack([kinds[h, kind[h]] for h in range(2)])[None].to(DEV)
+    q = torch.randn(1, n, 4, d, generator=g).bfloat16()
+    got = W.select_key_blocks(q.to(DEV), sums, nb * 64, block_size=64, topk=nb // 3, sink_blocks=0, local_blocks=1)
+    score = torch.einsum("nhd,hkd->nhk", q[0].double().view(n, 2, 2, d).sum(2), kinds.double())
+    assert (score.sort(-1).values.diff(dim=-1) > 1e-6).all()      # five different scores, far beyond any rounding
+    for i in range(n):
+        last = (nb * 64 - n + i) // 64      # the query's own block
+        for h in range(2):
+            order = sorted(range(last), key=lambda j: (-score[i, h, kind[h, j]].item(), j))
+            want = sorted(order[:nb // 3 - 1] + [last])
+            assert got.index[0, i, h].tolist() == want and got.num[0, i, h].item() == nb // 3

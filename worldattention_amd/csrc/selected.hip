@@ -21,9 +21,10 @@ __device__ __forceinline__ int64_t seen_tokens(const int32_t* kv_len, int64_t kv
 
 // =============================================================================================
 // Scores: (sum of a group's queries) . (block's key sum) in fp64, 16 queries x 16 blocks at a time
-// (v_mfma_f64_16x16x4): a query's sums and a key sum's products are exact in fp64 to 2^-52 of the score,
-// so the order of the products decides no choice. The sums are read once; a decoding step fills one
-// row of 16, which the fp64 matrix rate still hides behind the read.
+// (v_mfma_f64_16x16x4). D products and their sum are off by at most D 2^-52 of the sum of the products'
+// magnitudes, so only scores as close as that depend on the order of the products, of which there are two (a
+// single query's below); blocks of equal key sums take the same steps and tie in either. The sums are read
+// once; a decoding step fills one row of 16, which the fp64 matrix rate still hides behind the read.
 // =============================================================================================
 struct SelectParams {
   const bf16_t* q; int64_t q_sb, q_st, q_sh;
