@@ -1226,7 +1226,11 @@ __global__ void __launch_bounds__(kThreads) step_kernel(StepParams p) {
 // inside a segment grow with its length. Weights in us, fitted at 32,760 tokens of 12 x 128: 0.08 a token of a
 // round and rows launch (5 launches' worth in training, 1.4 with the state pass alone), 0.05 (0.2 with
 // derivatives) a segment, 2.8e-7 a token and token of segment. That call takes 21 segments of 1,600 tokens for its
-// output alone and 64 of 512 in training (the call 823 us; in 32 segments 888, 43 871, 86 923).
+// output alone and 64 of 512 in training (the call 823 us; in 32 segments 888, 43 871, 86 923). The weights and the
+// 256 are bf16's with D = 128, used for all: with D = 64 two workgroups fit a CU and half of a round stays empty (111
+// us for the same tokens and heads, 367 in training), and fp32's rows take longer than a weight says (4 heads of 8,190
+// tokens of 128: 80 us, 335 in training). Sequences count as full, whatever their lengths. "Training" is a call that
+// asks for the decays' gradient; with fixed decays the segments are the output's (590 us for the call above).
 int64_t segment_length(int64_t B, int64_t L, int64_t H, bool derivs) {
   const double rows = (double)(B * H);
   int64_t best = 0;
