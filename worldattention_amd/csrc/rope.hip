@@ -80,8 +80,8 @@ __device__ __forceinline__ void store_chunk(T* p, const Chunk<T, VEC>& c) {
 
 // A unit is the work of one thread at a time. Interleaved: VEC consecutive channels (the last unit of
 // an odd D holds one). Half-split: VEC pairs (p, p + P), or past the pairs VEC copied channels.
-// Bound by reading and writing every channel once: 40 heads x 32,760 tokens x 128 bf16 245 us (5.4 TB/s), one
-// token each of 16 sequences of 32 + 8 heads 3.5 us.
+// Bound by reading and writing every channel once: 40 heads x 32,760 tokens x 128 bf16 244 us (5.5 TB/s), one
+// token each of 16 sequences of 32 + 8 heads 3.7 us.
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(kThreads) rope_axes_kernel(RopeAxesParams p) {
   __shared__ float2 turn[kTurns];
