@@ -45,7 +45,7 @@ __device__ __forceinline__ double revolutions(int64_t position, double freq) {
   const double step = freq * kInv, low = fma(freq, kInv, -step) + freq * kInvLow;
   const int64_t tail = position & 2047;
   const double head = (double)(position - tail), whole = head * step;
-  // whole - rint(whole) is exact, as the product's rounding is; the other two terms stay below 2^12
+  // the difference is exact, and the first fma what the product rounded off; all but it stays below 2^12
   const double x = (whole - rint(whole)) + (fma(head, step, -whole) + fma(head, low, (double)tail * step));
   return x - rint(x);
 }

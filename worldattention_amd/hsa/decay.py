@@ -110,12 +110,13 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     * ``initial_state``: fp32 ``[B, H, D, Dv]``, the state before the first token (default 0).
     * ``lengths``: int32 ``[B]`` on the GPU: sequence ``b`` is its first ``lengths[b]`` tokens (clamped to
       ``[0, L]``); the tokens behind are not read, their outputs and gradients are 0.
-    * ``scale``: default ``D ** -0.5``.
+    * ``scale``: default ``D ** -0.5``; of any size, 0 too (the outputs are 0 then, the state is carried on).
 
-    At most 65,535 sequences times heads. Outputs have the inputs' dtype; the state is summed in fp32. Differentiable once, through both results, in
-    ``q``, ``k``, ``v``, ``log_decay`` and ``initial_state``. A value that is not finite in ``v`` (or, backwards,
-    in the gradient) reaches its 64-token neighbourhood, as it reaches a tile of softmax attention. To capture a
-    backward pass in a graph, capture its forward pass too, and let no eager graph of the same leaves live then.
+    At most 65,535 sequences times heads. Outputs have the inputs' dtype; the state is summed in fp32. Differentiable
+    once, through both results, in ``q``, ``k``, ``v``, ``log_decay`` and ``initial_state``. A value that is not finite in
+    ``v`` (or, backwards, in the gradient) reaches its 64-token neighbourhood, as it reaches a tile of softmax
+    attention. To capture a backward pass in a graph, capture its forward pass too, and let no eager graph of the same
+    leaves live then.
     """
     _check(q, k, v, log_decay, initial_state, "initial_state")
     bsz, length, heads, d = q.shape
@@ -162,7 +163,7 @@ def decay_linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_dec
                       scale: Optional[float] = None) -> torch.Tensor:
     """The recurrence for single tokens: ``[B, L, H, D]`` with ``L`` 1 (or a few, one after the other), ``state``
     ``[B, H, D, Dv]`` fp32 updated in place (sequences and heads in memory of their own), outputs ``[B, L, H, Dv]``
-    returned. Head dims up to 256. Not differentiable: inputs that ask for a gradient are refused while gradients
+    returned. Head dims up to 256, at most 65,535 sequences and as many heads. Not differentiable: inputs that ask for a gradient are refused while gradients
     are enabled."""
     _check(q, k, v, log_decay, state, "state")
     bsz, length, heads, d = q.shape

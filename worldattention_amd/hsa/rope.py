@@ -90,9 +90,9 @@ def rope_axes(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, 
       ``(p, p + P)``.
 
     bf16 or fp32; the angle's fraction of a revolution is exact to 2^-40 at any position (frequencies up to 1), the
-    rotation is fp32, one rounding. Returns new contiguous tensors (``q``'s,
-    or ``(q, k)``'s). Differentiable once in ``q`` and ``k``. To capture a backward pass in a graph, capture its
-    forward pass too, and let no eager graph of the same leaves live then.
+    rotation is fp32, one rounding. Returns new contiguous tensors (``q``'s, or ``(q, k)``'s). Differentiable once in
+    ``q`` and ``k``. To capture a backward pass in a graph, capture its forward pass too, and let no eager graph of
+    the same leaves live then.
     """
     sections = tuple(map(int, sections))
     if q.dim() != 4:

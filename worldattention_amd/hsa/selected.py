@@ -156,7 +156,8 @@ def select_key_blocks(q: torch.Tensor, k_block_sums: torch.Tensor, kv_len: KvLen
     The first ``sink_blocks`` and last ``local_blocks`` (at least the query's own) seen blocks are always
     chosen, then the highest of ``(sum of the group's queries) . (sum of the block's keys)``, in fp64; ties
     go to the lowest block. (Scores closer than the rounding of such a sum, ``D 2^-52`` of its products' magnitudes,
-    can rank differently for a single query and among several; equal key sums always tie.) A query before its sequence's first token gets none.
+    can rank differently for a single query and among several; equal key sums always tie.) A query before its
+    sequence's first token gets none.
     """
     _check_sums(k_block_sums, "k_block_sums")
     bsz, hk, _, d = k_block_sums.shape
