@@ -870,6 +870,75 @@ typedef struct wa_selected_attn_args {
 } wa_selected_attn_args;
 int wa_selected_attn(const wa_selected_attn_args* args, void* stream);
 
+/* Attention whose rows see up to two runs of keys each ("ranges"), with capped scores and a bias by
+ * distance. wa_key_ranges makes the ranges of a batch once, for every layer's calls: row i of sequence b
+ * sits at key position t = kv_len[b] - Lq + i (kv_len: device int32 [B], or NULL: kv_len_all; clamped to
+ * [0, Lk]) and sees, inside its document [first, end),
+ *   - its reach: keys below `end` or, with `causal`, below first + ((t - first) / chunk + 1) chunk (chunk 1:
+ *     its own token), and with window > 0 only those above t - window (and, not causal, below t + window);
+ *   - the document's first `sink` keys as far as it reaches, and its first `prefix` keys wherever it sits
+ *     (prefix: device int32 [B], or NULL: prefix_all).
+ * documents: device int32 borders, n_borders >= 2 of them in ascending order, documents_sb between
+ * sequences (0: shared); document d is [border d, border d + 1), and a token outside all of them sees nothing
+ * and is not seen. NULL: one document, [0, kv_len). `given` (device int32 [B, Lq, 4], each row the runs
+ * [0, 1) and [2, 3) as start and end; empty where end <= start) replaces all rules; it is clamped to [0, Lk].
+ * Written: rows int32 [B, Lq, 4] (disjoint runs, the lower one in 2, 3) and tiles int32
+ * [B, ceil(Lq / 64), WA_RANGE_TILE_INTS], what 64 rows see together. */
+#define WA_RANGE_TILE_INTS 12
+typedef struct wa_key_ranges_args {
+  int64_t B, Lq, Lk;
+  const int32_t* kv_len; int64_t kv_len_all;
+  const int32_t* given;
+  int32_t causal; int64_t chunk, window, sink;
+  const int32_t* prefix; int64_t prefix_all;
+  const int32_t* documents; int64_t documents_sb, n_borders;
+  int32_t* rows; int32_t* tiles;
+} wa_key_ranges_args;
+int wa_key_ranges(const wa_key_ranges_args* args, void* stream);
+
+/* o = softmax(s) V over the keys that a row sees, bf16, fp32 statistics:
+ *   x = scale q.k,  y = cap tanh(x / cap) (cap 0: x),  s = y - slopes[h] |t - j|  (slopes NULL: y).
+ * A row that sees nothing gets 0 and a log-sum-exp of -inf. Query heads hk (H / Hk) .. (hk + 1)(H / Hk) - 1
+ * read key head hk. q [B, Lq, H, D], k, v [B, Lk, Hk, D], D = 64 or 128, 16-byte aligned rows at most 2^23
+ * elements apart; rows / tiles as above for B sequences (ranges_sb 1) or one shared by all (0); kv_len as
+ * there (positions: read with slopes only). lse: fp32 [B, H, Lq], natural log. scale > 0 (0: D^-1/2). */
+typedef struct wa_ranged_fwd_args {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const void* k; int64_t k_sb, k_st, k_sh;
+  const void* v; int64_t v_sb, v_st, v_sh;
+  void* o; int64_t o_sb, o_st, o_sh;
+  float* lse;
+  const int32_t* rows; const int32_t* tiles; int32_t ranges_sb;
+  const int32_t* kv_len; int64_t kv_len_all;
+  const float* slopes;
+  int64_t B, H, Hk, Lq, Lk, D;
+  float scale, cap;
+  void* workspace;
+} wa_ranged_fwd_args;
+int64_t wa_ranged_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk, int64_t D);
+int wa_ranged_fwd(const wa_ranged_fwd_args* args, void* stream);
+
+/* Gradients of wa_ranged_fwd from its o and lse: dq, dk, dv in bf16 (contiguous [B, L, heads, D]), the
+ * gradient of a shared key head summed over its query heads, and dslopes fp32 [H] (NULL: not wanted). dlse
+ * (fp32 [B, H, Lq], NULL: 0): the gradient of lse. Everything is summed in a fixed order, without atomics. */
+typedef struct wa_ranged_bwd_args {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const void* k; int64_t k_sb, k_st, k_sh;
+  const void* v; int64_t v_sb, v_st, v_sh;
+  const void* o; int64_t o_sb, o_st, o_sh;
+  const void* dout; int64_t d_sb, d_st, d_sh;
+  const float* lse; const float* dlse;
+  const int32_t* rows; const int32_t* tiles; int32_t ranges_sb;
+  const int32_t* kv_len; int64_t kv_len_all;
+  const float* slopes;
+  int64_t B, H, Hk, Lq, Lk, D;
+  float scale, cap;
+  void* dq; void* dk; void* dv; float* dslopes;
+  void* workspace;
+} wa_ranged_bwd_args;
+int64_t wa_ranged_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk, int64_t D);
+int wa_ranged_bwd(const wa_ranged_bwd_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

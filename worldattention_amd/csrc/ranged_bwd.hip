@@ -1,0 +1,573 @@
+// Gradients of the ranged attention (ranged.hip). With P = exp(s - lse), dP = dO V^T and delta = rowsum(O dO) - dlse,
+//   dS = P (dP - delta),  dslope = -sum dS |t - j|,  dx = dS (1 - tanh^2),
+//   dQ = scale dx K,  dK = scale dx^T Q,  dV = P^T dO   (a shared key head: summed over its query heads).
+// Three launches: the rows' statistics, dQ (and the slopes'), dK and dV. The scores are formed again in each of the last two; that costs two
+// products more than forming them once, and needs neither atomics nor partial sums of dQ in memory.
+#include <algorithm>
+#include <type_traits>
+
+#include "ranges.h"
+#include "tile.h"
+
+namespace {
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+// dS is carried with this factor: the weights go from one wave to another as fp16 (11 significant bits), and 2^12 keeps weights down to
+// 2^-26 among its normal numbers. It is taken out where the gradients are written.
+constexpr float kLift = 4096.f;
+
+struct BwdParams {
+  const bf16_t* q; int64_t q_sb, q_st, q_sh;
+  const bf16_t* k; int64_t k_sb, k_st, k_sh;
+  const bf16_t* v; int64_t v_sb, v_st, v_sh;
+  const bf16_t* o; int64_t o_sb, o_st, o_sh;
+  const bf16_t* dout; int64_t d_sb, d_st, d_sh;
+  const float* lse; const float* dlse;
+  Ranges ranges;
+  const int32_t* kv_len; int64_t kv_len_all;
+  const float* slopes;
+  int B, H, Hk;
+  float scale, scale2, bend_in, cap2;
+  bf16_t* dq; bf16_t* dk; bf16_t* dv; float* dslopes;
+  // workspace
+  float* lse2;    // [B, H, Lq] log-sum-exp in units of log2; +inf where a row sees nothing: its weights come out 0
+  float* on;      // [B, H, Lq] 1, or 0 where a row sees a single key: its weight is 1 whatever the score, and its dS exactly 0
+  float* delta;   // [B, H, Lq] delta * on
+  float* slope_part;   // [H][B * q tiles]
+};
+
+// ---------------------------------------------------------------------------------------------
+// Rows' statistics: D / 8 lanes a row.
+// ---------------------------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(256) rows_kernel(BwdParams p, int64_t n_rows) {
+  constexpr int TPR = D / 8;
+  const int64_t u = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;   // (b, token, head): heads lie side by side
+  const int c0 = (threadIdx.x % TPR) * 8;
+  float s = 0.f;
+  int b = 0, i = 0, h = 0;
+  if (u < n_rows) {
+    h = (int)(u % p.H);
+    i = (int)(u / p.H % p.ranges.Lq);
+    b = (int)(u / p.H / p.ranges.Lq);
+    const bf16x8 o = *(const bf16x8*)(p.o + (int64_t)b * p.o_sb + (int64_t)i * p.o_st + (int64_t)h * p.o_sh + c0);
+    const bf16x8 d = *(const bf16x8*)(p.dout + (int64_t)b * p.d_sb + (int64_t)i * p.d_st + (int64_t)h * p.d_sh + c0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf((float)o[e], (float)d[e], s);
+  }
+#pragma unroll
+  for (int m = TPR / 2; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+  if (u < n_rows && threadIdx.x % TPR == 0) {
+    const int64_t r = ((int64_t)b * p.H + h) * p.ranges.Lq + i;
+    const int4 runs = p.ranges.row(b, i);
+    const bool one = (runs.y - runs.x) + (runs.w - runs.z) == 1;
+    const float l = p.lse[r], more = p.dlse ? p.dlse[r] : 0.f;
+    const bool none = l == -INFINITY;
+    p.lse2[r] = none ? INFINITY : l * WA_LOG2E;
+    p.on[r] = one ? 0.f : 1.f;
+    p.delta[r] = one || none ? (one && !none ? -more : 0.f) : s - more;
+  }
+}
+
+// A tile of 64 rows streamed into LDS by direct loads (tile.h's layout): rows from `rows` on read as zeros.
+template <int D, int NW>
+struct RowTile {
+  static constexpr int CPR = D / 8, RPI = 64 / CPR, NI = 64 / (RPI * NW);
+  int off[NI];
+  __device__ __forceinline__ void init(int64_t st, int w, int lane) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = (i * NW + w) * RPI + lane / CPR, pos = lane % CPR;
+      off[i] = ((int)(row * st) + (pos ^ dual_swizzle<D>(row)) * 8) * 2;
+    }
+  }
+  __device__ __forceinline__ void issue(bf16_t* lds, const bf16_t* first, int64_t st, int rows, int w) const {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)first, (short)0, rows > 0 ? (int)((min(rows, 64) - 1) * st + D) * 2 : 0, WA_BUF_DWORD3);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) lds_dma16(rs, lds + (i * NW + w) * RPI * D, off[i]);
+  }
+};
+
+template <int N> using IC = std::integral_constant<int, N>;
+
+// Top of a step: this wave's tile loads have landed and its LDS reads returned, then the workgroup's.
+__device__ __forceinline__ void step_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int first_position(const BwdParams& p, int b) {
+  return (int)min(max(p.kv_len ? (int64_t)p.kv_len[b] : p.kv_len_all, (int64_t)0), (int64_t)p.ranges.Lk) - p.ranges.Lq;
+}
+
+// ---------------------------------------------------------------------------------------------
+// dQ: one workgroup of four waves per 128 rows of a head over the 64-key steps that they see; K and V through two LDS stages each, a row
+// a lane. SLOPES: the slope's gradient besides, from sums over the row's keys of P, P dP, P dist and P dP dist in fp32: with them delta is
+// the row's own sum of P dP instead of one from the rounded output.
+// ---------------------------------------------------------------------------------------------
+template <int D, bool BENT, bool SLOPES>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ranged_dq_kernel(BwdParams p) {
+  constexpr int NW = 4, DC = D / 16, DT = D / 32, TILE = 64 * D;
+  using RT = RowTile<D, NW>;
+  __shared__ __attribute__((aligned(1024))) bf16_t kv0[2 * TILE];
+  __shared__ __attribute__((aligned(1024))) bf16_t kv1[2 * TILE];
+  __shared__ float s_part[NW];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5, l32 = lane & 31;
+  const int per = p.H / p.Hk, nbh = p.B * p.Hk, nq = (p.ranges.Lq + 127) / 128;
+  int u = (int)blockIdx.x;
+  const int bh = u % nbh;
+  u /= nbh;
+  const int h = (bh % p.Hk) * per + u % per, b = bh / p.Hk, qt = nq - 1 - u / per;
+  Steps st;
+  st.init(p.ranges, b, 2 * qt, 2);
+  const int qi = qt * 128 + w * 32 + l32;
+  const bool q_ok = qi < p.ranges.Lq;
+  const int row = q_ok ? qi : 0;
+  int4 runs = p.ranges.row(b, row);
+  if (!q_ok) runs = int4{0, 0, 0, 0};
+  bf16x8 qf[DC], dof[DC];
+  {
+    const bf16_t* qr = p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)row * p.q_st;
+    const bf16_t* dr = p.dout + (int64_t)b * p.d_sb + (int64_t)h * p.d_sh + (int64_t)row * p.d_st;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      const bf16x8 a = *(const bf16x8*)(qr + c * 16 + g * 8);
+      const bf16x8 d = *(const bf16x8*)(dr + c * 16 + g * 8);
+      qf[c] = q_ok ? a : bf16x8{};
+      dof[c] = q_ok ? d : bf16x8{};
+    }
+  }
+  const int64_t srow = ((int64_t)b * p.H + h) * p.ranges.Lq;
+  float lse2 = q_ok ? p.lse2[srow + row] : INFINITY;
+  float dl = q_ok ? p.delta[srow + row] : 0.f, on = q_ok ? p.on[srow + row] : 0.f;
+  Bend bend{p.bend_in, p.cap2, 0.f};
+  int pos = 0;   // the row's position
+  if (BENT && p.slopes) {
+    bend.slope2 = p.slopes[h] * WA_LOG2E;
+    pos = first_position(p, b) + qi;
+  }
+#pragma unroll
+  for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(qf[c]), "+v"(dof[c]));
+  asm volatile("" : "+v"(lse2), "+v"(dl), "+v"(on), "+v"(runs.x), "+v"(runs.y), "+v"(runs.z), "+v"(runs.w));
+
+  f32x16 dqacc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) dqacc[t] = f32x16{};
+  float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;   // sums of P, P dP, P dP dist, P dist
+
+  RT kt, vt;
+  kt.init(p.k_st, w, lane);
+  vt.init(p.v_st, w, lane);
+  const bf16_t* kb = p.k + (int64_t)b * p.k_sb + (int64_t)(bh % p.Hk) * p.k_sh;
+  const bf16_t* vb = p.v + (int64_t)b * p.v_sb + (int64_t)(bh % p.Hk) * p.v_sh;
+  auto issue = [&](bf16_t* kv, int t) {
+    const int key = st.key(t), rows = st.end(t) - key;
+    kt.issue(kv, kb + key * p.k_st, p.k_st, rows, w);
+    vt.issue(kv + TILE, vb + key * p.v_st, p.v_st, rows, w);
+  };
+  auto step = [&](auto S, int t) {
+    const bf16_t* kc = decltype(S)::value ? kv1 : kv0;
+    const bf16_t* vc = kc + TILE;
+    step_wait();
+    f32x16 sacc[2], pacc[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) sacc[x] = pacc[x] = f32x16{};
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        sacc[x] = wa_mfma32(tile_row8<D>(kc, x * 32 + l32, 2 * c + g), qf[c], sacc[x]);
+        pacc[x] = wa_mfma32(tile_row8<D>(vc, x * 32 + l32, 2 * c + g), dof[c], pacc[x]);
+      }
+    }
+    if (t + 1 < st.total) issue(decltype(S)::value ? kv0 : kv1, t + 1);   // the stage of step t - 1
+    const int key = st.key(t), end = st.end(t);
+    bf16x8 dsb[4];
+    // dS^T = P^T (dP^T - delta), packed in accumulator order for the next product
+    auto slopes_of = [&](float pr, float dp, float dist) {
+      const float pd = pr * dp, far = fabsf(dist);
+      a0 += pr;
+      a1 += pd;
+      a2 = fmaf(pd, far, a2);
+      a3 = fmaf(pr, far, a3);
+    };
+    auto weights = [&](auto masked) {
+      const RowRuns mine(runs, end);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int key0 = key + 32 * x + 4 * g;
+        const float far = (float)(key0 - pos);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = 8 * (r >> 2) + (r & 3);
+          float turn = 1.f, pr;
+          if constexpr (BENT) pr = __builtin_amdgcn_exp2f(bend(sacc[x][r], far + (float)at, turn) - lse2);
+          else pr = __builtin_amdgcn_exp2f(fmaf(sacc[x][r], p.scale2, -lse2));
+          float dp = pacc[x][r], ds = pr * fmaf(dp, on, -dl);
+          if constexpr (BENT) ds *= turn;
+          if constexpr (decltype(masked)::value) {
+            const bool seen = mine.sees(key0 + at);
+            ds = seen ? ds : 0.f;
+            if constexpr (SLOPES) {
+              pr = seen ? pr : 0.f;
+              dp = seen ? dp : 0.f;
+            }
+          }
+          if constexpr (SLOPES) slopes_of(pr, dp, far + (float)at);
+          dsb[x * 2 + (r >> 3)][r & 7] = (bf16_t)ds;
+        }
+      }
+    };
+    if (st.whole(key, end)) weights(std::false_type{});
+    else weights(std::true_type{});
+    // dQ[q, d] += dS[q, key] K[key, d]: A = dS (registers), B = K (transpose reads)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int tt = 0; tt < DT; ++tt) dqacc[tt] = wa_mfma32(dsb[c], tile_tr8<D>(kc, c, 32 * tt, lane), dqacc[tt]);
+    }
+  };
+  if (st.total > 0) issue(kv0, 0);
+  for (int t = 0; t < st.total; t += 2) {
+    step(IC<0>{}, t);
+    if (t + 1 < st.total) step(IC<1>{}, t + 1);
+  }
+  if constexpr (SLOPES) {
+    a0 += __shfl_xor(a0, 32, 64);
+    a1 += __shfl_xor(a1, 32, 64);
+    a2 += __shfl_xor(a2, 32, 64);
+    a3 += __shfl_xor(a3, 32, 64);
+    // the log-sum-exp's gradient shifts delta: it is what the rows' delta holds beyond the output's
+    float mine = 0.f;
+    if (a0 > 0.f) {
+      const float shift = p.dlse ? p.dlse[srow + row] : 0.f;
+      mine = on > 0.f ? a2 - (a1 / a0 - shift) * a3 : shift * a3;
+    } else if (a0 != a0) {
+      mine = a0;
+    }
+    float sum = g == 0 ? mine : 0.f;
+    sum = wa_wave_sum(sum);
+    if (lane == 0) s_part[w] = sum;
+    __syncthreads();
+    if (tid == 0) p.slope_part[((int64_t)h * p.B + b) * nq + qt] = -(s_part[0] + s_part[1] + s_part[2] + s_part[3]);
+  }
+  // accumulator lane (d = 32 t + l32, g) holds rows 32 w + 8 (r / 4) + 4 g + r % 4
+  bf16_t* out = p.dq + ((int64_t)b * p.ranges.Lq * p.H + h) * D + l32;
+#pragma unroll
+  for (int tt = 0; tt < DT; ++tt) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int i = qt * 128 + w * 32 + 8 * (r >> 2) + 4 * g + (r & 3);
+      if (i < p.ranges.Lq) out[(int64_t)i * p.H * D + 32 * tt] = (bf16_t)(dqacc[tt][r] * p.scale);
+    }
+  }
+}
+
+// The slopes' gradients: a workgroup a head, its parts added in a fixed order.
+__global__ void __launch_bounds__(256) slopes_kernel(BwdParams p, int n) {
+  __shared__ double s[256];
+  double x = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) x += (double)p.slope_part[(int64_t)blockIdx.x * n + i];
+  s[threadIdx.x] = x;
+  __syncthreads();
+  for (int m = 128; m >= 1; m >>= 1) {
+    if ((int)threadIdx.x < m) s[threadIdx.x] += s[threadIdx.x + m];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.dslopes[blockIdx.x] = (float)s[0];
+}
+
+// ---------------------------------------------------------------------------------------------
+// dK, dV: one workgroup per 64 keys of a key head, over the 64-row tiles that see one of them, for each query head of the group in turn.
+// Q, dO and the rows' statistics and runs stream through two LDS stages. Each 32 keys have two waves, a key a lane:
+//   the S-wave holds the keys and dV: S = Q K^T, P = exp2(s - lse2), P (1 - tanh^2) to LDS as fp16, dV += P^T dO;
+//   the dP-wave holds the values and dK: dP = dO V^T, dx from them, dK += dx^T Q.
+// ---------------------------------------------------------------------------------------------
+constexpr int kListMax = 1024;   // row tiles listed at a time: 65,536 rows
+
+template <int D, bool BENT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ranged_dkv_kernel(BwdParams p) {
+  constexpr int NW = 4, DC = D / 16, DT = D / 32, TILE = 64 * D;
+  using RT = RowTile<D, NW>;
+  // a stage: Q tile, dO tile, 64 lse2, 64 delta, 64 on, 64 rows' runs
+  constexpr int STATS = 2 * TILE, SS = STATS + 3 * 128 + 512;
+  __shared__ __attribute__((aligned(1024))) bf16_t qd0[SS];
+  __shared__ __attribute__((aligned(1024))) bf16_t qd1[SS];
+  __shared__ __attribute__((aligned(1024))) f16x4 s_p[2][2][4][64];
+  __shared__ int s_list[kListMax];   // row tile (from `base` on) | rows up to its last that sees anything << 10 | whole << 20
+  __shared__ int s_count[NW];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5, l32 = lane & 31, kg = w & 1;
+  const bool swave = w < 2;   // wave-uniform role
+  // a causal mask's first keys are seen by most rows: they start first
+  const int per = p.H / p.Hk, nbh = p.B * p.Hk;
+  const int bh = (int)blockIdx.x % nbh, key0 = (int)blockIdx.x / nbh * 64, hk = bh % p.Hk, b = bh / p.Hk;
+  const int kl = kg * 32 + l32, key = key0 + kl;
+  const bool k_ok = key < p.ranges.Lk;
+  const int key_end = min(key0 + 64, p.ranges.Lk);
+
+  bf16x8 kvf[DC];
+  {
+    const int kr = k_ok ? key : key0;
+    const bf16_t* src = swave ? p.k + (int64_t)b * p.k_sb + (int64_t)hk * p.k_sh + (int64_t)kr * p.k_st
+                              : p.v + (int64_t)b * p.v_sb + (int64_t)hk * p.v_sh + (int64_t)kr * p.v_st;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      const bf16x8 a = *(const bf16x8*)(src + c * 16 + g * 8);
+      kvf[c] = k_ok ? a : bf16x8{};
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(kvf[c]));
+  const int pos0 = BENT && p.slopes ? first_position(p, b) : 0;
+
+  f32x16 acc[DT];   // S-wave: dV^T; dP-wave: dK^T (lane = key, registers = channels)
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = f32x16{};
+  RT qt, dt;
+  qt.init(p.q_st, w, lane);
+  dt.init(p.d_st, w, lane);
+
+  for (int base = 0; base < p.ranges.n_tiles; base += kListMax) {
+    const int limit = min(base + kListMax, p.ranges.n_tiles);
+    int n = 0;
+    for (int i0 = base; i0 < limit; i0 += 256) {
+      const int i = i0 + tid;
+      bool any = false;
+      int entry = 0;
+      if (i < limit) {
+        const int32_t* r = p.ranges.tile(b, i);
+        any = (r[kUpLo] < key_end && r[kUpHi] > key0) || (r[kLowLo] < key_end && r[kLowHi] > key0);
+        const bool whole = (r[kUpIn0] <= key0 && r[kUpIn1] >= key_end) || (r[kLowIn0] <= key0 && r[kLowIn1] >= key_end);
+        entry = (i - base) | min(max(min(r[kRowEnd], p.ranges.Lq) - i * 64, 0), 64) << 10 | (whole ? 1 << 20 : 0);
+      }
+      const uint64_t mask = __ballot(any);
+      __syncthreads();   // s_count of the round before has been read
+      if (lane == 0) s_count[w] = __popcll(mask);
+      __syncthreads();
+      int at = n + __popcll(mask & ((1ull << lane) - 1));
+      for (int x = 0; x < w; ++x) at += s_count[x];
+      if (any) s_list[at] = entry;
+      n += s_count[0] + s_count[1] + s_count[2] + s_count[3];
+    }
+    __syncthreads();
+    n = __builtin_amdgcn_readfirstlane(n);
+    const int total = n * per;
+    int next_g = 0, next_i = 0;   // of the step issued next
+    auto issue = [&](bf16_t* qd) {
+      const int entry = __builtin_amdgcn_readfirstlane(s_list[next_i]), rows = entry >> 10 & 127;
+      const int row0 = (base + (entry & 1023)) * 64, h = hk * per + next_g;
+      qt.issue(qd, p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)row0 * p.q_st, p.q_st, rows, w);
+      dt.issue(qd + TILE, p.dout + (int64_t)b * p.d_sb + (int64_t)h * p.d_sh + (int64_t)row0 * p.d_st, p.d_st, rows, w);
+      const int64_t srow = ((int64_t)b * p.H + h) * p.ranges.Lq + row0;
+      float* stats = (float*)(qd + STATS);
+      const int count = min(64, p.ranges.Lq - row0);
+      if (w == 0) row_stats_dma(stats, p.lse2 + srow, count, lane);
+      if (w == 1) row_stats_dma(stats + 64, p.delta + srow, count, lane);
+      if (w == 2) row_stats_dma(stats + 128, p.on + srow, count, lane);
+      if (w == 3) {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(p.ranges.rows + ((int64_t)b * p.ranges.sb * p.ranges.Lq + row0) * 4), (short)0, count * 16, WA_BUF_DWORD3);
+        lds_dma16(rs, stats + 192, lane * 16);
+      }
+      if (++next_i == n) {
+        next_i = 0;
+        ++next_g;
+      }
+    };
+    int now_g = 0, now_i = 0;
+    float slope2 = BENT && p.slopes ? p.slopes[hk * per] * WA_LOG2E : 0.f;
+    auto step = [&](auto S, int t) {
+      const bf16_t* qc = decltype(S)::value ? qd1 : qd0;
+      const bf16_t* dc = qc + TILE;
+      const float* st_lse2 = (const float*)(qc + STATS);
+      const float* st_dl = st_lse2 + 64;
+      const float* st_on = st_lse2 + 128;
+      const int4* st_runs = (const int4*)(st_lse2 + 192);
+      step_wait();
+      const int entry = __builtin_amdgcn_readfirstlane(s_list[now_i]);
+      const int row0 = (base + (entry & 1023)) * 64;
+      const bool whole = entry >> 20;
+      // S[q, key] = Q K^T (S-wave) or dP[q, key] = dO V^T (dP-wave) per 32 rows; lane = key, registers = rows 32 x + 8 rq + 4 g + i
+      const bf16_t* at = swave ? qc : dc;
+      f32x16 sacc[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) sacc[x] = f32x16{};
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) sacc[x] = wa_mfma32(tile_row8<D>(at, x * 32 + l32, 2 * c + g), kvf[c], sacc[x]);
+      }
+      if (t + 1 < total) issue(decltype(S)::value ? qd0 : qd1);   // the stage of step t - 1
+      bf16x8 ab[4];
+      auto weights = [&](auto masked) {
+        const Bend bend{p.bend_in, p.cap2, slope2};
+        const float far = (float)(key - pos0 - row0 - 4 * g);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq) {
+            const int r0 = 32 * x + 8 * rq;
+            const f32x4 l4 = *(const f32x4*)(st_lse2 + r0 + 4 * g);
+            f16x4 p4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = rq * 4 + i;
+              float turn = 1.f, pr;
+              if constexpr (BENT) pr = __builtin_amdgcn_exp2f(bend(sacc[x][r], far - (float)(r0 + i), turn) - l4[i]);
+              else pr = __builtin_amdgcn_exp2f(fmaf(sacc[x][r], p.scale2, -l4[i]));
+              if constexpr (decltype(masked)::value) {
+                const RowRuns row(st_runs[r0 + 4 * g + i], INT32_MAX);
+                pr = row.sees(key) ? pr : 0.f;
+              }
+              ab[x * 2 + (r >> 3)][r & 7] = (bf16_t)pr;
+              p4[i] = (_Float16)(pr * (BENT ? kLift * turn : kLift));
+            }
+            s_p[kg][x][rq][lane] = p4;
+          }
+        }
+      };
+      if (swave) {
+        if (whole) weights(std::false_type{});
+        else weights(std::true_type{});
+      }
+      __syncthreads();   // the weights of both key halves are in LDS
+      if (!swave) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq) {
+            const int r0 = 32 * x + 8 * rq + 4 * g;
+            const f32x4 d4 = *(const f32x4*)(st_dl + r0), o4 = *(const f32x4*)(st_on + r0);
+            const f16x4 p4 = s_p[kg][x][rq][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = rq * 4 + i;
+              float ds = (float)p4[i] * fmaf(sacc[x][r], o4[i], -d4[i]);
+              if (!whole && p4[i] == (_Float16)0.f) ds = 0.f;   // what a masked key holds, NaN too, reaches nothing
+              ab[x * 2 + (r >> 3)][r & 7] = (bf16_t)ds;
+            }
+          }
+        }
+      }
+      // dV^T[d, key] += dO^T P (S-wave), dK^T[d, key] += Q^T dS (dP-wave): A by transpose reads, B from registers
+      const bf16_t* bt = swave ? dc : qc;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int tt = 0; tt < DT; ++tt) acc[tt] = wa_mfma32(tile_tr8<D>(bt, c, 32 * tt, lane), ab[c], acc[tt]);
+      }
+      if (++now_i == n) {
+        now_i = 0;
+        ++now_g;
+        if (BENT && p.slopes && now_g < per) slope2 = p.slopes[hk * per + now_g] * WA_LOG2E;
+      }
+    };
+    if (total > 0) issue(qd0);
+    for (int t = 0; t < total; t += 2) {
+      step(IC<0>{}, t);
+      if (t + 1 < total) step(IC<1>{}, t + 1);
+    }
+    __syncthreads();   // the list and the stages are free
+  }
+  // each lane holds its key's row: channels 32 tt + 8 rq + 4 g .. + 3 of tile tt. Rows are staged in LDS, row r's 16-byte chunk c at chunk
+  // c ^ swz(r), and written whole.
+  const float osc = swave ? 1.f : p.scale / kLift;
+  auto swz = [](int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); };
+  bf16_t* stg = swave ? qd1 : qd0;   // dV, dK
+#pragma unroll
+  for (int tt = 0; tt < DT; ++tt) {
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+      bf16x4 v4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v4[i] = (bf16_t)(acc[tt][rq * 4 + i] * osc);
+      *(bf16x4*)(stg + kl * D + (((4 * tt + rq) ^ swz(kl)) << 3) + 4 * g) = v4;
+    }
+  }
+  __syncthreads();
+  constexpr int CPR = D / 8;
+  const int rows = key_end - key0;
+  const int64_t first = (((int64_t)b * p.ranges.Lk + key0) * p.Hk + hk) * D, st = (int64_t)p.Hk * D;
+  for (int x = tid; x < rows * CPR; x += 256) {
+    const int r = x / CPR, c = x % CPR;
+    *(bf16x8*)(p.dk + first + r * st + c * 8) = *(const bf16x8*)(qd0 + r * D + ((c ^ swz(r)) << 3));
+    *(bf16x8*)(p.dv + first + r * st + c * 8) = *(const bf16x8*)(qd1 + r * D + ((c ^ swz(r)) << 3));
+  }
+}
+
+template <int D, bool BENT>
+void launch_bwd(const BwdParams& p, hipStream_t s) {
+  const int64_t n_rows = (int64_t)p.B * p.H * p.ranges.Lq, nq = (p.ranges.Lq + 127) / 128;
+  hipLaunchKernelGGL((rows_kernel<D>), dim3((unsigned)((n_rows + 2048 / D - 1) / (2048 / D))), dim3(256), 0, s, p, n_rows);
+  const dim3 gq((unsigned)(p.B * p.H * nq)), gk((unsigned)((int64_t)p.B * p.Hk * ((p.ranges.Lk + 63) / 64)));
+  if constexpr (BENT) {
+    if (p.dslopes) {
+      hipLaunchKernelGGL((ranged_dq_kernel<D, true, true>), gq, dim3(256), 0, s, p);
+      hipLaunchKernelGGL(slopes_kernel, dim3((unsigned)p.H), dim3(256), 0, s, p, (int)(p.B * nq));
+    } else {
+      hipLaunchKernelGGL((ranged_dq_kernel<D, true, false>), gq, dim3(256), 0, s, p);
+    }
+  } else {
+    hipLaunchKernelGGL((ranged_dq_kernel<D, false, false>), gq, dim3(256), 0, s, p);
+  }
+  hipLaunchKernelGGL((ranged_dkv_kernel<D, BENT>), gk, dim3(256), 0, s, p);
+}
+
+}  // namespace
+
+extern "C" int64_t wa_ranged_bwd_workspace_bytes(int64_t B, int64_t H, int64_t, int64_t Lq, int64_t, int64_t) {
+  return B * H * Lq * 12 + B * H * ((Lq + 127) / 128) * 4;
+}
+
+extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
+  WA_CHECK_ARG(a, "ranged_bwd: null args");
+  WA_CHECK_ARG(a->D == 64 || a->D == 128, "ranged_bwd: head dim must be 64 or 128, got %lld", (long long)a->D);
+  WA_CHECK_ARG(a->B >= 1 && a->Lq >= 1 && a->Lk >= 1 && a->Lq <= 1 << 30 && a->Lk <= 1 << 30 && a->Hk >= 1 && a->H >= a->Hk && a->H % a->Hk == 0,
+               "ranged_bwd: bad sizes B %lld Lq %lld Lk %lld heads %lld / %lld", (long long)a->B, (long long)a->Lq, (long long)a->Lk,
+               (long long)a->H, (long long)a->Hk);
+  WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->dout && a->lse && a->rows && a->tiles && a->dq && a->dk && a->dv && a->workspace &&
+               wa_aligned16(a->rows), "ranged_bwd: null tensor");
+  WA_CHECK_ARG(!a->dslopes || a->slopes, "ranged_bwd: dslopes without slopes");
+  auto rows16 = [](const void* x, int64_t sb, int64_t st, int64_t sh) {
+    return wa_aligned16(x) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0;
+  };
+  auto near = [](int64_t st) { return st >= 0 && st <= (int64_t)1 << 23; };
+  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->k, a->k_sb, a->k_st, a->k_sh) && rows16(a->v, a->v_sb, a->v_st, a->v_sh) &&
+               rows16(a->o, a->o_sb, a->o_st, a->o_sh) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh) && wa_aligned16(a->dq) && wa_aligned16(a->dk) &&
+               wa_aligned16(a->dv) && near(a->q_st) && near(a->k_st) && near(a->v_st) && near(a->d_st),
+               "ranged_bwd: rows must be 16-byte aligned, at most 2^23 elements apart");
+  WA_CHECK_ARG(a->scale >= 0.f && a->cap >= 0.f && a->scale < INFINITY && a->cap < INFINITY, "ranged_bwd: scale and cap must be finite and not below 0");
+  WA_CHECK_ARG(a->B * a->H * ((a->Lq + 127) / 128) <= INT32_MAX && a->B * a->Hk * ((a->Lk + 63) / 64) <= INT32_MAX && a->B * a->H * a->Lq / 16 <= INT32_MAX,
+               "ranged_bwd: too many rows");
+  BwdParams p{};
+  p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.k = (const bf16_t*)a->k; p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
+  p.v = (const bf16_t*)a->v; p.v_sb = a->v_sb; p.v_st = a->v_st; p.v_sh = a->v_sh;
+  p.o = (const bf16_t*)a->o; p.o_sb = a->o_sb; p.o_st = a->o_st; p.o_sh = a->o_sh;
+  p.dout = (const bf16_t*)a->dout; p.d_sb = a->d_sb; p.d_st = a->d_st; p.d_sh = a->d_sh;
+  p.lse = a->lse; p.dlse = a->dlse;
+  p.ranges = {a->rows, a->tiles, a->ranges_sb ? 1 : 0, (int)a->Lq, (int)a->Lk, (int)((a->Lq + kRangeRows - 1) / kRangeRows)};
+  p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.slopes = a->slopes;
+  p.B = (int)a->B; p.H = (int)a->H; p.Hk = (int)a->Hk;
+  p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->D) : a->scale;
+  p.scale2 = p.scale * WA_LOG2E;
+  p.bend_in = a->cap > 0.f ? 2.f * p.scale / a->cap * WA_LOG2E : p.scale2;
+  p.cap2 = a->cap * WA_LOG2E;
+  p.dq = (bf16_t*)a->dq; p.dk = (bf16_t*)a->dk; p.dv = (bf16_t*)a->dv; p.dslopes = a->dslopes;
+  const int64_t n = a->B * a->H * a->Lq;
+  p.lse2 = (float*)a->workspace;
+  p.on = p.lse2 + n;
+  p.delta = p.on + n;
+  p.slope_part = p.delta + n;
+  hipStream_t s = (hipStream_t)stream;
+  const bool bent = a->cap > 0.f || a->slopes;
+  if (a->D == 128) {
+    if (bent) launch_bwd<128, true>(p, s);
+    else launch_bwd<128, false>(p, s);
+  } else {
+    if (bent) launch_bwd<64, true>(p, s);
+    else launch_bwd<64, false>(p, s);
+  }
+  return wa_launch_status("ranged_bwd");
+}

@@ -11,6 +11,7 @@ from .attention import (
 from .kvcache import kv_append, new_block_sums
 from .block_sparse import block_sparse_attention, block_sparse_attention_reference, map_to_index
 from .decay import decay_linear_attention, decay_linear_step
+from .ranged import KeyRanges, key_ranges, ranged_attention
 from .rope import axis_frequencies, rope_axes
 from .selected import BlockSelection, attend_selected, select_key_blocks, selected_attention
 from .routing import (
@@ -42,6 +43,9 @@ __all__ = [
     "axis_frequencies",
     "decay_linear_attention",
     "decay_linear_step",
+    "KeyRanges",
+    "key_ranges",
+    "ranged_attention",
     "BlockSelection",
     "select_key_blocks",
     "selected_attention",
