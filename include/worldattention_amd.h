@@ -939,6 +939,73 @@ typedef struct wa_ranged_bwd_args {
 int64_t wa_ranged_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk, int64_t D);
 int wa_ranged_bwd(const wa_ranged_bwd_args* args, void* stream);
 
+/* A KV cache in 8 bits: codes k, v [B, cap, Hk, D] (int8 or e4m3, contiguous), and for each head and block of
+ * block_size (64 or 128) tokens one fp32 scale, k_scale / v_scale [B, Hk, blocks], blocks = ceil(cap / block_size);
+ * a token's value is code * scale. Scales are the smallest powers of two, from 2^-126 on, at which the block's
+ * values fit the codes (127 in int8, 448 in e4m3), so code * scale is exact in bf16. k_sums (fp32 [B, Hk, blocks,
+ * D], or NULL): each block's sum of the keys that the codes stand for, as wa_select_blocks reads it. D = 64 or 128. */
+#define WA_CODE_INT8 0
+#define WA_CODE_E4M3 1
+typedef struct wa_cache8 {
+  void* k; void* v;
+  float* k_scale; float* v_scale; float* k_sums;
+  int64_t B, cap, Hk, D, block_size;
+  int32_t code;
+} wa_cache8;
+
+/* Writes tokens [start, start + count) of every sequence: start from the device int32 [B] `start` (NULL:
+ * start_all), count = n or, with `lengths` (device int32 [B]), min(lengths[b], n). A sequence whose tokens do not fit
+ * the cache is left as it is. A block that is begun anew takes the new tokens' scale; one with earlier tokens takes the
+ * larger of its scale and theirs, and where that grows the earlier codes are rounded again (a token is off by less than
+ * one step in all). Codes are rounded to nearest even. A block that gets a value that is not finite has the scale NaN from
+ * then on. Tokens behind the written ones are not kept. k, v: bf16 or fp32 [B, n, Hk, D], 16-byte aligned rows. */
+typedef struct wa_kv8_append_args {
+  wa_cache8 cache;
+  const void* k; int64_t k_sb, k_st, k_sh;
+  const void* v; int64_t v_sb, v_st, v_sh;
+  int32_t dtype;
+  int64_t n;
+  const int32_t* start; int64_t start_all;
+  const int32_t* lengths;
+} wa_kv8_append_args;
+int wa_kv8_append(const wa_kv8_append_args* args, void* stream);
+
+/* Tokens [start, start + n) as values, bf16 or fp32 k_out, v_out [B, n, Hk, D] (contiguous); 0 outside the cache. With
+ * kv_len (device int32 [B]) or kv_len_all >= 0 only what `last` tokens at the sequence's end see under a window (0:
+ * everything) with sinks is written; kv_len_all < 0 and no kv_len: everything. */
+typedef struct wa_kv8_read_args {
+  wa_cache8 cache;
+  void* k_out; void* v_out;
+  int32_t dtype;
+  int64_t n;
+  const int32_t* start; int64_t start_all;
+  const int32_t* kv_len; int64_t kv_len_all;
+  int64_t last, window, sink;
+} wa_kv8_read_args;
+int wa_kv8_read(const wa_kv8_read_args* args, void* stream);
+
+/* Attention of the n newest tokens (query i sits at token kv_len[b] - n + i and sees the tokens up to its own) over the
+ * cache: scores, cap and slopes as in wa_ranged_fwd. window > 0: of these tokens only the `window` nearest and the first
+ * `sink`. With `index` (int32 [B, n, Hk, topk]) and `num` (int32 [B, n, Hk]) each query and key head attends to the
+ * seen tokens of the listed blocks (no window; any lists, as in wa_selected_attn). q, o: bf16 [B, n, H, D], 16-byte
+ * aligned rows; lse: fp32 [B, H, n]. A query that sees nothing gets 0 and -inf. Meant for few rows (n H / Hk): each
+ * 64 of them read the cache once. The workspace may be NULL where its size is 0. */
+typedef struct wa_kv8_attend_args {
+  wa_cache8 cache;
+  const void* q; int64_t q_sb, q_st, q_sh;
+  void* o; int64_t o_sb, o_st, o_sh;
+  float* lse;
+  int64_t n, H;
+  const int32_t* kv_len; int64_t kv_len_all;
+  const int32_t* index; const int32_t* num; int64_t topk;
+  int64_t window, sink;
+  const float* slopes;
+  float scale, cap;
+  void* workspace;
+} wa_kv8_attend_args;
+int64_t wa_kv8_attend_workspace_bytes(const wa_kv8_attend_args* args);
+int wa_kv8_attend(const wa_kv8_attend_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,7 @@ LIB_PATH = os.environ.get("WORLDATTENTION_AMD_LIB") or os.path.join(os.path.dirn
 
 WA_OK, WA_ERR_ARG, WA_ERR_UNSUPPORTED, WA_ERR_IO = 0, -1, -2, -3
 WA_F32, WA_BF16 = 0, 1
+WA_CODE_INT8, WA_CODE_E4M3 = 0, 1
 WA_ROUTE_GINI, WA_ROUTE_TOPK = 0, 1
 WA_EPI_PLAIN, WA_EPI_FUSE, WA_EPI_GATED = 0, 1, 2
 WA_LINEAR_LOWRANK, WA_LINEAR_ELU1 = 0, 1
@@ -442,6 +443,30 @@ RangedBwdArgs = _struct("wa_ranged_bwd_args", [
     ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("dslopes", c_void_p), ("workspace", c_void_p),
 ])
 
+Cache8 = _struct("wa_cache8", [
+    ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_sums", c_void_p),
+    ("B", c_int64), ("cap", c_int64), ("Hk", c_int64), ("D", c_int64), ("block_size", c_int64), ("code", c_int32),
+])
+
+Kv8AppendArgs = _struct("wa_kv8_append_args", [
+    ("cache", Cache8), ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
+    ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64), ("v_sh", c_int64), ("dtype", c_int32), ("n", c_int64),
+    ("start", c_void_p), ("start_all", c_int64), ("lengths", c_void_p),
+])
+
+Kv8ReadArgs = _struct("wa_kv8_read_args", [
+    ("cache", Cache8), ("k_out", c_void_p), ("v_out", c_void_p), ("dtype", c_int32), ("n", c_int64),
+    ("start", c_void_p), ("start_all", c_int64), ("kv_len", c_void_p), ("kv_len_all", c_int64),
+    ("last", c_int64), ("window", c_int64), ("sink", c_int64),
+])
+
+Kv8AttendArgs = _struct("wa_kv8_attend_args", [
+    ("cache", Cache8), ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+    ("o", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64), ("lse", c_void_p), ("n", c_int64), ("H", c_int64),
+    ("kv_len", c_void_p), ("kv_len_all", c_int64), ("index", c_void_p), ("num", c_void_p), ("topk", c_int64),
+    ("window", c_int64), ("sink", c_int64), ("slopes", c_void_p), ("scale", c_float), ("cap", c_float), ("workspace", c_void_p),
+])
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "wa_version": (c_int, []),
@@ -503,6 +528,10 @@ SIGNATURES = {
     "wa_ranged_fwd": (c_int, [POINTER(RangedFwdArgs), c_void_p]),
     "wa_ranged_bwd_workspace_bytes": (c_int64, [c_int64] * 6),
     "wa_ranged_bwd": (c_int, [POINTER(RangedBwdArgs), c_void_p]),
+    "wa_kv8_append": (c_int, [POINTER(Kv8AppendArgs), c_void_p]),
+    "wa_kv8_read": (c_int, [POINTER(Kv8ReadArgs), c_void_p]),
+    "wa_kv8_attend_workspace_bytes": (c_int64, [POINTER(Kv8AttendArgs)]),
+    "wa_kv8_attend": (c_int, [POINTER(Kv8AttendArgs), c_void_p]),
     "wa_hkv_gather_async": (c_int, [POINTER(HkvCopy), c_int64, c_void_p, c_void_p]),
     "wa_hkv_store_async": (c_int, [POINTER(HkvCopy), c_int64, c_void_p, c_void_p]),
 }

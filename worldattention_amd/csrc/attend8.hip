@@ -1,0 +1,459 @@
+// Attention of the newest tokens over an 8-bit KV cache (cache8.hip), all of it, a window with sinks, or chosen blocks. No reference counterpart.
+#include <algorithm>
+
+#include "codes.h"
+#include "ranges.h"
+#include "tile.h"
+
+namespace {
+
+// =============================================================================================
+// Rows are (query, head of the group) pairs of one key head; a unit of 16 RT rows walks its tiles of 32 keys once. A part of a unit (the
+// tiles that one workgroup takes) is shared by four waves, tile by tile, each with running maxima and sums of its own. A tile's codes come
+// straight into registers in the operands' order: a key row's 16 channels a load, where q takes its channels in the same order; a value
+// row's 8 channels a load, eight rows a lane, transposed as their halves are put together. Codes become bf16 exactly; a block's scales are
+// wave-uniform factors of the scores and of the weights (powers of two: the weights' rounding is that of the plain ones). Products are
+// v_mfma_f32_16x16x32: S^T = K Q^T, O^T += V^T P^T. The next tile's codes are asked for before the current ones are used. Bound by
+// reading the codes.
+// =============================================================================================
+struct AttendParams {
+  const bf16_t* q; int64_t q_sb, q_st, q_sh;
+  bf16_t* o; int64_t o_sb, o_st, o_sh;
+  float* lse;
+  const uint8_t* k; const uint8_t* v;
+  const float* k_scale; const float* v_scale;
+  const int32_t* kv_len; int64_t kv_len_all, cap;
+  const int32_t* index; const int32_t* num; int topk;
+  int64_t window, sink;
+  const float* slopes;
+  int n, H, Hk, nb, shift;        // shift: log2 of a block's tokens
+  int units, parts, per;          // row units of (sequence, key head, with lists: query); parts of a unit, tiles of a part
+  float scale2, bend_in, cap2;
+  float* part;                    // [unit][part][16 RT][D + 2]: maximum, sum, outputs
+};
+
+constexpr float kLowest = -3.4028234e38f;   // running maximum before the first key: below every score, and no difference of it is NaN
+constexpr float kSlack = 8.f;               // log2 of the growth that the running maximum lets pass
+
+__device__ __forceinline__ f32x4 mma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// A lane's value combined over the four 16-lane groups.
+template <typename Op>
+__device__ __forceinline__ float over_groups(float x, const Op& op) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float y = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <int D> struct ValueRow;     // a lane's part of a value row: D / 16 codes
+template <> struct ValueRow<128> { typedef u32x2 type; };
+template <> struct ValueRow<64> { typedef uint32_t type; };
+__device__ __forceinline__ uint32_t word(const u32x2& x, int i) { return x[i]; }
+__device__ __forceinline__ uint32_t word(uint32_t x, int) { return x; }
+
+// What a unit is and which tiles its rows see, the same in the walk and in the join.
+struct Unit {
+  int b, hk, i0, row0, rows, tiles;   // first query (with lists), first row, rows; tiles in all
+  int n0, s1;                         // without lists: the first n0 tiles, then those from s1 on
+  int64_t len;
+  template <int RT>
+  __device__ __forceinline__ void init(const AttendParams& p, int64_t u) {
+    const int G = p.H / p.Hk, of = p.index ? (G + 16 * RT - 1) / (16 * RT) : p.units;
+    // neighbouring workgroups take the key heads in turn: with eight of them each XCD's L2 sees one head's cache
+    hk = (int)(u % p.Hk);
+    u /= p.Hk;
+    const int chunk = (int)(u % of);
+    u /= of;
+    i0 = p.index ? (int)(u % p.n) : 0;
+    b = (int)(p.index ? u / p.n : u);
+    row0 = 16 * RT * chunk;
+    rows = min(16 * RT, (p.index ? G : p.n * G) - row0);
+    const int64_t held = p.kv_len ? (int64_t)p.kv_len[b] : p.kv_len_all;
+    len = min(max(held, (int64_t)0), p.cap);
+    n0 = s1 = 0;
+    if (p.index) {
+      tiles = max(0, min(p.num[((int64_t)b * p.n + i0) * p.Hk + hk], p.topk)) << (p.shift - 5);
+    } else {
+      const int64_t t0 = len - p.n + row0 / G, t1 = len - p.n + (row0 + rows - 1) / G;   // the rows' positions
+      const int end = (int)((t1 + 32) >> 5);          // tiles that the last row sees
+      if (t1 < 0) {
+        tiles = 0;
+      } else if (p.window > 0 && t0 - p.window + 1 > 0) {
+        n0 = (int)min((int64_t)end, (p.sink + 31) >> 5);
+        s1 = max(n0, (int)((t0 - p.window + 1) >> 5));
+        tiles = n0 + max(0, end - s1);
+      } else {
+        tiles = n0 = end;
+      }
+    }
+    tiles = __builtin_amdgcn_readfirstlane(tiles);
+  }
+  // Query and head (in its group) of row r of the unit.
+  __device__ __forceinline__ int query(const AttendParams& p, int r) const { return p.index ? i0 : (row0 + r) / (p.H / p.Hk); }
+  __device__ __forceinline__ int head(const AttendParams& p, int r) const {
+    const int G = p.H / p.Hk;
+    return hk * G + (p.index ? row0 + r : (row0 + r) % G);
+  }
+};
+
+__device__ __forceinline__ void write_row(const AttendParams& p, int b, int i, int h, int d, float sum, float top, float l) {
+  p.o[(int64_t)b * p.o_sb + (int64_t)i * p.o_st + (int64_t)h * p.o_sh + d] = (bf16_t)(l == 0.f ? 0.f : sum / l);
+  if (d == 0) p.lse[((int64_t)b * p.H + h) * p.n + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * WA_LN2;
+}
+
+template <typename Code, int D, int RT>
+__global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
+  constexpr int NW = 4, KC = D / 32, VC = D / 16, KL = D / 64;   // key products of a tile half; channels of a value row a lane holds; loads of a key row
+  typedef typename ValueRow<D>::type VRow;
+  __shared__ float so[NW][16][D + 4];
+  __shared__ float sm[NW][16], sl[NW][16];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, kg = lane >> 4;
+  const int64_t u = blockIdx.x / p.parts;
+  const int part = (int)(blockIdx.x % p.parts);
+  Unit unit;
+  unit.init<RT>(p, u);
+  const int t0 = part * p.per, t1 = min(unit.tiles, t0 + p.per);
+  if (t0 >= t1 && part > 0) return;
+  const bool alone = unit.tiles <= p.per;
+  const int b = unit.b, hk = unit.hk, window = (int)p.window, sink = (int)p.sink;
+
+  bf16x8 q[RT][KC];
+  int pos[RT], from[RT];   // the row's position: the last key that it sees; the first one of its window
+  float slope2[RT];
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    const int r = 16 * x + l16;
+    const bool ok = r < unit.rows;
+    const int i = unit.query(p, ok ? r : 0), h = unit.head(p, ok ? r : 0);
+    pos[x] = ok ? (int)(unit.len - p.n + i) : -1;
+    from[x] = window > 0 ? pos[x] - window + 1 : INT32_MIN;
+    slope2[x] = p.slopes ? p.slopes[h] * WA_LOG2E : 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {   // channels in the order in which the keys' come
+      q[x][c] = bf16x8{};
+      if (ok) q[x][c] = *(const bf16x8*)(p.q + (int64_t)b * p.q_sb + (int64_t)i * p.q_st + (int64_t)h * p.q_sh + 64 * (c >> 1) + 16 * kg + 8 * (c & 1));
+    }
+  }
+  const int64_t st = (int64_t)p.Hk * D;
+  const uint8_t* kb = p.k + ((int64_t)b * p.cap * p.Hk + hk) * D;
+  const uint8_t* vb = p.v + ((int64_t)b * p.cap * p.Hk + hk) * D;
+  const float* ksc = p.k_scale + ((int64_t)b * p.Hk + hk) * p.nb;
+  const float* vsc = p.v_scale + ((int64_t)b * p.Hk + hk) * p.nb;
+  const int32_t* list = p.index ? p.index + (((int64_t)b * p.n + unit.i0) * p.Hk + hk) * p.topk : nullptr;
+  const int last = p.index ? (int)(unit.len - p.n + unit.i0) : (int)(unit.len - p.n + (unit.row0 + unit.rows - 1) / (p.H / p.Hk));   // last key that any row sees
+  const int lowest = p.index ? last : (int)(unit.len - p.n + unit.row0 / (p.H / p.Hk));                                              // ... that every row sees
+
+  float m[RT], l[RT];
+  f32x4 o[RT][VC];
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    m[x] = kLowest;
+    l[x] = 0.f;
+#pragma unroll
+    for (int j = 0; j < VC; ++j) o[x][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // Ids of this wave's next 64 tiles sit in its lanes.
+  int ids = 0, ids_at = t1;
+  auto key_of = [&](int t) -> int {   // the tile's first key, -1 if none of its tokens is seen
+    if (!p.index) return (t < unit.n0 ? t : unit.s1 + t - unit.n0) * 32;
+    if (t >= ids_at + 64 * NW || t < ids_at) {
+      ids_at = t;
+      const int mine = t + lane * NW;
+      ids = mine < t1 ? list[mine >> (p.shift - 5)] : -1;
+    }
+    const int id = __builtin_amdgcn_readlane(ids, (t - ids_at) / NW);
+    const int64_t key = ((int64_t)id << p.shift) + (t & ((1 << (p.shift - 5)) - 1)) * 32;
+    return id < 0 || key > last ? -1 : (int)key;
+  };
+  struct Tile {
+    u32x4 k[2][KL];
+    VRow v[8];
+    float ks, vs;
+    int key;
+  };
+  auto load = [&](Tile& x, int t) {
+    x.key = -1;
+    while (t < t1 && (x.key = key_of(t)) < 0) t += NW;
+    if (x.key < 0) return t1;
+    const int live = min(32, last + 1 - x.key);   // behind the last token that any row sees its codes again
+    const uint8_t* kr = kb + x.key * st;
+    const uint8_t* vr = vb + x.key * st;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < KL; ++c) x.k[h][c] = *(const u32x4*)(kr + min(16 * h + l16, live - 1) * st + 64 * c + 16 * kg);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.v[e] = *(const VRow*)(vr + min(16 * (e >> 2) + 4 * kg + (e & 3), live - 1) * st + VC * l16);
+    x.ks = ksc[x.key >> p.shift];
+    x.vs = vsc[x.key >> p.shift];
+    return t;
+  };
+  auto use = [&](const Tile& x) {
+    bf16x8 ka[2][KC];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        u32x4 y;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t lo, hi;
+          Code::pairs(x.k[h][c >> 1][2 * (c & 1) + e], lo, hi);
+          y[2 * e] = lo;
+          y[2 * e + 1] = hi;
+        }
+        ka[h][c] = __builtin_bit_cast(bf16x8, y);
+      }
+    uint32_t vp[8][VC / 2];   // value rows as bf16 pairs of channels
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int j = 0; j < VC / 4; ++j) Code::pairs(word(x.v[e], j), vp[e][2 * j], vp[e][2 * j + 1]);
+    const bool whole = x.key + 31 <= lowest && ((window == 0) | (x.key > last - window) | (x.key + 31 < sink));
+    bf16x8 pr[RT];
+#pragma unroll
+    for (int y = 0; y < RT; ++y) {
+      f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) acc[h] = mma16(ka[h][c], q[y][c], acc[h]);
+      float s[8];
+      const int key0 = x.key + 4 * kg;
+      if (p.cap2 > 0.f || p.slopes) {
+        const Bend bend{p.bend_in * x.ks, p.cap2, slope2[y]};
+        const float far = (float)(pos[y] - key0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float unused;
+          s[e] = bend(acc[e >> 2][e & 3], far - (float)(16 * (e >> 2) + (e & 3)), unused);
+        }
+      } else {
+        const float by = p.scale2 * x.ks;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = acc[e >> 2][e & 3] * by;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // one comparison beside the other: as a chain of branches the window's was compiled to nothing
+          const int key = key0 + 16 * (e >> 2) + (e & 3);
+          const bool seen = (key <= pos[y]) & ((key >= from[y]) | (key < sink));
+          s[e] = seen ? s[e] : -INFINITY;
+        }
+      }
+      const float top = over_groups(fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))),
+                                    [](float a, float c) { return fmaxf(a, c); });
+      // the running maximum follows only when a score is 2^kSlack above it: weights of up to 2^kSlack are as exact
+      if (__any(top > m[y] + kSlack)) {
+        const float up = fmaxf(m[y], top), f = __builtin_amdgcn_exp2f(m[y] - up);
+        m[y] = up;
+        l[y] *= f;
+#pragma unroll
+        for (int j = 0; j < VC; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[y][j][r] *= f;
+      }
+      // weights times the values' scale round to bf16 for their product with the codes; the sum that divides them is of the unrounded ones
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float z = __builtin_amdgcn_exp2f(s[e] - m[y]);
+        pr[y][e] = (bf16_t)(s[e] == -INFINITY ? 0.f : z * x.vs);   // a scale of NaN reaches only rows that see its block
+        l[y] += z;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VC; ++j) {
+      u32x4 vt;     // channel j of the eight rows
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        vt[e] = __builtin_amdgcn_perm(vp[2 * e + 1][j / 2], vp[2 * e][j / 2], j % 2 ? 0x07060302 : 0x05040100);
+#pragma unroll
+      for (int y = 0; y < RT; ++y) o[y][j] = mma16(__builtin_bit_cast(bf16x8, vt), pr[y], o[y][j]);
+    }
+  };
+  {
+    Tile a, c;
+    int t = load(a, t0 + w);
+    while (a.key >= 0) {
+      t = load(c, t + NW);
+      use(a);
+      if (c.key < 0) break;
+      t = load(a, t + NW);
+      use(c);
+    }
+  }
+  // The waves' parts: each to the common maximum, then summed in wave order. Channel VC (4 kg + r) + j of row l16 is register r of
+  // accumulator j.
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    const float lw = over_groups(l[x], [](float a, float c) { return a + c; });
+    if (x > 0) __syncthreads();
+    if (kg == 0) {
+      sm[w][l16] = m[x];
+      sl[w][l16] = lw;
+    }
+    __syncthreads();
+    auto highest = [&](int r) { return fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])); };
+    const float f = __builtin_amdgcn_exp2f(m[x] - highest(l16));
+#pragma unroll
+    for (int j = 0; j < VC; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) so[w][l16][VC * (4 * kg + r) + j] = o[x][j][r] * f;
+    __syncthreads();
+    const int rows = min(16, unit.rows - 16 * x);
+    for (int y = tid; y < rows * D; y += 256) {
+      const int r = y / D, d = y % D;
+      const float top = highest(r);
+      float sum = 0.f, all = 0.f;
+#pragma unroll
+      for (int z = 0; z < NW; ++z) {
+        sum += so[z][r][d];
+        all += sl[z][r] * __builtin_amdgcn_exp2f(sm[z][r] - top);
+      }
+      if (alone) {
+        write_row(p, b, unit.query(p, 16 * x + r), unit.head(p, 16 * x + r), d, sum, top, all);
+      } else {
+        float* at = p.part + ((u * p.parts + part) * 16 * RT + 16 * x + r) * (D + 2);
+        at[2 + d] = sum;
+        if (d == 0) {
+          at[0] = top;
+          at[1] = all;
+        }
+      }
+    }
+  }
+}
+
+// The parts of units that have several, in their order: one wave per row.
+template <int D, int RT>
+__global__ void __launch_bounds__(256) join_kernel(AttendParams p, int64_t units) {
+  const int lane = threadIdx.x & 63;
+  const int64_t x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), u = x / (16 * RT);
+  const int r = (int)(x % (16 * RT));
+  if (u >= units) return;
+  Unit unit;
+  unit.init<RT>(p, u);
+  if (r >= unit.rows || unit.tiles <= p.per) return;
+  const int n = (unit.tiles + p.per - 1) / p.per;
+  constexpr int64_t kPart = 16 * RT * (D + 2);
+  const float* at = p.part + (u * p.parts * 16 * RT + r) * (D + 2);
+  float top = kLowest;
+  for (int s = lane; s < n; s += 64) top = fmaxf(top, at[s * kPart]);
+  top = wa_wave_max(top);
+  float l = 0.f, o[D / 64];
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float f = __builtin_amdgcn_exp2f(at[s * kPart] - top);
+    l += at[s * kPart + 1] * f;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] += at[s * kPart + 2 + lane + 64 * e] * f;
+  }
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) write_row(p, unit.b, unit.query(p, r), unit.head(p, r), lane + 64 * e, o[e], top, l);
+}
+
+// How a call is cut: row tiles of a unit, units, tiles of a part and parts.
+struct Cut {
+  int rt, units_of;
+  int64_t units;
+  int per, parts;
+};
+
+bool sized(const wa_kv8_attend_args& a) {
+  const wa_cache8& c = a.cache;
+  return c.B >= 1 && a.n >= 1 && c.cap >= 1 && c.cap <= 1 << 30 && c.Hk >= 1 && a.H >= c.Hk && a.H % c.Hk == 0 && a.H <= 65536 && a.n <= 1 << 24 &&
+         c.B <= 1 << 24 && a.n * (a.H / c.Hk) <= INT32_MAX && a.window >= 0 && a.sink >= 0 &&
+         (!a.index || (a.topk >= 1 && a.topk <= WA_SELECT_MAX_BLOCKS && a.window == 0));
+}
+
+Cut cut(const wa_kv8_attend_args& a) {
+  Cut c;
+  const int64_t G = a.H / a.cache.Hk, rows = a.index ? G : a.n * G;
+  c.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t of = (rows + 16 * c.rt - 1) / (16 * c.rt);
+  c.units_of = (int)of;
+  c.units = a.cache.B * a.cache.Hk * of * (a.index ? a.n : 1);
+  const int64_t tokens = a.kv_len ? a.cache.cap : std::min(std::max<int64_t>(a.kv_len_all, 0), a.cache.cap);
+  // at most: the sinks', and from the first row's window to the last row, each run with a partial tile at either end
+  const int64_t seen = a.window > 0 ? std::min(tokens, std::min(a.sink, tokens) + std::min(a.window, tokens) + a.n + 128) : tokens;
+  const int64_t tiles = a.index ? a.topk * (a.cache.block_size / 32) : (seen + 31) / 32;
+  // parts of at least 8 tiles (two a wave), about 2,048 workgroups where there is work for them: ragged sequences even out
+  const int64_t want = std::max<int64_t>(1, 2048 / c.units);
+  c.per = (int)std::max<int64_t>(8, (tiles + want - 1) / want);
+  c.parts = (int)std::max<int64_t>(1, (tiles + c.per - 1) / c.per);
+  return c;
+}
+
+template <typename Code, int D>
+void launch(const AttendParams& p, const Cut& c, hipStream_t s) {
+  const dim3 grid((unsigned)(c.units * c.parts)), block(256);
+  const dim3 rows((unsigned)((c.units * 16 * c.rt + 3) / 4));
+  if (c.rt == 1) hipLaunchKernelGGL((attend_kernel<Code, D, 1>), grid, block, 0, s, p);
+  else if (c.rt == 2) hipLaunchKernelGGL((attend_kernel<Code, D, 2>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((attend_kernel<Code, D, 4>), grid, block, 0, s, p);
+  if (c.parts == 1) return;
+  if (c.rt == 1) hipLaunchKernelGGL((join_kernel<D, 1>), rows, block, 0, s, p, c.units);
+  else if (c.rt == 2) hipLaunchKernelGGL((join_kernel<D, 2>), rows, block, 0, s, p, c.units);
+  else hipLaunchKernelGGL((join_kernel<D, 4>), rows, block, 0, s, p, c.units);
+}
+
+}  // namespace
+
+extern "C" int64_t wa_kv8_attend_workspace_bytes(const wa_kv8_attend_args* a) {
+  if (!a || !sized(*a)) return 0;
+  const Cut c = cut(*a);
+  return c.parts > 1 ? c.units * c.parts * 16 * c.rt * (a->cache.D + 2) * 4 : 0;
+}
+
+extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
+  WA_CHECK_ARG(a, "kv8_attend: null args");
+  const wa_cache8& c = a->cache;
+  WA_CHECK_ARG(c.D == 64 || c.D == 128, "kv8_attend: head dim must be 64 or 128, got %lld", (long long)c.D);
+  WA_CHECK_ARG(c.block_size == 64 || c.block_size == 128, "kv8_attend: block size must be 64 or 128, got %lld", (long long)c.block_size);
+  WA_CHECK_ARG(c.code == WA_CODE_INT8 || c.code == WA_CODE_E4M3, "kv8_attend: unknown code %d", c.code);
+  WA_CHECK_ARG(sized(*a), "kv8_attend: bad sizes B %lld n %lld cap %lld heads %lld / %lld window %lld sink %lld, or lists that are not of 1 .. %d ids without a window",
+               (long long)c.B, (long long)a->n, (long long)c.cap, (long long)a->H, (long long)c.Hk, (long long)a->window, (long long)a->sink, WA_SELECT_MAX_BLOCKS);
+  WA_CHECK_ARG(c.k && c.v && c.k_scale && c.v_scale && wa_aligned16(c.k) && wa_aligned16(c.v) && a->q && a->o && a->lse, "kv8_attend: null or misaligned tensor");
+  WA_CHECK_ARG(!a->index == !a->num, "kv8_attend: lists need counts");
+  auto rows16 = [](const void* x, int64_t sb, int64_t st, int64_t sh) {
+    return wa_aligned16(x) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0;
+  };
+  WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->o, a->o_sb, a->o_st, a->o_sh), "kv8_attend: rows must be 16-byte aligned");
+  WA_CHECK_ARG(a->scale >= 0.f && a->cap >= 0.f && a->scale < INFINITY && a->cap < INFINITY, "kv8_attend: scale and cap must be finite and not below 0");
+  const Cut k = cut(*a);
+  WA_CHECK_ARG(k.units * k.parts <= INT32_MAX && k.units * 16 * k.rt / 4 <= INT32_MAX, "kv8_attend: too many rows");
+  WA_CHECK_ARG(k.parts == 1 || a->workspace, "kv8_attend: a launch of %d parts needs a workspace", k.parts);
+  AttendParams p{};
+  p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.o = (bf16_t*)a->o; p.o_sb = a->o_sb; p.o_st = a->o_st; p.o_sh = a->o_sh;
+  p.lse = a->lse;
+  p.k = (const uint8_t*)c.k; p.v = (const uint8_t*)c.v; p.k_scale = c.k_scale; p.v_scale = c.v_scale;
+  p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.cap = c.cap;
+  p.index = a->index; p.num = a->num; p.topk = (int)a->topk;
+  p.window = std::min(a->window, (int64_t)1 << 30); p.sink = std::min(a->sink, (int64_t)1 << 30);
+  p.slopes = a->slopes;
+  p.n = (int)a->n; p.H = (int)a->H; p.Hk = (int)c.Hk;
+  p.nb = (int)((c.cap + c.block_size - 1) / c.block_size); p.shift = c.block_size == 64 ? 6 : 7;
+  p.units = k.units_of; p.parts = k.parts; p.per = k.per;
+  const float scale = a->scale == 0.f ? 1.f / sqrtf((float)c.D) : a->scale;
+  p.scale2 = scale * WA_LOG2E;
+  p.bend_in = a->cap > 0.f ? 2.f * scale / a->cap * WA_LOG2E : p.scale2;
+  p.cap2 = a->cap * WA_LOG2E;
+  p.part = (float*)a->workspace;
+  hipStream_t s = (hipStream_t)stream;
+  if (c.code == WA_CODE_INT8) {
+    if (c.D == 128) launch<Int8, 128>(p, k, s);
+    else launch<Int8, 64>(p, k, s);
+  } else {
+    if (c.D == 128) launch<E4m3, 128>(p, k, s);
+    else launch<E4m3, 64>(p, k, s);
+  }
+  return wa_launch_status("kv8_attend");
+}

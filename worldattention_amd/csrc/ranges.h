@@ -81,7 +81,7 @@ struct Steps {
 struct RowRuns {
   int up, up_n, low, low_n;
   __device__ __forceinline__ RowRuns(const int4& r, int end) : up(r.x), up_n(max(min(r.y, end) - r.x, 0)), low(r.z), low_n(max(min(r.w, end) - r.z, 0)) {}
-  __device__ __forceinline__ bool sees(int key) const { return (unsigned)(key - up) < (unsigned)up_n || (unsigned)(key - low) < (unsigned)low_n; }
+  __device__ __forceinline__ bool sees(int key) const { return ((unsigned)(key - up) < (unsigned)up_n) | ((unsigned)(key - low) < (unsigned)low_n); }
 };
 
 // Scores beyond the plain product, in units of log2: y = cap tanh(x / cap) with, e = exp(2 x / cap) and r = 1 / (e + 1),

@@ -10,6 +10,7 @@ from .attention import (
 )
 from .kvcache import kv_append, new_block_sums
 from .block_sparse import block_sparse_attention, block_sparse_attention_reference, map_to_index
+from .cache8 import attend_8bit, kv_append_8bit, kv_read_8bit, new_cache_8bit
 from .decay import decay_linear_attention, decay_linear_step
 from .ranged import KeyRanges, key_ranges, ranged_attention
 from .rope import axis_frequencies, rope_axes
@@ -46,6 +47,10 @@ __all__ = [
     "KeyRanges",
     "key_ranges",
     "ranged_attention",
+    "new_cache_8bit",
+    "kv_append_8bit",
+    "kv_read_8bit",
+    "attend_8bit",
     "BlockSelection",
     "select_key_blocks",
     "selected_attention",
