@@ -35,6 +35,8 @@ struct BwdParams {
   float* on;      // [B, H, Lq] 1, or 0 where a row sees a single key: its weight is 1 whatever the score, and its dS exactly 0
   float* delta;   // [B, H, Lq] delta * on
   float* slope_part;   // [H][B * q tiles]
+  float* part_kv;      // [parts][dK, dV][B, Lk, Hk, D] fp32, with parts > 1
+  int parts;
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -90,6 +92,104 @@ struct RowTile {
   }
 };
 
+// A lane's operands in a 64-row tile whose LDS address is a multiple of its size: rows l32 + 32 x, chunk 2 c + g (tile.h's tile_row8), and
+// transposed, rows of 16 c at columns 32 tt + l32 (tile_tr8). With the swizzle's exclusive ors a lane needs one address of either kind: what c and tt
+// turn are bits of it, what x and 16 c rows add is a constant (an address for each operand cost registers that the products' operands need).
+typedef __attribute__((address_space(3))) const bf16x8 lds_bf16x8;
+typedef __attribute__((address_space(3))) wa_s16x4 lds_s16x4;
+template <int D>
+struct TileReads {
+  uint32_t row, col;
+  __device__ __forceinline__ void init(int lane) {
+    const int l32 = lane & 31, g = lane >> 5, G = lane >> 4, r = (lane & 15) >> 2, q = lane & 3, i = 4 * (G >> 1) + r, at = 16 * (G & 1) + 4 * q;
+    row = (uint32_t)(l32 * D + (g ^ dual_swizzle<D>(l32)) * 8) * 2;
+    col = (uint32_t)(i * D + ((at >> 3) ^ dual_swizzle<D>(i)) * 8 + (at & 7)) * 2;
+  }
+  __device__ __forceinline__ static uint32_t address(const bf16_t* tile) { return (uint32_t)(size_t)WA_LDS_PTR(tile); }
+  __device__ __forceinline__ bf16x8 row8(uint32_t tile, int c, int x) const { return *(lds_bf16x8*)(size_t)(((tile | row) ^ 32 * c) + 64 * D * x); }
+  __device__ __forceinline__ bf16x8 tr8(uint32_t tile, int c, int tt) const {
+    bf16x8 a;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {   // eight rows on, whose swizzle differs in the lowest bit
+      const uint32_t at = ((tile | col) ^ (64 * tt) ^ (hf ? 16 * D + 16 : 0)) + 32 * D * c;
+      const bf16x4 b = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(size_t)at));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[4 * hf + e] = b[e];
+    }
+    return a;
+  }
+};
+
+// Products whose operands are read from LDS two at a time and kAhead pairs ahead: left to itself the compiler waits for each read right behind it.
+constexpr int kAhead = 1;
+typedef bf16x8 Operands[kAhead + 1][2];
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// acc[x] = rows 32 x .. of the tile times b^T. `first` reads the first operands.
+template <int D>
+struct RowsProduct {
+  static constexpr int N = D / 16;   // pairs: of one chunk c
+  __device__ __forceinline__ static void read(const TileReads<D>& rd, uint32_t lds, Operands& a, int i) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) a[i % (kAhead + 1)][y] = rd.row8(lds, i, y);
+  }
+  __device__ __forceinline__ static void first(const TileReads<D>& rd, uint32_t lds, Operands& a) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) read(rd, lds, a, i);
+  }
+  __device__ __forceinline__ static void run(const TileReads<D>& rd, uint32_t lds, const bf16x8 (&b)[D / 16], f32x16 (&acc)[2], Operands& a) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i + kAhead < N) read(rd, lds, a, i + kAhead);
+      in_order();
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[y] = wa_mfma32(a[i % (kAhead + 1)][y], b[i], i == 0 ? f32x16{} : acc[y]);
+      in_order();
+    }
+  }
+};
+// acc[tt] += (the tile's columns 32 tt ..)^T times b, over the tile's 64 rows.
+template <int D>
+struct ColsProduct {
+  static constexpr int DT = D / 32, N = 2 * DT;
+  __device__ __forceinline__ static void read(const TileReads<D>& rd, uint32_t lds, Operands& a, int i) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) a[i % (kAhead + 1)][y] = rd.tr8(lds, (2 * i + y) / DT, (2 * i + y) % DT);
+  }
+  __device__ __forceinline__ static void first(const TileReads<D>& rd, uint32_t lds, Operands& a) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) read(rd, lds, a, i);
+  }
+  __device__ __forceinline__ static void run(const TileReads<D>& rd, uint32_t lds, const bf16x8 (&b)[4], f32x16 (&acc)[DT], Operands& a) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i + kAhead < N) read(rd, lds, a, i + kAhead);
+      in_order();
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[(2 * i + y) % DT] = wa_mfma32(a[i % (kAhead + 1)][y], b[(2 * i + y) / DT], acc[(2 * i + y) % DT]);
+      in_order();
+    }
+  }
+};
+
+// a b, and 0 where either is 0, whatever the other.
+__device__ __forceinline__ float zero_mul(float a, float b) {
+  float x;
+  asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(x) : "v"(a), "v"(b));
+  return x;
+}
+
+// Four values as bf16 into places 4 x .. of an operand.
+__device__ __forceinline__ void put4(bf16x8& a, int x, const float (&f)[4]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bf16x2 p = __builtin_convertvector(f32x2{f[2 * i], f[2 * i + 1]}, bf16x2);
+    a[4 * x + 2 * i] = p[0];
+    a[4 * x + 2 * i + 1] = p[1];
+  }
+}
+
 template <int N> using IC = std::integral_constant<int, N>;
 
 // Top of a step: this wave's tile loads have landed and its LDS reads returned, then the workgroup's.
@@ -108,8 +208,8 @@ template <int D, bool BENT, bool SLOPES>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ranged_dq_kernel(BwdParams p) {
   constexpr int NW = 4, DC = D / 16, DT = D / 32, TILE = 64 * D;
   using RT = RowTile<D, NW>;
-  __shared__ __attribute__((aligned(1024))) bf16_t kv0[2 * TILE];
-  __shared__ __attribute__((aligned(1024))) bf16_t kv1[2 * TILE];
+  __shared__ __attribute__((aligned(2 * TILE))) bf16_t kv0[2 * TILE];
+  __shared__ __attribute__((aligned(2 * TILE))) bf16_t kv1[2 * TILE];
   __shared__ float s_part[NW];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, l32 = lane & 31;
@@ -165,72 +265,80 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
     kt.issue(kv, kb + key * p.k_st, p.k_st, rows, w);
     vt.issue(kv + TILE, vb + key * p.v_st, p.v_st, rows, w);
   };
-  auto step = [&](auto S, int t) {
-    const bf16_t* kc = decltype(S)::value ? kv1 : kv0;
-    const bf16_t* vc = kc + TILE;
-    step_wait();
-    f32x16 sacc[2], pacc[2];
+  TileReads<D> rd;
+  rd.init(lane);
+  auto slopes_of = [&](float pr, float dp, float dist) {
+    const float pd = pr * dp, far = fabsf(dist);
+    a0 += pr;
+    a1 += pd;
+    a2 = fmaf(pd, far, a2);
+    a3 = fmaf(pr, far, a3);
+  };
+  // 32 keys at a time: S^T = K Q^T and dP^T = V dO^T in turn, then dS^T = P^T (dP^T - delta), packed in accumulator order for the next product
+  // (both halves' products first, their exponentials after, took 64 more registers than there are).
+  auto half = [&](uint32_t kc, uint32_t vc, int x, int key0, int end, bool whole, bf16x8* dsb) {
+    f32x16 s, dp;
+    Operands a;
+    auto read = [&](int c) {
+      a[c % (kAhead + 1)][0] = rd.row8(kc, c, x);
+      a[c % (kAhead + 1)][1] = rd.row8(vc, c, x);
+    };
 #pragma unroll
-    for (int x = 0; x < 2; ++x) sacc[x] = pacc[x] = f32x16{};
+    for (int c = 0; c < kAhead; ++c) read(c);
 #pragma unroll
     for (int c = 0; c < DC; ++c) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        sacc[x] = wa_mfma32(tile_row8<D>(kc, x * 32 + l32, 2 * c + g), qf[c], sacc[x]);
-        pacc[x] = wa_mfma32(tile_row8<D>(vc, x * 32 + l32, 2 * c + g), dof[c], pacc[x]);
-      }
+      if (c + kAhead < DC) read(c + kAhead);
+      in_order();
+      s = wa_mfma32(a[c % (kAhead + 1)][0], qf[c], c == 0 ? f32x16{} : s);
+      dp = wa_mfma32(a[c % (kAhead + 1)][1], dof[c], c == 0 ? f32x16{} : dp);
+      in_order();
     }
-    if (t + 1 < st.total) issue(decltype(S)::value ? kv0 : kv1, t + 1);   // the stage of step t - 1
-    const int key = st.key(t), end = st.end(t);
-    bf16x8 dsb[4];
-    // dS^T = P^T (dP^T - delta), packed in accumulator order for the next product
-    auto slopes_of = [&](float pr, float dp, float dist) {
-      const float pd = pr * dp, far = fabsf(dist);
-      a0 += pr;
-      a1 += pd;
-      a2 = fmaf(pd, far, a2);
-      a3 = fmaf(pr, far, a3);
-    };
     auto weights = [&](auto masked) {
       const RowRuns mine(runs, end);
+      const float far = (float)(key0 - pos);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int key0 = key + 32 * x + 4 * g;
-        const float far = (float)(key0 - pos);
+      for (int r4 = 0; r4 < 4; ++r4) {
+        float out[4];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = 8 * (r >> 2) + (r & 3);
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * r4 + i, at = 8 * r4 + i;
           float turn = 1.f, pr;
-          if constexpr (BENT) pr = __builtin_amdgcn_exp2f(bend(sacc[x][r], far + (float)at, turn) - lse2);
-          else pr = __builtin_amdgcn_exp2f(fmaf(sacc[x][r], p.scale2, -lse2));
-          float dp = pacc[x][r], ds = pr * fmaf(dp, on, -dl);
+          if constexpr (BENT) pr = __builtin_amdgcn_exp2f(bend(s[r], far + (float)at, turn) - lse2);
+          else pr = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lse2));
+          float d = dp[r], ds = pr * fmaf(d, on, -dl);
           if constexpr (BENT) ds *= turn;
           if constexpr (decltype(masked)::value) {
             const bool seen = mine.sees(key0 + at);
             ds = seen ? ds : 0.f;
             if constexpr (SLOPES) {
               pr = seen ? pr : 0.f;
-              dp = seen ? dp : 0.f;
+              d = seen ? d : 0.f;
             }
           }
-          if constexpr (SLOPES) slopes_of(pr, dp, far + (float)at);
-          dsb[x * 2 + (r >> 3)][r & 7] = (bf16_t)ds;
+          if constexpr (SLOPES) slopes_of(pr, d, far + (float)at);
+          out[i] = ds;
         }
+        put4(dsb[r4 >> 1], r4 & 1, out);
+        if constexpr (BENT) in_order();
       }
     };
-    if (st.whole(key, end)) weights(std::false_type{});
+    if (whole) weights(std::false_type{});
     else weights(std::true_type{});
-    // dQ[q, d] += dS[q, key] K[key, d]: A = dS (registers), B = K (transpose reads)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-#pragma unroll
-      for (int tt = 0; tt < DT; ++tt) dqacc[tt] = wa_mfma32(dsb[c], tile_tr8<D>(kc, c, 32 * tt, lane), dqacc[tt]);
-    }
   };
   if (st.total > 0) issue(kv0, 0);
-  for (int t = 0; t < st.total; t += 2) {
-    step(IC<0>{}, t);
-    if (t + 1 < st.total) step(IC<1>{}, t + 1);
+  for (int t = 0; t < st.total; ++t) {
+    const uint32_t kc = rd.address(t & 1 ? kv1 : kv0), vc = kc + 2 * TILE;
+    step_wait();
+    if (t + 1 < st.total) issue(t & 1 ? kv0 : kv1, t + 1);   // the stage of step t - 1
+    const int key = st.key(t), end = st.end(t);
+    const bool whole = st.whole(key, end);
+    bf16x8 dsb[4];
+    half(kc, vc, 0, key + 4 * g, end, whole, dsb);
+    half(kc, vc, 1, key + 32 + 4 * g, end, whole, dsb + 2);
+    // dQ^T[d, q] += K^T dS^T: A by transpose reads, B from registers (a row a lane)
+    Operands a;
+    ColsProduct<D>::first(rd, kc, a);
+    ColsProduct<D>::run(rd, kc, dsb, dqacc, a);
   }
   if constexpr (SLOPES) {
     a0 += __shfl_xor(a0, 32, 64);
@@ -251,14 +359,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
     __syncthreads();
     if (tid == 0) p.slope_part[((int64_t)h * p.B + b) * nq + qt] = -(s_part[0] + s_part[1] + s_part[2] + s_part[3]);
   }
-  // accumulator lane (d = 32 t + l32, g) holds rows 32 w + 8 (r / 4) + 4 g + r % 4
-  bf16_t* out = p.dq + ((int64_t)b * p.ranges.Lq * p.H + h) * D + l32;
+  // channel 32 tt + 8 rq + 4 g + i of row l32 is register 4 rq + i of accumulator tt
+  if (!q_ok) return;
+  bf16_t* out = p.dq + (((int64_t)b * p.ranges.Lq + qi) * p.H + h) * D + 4 * g;
 #pragma unroll
   for (int tt = 0; tt < DT; ++tt) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int i = qt * 128 + w * 32 + 8 * (r >> 2) + 4 * g + (r & 3);
-      if (i < p.ranges.Lq) out[(int64_t)i * p.H * D + 32 * tt] = (bf16_t)(dqacc[tt][r] * p.scale);
+    for (int rq = 0; rq < 4; ++rq) {
+      bf16x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (bf16_t)(dqacc[tt][4 * rq + i] * p.scale);
+      *(bf16x4*)(out + 32 * tt + 8 * rq) = x;
     }
   }
 }
@@ -278,33 +389,41 @@ __global__ void __launch_bounds__(256) slopes_kernel(BwdParams p, int n) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// dK, dV: one workgroup per 64 keys of a key head, over the 64-row tiles that see one of them, for each query head of the group in turn.
-// Q, dO and the rows' statistics and runs stream through two LDS stages. Each 32 keys have two waves, a key a lane:
-//   the S-wave holds the keys and dV: S = Q K^T, P = exp2(s - lse2), P (1 - tanh^2) to LDS as fp16, dV += P^T dO;
-//   the dP-wave holds the values and dK: dP = dO V^T, dx from them, dK += dx^T Q.
+// dK, dV: one workgroup of eight waves per 128 keys of a key head, over the 64-row tiles that see one of them, for each query head of the
+// group in turn. Each 32 keys have two waves, on one SIMD, a key a lane:
+//   the S-wave holds the keys and dV. Phase t: S = Q K^T of step t, P = exp2(s - lse2), P (1 - tanh^2) to LDS as fp16, dV += P^T dO;
+//   the dP-wave holds the values and dK, a step behind. Phase t: dx of step t - 1 from its dP and the weights in LDS, dK += dx^T Q, then
+//   dP = dO V^T of step t.
+// So one wave's products run under the other's exponentials, with one barrier a step. Q, dO and the rows' statistics and runs stream two steps ahead
+// into rings of four (Q is read by both phases), three and four stages; the weights have two. A workgroup takes 156 KiB of LDS at D = 128.
+// PARTS: the steps are cut into runs for workgroups of their own, whose fp32 sums another launch adds up in their order.
 // ---------------------------------------------------------------------------------------------
 constexpr int kListMax = 1024;   // row tiles listed at a time: 65,536 rows
+constexpr int kKeys = 128;       // of a workgroup
 
 template <int D, bool BENT>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ranged_dkv_kernel(BwdParams p) {
-  constexpr int NW = 4, DC = D / 16, DT = D / 32, TILE = 64 * D;
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) ranged_dkv_kernel(BwdParams p) {
+  constexpr int NW = 8, DC = D / 16, DT = D / 32, TILE = 64 * D;
   using RT = RowTile<D, NW>;
-  // a stage: Q tile, dO tile, 64 lse2, 64 delta, 64 on, 64 rows' runs
-  constexpr int STATS = 2 * TILE, SS = STATS + 3 * 128 + 512;
-  __shared__ __attribute__((aligned(1024))) bf16_t qd0[SS];
-  __shared__ __attribute__((aligned(1024))) bf16_t qd1[SS];
-  __shared__ __attribute__((aligned(1024))) f16x4 s_p[2][2][4][64];
+  constexpr int STATS = 192 + 256;   // floats of a stage: 64 lse2, 64 delta, 64 on, 64 rows' runs
+  __shared__ __attribute__((aligned(2 * TILE))) bf16_t s_q[4 * TILE];   // tiles at multiples of their size (TileReads)
+  __shared__ __attribute__((aligned(2 * TILE))) bf16_t s_do[3 * TILE];
+  __shared__ __attribute__((aligned(1024))) f16x4 s_p[2][4][2][4][64];
+  __shared__ __attribute__((aligned(1024))) float s_stats[4 * STATS];
   __shared__ int s_list[kListMax];   // row tile (from `base` on) | rows up to its last that sees anything << 10 | whole << 20
   __shared__ int s_count[NW];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 5, l32 = lane & 31, kg = w & 1;
-  const bool swave = w < 2;   // wave-uniform role
+  const int g = lane >> 5, l32 = lane & 31, kg = w & 3;
+  const bool swave = w < 4;   // wave-uniform role
   // a causal mask's first keys are seen by most rows: they start first
   const int per = p.H / p.Hk, nbh = p.B * p.Hk;
-  const int bh = (int)blockIdx.x % nbh, key0 = (int)blockIdx.x / nbh * 64, hk = bh % p.Hk, b = bh / p.Hk;
+  int u = (int)blockIdx.x;
+  const int bh = u % nbh, hk = bh % p.Hk, b = bh / p.Hk;
+  u /= nbh;
+  const int part = u % p.parts, key0 = u / p.parts * kKeys;
   const int kl = kg * 32 + l32, key = key0 + kl;
   const bool k_ok = key < p.ranges.Lk;
-  const int key_end = min(key0 + 64, p.ranges.Lk);
+  const int key_end = min(key0 + kKeys, p.ranges.Lk);
 
   bf16x8 kvf[DC];
   {
@@ -327,11 +446,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   RT qt, dt;
   qt.init(p.q_st, w, lane);
   dt.init(p.d_st, w, lane);
+  TileReads<D> rd;
+  rd.init(lane);
 
   for (int base = 0; base < p.ranges.n_tiles; base += kListMax) {
     const int limit = min(base + kListMax, p.ranges.n_tiles);
     int n = 0;
-    for (int i0 = base; i0 < limit; i0 += 256) {
+    for (int i0 = base; i0 < limit; i0 += 64 * NW) {
       const int i = i0 + tid;
       bool any = false;
       int entry = 0;
@@ -346,135 +467,200 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
       if (lane == 0) s_count[w] = __popcll(mask);
       __syncthreads();
       int at = n + __popcll(mask & ((1ull << lane) - 1));
-      for (int x = 0; x < w; ++x) at += s_count[x];
+#pragma unroll
+      for (int x = 0; x < NW; ++x) {
+        const int c = s_count[x];
+        if (x < w) at += c;
+        n += c;
+      }
       if (any) s_list[at] = entry;
-      n += s_count[0] + s_count[1] + s_count[2] + s_count[3];
     }
     __syncthreads();
     n = __builtin_amdgcn_readfirstlane(n);
-    const int total = n * per;
-    int next_g = 0, next_i = 0;   // of the step issued next
-    auto issue = [&](bf16_t* qd) {
-      const int entry = __builtin_amdgcn_readfirstlane(s_list[next_i]), rows = entry >> 10 & 127;
-      const int row0 = (base + (entry & 1023)) * 64, h = hk * per + next_g;
-      qt.issue(qd, p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)row0 * p.q_st, p.q_st, rows, w);
-      dt.issue(qd + TILE, p.dout + (int64_t)b * p.d_sb + (int64_t)h * p.d_sh + (int64_t)row0 * p.d_st, p.d_st, rows, w);
-      const int64_t srow = ((int64_t)b * p.H + h) * p.ranges.Lq + row0;
-      float* stats = (float*)(qd + STATS);
-      const int count = min(64, p.ranges.Lq - row0);
-      if (w == 0) row_stats_dma(stats, p.lse2 + srow, count, lane);
-      if (w == 1) row_stats_dma(stats + 64, p.delta + srow, count, lane);
-      if (w == 2) row_stats_dma(stats + 128, p.on + srow, count, lane);
-      if (w == 3) {
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(p.ranges.rows + ((int64_t)b * p.ranges.sb * p.ranges.Lq + row0) * 4), (short)0, count * 16, WA_BUF_DWORD3);
-        lds_dma16(rs, stats + 192, lane * 16);
-      }
-      if (++next_i == n) {
-        next_i = 0;
-        ++next_g;
-      }
-    };
-    int now_g = 0, now_i = 0;
-    float slope2 = BENT && p.slopes ? p.slopes[hk * per] * WA_LOG2E : 0.f;
-    auto step = [&](auto S, int t) {
-      const bf16_t* qc = decltype(S)::value ? qd1 : qd0;
-      const bf16_t* dc = qc + TILE;
-      const float* st_lse2 = (const float*)(qc + STATS);
-      const float* st_dl = st_lse2 + 64;
-      const float* st_on = st_lse2 + 128;
-      const int4* st_runs = (const int4*)(st_lse2 + 192);
-      step_wait();
-      const int entry = __builtin_amdgcn_readfirstlane(s_list[now_i]);
-      const int row0 = (base + (entry & 1023)) * 64;
-      const bool whole = entry >> 20;
-      // S[q, key] = Q K^T (S-wave) or dP[q, key] = dO V^T (dP-wave) per 32 rows; lane = key, registers = rows 32 x + 8 rq + 4 g + i
-      const bf16_t* at = swave ? qc : dc;
-      f32x16 sacc[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) sacc[x] = f32x16{};
-#pragma unroll
-      for (int c = 0; c < DC; ++c) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) sacc[x] = wa_mfma32(tile_row8<D>(at, x * 32 + l32, 2 * c + g), kvf[c], sacc[x]);
-      }
-      if (t + 1 < total) issue(decltype(S)::value ? qd0 : qd1);   // the stage of step t - 1
-      bf16x8 ab[4];
-      auto weights = [&](auto masked) {
-        const Bend bend{p.bend_in, p.cap2, slope2};
-        const float far = (float)(key - pos0 - row0 - 4 * g);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-          for (int rq = 0; rq < 4; ++rq) {
-            const int r0 = 32 * x + 8 * rq;
-            const f32x4 l4 = *(const f32x4*)(st_lse2 + r0 + 4 * g);
-            f16x4 p4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = rq * 4 + i;
-              float turn = 1.f, pr;
-              if constexpr (BENT) pr = __builtin_amdgcn_exp2f(bend(sacc[x][r], far - (float)(r0 + i), turn) - l4[i]);
-              else pr = __builtin_amdgcn_exp2f(fmaf(sacc[x][r], p.scale2, -l4[i]));
-              if constexpr (decltype(masked)::value) {
-                const RowRuns row(st_runs[r0 + 4 * g + i], INT32_MAX);
-                pr = row.sees(key) ? pr : 0.f;
-              }
-              ab[x * 2 + (r >> 3)][r & 7] = (bf16_t)pr;
-              p4[i] = (_Float16)(pr * (BENT ? kLift * turn : kLift));
-            }
-            s_p[kg][x][rq][lane] = p4;
+    const int all = n * per;
+    const int first = (int)((int64_t)all * part / p.parts), total = (int)((int64_t)all * (part + 1) / p.parts) - first;
+    if (total > 0) {
+      int next_g = first / n, next_i = first % n, next_do = 0, now_do = 0;   // of the step issued next
+      int now_g = next_g, now_i = next_i;
+      // The next step's list entry is read while the present one is issued, and a head's addresses are formed once: what an issue takes from the
+      // waves is scalar work that nothing hides.
+      int next_entry = s_list[next_i];
+      const bf16_t* qh = p.q + (int64_t)b * p.q_sb + (int64_t)(hk * per + next_g) * p.q_sh;
+      const bf16_t* dh = p.dout + (int64_t)b * p.d_sb + (int64_t)(hk * per + next_g) * p.d_sh;
+      const float* stat = w == 0 ? p.lse2 : w == 1 ? p.delta : p.on;   // the row statistics that this wave streams
+      stat += ((int64_t)b * p.H + hk * per + next_g) * p.ranges.Lq;
+      const int32_t* runs = p.ranges.rows + (int64_t)b * p.ranges.sb * p.ranges.Lq * 4;
+      auto issue = [&](int t) {
+        if (t >= total) return;
+        const int entry = __builtin_amdgcn_readfirstlane(next_entry), rows = entry >> 10 & 127, row0 = (base + (entry & 1023)) * 64;
+        const bf16_t *qn = qh, *dn = dh;
+        const float* sn = stat;
+        if (++next_i == n) {
+          next_i = 0;
+          qh += p.q_sh;
+          dh += p.d_sh;
+          stat += p.ranges.Lq;
+        }
+        next_entry = s_list[next_i];
+        qt.issue(s_q + (t & 3) * TILE, qn + row0 * p.q_st, p.q_st, rows, w);
+        dt.issue(s_do + next_do * TILE, dn + row0 * p.d_st, p.d_st, rows, w);
+        next_do = next_do == 2 ? 0 : next_do + 1;
+        if (w < 4) {
+          float* to = s_stats + (t & 3) * STATS + 64 * w;
+          const int count = min(64, p.ranges.Lq - row0);
+          if (w < 3) {
+            row_stats_dma(to, sn + row0, count, lane);
+          } else {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(runs + (int64_t)row0 * 4), (short)0, count * 16, WA_BUF_DWORD3);
+            lds_dma16(rs, to, lane * 16);
           }
         }
       };
+      // Top of phase t: this wave's loads of step t have landed (those of step t + 1, five of an S-wave's and four of a dP-wave's at
+      // D = 128, may be on their way) and its LDS reads returned, then the workgroup's.
+      auto top = [&](int t) {
+        if (t + 1 >= total) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else if (swave) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * RT::NI + 1) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * RT::NI) : "memory");
+      };
+      issue(0);
+      issue(1);
       if (swave) {
-        if (whole) weights(std::false_type{});
-        else weights(std::true_type{});
-      }
-      __syncthreads();   // the weights of both key halves are in LDS
-      if (!swave) {
+        float slope2 = BENT && p.slopes ? p.slopes[hk * per + now_g] * WA_LOG2E : 0.f;
+        for (int t = 0; t < total; ++t) {
+          top(t);
+          const uint32_t qc = rd.address(s_q + (t & 3) * TILE);
+          const uint32_t dc = rd.address(s_do + now_do * TILE);
+          const float* st_lse2 = s_stats + (t & 3) * STATS;
+          const int4* st_runs = (const int4*)(st_lse2 + 192);
+          const int entry = __builtin_amdgcn_readfirstlane(s_list[now_i]);
+          const int row0 = (base + (entry & 1023)) * 64;
+          // S[q, key] = Q K^T per 32 rows; lane = key, registers = rows 32 x + 8 rq + 4 g + i
+          f32x16 sacc[2];
+          Operands a;
+          RowsProduct<D>::first(rd, qc, a);
+          RowsProduct<D>::run(rd, qc, kvf, sacc, a);
+          issue(t + 2);
+          ColsProduct<D>::first(rd, dc, a);   // under the exponentials
+          in_order();
+          bf16x8 ab[4];
+          auto weights = [&](auto masked) {
+            const Bend bend{p.bend_in, p.cap2, slope2};
+            const float far = (float)(key - pos0 - row0 - 4 * g);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < 2; ++x) {
 #pragma unroll
-          for (int rq = 0; rq < 4; ++rq) {
-            const int r0 = 32 * x + 8 * rq + 4 * g;
-            const f32x4 d4 = *(const f32x4*)(st_dl + r0), o4 = *(const f32x4*)(st_on + r0);
-            const f16x4 p4 = s_p[kg][x][rq][lane];
+              for (int rq = 0; rq < 4; ++rq) {
+                const int r0 = 32 * x + 8 * rq;
+                const f32x4 l4 = *(const f32x4*)(st_lse2 + r0 + 4 * g);
+                f16x4 p4;
+                float pw[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = rq * 4 + i;
-              float ds = (float)p4[i] * fmaf(sacc[x][r], o4[i], -d4[i]);
-              if (!whole && p4[i] == (_Float16)0.f) ds = 0.f;   // what a masked key holds, NaN too, reaches nothing
-              ab[x * 2 + (r >> 3)][r & 7] = (bf16_t)ds;
+                for (int i = 0; i < 4; ++i) {
+                  const int r = rq * 4 + i;
+                  float turn = 1.f, pr;
+                  if constexpr (BENT) pr = __builtin_amdgcn_exp2f(bend(sacc[x][r], far - (float)(r0 + i), turn) - l4[i]);
+                  else pr = __builtin_amdgcn_exp2f(fmaf(sacc[x][r], p.scale2, -l4[i]));
+                  if constexpr (decltype(masked)::value) {
+                    const RowRuns row(st_runs[r0 + 4 * g + i], INT32_MAX);
+                    pr = row.sees(key) ? pr : 0.f;
+                  }
+                  pw[i] = pr;
+                  p4[i] = (_Float16)(pr * (BENT ? kLift * turn : kLift));
+                }
+                put4(ab[x * 2 + (rq >> 1)], rq & 1, pw);
+                s_p[t & 1][kg][x][rq][lane] = p4;
+                if (decltype(masked)::value || rq % 2) in_order();   // few rows' statistics in registers at a time
+              }
             }
+          };
+          if (entry >> 20) weights(std::false_type{});
+          else weights(std::true_type{});
+          // dV^T[d, key] += dO^T P: A by transpose reads, B from registers
+          ColsProduct<D>::run(rd, dc, ab, acc, a);
+          now_do = now_do == 2 ? 0 : now_do + 1;
+          if (++now_i == n) {
+            now_i = 0;
+            ++now_g;
+            if (BENT && p.slopes && now_g < per) slope2 = p.slopes[hk * per + now_g] * WA_LOG2E;
           }
         }
-      }
-      // dV^T[d, key] += dO^T P (S-wave), dK^T[d, key] += Q^T dS (dP-wave): A by transpose reads, B from registers
-      const bf16_t* bt = swave ? dc : qc;
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // phase `total`
+      } else {
+        f32x16 dp[2];
+        auto product = [&](int t) {   // dP[q, key] = dO V^T
+          const uint32_t dc = rd.address(s_do + now_do * TILE);
+          Operands a;
+          RowsProduct<D>::first(rd, dc, a);
+          RowsProduct<D>::run(rd, dc, kvf, dp, a);
+          now_do = now_do == 2 ? 0 : now_do + 1;
+        };
+        auto gradient = [&](int t) {   // dK^T[d, key] += Q^T dS
+          const uint32_t qc = rd.address(s_q + (t & 3) * TILE);
+          const float* st_dl = s_stats + (t & 3) * STATS + 64;
+          const float* st_on = st_dl + 64;
+          bf16x8 ab[4];
+          Operands a;
+          ColsProduct<D>::first(rd, qc, a);
+          in_order();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+          for (int x = 0; x < 2; ++x) {
 #pragma unroll
-        for (int tt = 0; tt < DT; ++tt) acc[tt] = wa_mfma32(tile_tr8<D>(bt, c, 32 * tt, lane), ab[c], acc[tt]);
+            for (int rq = 0; rq < 4; ++rq) {
+              const int r0 = 32 * x + 8 * rq + 4 * g;
+              const f32x4 d4 = *(const f32x4*)(st_dl + r0), o4 = *(const f32x4*)(st_on + r0);
+              const f16x4 p4 = s_p[t & 1][kg][x][rq][lane];
+              float ds[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = rq * 4 + i;
+                // a product that is 0 where the weight is: what a masked key holds, NaN too, reaches nothing
+                ds[i] = zero_mul((float)p4[i], fmaf(dp[x][r], o4[i], -d4[i]));
+              }
+              put4(ab[x * 2 + (rq >> 1)], rq & 1, ds);
+              if (rq % 2) in_order();
+            }
+          }
+          ColsProduct<D>::run(rd, qc, ab, acc, a);
+        };
+        top(0);
+        issue(2);
+        product(0);
+        for (int t = 1; t < total; ++t) {
+          top(t);
+          gradient(t - 1);
+          issue(t + 2);
+          product(t);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        gradient(total - 1);
       }
-      if (++now_i == n) {
-        now_i = 0;
-        ++now_g;
-        if (BENT && p.slopes && now_g < per) slope2 = p.slopes[hk * per + now_g] * WA_LOG2E;
-      }
-    };
-    if (total > 0) issue(qd0);
-    for (int t = 0; t < total; t += 2) {
-      step(IC<0>{}, t);
-      if (t + 1 < total) step(IC<1>{}, t + 1);
     }
     __syncthreads();   // the list and the stages are free
   }
-  // each lane holds its key's row: channels 32 tt + 8 rq + 4 g .. + 3 of tile tt. Rows are staged in LDS, row r's 16-byte chunk c at chunk
-  // c ^ swz(r), and written whole.
+  // each lane holds its key's row: channels 32 tt + 8 rq + 4 g .. + 3 of tile tt
   const float osc = swave ? 1.f : p.scale / kLift;
+  const int rows = key_end - key0;
+  const int64_t at0 = (((int64_t)b * p.ranges.Lk + key0) * p.Hk + hk) * D, st = (int64_t)p.Hk * D;
+  if (p.parts > 1) {
+    if (!k_ok) return;
+    const int64_t size = (int64_t)p.B * p.ranges.Lk * st;
+    float* dst = p.part_kv + ((int64_t)part * 2 + (swave ? 1 : 0)) * size + at0 + kl * st + 4 * g;
+#pragma unroll
+    for (int tt = 0; tt < DT; ++tt) {
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        f32x4 v4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v4[i] = acc[tt][rq * 4 + i] * osc;
+        *(f32x4*)(dst + 32 * tt + 8 * rq) = v4;
+      }
+    }
+    return;
+  }
+  // Rows are staged in LDS, row r's 16-byte chunk c at chunk c ^ swz(r), and written whole.
   auto swz = [](int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); };
-  bf16_t* stg = swave ? qd1 : qd0;   // dV, dK
+  bf16_t* stg = s_q + (swave ? 2 * TILE : 0);   // dK, dV
 #pragma unroll
   for (int tt = 0; tt < DT; ++tt) {
 #pragma unroll
@@ -487,20 +673,47 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   }
   __syncthreads();
   constexpr int CPR = D / 8;
-  const int rows = key_end - key0;
-  const int64_t first = (((int64_t)b * p.ranges.Lk + key0) * p.Hk + hk) * D, st = (int64_t)p.Hk * D;
-  for (int x = tid; x < rows * CPR; x += 256) {
+  for (int x = tid; x < rows * CPR; x += 64 * NW) {
     const int r = x / CPR, c = x % CPR;
-    *(bf16x8*)(p.dk + first + r * st + c * 8) = *(const bf16x8*)(qd0 + r * D + ((c ^ swz(r)) << 3));
-    *(bf16x8*)(p.dv + first + r * st + c * 8) = *(const bf16x8*)(qd1 + r * D + ((c ^ swz(r)) << 3));
+    *(bf16x8*)(p.dk + at0 + r * st + c * 8) = *(const bf16x8*)(s_q + r * D + ((c ^ swz(r)) << 3));
+    *(bf16x8*)(p.dv + at0 + r * st + c * 8) = *(const bf16x8*)(s_q + 2 * TILE + r * D + ((c ^ swz(r)) << 3));
   }
+}
+
+// dK and dV of a launch in parts: the parts' sums in their order, eight channels a thread.
+__global__ void __launch_bounds__(256) parts_kernel(BwdParams p, int64_t size) {
+  const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (x >= 2 * size) return;
+  const float* src = p.part_kv + x;
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = 0.f;
+  for (int i = 0; i < p.parts; ++i) {
+    const f32x4 a = *(const f32x4*)(src + 2 * size * i), c = *(const f32x4*)(src + 2 * size * i + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[e] += a[e];
+      s[4 + e] += c[e];
+    }
+  }
+  bf16x8 o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = (bf16_t)s[e];
+  *(bf16x8*)(x < size ? p.dk + x : p.dv + (x - size)) = o;
+}
+
+// Runs that the steps of 128 keys are cut into: about two workgroups a CU, but none without a query head of its own (the runs' fp32 sums are
+// written and read once more).
+int kv_parts(int64_t B, int64_t H, int64_t Hk, int64_t Lk) {
+  const int64_t groups = B * Hk * ((Lk + kKeys - 1) / kKeys);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(H / Hk, 512 / groups));
 }
 
 template <int D, bool BENT>
 void launch_bwd(const BwdParams& p, hipStream_t s) {
   const int64_t n_rows = (int64_t)p.B * p.H * p.ranges.Lq, nq = (p.ranges.Lq + 127) / 128;
   hipLaunchKernelGGL((rows_kernel<D>), dim3((unsigned)((n_rows + 2048 / D - 1) / (2048 / D))), dim3(256), 0, s, p, n_rows);
-  const dim3 gq((unsigned)(p.B * p.H * nq)), gk((unsigned)((int64_t)p.B * p.Hk * ((p.ranges.Lk + 63) / 64)));
+  const dim3 gq((unsigned)(p.B * p.H * nq)), gk((unsigned)((int64_t)p.B * p.Hk * ((p.ranges.Lk + kKeys - 1) / kKeys) * p.parts));
   if constexpr (BENT) {
     if (p.dslopes) {
       hipLaunchKernelGGL((ranged_dq_kernel<D, true, true>), gq, dim3(256), 0, s, p);
@@ -511,13 +724,20 @@ void launch_bwd(const BwdParams& p, hipStream_t s) {
   } else {
     hipLaunchKernelGGL((ranged_dq_kernel<D, false, false>), gq, dim3(256), 0, s, p);
   }
-  hipLaunchKernelGGL((ranged_dkv_kernel<D, BENT>), gk, dim3(256), 0, s, p);
+  hipLaunchKernelGGL((ranged_dkv_kernel<D, BENT>), gk, dim3(512), 0, s, p);
+  if (p.parts > 1) {
+    const int64_t size = (int64_t)p.B * p.ranges.Lk * p.Hk * D;
+    hipLaunchKernelGGL(parts_kernel, dim3((unsigned)((size / 4 + 255) / 256)), dim3(256), 0, s, p, size);
+  }
 }
 
 }  // namespace
 
-extern "C" int64_t wa_ranged_bwd_workspace_bytes(int64_t B, int64_t H, int64_t, int64_t Lq, int64_t, int64_t) {
-  return B * H * Lq * 12 + B * H * ((Lq + 127) / 128) * 4;
+extern "C" int64_t wa_ranged_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk, int64_t D) {
+  if (B < 1 || Hk < 1 || H < Hk || Lk < 1) return 0;
+  const int parts = kv_parts(B, H, Hk, Lk);
+  const int64_t rows = (B * H * Lq * 12 + B * H * ((Lq + 127) / 128) * 4 + 15) / 16 * 16;
+  return rows + (parts > 1 ? parts * 2 * B * Lk * Hk * D * 4 : 0);
 }
 
 extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
@@ -535,10 +755,10 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   auto near = [](int64_t st) { return st >= 0 && st <= (int64_t)1 << 23; };
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->k, a->k_sb, a->k_st, a->k_sh) && rows16(a->v, a->v_sb, a->v_st, a->v_sh) &&
                rows16(a->o, a->o_sb, a->o_st, a->o_sh) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh) && wa_aligned16(a->dq) && wa_aligned16(a->dk) &&
-               wa_aligned16(a->dv) && near(a->q_st) && near(a->k_st) && near(a->v_st) && near(a->d_st),
+               wa_aligned16(a->dv) && wa_aligned16(a->workspace) && near(a->q_st) && near(a->k_st) && near(a->v_st) && near(a->d_st),
                "ranged_bwd: rows must be 16-byte aligned, at most 2^23 elements apart");
   WA_CHECK_ARG(a->scale >= 0.f && a->cap >= 0.f && a->scale < INFINITY && a->cap < INFINITY, "ranged_bwd: scale and cap must be finite and not below 0");
-  WA_CHECK_ARG(a->B * a->H * ((a->Lq + 127) / 128) <= INT32_MAX && a->B * a->Hk * ((a->Lk + 63) / 64) <= INT32_MAX && a->B * a->H * a->Lq / 16 <= INT32_MAX,
+  WA_CHECK_ARG(a->B * a->H * ((a->Lq + 127) / 128) <= INT32_MAX && a->B * a->H * ((a->Lk + 63) / 64) <= INT32_MAX && a->B * a->Lk * a->Hk * a->D / 1024 <= INT32_MAX && a->B * a->H * a->Lq / 16 <= INT32_MAX,
                "ranged_bwd: too many rows");
   BwdParams p{};
   p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
@@ -560,6 +780,8 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   p.on = p.lse2 + n;
   p.delta = p.on + n;
   p.slope_part = p.delta + n;
+  p.parts = kv_parts(a->B, a->H, a->Hk, a->Lk);
+  p.part_kv = (float*)((char*)a->workspace + (n * 12 + a->B * a->H * ((a->Lq + 127) / 128) * 4 + 15) / 16 * 16);
   hipStream_t s = (hipStream_t)stream;
   const bool bent = a->cap > 0.f || a->slopes;
   if (a->D == 128) {
