@@ -28,7 +28,7 @@ struct AttendParams {
   const float* slopes;
   int n, H, Hk, nb, shift;        // shift: log2 of a block's tokens
   int units, parts, per;          // row units of (sequence, key head, with lists: query); parts of a unit, tiles of a part
-  float scale2, bend_in, cap2;
+  Bend bend;
   float* part;                    // [unit][part][16 RT][D + 2]: maximum, sum, outputs
 };
 
@@ -105,7 +105,7 @@ __device__ __forceinline__ void write_row(const AttendParams& p, int b, int i, i
 }
 
 template <typename Code, int D, int RT>
-__global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
+__global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) attend_kernel(AttendParams p) {
   constexpr int NW = 4, KC = D / 32, VC = D / 16, KL = D / 64;   // key products of a tile half; channels of a value row a lane holds; loads of a key row
   typedef typename ValueRow<D>::type VRow;
   __shared__ float so[NW][16][D + 4];
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
       if (ok) q[x][c] = *(const bf16x8*)(p.q + (int64_t)b * p.q_sb + (int64_t)i * p.q_st + (int64_t)h * p.q_sh + 64 * (c >> 1) + 16 * kg + 8 * (c & 1));
     }
   }
-  const int64_t st = (int64_t)p.Hk * D;
+  const int st = p.Hk * D;   // at most 2^23
   const uint8_t* kb = p.k + ((int64_t)b * p.cap * p.Hk + hk) * D;
   const uint8_t* vb = p.v + ((int64_t)b * p.cap * p.Hk + hk) * D;
   const float* ksc = p.k_scale + ((int64_t)b * p.Hk + hk) * p.nb;
@@ -169,6 +169,12 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
     const int64_t key = ((int64_t)id << p.shift) + (t & ((1 << (p.shift - 5)) - 1)) * 32;
     return id < 0 || key > last ? -1 : (int)key;
   };
+  // The lane's places in a tile: key rows 16 h + l16, value rows 16 (e / 4) + 4 kg + e % 4.
+  int k_off[2], v_off[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) k_off[h] = (16 * h + l16) * st + 16 * kg;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v_off[e] = (16 * (e >> 2) + 4 * kg + (e & 3)) * st + VC * l16;
   struct Tile {
     u32x4 k[2][KL];
     VRow v[8];
@@ -179,15 +185,19 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
     x.key = -1;
     while (t < t1 && (x.key = key_of(t)) < 0) t += NW;
     if (x.key < 0) return t1;
-    const int live = min(32, last + 1 - x.key);   // behind the last token that any row sees its codes again
-    const uint8_t* kr = kb + x.key * st;
-    const uint8_t* vr = vb + x.key * st;
+    // from the last token that any row sees on the codes read as zeros
+    const int bytes = (min(32, last + 1 - x.key) - 1) * st + D;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + (int64_t)x.key * st), (short)0, bytes, WA_BUF_DWORD3);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + (int64_t)x.key * st), (short)0, bytes, WA_BUF_DWORD3);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int c = 0; c < KL; ++c) x.k[h][c] = *(const u32x4*)(kr + min(16 * h + l16, live - 1) * st + 64 * c + 16 * kg);
+      for (int c = 0; c < KL; ++c) x.k[h][c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[h] + 64 * c, 0, 0));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x.v[e] = *(const VRow*)(vr + min(16 * (e >> 2) + 4 * kg + (e & 3), live - 1) * st + VC * l16);
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (D == 128) x.v[e] = __builtin_bit_cast(VRow, __builtin_amdgcn_raw_buffer_load_b64(vr, v_off[e], 0, 0));
+      else x.v[e] = __builtin_amdgcn_raw_buffer_load_b32(vr, v_off[e], 0, 0);
+    }
     x.ks = ksc[x.key >> p.shift];
     x.vs = vsc[x.key >> p.shift];
     return t;
@@ -208,11 +218,6 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
         }
         ka[h][c] = __builtin_bit_cast(bf16x8, y);
       }
-    uint32_t vp[8][VC / 2];   // value rows as bf16 pairs of channels
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-      for (int j = 0; j < VC / 4; ++j) Code::pairs(word(x.v[e], j), vp[e][2 * j], vp[e][2 * j + 1]);
     const bool whole = x.key + 31 <= lowest && ((window == 0) | (x.key > last - window) | (x.key + 31 < sink));
     bf16x8 pr[RT];
 #pragma unroll
@@ -224,16 +229,25 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
         for (int h = 0; h < 2; ++h) acc[h] = mma16(ka[h][c], q[y][c], acc[h]);
       float s[8];
       const int key0 = x.key + 4 * kg;
-      if (p.cap2 > 0.f || p.slopes) {
-        const Bend bend{p.bend_in * x.ks, p.cap2, slope2[y]};
+      if (p.bend.cap2 > 0.f || p.slopes) {
+        Bend bend = p.bend;       // of scores of the codes: the keys' scale (a power of two) goes with the scores' own
+        bend.scale2 *= x.ks;
+        bend.in *= x.ks;
+        bend.in2 *= x.ks;
+        bend.slope2 = slope2[y];
         const float far = (float)(pos[y] - key0);
+        float most = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float unused;
-          s[e] = bend(acc[e >> 2][e & 3], far - (float)(16 * (e >> 2) + (e & 3)), unused);
-        }
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(acc[e >> 2][e & 3]));
+        by_form(bend.form(most), [&](auto form) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float unused;
+            s[e] = bend.bent<decltype(form)::value>(acc[e >> 2][e & 3], far - (float)(16 * (e >> 2) + (e & 3)), unused);
+          }
+        });
       } else {
-        const float by = p.scale2 * x.ks;
+        const float by = p.bend.scale2 * x.ks;
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] = acc[e >> 2][e & 3] * by;
       }
@@ -268,10 +282,10 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
     }
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
-      u32x4 vt;     // channel j of the eight rows
+      uint32_t rows[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        vt[e] = __builtin_amdgcn_perm(vp[2 * e + 1][j / 2], vp[2 * e][j / 2], j % 2 ? 0x07060302 : 0x05040100);
+      for (int e = 0; e < 8; ++e) rows[e] = word(x.v[e], j / 4);
+      const u32x4 vt = Code::column(rows, j % 4);   // channel j of the eight rows
 #pragma unroll
       for (int y = 0; y < RT; ++y) o[y][j] = mma16(__builtin_bit_cast(bf16x8, vt), pr[y], o[y][j]);
     }
@@ -384,8 +398,8 @@ Cut cut(const wa_kv8_attend_args& a) {
   // at most: the sinks', and from the first row's window to the last row, each run with a partial tile at either end
   const int64_t seen = a.window > 0 ? std::min(tokens, std::min(a.sink, tokens) + std::min(a.window, tokens) + a.n + 128) : tokens;
   const int64_t tiles = a.index ? a.topk * (a.cache.block_size / 32) : (seen + 31) / 32;
-  // parts of at least 8 tiles (two a wave), about 2,048 workgroups where there is work for them: ragged sequences even out
-  const int64_t want = std::max<int64_t>(1, 2048 / c.units);
+  // parts of at least 8 tiles (two a wave), about 4,096 workgroups where there is work for them: ragged sequences even out
+  const int64_t want = std::max<int64_t>(1, 4096 / c.units);
   c.per = (int)std::max<int64_t>(8, (tiles + want - 1) / want);
   c.parts = (int)std::max<int64_t>(1, (tiles + c.per - 1) / c.per);
   return c;
@@ -426,7 +440,8 @@ extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
     return wa_aligned16(x) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0;
   };
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->o, a->o_sb, a->o_st, a->o_sh), "kv8_attend: rows must be 16-byte aligned");
-  WA_CHECK_ARG(a->scale >= 0.f && a->cap >= 0.f && a->scale < INFINITY && a->cap < INFINITY, "kv8_attend: scale and cap must be finite and not below 0");
+  WA_CHECK_ARG(a->scale >= 0.f && a->scale < INFINITY && (a->cap == 0.f || (a->cap >= 1e-6f && a->cap <= 1e6f && a->scale <= 1e30f)),
+               "kv8_attend: scale must be finite and not below 0, cap 0 or 1e-6 .. 1e6 (with a scale of at most 1e30)");
   const Cut k = cut(*a);
   WA_CHECK_ARG(k.units * k.parts <= INT32_MAX && k.units * 16 * k.rt / 4 <= INT32_MAX, "kv8_attend: too many rows");
   WA_CHECK_ARG(k.parts == 1 || a->workspace, "kv8_attend: a launch of %d parts needs a workspace", k.parts);
@@ -443,9 +458,7 @@ extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
   p.nb = (int)((c.cap + c.block_size - 1) / c.block_size); p.shift = c.block_size == 64 ? 6 : 7;
   p.units = k.units_of; p.parts = k.parts; p.per = k.per;
   const float scale = a->scale == 0.f ? 1.f / sqrtf((float)c.D) : a->scale;
-  p.scale2 = scale * WA_LOG2E;
-  p.bend_in = a->cap > 0.f ? 2.f * scale / a->cap * WA_LOG2E : p.scale2;
-  p.cap2 = a->cap * WA_LOG2E;
+  p.bend = bend_of(scale, a->cap);
   p.part = (float*)a->workspace;
   hipStream_t s = (hipStream_t)stream;
   if (c.code == WA_CODE_INT8) {

@@ -30,6 +30,14 @@ struct Int8 {
     lo = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
     hi = __builtin_amdgcn_perm(__float_as_uint(e), __float_as_uint(d), 0x07060302);
   }
+  // The operand that holds a column of eight rows: column j of the four that each row's word has.
+  __device__ __forceinline__ static u32x4 column(const uint32_t (&rows)[8], int j) {
+    u32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      x[e] = __builtin_amdgcn_perm(__float_as_uint((float)(int8_t)(rows[2 * e + 1] >> (8 * j))), __float_as_uint((float)(int8_t)(rows[2 * e] >> (8 * j))), 0x07060302);
+    return x;
+  }
 };
 
 struct E4m3 {
@@ -58,6 +66,22 @@ struct E4m3 {
   __device__ __forceinline__ static void pairs(uint32_t c, uint32_t& lo, uint32_t& hi) {
     lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false));
     hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true));
+  }
+  __device__ __forceinline__ static u32x4 column(const uint32_t (&rows)[8], int j) {
+    u32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t a, b;
+      if (j < 2) {
+        a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rows[2 * e], 1.f, false));
+        b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rows[2 * e + 1], 1.f, false));
+      } else {
+        a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rows[2 * e], 1.f, true));
+        b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rows[2 * e + 1], 1.f, true));
+      }
+      x[e] = __builtin_amdgcn_perm(b, a, j % 2 ? 0x07060302 : 0x05040100);
+    }
+    return x;
   }
 };
 

@@ -119,7 +119,7 @@ struct FwdParams {
   const int32_t* kv_len; int64_t kv_len_all;
   const float* slopes;
   int B, H, Hk;
-  float scale2, bend_in, cap2;
+  Bend bend;
 };
 
 // Running maximum before the first key: below every score, and finite, so that no difference of it is NaN where a row sees nothing yet.
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
       qf[qt][c] = q_ok[qt] ? t : bf16x8{};
     }
   }
-  Bend bend{p.bend_in, p.cap2, 0.f};
+  Bend bend = p.bend;
   int pos0 = 0;
   if (BENT && p.slopes) {
     bend.slope2 = p.slopes[h] * WA_LOG2E;
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
 #pragma unroll
     for (int c = 0; c < 4; ++c) P[c][qt] = bf16x8{};
   }
-  const float sl2 = BENT ? 1.f : p.scale2;
+  const float sl2 = BENT ? 1.f : p.bend.scale2;
   // Before a half's exponentials: its scores bent, and those of keys that the row does not see at -inf (lane (l32, g) holds keys
   // 32 KH + 8 (r / 4) + 4 g + r % 4 of step s).
   auto ready = [&](auto half, int s) {
@@ -231,11 +231,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         const float far = (float)(key0 - pos0 - qi[qt]);
+        f32x16 x = S[KH][qt];   // a copy: an array that the forms' branches reach into goes to memory
+        auto bend_all = [&](auto form) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float unused;
-          S[KH][qt][r] = bend(S[KH][qt][r], far + (float)(8 * (r >> 2) + (r & 3)), unused);
-        }
+          for (int r = 0; r < 16; ++r) {
+            float unused;
+            x[r] = bend.bent<decltype(form)::value>(x[r], far + (float)(8 * (r >> 2) + (r & 3)), unused);
+          }
+        };
+        float most = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(x[r]));
+        by_form(bend.form(most), bend_all);
+        S[KH][qt] = x;
       }
     }
     if (!st.whole(key, end)) {
@@ -379,7 +387,8 @@ extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   WA_CHECK_ARG(rows16(a->q, a->q_sb, a->q_st, a->q_sh) && rows16(a->k, a->k_sb, a->k_st, a->k_sh) && rows16(a->v, a->v_sb, a->v_st, a->v_sh) &&
                rows16(a->o, a->o_sb, a->o_st, a->o_sh) && near(a->k_st) && near(a->v_st),
                "ranged_fwd: rows must be 16-byte aligned, keys and values at most 2^23 elements apart");
-  WA_CHECK_ARG(a->scale >= 0.f && a->cap >= 0.f && a->scale < INFINITY && a->cap < INFINITY, "ranged_fwd: scale and cap must be finite and not below 0");
+  WA_CHECK_ARG(a->scale >= 0.f && a->scale < INFINITY && (a->cap == 0.f || (a->cap >= 1e-6f && a->cap <= 1e6f && a->scale <= 1e30f)),
+               "ranged_fwd: scale must be finite and not below 0, cap 0 or 1e-6 .. 1e6 (with a scale of at most 1e30)");
   FwdParams p{};
   p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.k = (const bf16_t*)a->k; p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
@@ -390,9 +399,7 @@ extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.slopes = a->slopes;
   p.B = (int)a->B; p.H = (int)a->H; p.Hk = (int)a->Hk;
   const float scale = a->scale == 0.f ? 1.f / sqrtf((float)a->D) : a->scale;
-  p.scale2 = scale * WA_LOG2E;
-  p.bend_in = a->cap > 0.f ? 2.f * scale / a->cap * WA_LOG2E : p.scale2;
-  p.cap2 = a->cap * WA_LOG2E;
+  p.bend = bend_of(scale, a->cap);
   WA_CHECK_ARG(a->B * a->H * ((a->Lq + 127) / 128) <= INT32_MAX, "ranged_fwd: too many rows");
   const bool bent = a->cap > 0.f || a->slopes;
   if (a->D == 128) launch_fwd<128, 1>(p, bent, (hipStream_t)stream);

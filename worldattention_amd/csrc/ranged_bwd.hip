@@ -28,7 +28,8 @@ struct BwdParams {
   const int32_t* kv_len; int64_t kv_len_all;
   const float* slopes;
   int B, H, Hk;
-  float scale, scale2, bend_in, cap2;
+  float scale;
+  Bend bend;
   bf16_t* dq; bf16_t* dk; bf16_t* dv; float* dslopes;
   // workspace
   float* lse2;    // [B, H, Lq] log-sum-exp in units of log2; +inf where a row sees nothing: its weights come out 0
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   const int64_t srow = ((int64_t)b * p.H + h) * p.ranges.Lq;
   float lse2 = q_ok ? p.lse2[srow + row] : INFINITY;
   float dl = q_ok ? p.delta[srow + row] : 0.f, on = q_ok ? p.on[srow + row] : 0.f;
-  Bend bend{p.bend_in, p.cap2, 0.f};
+  Bend bend = p.bend;
   int pos = 0;   // the row's position
   if (BENT && p.slopes) {
     bend.slope2 = p.slopes[h] * WA_LOG2E;
@@ -293,37 +294,47 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
       dp = wa_mfma32(a[c % (kAhead + 1)][1], dof[c], c == 0 ? f32x16{} : dp);
       in_order();
     }
-    auto weights = [&](auto masked) {
+    auto weights = [&](auto form) {
       const RowRuns mine(runs, end);
       const float far = (float)(key0 - pos);
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        float out[4];
+        float out[4], pr[4], d[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = 4 * r4 + i, at = 8 * r4 + i;
-          float turn = 1.f, pr;
-          if constexpr (BENT) pr = __builtin_amdgcn_exp2f(bend(s[r], far + (float)at, turn) - lse2);
-          else pr = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lse2));
-          float d = dp[r], ds = pr * fmaf(d, on, -dl);
-          if constexpr (BENT) ds *= turn;
-          if constexpr (decltype(masked)::value) {
-            const bool seen = mine.sees(key0 + at);
-            ds = seen ? ds : 0.f;
-            if constexpr (SLOPES) {
-              pr = seen ? pr : 0.f;
-              d = seen ? d : 0.f;
-            }
+          const int r = 4 * r4 + i;
+          float turn = 1.f;
+          d[i] = dp[r];
+          if constexpr (BENT) pr[i] = __builtin_amdgcn_exp2f(bend.bent<decltype(form)::value>(s[r], far + (float)(8 * r4 + i), turn) - lse2);
+          else pr[i] = __builtin_amdgcn_exp2f(fmaf(s[r], bend.scale2, -lse2));
+          out[i] = pr[i] * fmaf(d[i], on, -dl);
+          if constexpr (BENT) out[i] *= turn;
+        }
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool seen = mine.sees(key0 + 8 * r4 + i);
+            out[i] = seen ? out[i] : 0.f;
+            pr[i] = seen ? pr[i] : 0.f;
+            d[i] = seen ? d[i] : 0.f;
           }
-          if constexpr (SLOPES) slopes_of(pr, d, far + (float)at);
-          out[i] = ds;
+        }
+        if constexpr (SLOPES) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) slopes_of(pr[i], d[i], far + (float)(8 * r4 + i));
         }
         put4(dsb[r4 >> 1], r4 & 1, out);
         if constexpr (BENT) in_order();
       }
     };
-    if (whole) weights(std::false_type{});
-    else weights(std::true_type{});
+    if constexpr (BENT) {
+      float most = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[r]));
+      by_form(bend.form(most), weights);
+    } else {
+      weights(FormTag<kBias>{});
+    }
   };
   if (st.total > 0) issue(kv0, 0);
   for (int t = 0; t < st.total; ++t) {
@@ -526,7 +537,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
       issue(0);
       issue(1);
       if (swave) {
-        float slope2 = BENT && p.slopes ? p.slopes[hk * per + now_g] * WA_LOG2E : 0.f;
+        Bend bend = p.bend;
+        if (BENT && p.slopes) bend.slope2 = p.slopes[hk * per + now_g] * WA_LOG2E;
         for (int t = 0; t < total; ++t) {
           top(t);
           const uint32_t qc = rd.address(s_q + (t & 3) * TILE);
@@ -544,8 +556,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
           ColsProduct<D>::first(rd, dc, a);   // under the exponentials
           in_order();
           bf16x8 ab[4];
-          auto weights = [&](auto masked) {
-            const Bend bend{p.bend_in, p.cap2, slope2};
+          const bool whole = entry >> 20;
+          auto weights = [&](auto form) {
             const float far = (float)(key - pos0 - row0 - 4 * g);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
@@ -553,36 +565,36 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
               for (int rq = 0; rq < 4; ++rq) {
                 const int r0 = 32 * x + 8 * rq;
                 const f32x4 l4 = *(const f32x4*)(st_lse2 + r0 + 4 * g);
-                f16x4 p4;
-                float pw[4];
+                float pr[4], turn[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  const int r = rq * 4 + i;
-                  float turn = 1.f, pr;
-                  if constexpr (BENT) pr = __builtin_amdgcn_exp2f(bend(sacc[x][r], far - (float)(r0 + i), turn) - l4[i]);
-                  else pr = __builtin_amdgcn_exp2f(fmaf(sacc[x][r], p.scale2, -l4[i]));
-                  if constexpr (decltype(masked)::value) {
-                    const RowRuns row(st_runs[r0 + 4 * g + i], INT32_MAX);
-                    pr = row.sees(key) ? pr : 0.f;
-                  }
-                  pw[i] = pr;
-                  p4[i] = (_Float16)(pr * (BENT ? kLift * turn : kLift));
+                  const float s = sacc[x][rq * 4 + i];
+                  turn[i] = 1.f;
+                  if constexpr (BENT) pr[i] = __builtin_amdgcn_exp2f(bend.bent<decltype(form)::value>(s, far - (float)(r0 + i), turn[i]) - l4[i]);
+                  else pr[i] = __builtin_amdgcn_exp2f(fmaf(s, bend.scale2, -l4[i]));
                 }
-                put4(ab[x * 2 + (rq >> 1)], rq & 1, pw);
+                if (!whole) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) pr[i] = RowRuns(st_runs[r0 + 4 * g + i], INT32_MAX).sees(key) ? pr[i] : 0.f;
+                }
+                f16x4 p4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p4[i] = (_Float16)(pr[i] * (BENT ? kLift * turn[i] : kLift));
+                put4(ab[x * 2 + (rq >> 1)], rq & 1, pr);
                 s_p[t & 1][kg][x][rq][lane] = p4;
-                if (decltype(masked)::value || rq % 2) in_order();   // few rows' statistics in registers at a time
+                if (BENT || rq % 2) in_order();   // few rows' statistics in registers at a time
               }
             }
           };
-          if (entry >> 20) weights(std::false_type{});
-          else weights(std::true_type{});
+          if constexpr (BENT) by_form(bend.form(largest<2>(sacc)), weights);
+          else weights(FormTag<kBias>{});
           // dV^T[d, key] += dO^T P: A by transpose reads, B from registers
           ColsProduct<D>::run(rd, dc, ab, acc, a);
           now_do = now_do == 2 ? 0 : now_do + 1;
           if (++now_i == n) {
             now_i = 0;
             ++now_g;
-            if (BENT && p.slopes && now_g < per) slope2 = p.slopes[hk * per + now_g] * WA_LOG2E;
+            if (BENT && p.slopes && now_g < per) bend.slope2 = p.slopes[hk * per + now_g] * WA_LOG2E;
           }
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // phase `total`
@@ -757,7 +769,8 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
                rows16(a->o, a->o_sb, a->o_st, a->o_sh) && rows16(a->dout, a->d_sb, a->d_st, a->d_sh) && wa_aligned16(a->dq) && wa_aligned16(a->dk) &&
                wa_aligned16(a->dv) && wa_aligned16(a->workspace) && near(a->q_st) && near(a->k_st) && near(a->v_st) && near(a->d_st),
                "ranged_bwd: rows must be 16-byte aligned, at most 2^23 elements apart");
-  WA_CHECK_ARG(a->scale >= 0.f && a->cap >= 0.f && a->scale < INFINITY && a->cap < INFINITY, "ranged_bwd: scale and cap must be finite and not below 0");
+  WA_CHECK_ARG(a->scale >= 0.f && a->scale < INFINITY && (a->cap == 0.f || (a->cap >= 1e-6f && a->cap <= 1e6f && a->scale <= 1e30f)),
+               "ranged_bwd: scale must be finite and not below 0, cap 0 or 1e-6 .. 1e6 (with a scale of at most 1e30)");
   WA_CHECK_ARG(a->B * a->H * ((a->Lq + 127) / 128) <= INT32_MAX && a->B * a->H * ((a->Lk + 63) / 64) <= INT32_MAX && a->B * a->Lk * a->Hk * a->D / 1024 <= INT32_MAX && a->B * a->H * a->Lq / 16 <= INT32_MAX,
                "ranged_bwd: too many rows");
   BwdParams p{};
@@ -771,9 +784,7 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.slopes = a->slopes;
   p.B = (int)a->B; p.H = (int)a->H; p.Hk = (int)a->Hk;
   p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->D) : a->scale;
-  p.scale2 = p.scale * WA_LOG2E;
-  p.bend_in = a->cap > 0.f ? 2.f * p.scale / a->cap * WA_LOG2E : p.scale2;
-  p.cap2 = a->cap * WA_LOG2E;
+  p.bend = bend_of(p.scale, a->cap);
   p.dq = (bf16_t*)a->dq; p.dk = (bf16_t*)a->dk; p.dv = (bf16_t*)a->dv; p.dslopes = a->dslopes;
   const int64_t n = a->B * a->H * a->Lq;
   p.lse2 = (float*)a->workspace;

@@ -84,21 +84,61 @@ struct RowRuns {
   __device__ __forceinline__ bool sees(int key) const { return ((unsigned)(key - up) < (unsigned)up_n) | ((unsigned)(key - low) < (unsigned)low_n); }
 };
 
-// Scores beyond the plain product, in units of log2: y = cap tanh(x / cap) with, e = exp(2 x / cap) and r = 1 / (e + 1),
-//   tanh = 1 - 2 r   and its derivative   1 - tanh^2 = 4 e r r,
-// the first off by a few 2^-24 of the cap wherever x is (e = inf gives r = 0), the second by a few 2^-24 of itself; then the distance's bias.
+// Scores beyond the plain product, in units of log2: cap tanh(x / cap), x = scale s, less the distance's bias. Which form of the tanh is right for all of
+// a wave's scores is asked once for a tile:
+//   kBias   no cap;
+//   kNear   |x| <= cap / 2: tanh(z) = z P(z^2), P of degree 4 fitted to 1.5e-8 of the value (a weighted least-squares fit of tanh(z) / z on
+//           [0, 1/4] with the leading 1 kept). More exact than the other, and less work: eight plain instructions for two transcendental ones and four
+//           (a training step of 8,190 packed tokens, 16 heads, cap 30: see ranged.hip);
+//   kFar    e = exp(2 z), r = 1 / (e + 1): tanh = 1 - 2 r, off by a few 2^-24 of the cap wherever z is (e = inf gives r = 0); its derivative
+//           4 e r r, off by a few 2^-24 of itself.
+enum BendForm { kBias, kNear, kFar };
 struct Bend {
-  float in, cap2, slope2;   // 2 scale / cap log2(e) with a cap, else scale log2(e); cap log2(e) or 0; slope log2(e)
-  __device__ __forceinline__ float operator()(float s, float dist, float& turn) const {
-    float y = s * in;
+  float scale2, in, in2, cap2, slope2;   // scale log2(e); scale / cap; 2 scale / cap log2(e); cap log2(e) or 0; slope log2(e)
+  // The form for scores of at most `most`, the same in all of the wave's lanes.
+  __device__ __forceinline__ BendForm form(float most) const {
+    if (!(cap2 > 0.f)) return kBias;
+    return __any(most * in > 0.5f) ? kFar : kNear;
+  }
+  template <BendForm FORM>
+  __device__ __forceinline__ float bent(float s, float dist, float& turn) const {
+    float y;
     turn = 1.f;
-    if (cap2 > 0.f) {       // uniform over the launch
-      const float e = __builtin_amdgcn_exp2f(y), r = __builtin_amdgcn_rcpf(e + 1.f);
+    if constexpr (FORM == kBias) {
+      y = s * scale2;
+    } else if constexpr (FORM == kNear) {
+      const float z = s * in, u = z * z;
+      const float q = fmaf(u, fmaf(u, fmaf(u, fmaf(u, 0x1.1a7b9cp-6f, -0x1.b28c5ep-5f), 0x1.10e9fcp-3f), -0x1.5554d6p-2f), 1.f);
+      const float t = z * q;
+      y = t * cap2;
+      turn = fmaf(-t, t, 1.f);
+    } else {
+      const float e = __builtin_amdgcn_exp2f(s * in2), r = __builtin_amdgcn_rcpf(e + 1.f);
       y = fmaf(-2.f * cap2, r, cap2);
       turn = fminf(e, 0x1p100f) * 4.f * r * r;
     }
     return fmaf(-slope2, fabsf(dist), y);
   }
 };
+template <int N>
+__device__ __forceinline__ float largest(const f32x16 (&s)[N]) {
+  float x = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x = fmaxf(x, fabsf(s[i][r]));
+  return x;
+}
+template <BendForm F> struct FormTag { static constexpr BendForm value = F; };
+// run(FormTag<form>)
+template <typename Run>
+__device__ __forceinline__ void by_form(BendForm form, const Run& run) {
+  if (form == kBias) run(FormTag<kBias>{});
+  else if (form == kNear) run(FormTag<kNear>{});
+  else run(FormTag<kFar>{});
+}
+static inline Bend bend_of(float scale, float cap) {
+  return {scale * WA_LOG2E, cap > 0.f ? scale / cap : 0.f, cap > 0.f ? 2.f * scale / cap * WA_LOG2E : 0.f, cap * WA_LOG2E, 0.f};
+}
 
 }  // namespace

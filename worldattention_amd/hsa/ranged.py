@@ -203,6 +203,8 @@ def check_scores(d: int, heads: int, scale, cap, slopes) -> tuple[float, float]:
         raise ValueError(f"scale must be above 0 and finite in fp32, got {scale}")
     if not 0.0 <= cap <= 1e6 or (cap > 0.0 and not 1e-6 <= cap):
         raise ValueError(f"cap must be between 1e-6 and 1e6 (None or 0: no cap), got {cap}")
+    if cap > 0.0 and scale > 1e30:
+        raise ValueError(f"scale must be at most 1e30 with a cap, got {scale}")
     if slopes is not None and (tuple(slopes.shape) != (heads,) or slopes.dtype is not torch.float32):
         raise ValueError(f"slopes must be fp32 [{heads}], got {slopes.dtype} {tuple(slopes.shape)}")
     return scale, cap
