@@ -230,21 +230,18 @@ __global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) attend_kernel(AttendPara
       float s[8];
       const int key0 = x.key + 4 * kg;
       if (p.bend.cap2 > 0.f || p.slopes) {
-        Bend bend = p.bend;       // of scores of the codes: the keys' scale (a power of two) goes with the scores' own
-        bend.scale2 *= x.ks;
-        bend.in *= x.ks;
-        bend.in2 *= x.ks;
+        Bend bend = p.bend;
         bend.slope2 = slope2[y];
         const float far = (float)(pos[y] - key0);
-        float most = 0.f;
+        float most = 0.f, unused;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(acc[e >> 2][e & 3]));
+        for (int e = 0; e < 8; ++e) {
+          s[e] = acc[e >> 2][e & 3] * x.ks;
+          most = fmaxf(most, fabsf(s[e]));
+        }
         by_form(bend.form(most), [&](auto form) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float unused;
-            s[e] = bend.bent<decltype(form)::value>(acc[e >> 2][e & 3], far - (float)(16 * (e >> 2) + (e & 3)), unused);
-          }
+          for (int e = 0; e < 8; ++e) s[e] = bend.bent<decltype(form)::value>(s[e], far - (float)(16 * (e >> 2) + (e & 3)), unused);
         });
       } else {
         const float by = p.bend.scale2 * x.ks;

@@ -120,6 +120,9 @@ struct FwdParams {
   const float* slopes;
   int B, H, Hk;
   Bend bend;
+  int splits;       // parts of a workgroup's steps
+  float* part_o;    // [splits][B, H, Lq, D] sums of parts' weighted values
+  float* part_ml;   // [splits][B, H, Lq][2] their maxima and sums
 };
 
 // Running maximum before the first key: below every score, and finite, so that no difference of it is NaN where a row sees nothing yet.
@@ -141,9 +144,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
   int u = (int)blockIdx.x;
   const int bh = u % nbh;
   u /= nbh;
-  const int h = (bh % p.Hk) * per + u % per, b = bh / p.Hk, qt0 = nq - 1 - u / per;
+  const int h = (bh % p.Hk) * per + u % per, b = bh / p.Hk;
+  u /= per;
+  const int split = u % p.splits, qt0 = nq - 1 - u / p.splits;
   Steps st;
   st.init(p.ranges, b, qt0 * (BM / kRangeRows), BM / kRangeRows);
+  st.cut(split, p.splits);
 
   int qi[QT];
   bool q_ok[QT];
@@ -323,6 +329,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
   for (int qt = 0; qt < QT; ++qt) {
     const float l = l_i[qt] + __shfl_xor(l_i[qt], 32, 64);
     if (!q_ok[qt]) continue;
+    const int64_t row = ((int64_t)b * p.H + h) * p.ranges.Lq + qi[qt];
+    if (p.splits > 1) {
+      const int64_t at = split * ((int64_t)p.B * p.H * p.ranges.Lq) + row;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq)
+          *(f32x4*)(p.part_o + at * D + 32 * t + 8 * rq + 4 * g) =
+              f32x4{oacc[qt][t][4 * rq], oacc[qt][t][4 * rq + 1], oacc[qt][t][4 * rq + 2], oacc[qt][t][4 * rq + 3]};
+      }
+      if (g == 0) {
+        p.part_ml[2 * at] = m_i[qt];
+        p.part_ml[2 * at + 1] = l;
+      }
+      continue;
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bf16_t* at = p.o + (int64_t)b * p.o_sb + (int64_t)qi[qt] * p.o_st + (int64_t)h * p.o_sh + 4 * g;
 #pragma unroll
@@ -335,15 +357,58 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
         *(bf16x4*)(at + 32 * t + 8 * rq) = x;
       }
     }
-    if (g == 0) p.lse[((int64_t)b * p.H + h) * p.ranges.Lq + qi[qt]] = l == 0.f ? -INFINITY : (m_i[qt] + log2f(l)) * WA_LN2;
+    if (g == 0) p.lse[row] = l == 0.f ? -INFINITY : (m_i[qt] + log2f(l)) * WA_LN2;
   }
+}
+
+// The parts of a split launch, in their order: D / 8 lanes a row.
+template <int D>
+__global__ void __launch_bounds__(256) join_kernel(FwdParams p, int64_t n_rows) {
+  constexpr int TPR = D / 8;
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int c0 = threadIdx.x % TPR * 8;
+  if (row >= n_rows) return;
+  float top = kNoMax;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[2 * (s * n_rows + row)]);
+  float l = 0.f, o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const int64_t at = s * n_rows + row;
+    const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - top);
+    l += p.part_ml[2 * at + 1] * f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const f32x4 x = *(const f32x4*)(p.part_o + at * D + c0 + 4 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[4 * c + e] += x[e] * f;
+    }
+  }
+  const int i = (int)(row % p.ranges.Lq), h = (int)(row / p.ranges.Lq % p.H), b = (int)(row / p.ranges.Lq / p.H);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  bf16x8 x;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (bf16_t)(o[e] * inv);
+  *(bf16x8*)(p.o + (int64_t)b * p.o_sb + (int64_t)i * p.o_st + (int64_t)h * p.o_sh + c0) = x;
+  if (c0 == 0) p.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * WA_LN2;
+}
+
+// Parts of a workgroup's steps: while the rows alone leave a CU without its two workgroups, but none below 16 steps (a part's sums are written and
+// read once more, and a second launch joins them).
+int fwd_splits(int64_t B, int64_t H, int64_t Lq, int64_t Lk) {
+  const int64_t groups = B * H * ((Lq + 127) / 128);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(512 / groups, (Lk + 63) / 64 / 16));
 }
 
 template <int D, int QT>
 void launch_fwd(const FwdParams& p, bool bent, hipStream_t s) {
-  const int64_t grid = (int64_t)p.B * p.H * ((p.ranges.Lq + 128 * QT - 1) / (128 * QT));
+  const int64_t grid = (int64_t)p.B * p.H * ((p.ranges.Lq + 128 * QT - 1) / (128 * QT)) * p.splits;
   if (bent) hipLaunchKernelGGL((ranged_fwd_kernel<D, QT, true>), dim3((unsigned)grid), dim3(256), 0, s, p);
   else hipLaunchKernelGGL((ranged_fwd_kernel<D, QT, false>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  if (p.splits > 1) {
+    const int64_t n_rows = (int64_t)p.B * p.H * p.ranges.Lq, per = 2048 / D;
+    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)((n_rows + per - 1) / per)), dim3(256), 0, s, p, n_rows);
+  }
 }
 
 }  // namespace
@@ -371,7 +436,11 @@ extern "C" int wa_key_ranges(const wa_key_ranges_args* a, void* stream) {
   return wa_launch_status("key_ranges");
 }
 
-extern "C" int64_t wa_ranged_fwd_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+extern "C" int64_t wa_ranged_fwd_workspace_bytes(int64_t B, int64_t H, int64_t, int64_t Lq, int64_t Lk, int64_t D) {
+  if (B < 1 || H < 1 || Lq < 1 || Lk < 1) return 0;
+  const int splits = fwd_splits(B, H, Lq, Lk);
+  return splits > 1 ? splits * B * H * Lq * (D + 2) * 4 : 0;
+}
 
 extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   WA_CHECK_ARG(a, "ranged_fwd: null args");
@@ -401,6 +470,10 @@ extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   const float scale = a->scale == 0.f ? 1.f / sqrtf((float)a->D) : a->scale;
   p.bend = bend_of(scale, a->cap);
   WA_CHECK_ARG(a->B * a->H * ((a->Lq + 127) / 128) <= INT32_MAX, "ranged_fwd: too many rows");
+  p.splits = fwd_splits(a->B, a->H, a->Lq, a->Lk);
+  WA_CHECK_ARG(p.splits == 1 || (a->workspace && wa_aligned16(a->workspace)), "ranged_fwd: a launch in %d parts needs a workspace", p.splits);
+  p.part_o = (float*)a->workspace;
+  p.part_ml = p.part_o + p.splits * a->B * a->H * a->Lq * a->D;
   const bool bent = a->cap > 0.f || a->slopes;
   if (a->D == 128) launch_fwd<128, 1>(p, bent, (hipStream_t)stream);
   else launch_fwd<64, 1>(p, bent, (hipStream_t)stream);

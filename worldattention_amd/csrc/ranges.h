@@ -32,7 +32,7 @@ struct Ranges {
 // The 64-key steps that N consecutive tiles of rows walk: one or two runs of keys (the hulls, joined where they touch), cut into
 // steps from each run's first key on. All values are wave-uniform.
 struct Steps {
-  int s0, e0, s1, e1, n0, total;
+  int s0, e0, s1, e1, n0, first, total;
   int up0, up1, low0, low1;   // keys that every row holds in its upper / lower run
   __device__ __forceinline__ void init(const Ranges& p, int b, int tile, int n) {
     int v[8] = {INT32_MAX, 0, INT32_MAX, 0, 0, INT32_MAX, 0, INT32_MAX};
@@ -65,12 +65,19 @@ struct Steps {
       e0 = up && low ? max(v[1], v[3]) : up ? v[1] : v[3];
     }
     n0 = (e0 - s0 + 63) / 64;
+    first = 0;
     total = n0 + (e1 - s1 + 63) / 64;
     up0 = v[4]; up1 = v[5]; low0 = v[6]; low1 = v[7];
   }
+  // The steps of part `part` of `parts` alone.
+  __device__ __forceinline__ void cut(int part, int parts) {
+    if (parts == 1) return;
+    first = (int)((int64_t)total * part / parts);
+    total = (int)((int64_t)total * (part + 1) / parts) - first;
+  }
   // Step i's first key, and the end of the run it is in.
-  __device__ __forceinline__ int key(int i) const { return i < n0 ? s0 + 64 * i : s1 + 64 * (i - n0); }
-  __device__ __forceinline__ int end(int i) const { return i < n0 ? e0 : e1; }
+  __device__ __forceinline__ int key(int i) const { return first + i < n0 ? s0 + 64 * (first + i) : s1 + 64 * (first + i - n0); }
+  __device__ __forceinline__ int end(int i) const { return first + i < n0 ? e0 : e1; }
   // Whether every row sees all 64 keys from `key` on (which lie before `end`).
   __device__ __forceinline__ bool whole(int key, int end) const {
     return key + 64 <= end && ((key >= up0 && key + 64 <= up1) || (key >= low0 && key + 64 <= low1));
@@ -88,38 +95,60 @@ struct RowRuns {
 // a wave's scores is asked once for a tile:
 //   kBias   no cap;
 //   kNear   |x| <= cap / 2: tanh(z) = z P(z^2), P of degree 4 fitted to 1.5e-8 of the value (a weighted least-squares fit of tanh(z) / z on
-//           [0, 1/4] with the leading 1 kept). More exact than the other, and less work: eight plain instructions for two transcendental ones and four
-//           (a training step of 8,190 packed tokens, 16 heads, cap 30: see ranged.hip);
+//           [0, 1/4] with the leading 1 kept), with the scale in its coefficients: six instructions, more exact than kFar and half its work;
 //   kFar    e = exp(2 z), r = 1 / (e + 1): tanh = 1 - 2 r, off by a few 2^-24 of the cap wherever z is (e = inf gives r = 0); its derivative
 //           4 e r r, off by a few 2^-24 of itself.
 enum BendForm { kBias, kNear, kFar };
 struct Bend {
-  float scale2, in, in2, cap2, slope2;   // scale log2(e); scale / cap; 2 scale / cap log2(e); cap log2(e) or 0; slope log2(e)
+  float near;                 // largest |s| for kNear (below 0: none; the coefficients' powers of the scale would leave fp32)
+  float scale2, in2, cap2;    // scale log2(e); 2 scale / cap log2(e); cap log2(e) or 0
+  float c[4], icap2;          // kNear's coefficients of s^2 and its powers; 1 / cap2
+  float slope2;               // slope log2(e)
   // The form for scores of at most `most`, the same in all of the wave's lanes.
   __device__ __forceinline__ BendForm form(float most) const {
     if (!(cap2 > 0.f)) return kBias;
-    return __any(most * in > 0.5f) ? kFar : kNear;
+    return __any(most > near) ? kFar : kNear;
+  }
+  // The score before the bias, and the cap's derivative there.
+  template <BendForm FORM>
+  __device__ __forceinline__ float capped(float s, float& turn) const {
+    turn = 1.f;
+    if constexpr (FORM == kBias) {
+      return s * scale2;
+    } else if constexpr (FORM == kNear) {
+      const float u = s * s, y = s * fmaf(u, fmaf(u, fmaf(u, fmaf(u, c[3], c[2]), c[1]), c[0]), scale2), t = y * icap2;
+      turn = fmaf(-t, t, 1.f);
+      return y;
+    } else {
+      const float e = __builtin_amdgcn_exp2f(s * in2), r = __builtin_amdgcn_rcpf(e + 1.f);
+      turn = fminf(e, 0x1p100f) * 4.f * r * r;
+      return fmaf(-2.f * cap2, r, cap2);
+    }
   }
   template <BendForm FORM>
   __device__ __forceinline__ float bent(float s, float dist, float& turn) const {
-    float y;
-    turn = 1.f;
-    if constexpr (FORM == kBias) {
-      y = s * scale2;
-    } else if constexpr (FORM == kNear) {
-      const float z = s * in, u = z * z;
-      const float q = fmaf(u, fmaf(u, fmaf(u, fmaf(u, 0x1.1a7b9cp-6f, -0x1.b28c5ep-5f), 0x1.10e9fcp-3f), -0x1.5554d6p-2f), 1.f);
-      const float t = z * q;
-      y = t * cap2;
-      turn = fmaf(-t, t, 1.f);
-    } else {
-      const float e = __builtin_amdgcn_exp2f(s * in2), r = __builtin_amdgcn_rcpf(e + 1.f);
-      y = fmaf(-2.f * cap2, r, cap2);
-      turn = fminf(e, 0x1p100f) * 4.f * r * r;
-    }
-    return fmaf(-slope2, fabsf(dist), y);
+    return fmaf(-slope2, fabsf(dist), capped<FORM>(s, turn));
   }
 };
+static inline Bend bend_of(float scale, float cap) {
+  Bend b{};
+  b.scale2 = scale * WA_LOG2E;
+  b.near = -1.f;
+  if (cap > 0.f) {
+    const float in = scale / cap, u = in * in;
+    b.in2 = 2.f * in * WA_LOG2E;
+    b.cap2 = cap * WA_LOG2E;
+    b.icap2 = 1.f / b.cap2;
+    if (in >= 0x1p-15f && in <= 0x1p15f) {   // powers up to the eighth, and |s| <= 2^14, stay normal
+      b.near = 0.5f / in;
+      b.c[0] = -0x1.5554d6p-2f * u * b.scale2;
+      b.c[1] = 0x1.10e9fcp-3f * u * u * b.scale2;
+      b.c[2] = -0x1.b28c5ep-5f * u * u * u * b.scale2;
+      b.c[3] = 0x1.1a7b9cp-6f * u * u * u * u * b.scale2;
+    }
+  }
+  return b;
+}
 template <int N>
 __device__ __forceinline__ float largest(const f32x16 (&s)[N]) {
   float x = 0.f;
@@ -137,8 +166,4 @@ __device__ __forceinline__ void by_form(BendForm form, const Run& run) {
   else if (form == kNear) run(FormTag<kNear>{});
   else run(FormTag<kFar>{});
 }
-static inline Bend bend_of(float scale, float cap) {
-  return {scale * WA_LOG2E, cap > 0.f ? scale / cap : 0.f, cap > 0.f ? 2.f * scale / cap * WA_LOG2E : 0.f, cap * WA_LOG2E, 0.f};
-}
-
 }  // namespace
