@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   int u = (int)blockIdx.x;
   const int bh = u % nbh;
   u /= nbh;
-  const int h = (bh % p.Hk) * per + u % per, b = bh / p.Hk, qt = nq - 1 - u / per;
+  const int h = (bh % p.Hk) * per + u % per, b = bh / p.Hk, qt = p.ranges.row_tile(b, u / per);
   Steps st;
   st.init(p.ranges, b, 2 * qt, 2);
   const int qi = qt * 128 + w * 32 + l32;
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(256) slopes_kernel(BwdParams p, int n) {
 // PARTS: the steps are cut into runs for workgroups of their own, whose fp32 sums another launch adds up in their order.
 // ---------------------------------------------------------------------------------------------
 constexpr int kListMax = 1024;   // row tiles listed at a time: 65,536 rows
-constexpr int kKeys = 128;       // of a workgroup
+constexpr int kKeys = 128;       // of a workgroup, as the order of the key tiles has them
 
 template <int D, bool BENT>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) ranged_dkv_kernel(BwdParams p) {
@@ -426,12 +426,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, l32 = lane & 31, kg = w & 3;
   const bool swave = w < 4;   // wave-uniform role
-  // a causal mask's first keys are seen by most rows: they start first
   const int per = p.H / p.Hk, nbh = p.B * p.Hk;
   int u = (int)blockIdx.x;
   const int bh = u % nbh, hk = bh % p.Hk, b = bh / p.Hk;
   u /= nbh;
-  const int part = u % p.parts, key0 = u / p.parts * kKeys;
+  const int part = u % p.parts, key0 = p.ranges.key_tile(b, u / p.parts) * kKeys;
   const int kl = kg * 32 + l32, key = key0 + kl;
   const bool k_ok = key < p.ranges.Lk;
   const int key_end = min(key0 + kKeys, p.ranges.Lk);
@@ -758,7 +757,7 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   WA_CHECK_ARG(a->B >= 1 && a->Lq >= 1 && a->Lk >= 1 && a->Lq <= 1 << 30 && a->Lk <= 1 << 30 && a->Hk >= 1 && a->H >= a->Hk && a->H % a->Hk == 0,
                "ranged_bwd: bad sizes B %lld Lq %lld Lk %lld heads %lld / %lld", (long long)a->B, (long long)a->Lq, (long long)a->Lk,
                (long long)a->H, (long long)a->Hk);
-  WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->dout && a->lse && a->rows && a->tiles && a->dq && a->dk && a->dv && a->workspace &&
+  WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->dout && a->lse && a->rows && a->tiles && a->order && a->dq && a->dk && a->dv && a->workspace &&
                wa_aligned16(a->rows), "ranged_bwd: null tensor");
   WA_CHECK_ARG(!a->dslopes || a->slopes, "ranged_bwd: dslopes without slopes");
   auto rows16 = [](const void* x, int64_t sb, int64_t st, int64_t sh) {
@@ -780,7 +779,7 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   p.o = (const bf16_t*)a->o; p.o_sb = a->o_sb; p.o_st = a->o_st; p.o_sh = a->o_sh;
   p.dout = (const bf16_t*)a->dout; p.d_sb = a->d_sb; p.d_st = a->d_st; p.d_sh = a->d_sh;
   p.lse = a->lse; p.dlse = a->dlse;
-  p.ranges = {a->rows, a->tiles, a->ranges_sb ? 1 : 0, (int)a->Lq, (int)a->Lk, (int)((a->Lq + kRangeRows - 1) / kRangeRows)};
+  p.ranges = {a->rows, a->tiles, a->ranges_sb ? 1 : 0, (int)a->Lq, (int)a->Lk, (int)((a->Lq + kRangeRows - 1) / kRangeRows), a->order};
   p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.slopes = a->slopes;
   p.B = (int)a->B; p.H = (int)a->H; p.Hk = (int)a->Hk;
   p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->D) : a->scale;

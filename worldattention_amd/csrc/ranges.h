@@ -15,6 +15,14 @@ struct Ranges {
   const int32_t* rows;
   const int32_t* tiles;
   int sb, Lq, Lk, n_tiles;   // sb: 0 where the batch shares one set
+  const int32_t* order;      // of each set: 128-row tiles and then 128-key tiles, those with the most steps first
+  __device__ __forceinline__ int row_tiles() const { return (Lq + 127) / 128; }
+  __device__ __forceinline__ int key_tiles() const { return (Lk + 127) / 128; }
+  __device__ __forceinline__ int row_tile(int b, int i) const { return placed(order + (int64_t)b * sb * (row_tiles() + key_tiles()) + i, row_tiles()); }
+  __device__ __forceinline__ int key_tile(int b, int i) const {
+    return placed(order + (int64_t)b * sb * (row_tiles() + key_tiles()) + row_tiles() + i, key_tiles());
+  }
+  __device__ __forceinline__ static int placed(const int32_t* at, int n) { return __builtin_amdgcn_readfirstlane(min(max(*at, 0), n - 1)); }
   __device__ __forceinline__ const int32_t* tile(int b, int i) const {
     return tiles + ((int64_t)b * sb * n_tiles + i) * WA_RANGE_TILE_INTS;
   }
@@ -34,7 +42,8 @@ struct Ranges {
 struct Steps {
   int s0, e0, s1, e1, n0, first, total;
   int up0, up1, low0, low1;   // keys that every row holds in its upper / lower run
-  __device__ __forceinline__ void init(const Ranges& p, int b, int tile, int n) {
+  // Any lanes' tiles.
+  __device__ __forceinline__ void of(const Ranges& p, int b, int tile, int n) {
     int v[8] = {INT32_MAX, 0, INT32_MAX, 0, 0, INT32_MAX, 0, INT32_MAX};
     for (int i = tile; i < min(tile + n, p.n_tiles); ++i) {
       const int32_t* t = p.tile(b, i);
@@ -42,19 +51,12 @@ struct Steps {
       for (int run = 0; run < 2; ++run) {
         const int lo = t[2 * run], hi = t[2 * run + 1];
         if (hi > lo) {
-          v[2 * run] = min(v[2 * run], lo);
-          v[2 * run + 1] = max(v[2 * run + 1], hi);
+          v[2 * run] = min(v[2 * run], max(lo, 0));
+          v[2 * run + 1] = max(v[2 * run + 1], min(hi, p.Lk));
         }
         v[4 + 2 * run] = max(v[4 + 2 * run], t[4 + 2 * run]);
         v[5 + 2 * run] = min(v[5 + 2 * run], t[5 + 2 * run]);
       }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __builtin_amdgcn_readfirstlane(v[i]);
-#pragma unroll
-    for (int run = 0; run < 2; ++run) {
-      v[2 * run] = max(v[2 * run], 0);
-      v[2 * run + 1] = min(v[2 * run + 1], p.Lk);
     }
     const bool up = v[1] > v[0], low = v[3] > v[2];
     s0 = e0 = s1 = e1 = 0;
@@ -68,6 +70,13 @@ struct Steps {
     first = 0;
     total = n0 + (e1 - s1 + 63) / 64;
     up0 = v[4]; up1 = v[5]; low0 = v[6]; low1 = v[7];
+  }
+  // One wave's.
+  __device__ __forceinline__ void init(const Ranges& p, int b, int tile, int n) {
+    of(p, b, tile, n);
+    int* const all[] = {&s0, &e0, &s1, &e1, &n0, &total, &up0, &up1, &low0, &low1};
+#pragma unroll
+    for (int* x : all) *x = __builtin_amdgcn_readfirstlane(*x);
   }
   // The steps of part `part` of `parts` alone.
   __device__ __forceinline__ void cut(int part, int parts) {

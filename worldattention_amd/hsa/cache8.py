@@ -15,7 +15,7 @@ from typing import Optional, Union
 import torch
 
 from .. import _lib
-from .ranged import _count, _forward, check_scores, key_ranges
+from .ranged import _count, _forward, _make_ranges, check_scores
 from .selected import BlockSelection, KvLen, _no_gradient
 
 __all__ = ["new_cache_8bit", "kv_append_8bit", "kv_read_8bit", "attend_8bit"]
@@ -200,7 +200,8 @@ def attend_8bit(q: torch.Tensor, kv_cache: dict, kv_len: KvLen, *, scale: Option
     if chosen is None and n * (heads // hk) > _FEW_ROWS:
         tokens = max_len if lens is not None else min(max(len_all, 0), max_len)
         k, v = _read(c, dev, None, 0, tokens, torch.bfloat16, (len_ptr, len_all if lens is None else 0), n, window, sink)
-        ranges = key_ranges(bsz, n, tokens, window=window or None, sink=sink, kv_len=len_all if lens is None else lens, device=dev)
+        ranges = _make_ranges(bsz, n, tokens, window=window or None, sink=sink, kv_len=len_all if lens is None else lens, device=dev,
+                              in_order=True)   # for one call: not worth sorting
         if not 0 <= q.stride(1) <= 1 << 23:
             q = q.clone(memory_format=torch.contiguous_format)
         return _forward(q, k, v, slopes, ranges, scale, cap)

@@ -29,6 +29,7 @@ class KeyRanges(NamedTuple):
 
     rows: torch.Tensor                    # int32 [B or 1, Lq, 4]: two disjoint runs of keys, the lower one second
     tiles: torch.Tensor                   # int32 [B or 1, ceil(Lq / 64), 12]: what 64 rows see together
+    order: torch.Tensor                   # int32 [B or 1, ceil(Lq / 128) + ceil(Lk / 128)]: tiles of rows and of keys, most work first
     kv_len: Union[int, torch.Tensor]      # row i sits at key position kv_len - Lq + i
     q_len: int
     k_len: int
@@ -73,6 +74,11 @@ def key_ranges(batch: int, q_len: int, k_len: int, *, causal: bool = True, chunk
     key in both counts once; positions are used by a bias alone). A batch whose rules do not differ shares one set. Nothing is
     read back to the host, so ranges can be made, and captured, with device lengths.
     """
+    return _make_ranges(batch, q_len, k_len, causal, chunk, window, sink, prefix, documents, lengths, kv_len, given, device)
+
+
+def _make_ranges(batch, q_len, k_len, causal=True, chunk=1, window=None, sink=0, prefix=0, documents=None, lengths=None, kv_len=None,
+                 given=None, device=None, in_order=False) -> KeyRanges:
     batch, q_len, k_len = _count(batch, "batch", 0), _count(q_len, "q_len", 0), _count(k_len, "k_len", 0)
     if q_len > _MOST or k_len > _MOST:
         raise ValueError(f"at most {_MOST} tokens, got {q_len} and {k_len}")
@@ -119,12 +125,13 @@ def key_ranges(batch: int, q_len: int, k_len: int, *, causal: bool = True, chunk
         raise ValueError(f"tensors on {dev}, device {device}")
     rows = torch.empty((sets, q_len, 4), dtype=torch.int32, device=dev)
     tiles = torch.empty((sets, -(-q_len // 64), 12), dtype=torch.int32, device=dev)
+    order = torch.empty((sets, -(-q_len // 128) - (-k_len // 128)), dtype=torch.int32, device=dev)
     if rows.numel():
         args = _lib.KeyRangesArgs(sets, q_len, k_len, _lib.ptr(kv_t), kv_all, _lib.ptr(given), int(bool(causal)), chunk, window,
                                   sink, _lib.ptr(prefix_t), prefix_all, _lib.ptr(documents), docs_sb, n_borders, rows.data_ptr(),
-                                  tiles.data_ptr())
+                                  tiles.data_ptr(), order.data_ptr(), int(in_order))
         _lib.launch("wa_key_ranges", args, dev)
-    return KeyRanges(rows, tiles, kv_all if kv_t is None else kv_t, q_len, k_len)
+    return KeyRanges(rows, tiles, order, kv_all if kv_t is None else kv_t, q_len, k_len)
 
 
 def _ready(t: torch.Tensor) -> torch.Tensor:
@@ -137,7 +144,7 @@ def _ready(t: torch.Tensor) -> torch.Tensor:
 def _range_args(ranges: KeyRanges):
     kv = ranges.kv_len
     tensor = isinstance(kv, torch.Tensor)
-    return (ranges.rows.data_ptr(), ranges.tiles.data_ptr(), int(ranges.rows.shape[0] > 1), kv.data_ptr() if tensor else None,
+    return (ranges.rows.data_ptr(), ranges.tiles.data_ptr(), ranges.order.data_ptr(), int(ranges.rows.shape[0] > 1), kv.data_ptr() if tensor else None,
             0 if tensor else kv)
 
 
@@ -158,24 +165,23 @@ def _forward(q, k, v, slopes, ranges, scale, cap):
 
 class _Ranged(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, slopes, rows, tiles, kv_len, q_len, k_len, scale, cap):
+    def forward(ctx, q, k, v, slopes, ranges, scale, cap):
         ctx.set_materialize_grads(False)
-        ranges = KeyRanges(rows, tiles, kv_len, q_len, k_len)
         out, lse = _forward(q, k, v, slopes, ranges, scale, cap)
-        held = kv_len if isinstance(kv_len, torch.Tensor) else None
-        ctx.save_for_backward(q, k, v, slopes, out, lse, rows, tiles, held)
-        ctx.rest = (kv_len if held is None else None, q_len, k_len, scale, cap)
+        held = ranges.kv_len if isinstance(ranges.kv_len, torch.Tensor) else None
+        ctx.save_for_backward(q, k, v, slopes, out, lse, ranges.rows, ranges.tiles, ranges.order, held)
+        ctx.rest = (None if held is not None else ranges.kv_len, ranges.q_len, ranges.k_len, scale, cap)
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dlse):
-        none = (None,) * 7
+        none = (None,) * 3
         if dout is None and dlse is None:
             return None, None, None, None, *none
-        q, k, v, slopes, out, lse, rows, tiles, held = ctx.saved_tensors
+        q, k, v, slopes, out, lse, rows, tiles, order, held = ctx.saved_tensors
         kv_len, q_len, k_len, scale, cap = ctx.rest
-        ranges = KeyRanges(rows, tiles, kv_len if held is None else held, q_len, k_len)
+        ranges = KeyRanges(rows, tiles, order, kv_len if held is None else held, q_len, k_len)
         dev = q.device
         bsz, n, heads, d = q.shape
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
@@ -239,23 +245,23 @@ def ranged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ranges: 
     if ranges.q_len != n or ranges.k_len != k.shape[1] or ranges.rows.shape[0] not in (1, bsz):
         raise ValueError(f"ranges of {ranges.rows.shape[0]} sequences, {ranges.q_len} rows and {ranges.k_len} keys do not fit "
                          f"{bsz}, {n} and {k.shape[1]}")
-    if (tuple(ranges.rows.shape[1:]) != (n, 4) or ranges.tiles.shape != (ranges.rows.shape[0], -(-n // 64), 12)
-            or not ranges.rows.is_contiguous() or not ranges.tiles.is_contiguous()
-            or ranges.rows.dtype is not torch.int32 or ranges.tiles.dtype is not torch.int32):
+    sets = ranges.rows.shape[0]
+    shapes = ((sets, n, 4), (sets, -(-n // 64), 12), (sets, -(-n // 128) - (-k.shape[1] // 128)))
+    if any(t.shape != s or t.dtype is not torch.int32 or not t.is_contiguous() for t, s in zip(ranges, shapes)):
         raise ValueError("ranges must be as key_ranges makes them")
     dp = padded_head_dim(d)
     scale, cap = check_scores(d, heads, scale, cap, slopes)
     if isinstance(ranges.kv_len, torch.Tensor) and tuple(ranges.kv_len.shape) != (bsz,):
         raise ValueError(f"ranges' kv_len is of {tuple(ranges.kv_len.shape)}, the batch of {bsz}")
     _lib.refuse_tangents(q, k, v, slopes)
-    _lib.require_gpu(q, k, v, slopes, ranges.rows, ranges.tiles, ranges.kv_len if isinstance(ranges.kv_len, torch.Tensor) else None)
+    _lib.require_gpu(q, k, v, slopes, *ranges[:3], ranges.kv_len if isinstance(ranges.kv_len, torch.Tensor) else None)
     if d != dp:
         q, k, v = (torch.nn.functional.pad(t, (0, dp - d)) for t in (q, k, v))
     q, k, v = _ready(q), _ready(k), _ready(v)
     slopes = None if slopes is None else slopes.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (slopes is not None and slopes.requires_grad)):
-        out, lse = _Ranged.apply(q, k, v, slopes, *ranges, scale, cap)
+        out, lse = _Ranged.apply(q, k, v, slopes, ranges, scale, cap)
     else:
         out, lse = _forward(q, k, v, slopes, ranges, scale, cap)
     if d != dp:
