@@ -9,12 +9,12 @@ namespace {
 
 // =============================================================================================
 // Rows are (query, head of the group) pairs of one key head; a unit of 16 RT rows walks its tiles of 32 keys once. A part of a unit (the
-// tiles that one workgroup takes) is shared by four waves, tile by tile, each with running maxima and sums of its own. A tile's codes come
-// straight into registers in the operands' order: a key row's 16 channels a load, where q takes its channels in the same order; a value
-// row's 8 channels a load, eight rows a lane, transposed as their halves are put together. Codes become bf16 exactly; a block's scales are
-// wave-uniform factors of the scores and of the weights (powers of two: the weights' rounding is that of the plain ones). Products are
-// v_mfma_f32_16x16x32: S^T = K Q^T, O^T += V^T P^T. The next tile's codes are asked for before the current ones are used. Bound by
-// reading the codes.
+// tiles that one workgroup takes) is shared by four waves, tile by tile, each with running maxima and sums of its own. A wave's codes stream through
+// two LDS stages of its own by direct loads, whole rows at a time: a stage is read into registers and filled again, two tiles on, before the tile is
+// used, so a CU has 128 KB on their way (one tile ahead in registers, 64 KB, and rows in halves: 32 ragged sequences of up to 32,768 tokens, 8 key heads,
+// 283 us). Codes become bf16 exactly; a block's scales are wave-uniform factors of the scores and of the weights (powers of two: the weights' rounding
+// is that of the plain ones). Products are v_mfma_f32_16x16x32: S^T = K Q^T, O^T += V^T P^T; row a = 4 x + y of the former is key 4 y + x of
+// its 16, which puts value rows that are read together in different banks. Bound by reading the codes.
 // =============================================================================================
 struct AttendParams {
   const bf16_t* q; int64_t q_sb, q_st, q_sh;
@@ -105,10 +105,11 @@ __device__ __forceinline__ void write_row(const AttendParams& p, int b, int i, i
 }
 
 template <typename Code, int D, int RT>
-__global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) attend_kernel(AttendParams p) {
+__global__ void __launch_bounds__(256, D == 128 && RT == 4 ? 1 : 2) attend_kernel(AttendParams p) {
   constexpr int NW = 4, KC = D / 32, VC = D / 16, KL = D / 64;   // key products of a tile half; channels of a value row a lane holds; loads of a key row
   typedef typename ValueRow<D>::type VRow;
-  __shared__ float so[NW][16][D + 4];
+  static_assert(NW * 4 * 32 * D >= NW * 16 * (D + 4) * 4, "the waves' outputs fit their drained rings");
+  __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * 32 * D];   // of each wave two stages of keys and values; then the waves' outputs
   __shared__ float sm[NW][16], sl[NW][16];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, kg = lane >> 4;
   const int64_t u = blockIdx.x / p.parts;
@@ -169,66 +170,92 @@ __global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) attend_kernel(AttendPara
     const int64_t key = ((int64_t)id << p.shift) + (t & ((1 << (p.shift - 5)) - 1)) * 32;
     return id < 0 || key > last ? -1 : (int)key;
   };
-  // The lane's places in a tile: key rows 16 h + l16, value rows 16 (e / 4) + 4 kg + e % 4.
-  int k_off[2], v_off[8];
+  // A tile's codes in LDS: 16-byte chunk c of row r in slot c ^ swizzle(r). Direct load i fills rows i RPL .. + RPL.
+  constexpr int CPR = D / 16, RPL = 64 / CPR, LOADS = 32 / RPL, HALF = 32 * D;
+  auto swizzle = [](int r) { return D == 128 ? (r >> 1) & 7 : (r >> 2) & 3; };
+  char* const ring = lds + w * 4 * HALF;
+  int off[LOADS];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) k_off[h] = (16 * h + l16) * st + 16 * kg;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v_off[e] = (16 * (e >> 2) + 4 * kg + (e & 3)) * st + VC * l16;
+  for (int i = 0; i < LOADS; ++i) {
+    const int r = i * RPL + lane / CPR;
+    off[i] = r * st + ((lane % CPR) ^ swizzle(r)) * 16;
+  }
+  const int ky = (l16 & 3) * 4 + (l16 >> 2);   // the key of operand row l16
   struct Tile {
-    u32x4 k[2][KL];
-    VRow v[8];
     float ks, vs;
     int key;
   };
-  auto load = [&](Tile& x, int t) {
+  int next = t0 + w;
+  auto issue = [&](Tile& x, int stage) {   // the wave's next tile with seen tokens
     x.key = -1;
-    while (t < t1 && (x.key = key_of(t)) < 0) t += NW;
-    if (x.key < 0) return t1;
+    while (next < t1 && (x.key = key_of(next)) < 0) next += NW;
+    next += NW;
+    if (x.key < 0) return;
     // from the last token that any row sees on the codes read as zeros
     const int bytes = (min(32, last + 1 - x.key) - 1) * st + D;
     const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + (int64_t)x.key * st), (short)0, bytes, WA_BUF_DWORD3);
     const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + (int64_t)x.key * st), (short)0, bytes, WA_BUF_DWORD3);
+    char* const to = ring + stage * 2 * HALF;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < LOADS; ++i) lds_dma16(kr, to + i * 1024, off[i]);
 #pragma unroll
-      for (int c = 0; c < KL; ++c) x.k[h][c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[h] + 64 * c, 0, 0));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (D == 128) x.v[e] = __builtin_bit_cast(VRow, __builtin_amdgcn_raw_buffer_load_b64(vr, v_off[e], 0, 0));
-      else x.v[e] = __builtin_amdgcn_raw_buffer_load_b32(vr, v_off[e], 0, 0);
-    }
+    for (int i = 0; i < LOADS; ++i) lds_dma16(vr, to + HALF + i * 1024, off[i]);
     x.ks = ksc[x.key >> p.shift];
     x.vs = vsc[x.key >> p.shift];
-    return t;
   };
-  auto use = [&](const Tile& x) {
-    bf16x8 ka[2][KC];
+  // Tile x of `stage`, with tile y behind it on its way: x's place is taken by the tile after y.
+  auto use = [&](Tile& x0, const Tile& y0, int stage) {
+    const Tile x = x0;
+    if (y0.key >= 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const char* at = ring + stage * 2 * HALF;
+    u32x4 kc[2][KL];
+    VRow vc[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
+      for (int c = 0; c < KL; ++c) kc[h][c] = *(const u32x4*)(at + (16 * h + ky) * D + ((4 * c + kg) ^ swizzle(ky)) * 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int r = 16 * (e >> 2) + 4 * (e & 3) + kg;
+      vc[e] = *(const VRow*)(at + HALF + r * D + (((VC * l16) >> 4) ^ swizzle(r)) * 16 + ((VC * l16) & 15));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < KL; ++c) asm volatile("" : "+v"(kc[h][c]));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(vc[e]));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before it is filled again
+    issue(x0, stage);
+    // the halves' keys one after the other: what is converted is used at once
+    f32x4 scores[RT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int y = 0; y < RT; ++y) scores[y][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
       for (int c = 0; c < KC; ++c) {
-        u32x4 y;
+        u32x4 k;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint32_t lo, hi;
-          Code::pairs(x.k[h][c >> 1][2 * (c & 1) + e], lo, hi);
-          y[2 * e] = lo;
-          y[2 * e + 1] = hi;
+          Code::pairs(kc[h][c >> 1][2 * (c & 1) + e], lo, hi);
+          k[2 * e] = lo;
+          k[2 * e + 1] = hi;
         }
-        ka[h][c] = __builtin_bit_cast(bf16x8, y);
+#pragma unroll
+        for (int y = 0; y < RT; ++y) scores[y][h] = mma16(__builtin_bit_cast(bf16x8, k), q[y][c], scores[y][h]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     const bool whole = x.key + 31 <= lowest && ((window == 0) | (x.key > last - window) | (x.key + 31 < sink));
     bf16x8 pr[RT];
 #pragma unroll
     for (int y = 0; y < RT; ++y) {
-      f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) acc[h] = mma16(ka[h][c], q[y][c], acc[h]);
+      const f32x4(&acc)[2] = scores[y];
       float s[8];
-      const int key0 = x.key + 4 * kg;
+      const int key0 = x.key + kg;
       if (p.bend.cap2 > 0.f || p.slopes) {
         Bend bend = p.bend;
         bend.slope2 = slope2[y];
@@ -241,7 +268,7 @@ __global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) attend_kernel(AttendPara
         }
         by_form(bend.form(most), [&](auto form) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[e] = bend.bent<decltype(form)::value>(s[e], far - (float)(16 * (e >> 2) + (e & 3)), unused);
+          for (int e = 0; e < 8; ++e) s[e] = bend.bent<decltype(form)::value>(s[e], far - (float)(16 * (e >> 2) + 4 * (e & 3)), unused);
         });
       } else {
         const float by = p.bend.scale2 * x.ks;
@@ -252,7 +279,7 @@ __global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) attend_kernel(AttendPara
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           // one comparison beside the other: as a chain of branches the window's was compiled to nothing
-          const int key = key0 + 16 * (e >> 2) + (e & 3);
+          const int key = key0 + 16 * (e >> 2) + 4 * (e & 3);
           const bool seen = (key <= pos[y]) & ((key >= from[y]) | (key < sink));
           s[e] = seen ? s[e] : -INFINITY;
         }
@@ -281,23 +308,28 @@ __global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) attend_kernel(AttendPara
     for (int j = 0; j < VC; ++j) {
       uint32_t rows[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) rows[e] = word(x.v[e], j / 4);
+      for (int e = 0; e < 8; ++e) rows[e] = word(vc[e], j / 4);
       const u32x4 vt = Code::column(rows, j % 4);   // channel j of the eight rows
 #pragma unroll
       for (int y = 0; y < RT; ++y) o[y][j] = mma16(__builtin_bit_cast(bf16x8, vt), pr[y], o[y][j]);
+      if (j % 2) __builtin_amdgcn_sched_barrier(0);
     }
   };
   {
+#pragma unroll
+    for (int x = 0; x < RT; ++x)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) asm volatile("" : "+v"(q[x][c]));   // here before the first tiles are asked for
     Tile a, c;
-    int t = load(a, t0 + w);
+    issue(a, 0);
+    issue(c, 1);
     while (a.key >= 0) {
-      t = load(c, t + NW);
-      use(a);
+      use(a, c, 0);
       if (c.key < 0) break;
-      t = load(a, t + NW);
-      use(c);
+      use(c, a, 1);
     }
   }
+  float(*so)[16][D + 4] = (float(*)[16][D + 4])lds;
   // The waves' parts: each to the common maximum, then summed in wave order. Channel VC (4 kg + r) + j of row l16 is register r of
   // accumulator j.
 #pragma unroll

@@ -713,11 +713,11 @@ __global__ void __launch_bounds__(256) parts_kernel(BwdParams p, int64_t size) {
   *(bf16x8*)(x < size ? p.dk + x : p.dv + (x - size)) = o;
 }
 
-// Runs that the steps of 128 keys are cut into: about two workgroups a CU, but none without a query head of its own (the runs' fp32 sums are
-// written and read once more).
-int kv_parts(int64_t B, int64_t H, int64_t Hk, int64_t Lk) {
-  const int64_t groups = B * Hk * ((Lk + kKeys - 1) / kKeys);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(H / Hk, 512 / groups));
+// Runs that the steps of 128 keys are cut into: about two workgroups a CU, but none of fewer than four steps, and at most eight (the runs' fp32 sums
+// are written and read once more).
+int kv_parts(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk) {
+  const int64_t groups = B * Hk * ((Lk + kKeys - 1) / kKeys), steps = H / Hk * ((Lq + 63) / 64);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / groups, steps / 4, 8}));
 }
 
 template <int D, bool BENT>
@@ -745,8 +745,8 @@ void launch_bwd(const BwdParams& p, hipStream_t s) {
 }  // namespace
 
 extern "C" int64_t wa_ranged_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk, int64_t D) {
-  if (B < 1 || Hk < 1 || H < Hk || Lk < 1) return 0;
-  const int parts = kv_parts(B, H, Hk, Lk);
+  if (B < 1 || Hk < 1 || H < Hk || Lq < 1 || Lk < 1) return 0;
+  const int parts = kv_parts(B, H, Hk, Lq, Lk);
   const int64_t rows = (B * H * Lq * 12 + B * H * ((Lq + 127) / 128) * 4 + 15) / 16 * 16;
   return rows + (parts > 1 ? parts * 2 * B * Lk * Hk * D * 4 : 0);
 }
@@ -790,7 +790,7 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   p.on = p.lse2 + n;
   p.delta = p.on + n;
   p.slope_part = p.delta + n;
-  p.parts = kv_parts(a->B, a->H, a->Hk, a->Lk);
+  p.parts = kv_parts(a->B, a->H, a->Hk, a->Lq, a->Lk);
   p.part_kv = (float*)((char*)a->workspace + (n * 12 + a->B * a->H * ((a->Lq + 127) / 128) * 4 + 15) / 16 * 16);
   hipStream_t s = (hipStream_t)stream;
   const bool bent = a->cap > 0.f || a->slopes;
