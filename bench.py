@@ -79,7 +79,7 @@ def copy_calibration(dev) -> None:
 
 # The sources the sparse forward kernel is built from: a counter summary under profiles/ records
 # their fingerprint, and its figures are used only while the sources still match it.
-SPARSE_KERNEL_SOURCES = ("worldattention_amd/csrc/bsa_fwd.hip", "worldattention_amd/csrc/tile.h",
+SPARSE_KERNEL_SOURCES = ("worldattention_amd/csrc/bsa_fwd.hip", "worldattention_amd/csrc/pipe.h", "worldattention_amd/csrc/tile.h",
                          "worldattention_amd/csrc/common.h")
 
 
