@@ -883,8 +883,9 @@ int wa_selected_attn(const wa_selected_attn_args* args, void* stream);
  * and is not seen. NULL: one document, [0, kv_len). `given` (device int32 [B, Lq, 4], each row the runs
  * [0, 1) and [2, 3) as start and end; empty where end <= start) replaces all rules; it is clamped to [0, Lk].
  * Written: rows int32 [B, Lq, 4] (disjoint runs, the lower one in 2, 3) and tiles int32
- * [B, ceil(Lq / 64), WA_RANGE_TILE_INTS], what 64 rows see together; order int32 [B, ceil(Lq / 128) + ceil(Lk / 128)],
- * tiles of rows and of keys, those with the most work first (in_order: the last rows and the first keys first, at no cost). */
+ * [B, ceil(Lq / 64), WA_RANGE_TILE_INTS], what 64 rows see together; order int32 [B, ceil(Lq / 128) +
+ * ceil(Lk / 128) + 1], tiles of rows and of keys, those with the most work first (in_order: the last rows and the first
+ * keys first, at no cost), and the first row's position. */
 #define WA_RANGE_TILE_INTS 12
 typedef struct wa_key_ranges_args {
   int64_t B, Lq, Lk;
@@ -902,8 +903,7 @@ int wa_key_ranges(const wa_key_ranges_args* args, void* stream);
  *   x = scale q.k,  y = cap tanh(x / cap) (cap 0: x),  s = y - slopes[h] |t - j|  (slopes NULL: y).
  * A row that sees nothing gets 0 and a log-sum-exp of -inf. Query heads hk (H / Hk) .. (hk + 1)(H / Hk) - 1
  * read key head hk. q [B, Lq, H, D], k, v [B, Lk, Hk, D], D = 64 or 128, 16-byte aligned rows at most 2^23
- * elements apart; rows / tiles / order as above for B sequences (ranges_sb 1) or one shared by all (0); kv_len as
- * there (positions: read with slopes only). lse: fp32 [B, H, Lq], natural log. scale > 0 (0: D^-1/2). */
+ * elements apart; rows / tiles / order as above for B sequences (ranges_sb 1) or one shared by all (0). lse: fp32 [B, H, Lq], natural log. scale > 0 (0: D^-1/2). */
 typedef struct wa_ranged_fwd_args {
   const void* q; int64_t q_sb, q_st, q_sh;
   const void* k; int64_t k_sb, k_st, k_sh;
@@ -911,7 +911,6 @@ typedef struct wa_ranged_fwd_args {
   void* o; int64_t o_sb, o_st, o_sh;
   float* lse;
   const int32_t* rows; const int32_t* tiles; const int32_t* order; int32_t ranges_sb;
-  const int32_t* kv_len; int64_t kv_len_all;
   const float* slopes;
   int64_t B, H, Hk, Lq, Lk, D;
   float scale, cap;
@@ -931,7 +930,6 @@ typedef struct wa_ranged_bwd_args {
   const void* dout; int64_t d_sb, d_st, d_sh;
   const float* lse; const float* dlse;
   const int32_t* rows; const int32_t* tiles; const int32_t* order; int32_t ranges_sb;
-  const int32_t* kv_len; int64_t kv_len_all;
   const float* slopes;
   int64_t B, H, Hk, Lq, Lk, D;
   float scale, cap;

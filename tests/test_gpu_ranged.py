@@ -45,9 +45,8 @@ def _inputs(b, n, m, h, hk, d, seed=0, size=1.0):
     return q, k, v, do
 
 
-def check(q, k, v, do, ranges, mask, *, scale=None, cap=None, slopes=None, dlse=None):
+def check(q, k, v, do, ranges, mask, *, scale=None, cap=None, slopes=None, dlse=None, kv_len=None):
     """One call and its gradients against the definition."""
-    kv_len = ranges.kv_len
     leaves = [t.detach().requires_grad_(True) for t in (q, k, v)] + ([] if slopes is None else [slopes.detach().requires_grad_(True)])
     out, lse = W.ranged_attention(*leaves[:3], ranges, scale=scale, cap=cap, slopes=leaves[3] if slopes is not None else None, return_lse=True)
     outs, gouts = [out], [do]
@@ -158,7 +157,7 @@ def test_caps_slopes_and_the_log_sum_exps_gradient(d, cap, slopes, dlse):
     rules = dict(window=150, sink=7, kv_len=[330, 201])
     ranges = _ranges(b, n, m, rules)
     g = torch.Generator().manual_seed(1)
-    check(q, k, v, do, ranges, OR.seen(b, n, m, **rules), cap=cap, scale=0.11,
+    check(q, k, v, do, ranges, OR.seen(b, n, m, **rules), cap=cap, scale=0.11, kv_len=rules["kv_len"],
           slopes=torch.tensor([0.5, 0.0, 0.03, -0.01], device=DEV) if slopes else None,
           dlse=torch.randn(b, h, n, generator=g).to(DEV) if dlse else None)
 
@@ -319,3 +318,57 @@ def test_captured_steps():
             torch.cuda.synchronize()
             for x, y in zip(got, step()):
                 assert torch.equal(x, y), turn
+
+
+def test_ranges_keep_what_they_were_made_from():
+    """Lengths that a program counts up after the ranges were made change neither the rows nor their positions."""
+    b, n = 2, 100
+    q, k, v, _ = _inputs(b, n, n, 2, 2, 64, seed=30)
+    lens, slopes = _i32([100, 60]), torch.tensor([0.3, 0.1], device=DEV)
+    ranges = W.key_ranges(b, n, n, kv_len=lens)
+    first = W.ranged_attention(q, k, v, ranges, slopes=slopes)
+    lens += 7
+    assert torch.equal(first, W.ranged_attention(q, k, v, ranges, slopes=slopes))
+
+
+@pytest.mark.parametrize("dlse", [False, True])
+def test_single_keys_with_the_log_sum_exps_gradient(dlse):
+    """One key: the weight's gradient is 0, the log-sum-exp's is its score's."""
+    q, k, v, do = _inputs(1, 200, 200, 2, 2, 64, seed=31)
+    g = torch.Generator().manual_seed(2)
+    check(q, k, v, do, _ranges(1, 200, 200, dict(window=1)), OR.seen(1, 200, 200, window=1), cap=6.0,
+          slopes=torch.tensor([0.2, 0.1], device=DEV), dlse=torch.randn(1, 2, 200, generator=g).to(DEV) if dlse else None)
+
+
+@pytest.mark.parametrize("n,m", [(5, 4000), (130, 5000)])
+def test_few_rows_over_many_keys(n, m):
+    """Launches whose rows are too few to fill the GPU: steps in parts, joined; keys in runs."""
+    q, k, v, do = _inputs(1, n, m, 2, 1, 128, seed=n)
+    for rules in (dict(), dict(window=700, sink=40), dict(kv_len=[m - 64])):
+        check(q, k, v, do, _ranges(1, n, m, rules), OR.seen(1, n, m, **rules), cap=15.0)
+
+
+def test_offsets_that_pass_32_bits():
+    """Sequences and heads further apart than 2^31 elements."""
+    n, d = 150, 64
+    g = torch.Generator().manual_seed(33)
+    pool = torch.zeros(((1 << 31) + 4096 * 64,), dtype=torch.bfloat16, device=DEV)
+    far = torch.as_strided(pool, (2, n, 1, d), ((1 << 31) + 64, 2 * d, d, 1))
+    far.copy_(torch.randn(2, n, 1, d, generator=g))
+    q, k, v, do = _inputs(2, n, n, 1, 1, d, seed=34)
+    check(far, far, far, do, _ranges(2, n, n, dict()), OR.seen(2, n, n))
+
+
+def test_scores_at_the_ends_of_fp32():
+    """Scores near the lowest numbers of fp32 still weigh their keys; infinite ones give NaN, as a softmax of them does."""
+    n, d = 70, 64
+    q, k, v, _ = _inputs(1, n, n, 1, 1, d, seed=35)
+    q.fill_(1.0)
+    k.zero_()
+    k[..., 0] = -3.0e38
+    out, lse = W.ranged_attention(q, k, v, _ranges(1, n, n, dict()), scale=0.5, return_lse=True)
+    want = torch.cumsum(v[0, :, 0].double(), 0) / torch.arange(1, n + 1, device=DEV)[:, None]
+    assert ((out[0, :, 0].double() - want).abs() <= 2.0 ** -7 * (1 + want.abs())).all() and lse.isfinite().all()
+    k[0, 40, 0, 1] = math.inf
+    out = W.ranged_attention(q, k, v, _ranges(1, n, n, dict(documents=[0, 40, 41, 70])))
+    assert out[0, 40].isnan().all()

@@ -426,8 +426,8 @@ RangedFwdArgs = _struct("wa_ranged_fwd_args", [
     ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
     ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64), ("v_sh", c_int64),
     ("o", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
-    ("lse", c_void_p), ("rows", c_void_p), ("tiles", c_void_p), ("order", c_void_p), ("ranges_sb", c_int32), ("kv_len", c_void_p),
-    ("kv_len_all", c_int64), ("slopes", c_void_p), ("B", c_int64), ("H", c_int64), ("Hk", c_int64), ("Lq", c_int64),
+    ("lse", c_void_p), ("rows", c_void_p), ("tiles", c_void_p), ("order", c_void_p), ("ranges_sb", c_int32),
+    ("slopes", c_void_p), ("B", c_int64), ("H", c_int64), ("Hk", c_int64), ("Lq", c_int64),
     ("Lk", c_int64), ("D", c_int64), ("scale", c_float), ("cap", c_float), ("workspace", c_void_p),
 ])
 
@@ -438,7 +438,7 @@ RangedBwdArgs = _struct("wa_ranged_bwd_args", [
     ("o", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
     ("dout", c_void_p), ("d_sb", c_int64), ("d_st", c_int64), ("d_sh", c_int64),
     ("lse", c_void_p), ("dlse", c_void_p), ("rows", c_void_p), ("tiles", c_void_p), ("order", c_void_p), ("ranges_sb", c_int32),
-    ("kv_len", c_void_p), ("kv_len_all", c_int64), ("slopes", c_void_p), ("B", c_int64), ("H", c_int64), ("Hk", c_int64),
+    ("slopes", c_void_p), ("B", c_int64), ("H", c_int64), ("Hk", c_int64),
     ("Lq", c_int64), ("Lk", c_int64), ("D", c_int64), ("scale", c_float), ("cap", c_float),
     ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("dslopes", c_void_p), ("workspace", c_void_p),
 ])

@@ -36,8 +36,12 @@ __device__ int4 ordered(int64_t a0, int64_t a1, int64_t b0, int64_t b1, int Lk) 
   return r;
 }
 
+__device__ __forceinline__ int64_t held_tokens(const RulesParams& p, int b) {
+  return min(max(p.kv_len ? (int64_t)p.kv_len[b] : p.kv_len_all, (int64_t)0), (int64_t)p.Lk);
+}
+
 __device__ int4 by_rules(const RulesParams& p, int b, int i) {
-  const int64_t len = min(max(p.kv_len ? (int64_t)p.kv_len[b] : p.kv_len_all, (int64_t)0), (int64_t)p.Lk);
+  const int64_t len = held_tokens(p, b);
   const int64_t t = len - p.Lq + i;
   if (t < 0) return int4{0, 0, 0, 0};
   int64_t first = 0, end = len;
@@ -108,10 +112,11 @@ __global__ void __launch_bounds__(256) ranges_kernel(RulesParams p) {
 // of a set; a tile's place is the number of tiles before it, in ascending order where there are too many to count against each other.
 constexpr int kOrderMax = 4096;
 
-__global__ void __launch_bounds__(1024) order_kernel(Ranges p, int32_t* order, int sorted) {
+__global__ void __launch_bounds__(1024) order_kernel(Ranges p, RulesParams rules, int32_t* order, int sorted) {
   __shared__ int s_steps[kOrderMax], s_place[kOrderMax];
   const int set = blockIdx.x >> 1, keys = blockIdx.x & 1, tid = threadIdx.x, n = keys ? p.key_tiles() : p.row_tiles();
-  int32_t* out = order + (int64_t)set * (p.row_tiles() + p.key_tiles()) + (keys ? p.row_tiles() : 0);
+  int32_t* out = order + (int64_t)set * (p.row_tiles() + p.key_tiles() + 1) + (keys ? p.row_tiles() : 0);
+  if (keys && tid == 0) out[n] = (int)(held_tokens(rules, set) - p.Lq);
   if (n > kOrderMax || !sorted) {   // right for a causal mask: the last rows, the first keys
     for (int i = tid; i < n; i += 1024) out[i] = keys ? i : n - 1 - i;
     return;
@@ -150,7 +155,7 @@ __global__ void __launch_bounds__(1024) order_kernel(Ranges p, int32_t* order, i
 }
 
 // ---------------------------------------------------------------------------------------------
-// Forward. One workgroup of four waves per 128 QT rows of a head, one pass over the 64-key steps that its rows see, each with the
+// Forward. One workgroup of four waves per 128 rows of a head, one pass over the 64-key steps that its rows see, each with the
 // running maximum and sum of its softmax; the step loop is pipe.h's: while a half-step's products run, the exponentials of the one before
 // it do. A step that every row sees whole needs no mask; the others compare each key with the row's two runs, a row a lane.
 // A run's first step starts at its first key and its last one ends with it: keys that no row of the workgroup sees are not read.
@@ -162,7 +167,6 @@ struct FwdParams {
   bf16_t* o; int64_t o_sb, o_st, o_sh;
   float* lse;
   Ranges ranges;
-  const int32_t* kv_len; int64_t kv_len_all;
   const float* slopes;
   int B, H, Hk;
   Bend bend;
@@ -174,9 +178,9 @@ struct FwdParams {
 // Running maximum before the first key: below every score, and finite, so that no difference of it is NaN where a row sees nothing yet.
 constexpr float kNoMax = -3.4028234e38f;
 
-template <int D, int QT, bool BENT>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 1 ? 2 : 1))) ranged_fwd_kernel(FwdParams p) {
-  constexpr int NW = 4, BM = 128 * QT, DC = D / 16, DT = D / 32, TILE = 64 * D;
+template <int D, bool BENT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ranged_fwd_kernel(FwdParams p) {
+  constexpr int NW = 4, QT = 1, BM = 32 * NW * QT, DC = D / 16, DT = D / 32, TILE = 64 * D;
   using NT = NextTile<D, NW>;
   __shared__ __attribute__((aligned(1024))) bf16_t ks0[TILE];
   __shared__ __attribute__((aligned(1024))) bf16_t ks1[TILE];
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
   int pos0 = 0;
   if (BENT && p.slopes) {
     bend.slope2 = p.slopes[h] * WA_LOG2E;
-    pos0 = (int)min(max(p.kv_len ? (int64_t)p.kv_len[b] : p.kv_len_all, (int64_t)0), (int64_t)p.ranges.Lk) - p.ranges.Lq;
+    pos0 = p.ranges.position(b);
   }
 
   const bf16_t* kb = p.k + (int64_t)b * p.k_sb + (int64_t)(bh % p.Hk) * p.k_sh;
@@ -274,7 +278,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
 #pragma unroll
     for (int c = 0; c < 4; ++c) P[c][qt] = bf16x8{};
   }
+  // Scores are scaled in the exponential's multiply-add: its product is not rounded and the running maximum is, which the weights of a row
+  // share while that rounding is small. From a maximum of 2^20 on (a rounding of 2^-4 of a power) the wave forms each half's weights again,
+  // from scores that are rounded as the maximum is.
+  constexpr float kLarge = 0x1p20f;
   const float sl2 = BENT ? 1.f : p.bend.scale2;
+  float most_sum = 65536.f;   // of a row's weights in a half; behind it, the half's weights are formed again
   // Before a half's exponentials: its scores bent, and those of keys that the row does not see at -inf (lane (l32, g) holds keys
   // 32 KH + 8 (r / 4) + 4 g + r % 4 of step s).
   auto ready = [&](auto half, int s) {
@@ -313,7 +322,27 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QT == 
   };
   auto accept = [&](auto half) {
     constexpr int KH = decltype(half)::value;
-    if (pipe_check<QT>(rs)) pipe_rescale<D, QT, KH>(S[KH], P, oacc, m_i, l_i, rs, sl2);
+    bool again = false;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) again |= !(rs[qt] <= most_sum);
+    if (__any(again)) {
+      if constexpr (BENT) {
+        pipe_rescale<D, QT, KH>(S[KH], P, oacc, m_i, l_i, rs, sl2);
+      } else {
+        float most = kNoMax;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, S[KH][qt][r]);
+        const bool large = most_sum < 0.f || __any(most != kNoMax && fabsf(most) * sl2 > kLarge);
+        if (large) most_sum = -1.f;
+        const float before = large ? sl2 : 1.f;
+        f32x16 x[QT];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) x[qt] = S[KH][qt] * before;
+        pipe_rescale<D, QT, KH>(x, P, oacc, m_i, l_i, rs, large ? 1.f : sl2);
+      }
+    }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) l_i[qt] += rs[qt];
   };
@@ -447,11 +476,11 @@ int fwd_splits(int64_t B, int64_t H, int64_t Lq, int64_t Lk) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(512 / groups, (Lk + 63) / 64 / 16));
 }
 
-template <int D, int QT>
+template <int D>
 void launch_fwd(const FwdParams& p, bool bent, hipStream_t s) {
-  const int64_t grid = (int64_t)p.B * p.H * ((p.ranges.Lq + 128 * QT - 1) / (128 * QT)) * p.splits;
-  if (bent) hipLaunchKernelGGL((ranged_fwd_kernel<D, QT, true>), dim3((unsigned)grid), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((ranged_fwd_kernel<D, QT, false>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  const int64_t grid = (int64_t)p.B * p.H * ((p.ranges.Lq + 127) / 128) * p.splits;
+  if (bent) hipLaunchKernelGGL((ranged_fwd_kernel<D, true>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((ranged_fwd_kernel<D, false>), dim3((unsigned)grid), dim3(256), 0, s, p);
   if (p.splits > 1) {
     const int64_t n_rows = (int64_t)p.B * p.H * p.ranges.Lq, per = 2048 / D;
     hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)((n_rows + per - 1) / per)), dim3(256), 0, s, p, n_rows);
@@ -481,7 +510,7 @@ extern "C" int wa_key_ranges(const wa_key_ranges_args* a, void* stream) {
   WA_CHECK_ARG(a->B <= 1 << 30 && grid <= INT32_MAX, "key_ranges: too many rows");
   hipLaunchKernelGGL(ranges_kernel, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, p);
   const Ranges made{a->rows, a->tiles, 1, p.Lq, p.Lk, p.n_tiles, nullptr};
-  hipLaunchKernelGGL(order_kernel, dim3((unsigned)(2 * a->B)), dim3(1024), 0, (hipStream_t)stream, made, a->order, a->in_order ? 0 : 1);
+  hipLaunchKernelGGL(order_kernel, dim3((unsigned)(2 * a->B)), dim3(1024), 0, (hipStream_t)stream, made, p, a->order, a->in_order ? 0 : 1);
   return wa_launch_status("key_ranges");
 }
 
@@ -514,7 +543,7 @@ extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   p.o = (bf16_t*)a->o; p.o_sb = a->o_sb; p.o_st = a->o_st; p.o_sh = a->o_sh;
   p.lse = a->lse;
   p.ranges = {a->rows, a->tiles, a->ranges_sb ? 1 : 0, (int)a->Lq, (int)a->Lk, (int)((a->Lq + kRangeRows - 1) / kRangeRows), a->order};
-  p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.slopes = a->slopes;
+  p.slopes = a->slopes;
   p.B = (int)a->B; p.H = (int)a->H; p.Hk = (int)a->Hk;
   const float scale = a->scale == 0.f ? 1.f / sqrtf((float)a->D) : a->scale;
   p.bend = bend_of(scale, a->cap);
@@ -524,7 +553,7 @@ extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   p.part_o = (float*)a->workspace;
   p.part_ml = p.part_o + p.splits * a->B * a->H * a->Lq * a->D;
   const bool bent = a->cap > 0.f || a->slopes;
-  if (a->D == 128) launch_fwd<128, 1>(p, bent, (hipStream_t)stream);
-  else launch_fwd<64, 1>(p, bent, (hipStream_t)stream);
+  if (a->D == 128) launch_fwd<128>(p, bent, (hipStream_t)stream);
+  else launch_fwd<64>(p, bent, (hipStream_t)stream);
   return wa_launch_status("ranged_fwd");
 }

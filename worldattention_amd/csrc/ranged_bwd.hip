@@ -25,7 +25,6 @@ struct BwdParams {
   const bf16_t* dout; int64_t d_sb, d_st, d_sh;
   const float* lse; const float* dlse;
   Ranges ranges;
-  const int32_t* kv_len; int64_t kv_len_all;
   const float* slopes;
   int B, H, Hk;
   float scale;
@@ -191,14 +190,9 @@ __device__ __forceinline__ void put4(bf16x8& a, int x, const float (&f)[4]) {
   }
 }
 
-template <int N> using IC = std::integral_constant<int, N>;
 
 // Top of a step: this wave's tile loads have landed and its LDS reads returned, then the workgroup's.
 __device__ __forceinline__ void step_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
-__device__ __forceinline__ int first_position(const BwdParams& p, int b) {
-  return (int)min(max(p.kv_len ? (int64_t)p.kv_len[b] : p.kv_len_all, (int64_t)0), (int64_t)p.ranges.Lk) - p.ranges.Lq;
-}
 
 // ---------------------------------------------------------------------------------------------
 // dQ: one workgroup of four waves per 128 rows of a head over the 64-key steps that they see; K and V through two LDS stages each, a row
@@ -245,7 +239,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   int pos = 0;   // the row's position
   if (BENT && p.slopes) {
     bend.slope2 = p.slopes[h] * WA_LOG2E;
-    pos = first_position(p, b) + qi;
+    pos = p.ranges.position(b) + qi;
   }
 #pragma unroll
   for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(qf[c]), "+v"(dof[c]));
@@ -407,7 +401,7 @@ __global__ void __launch_bounds__(256) slopes_kernel(BwdParams p, int n) {
 //   dP = dO V^T of step t.
 // So one wave's products run under the other's exponentials, with one barrier a step. Q, dO and the rows' statistics and runs stream two steps ahead
 // into rings of four (Q is read by both phases), three and four stages; the weights have two. A workgroup takes 156 KiB of LDS at D = 128.
-// PARTS: the steps are cut into runs for workgroups of their own, whose fp32 sums another launch adds up in their order.
+// parts > 1: the steps are cut into runs for workgroups of their own, whose fp32 sums another launch adds up in their order.
 // ---------------------------------------------------------------------------------------------
 constexpr int kListMax = 1024;   // row tiles listed at a time: 65,536 rows
 constexpr int kKeys = 128;       // of a workgroup, as the order of the key tiles has them
@@ -448,7 +442,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
   }
 #pragma unroll
   for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(kvf[c]));
-  const int pos0 = BENT && p.slopes ? first_position(p, b) : 0;
+  const int pos0 = BENT && p.slopes ? p.ranges.position(b) : 0;
 
   f32x16 acc[DT];   // S-wave: dV^T; dP-wave: dK^T (lane = key, registers = channels)
 #pragma unroll
@@ -780,7 +774,7 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   p.dout = (const bf16_t*)a->dout; p.d_sb = a->d_sb; p.d_st = a->d_st; p.d_sh = a->d_sh;
   p.lse = a->lse; p.dlse = a->dlse;
   p.ranges = {a->rows, a->tiles, a->ranges_sb ? 1 : 0, (int)a->Lq, (int)a->Lk, (int)((a->Lq + kRangeRows - 1) / kRangeRows), a->order};
-  p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all; p.slopes = a->slopes;
+  p.slopes = a->slopes;
   p.B = (int)a->B; p.H = (int)a->H; p.Hk = (int)a->Hk;
   p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->D) : a->scale;
   p.bend = bend_of(p.scale, a->cap);

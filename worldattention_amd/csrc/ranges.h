@@ -15,13 +15,13 @@ struct Ranges {
   const int32_t* rows;
   const int32_t* tiles;
   int sb, Lq, Lk, n_tiles;   // sb: 0 where the batch shares one set
-  const int32_t* order;      // of each set: 128-row tiles and then 128-key tiles, those with the most steps first
+  const int32_t* order;      // of each set: 128-row tiles and then 128-key tiles, those with the most steps first; the first row's position
   __device__ __forceinline__ int row_tiles() const { return (Lq + 127) / 128; }
   __device__ __forceinline__ int key_tiles() const { return (Lk + 127) / 128; }
-  __device__ __forceinline__ int row_tile(int b, int i) const { return placed(order + (int64_t)b * sb * (row_tiles() + key_tiles()) + i, row_tiles()); }
-  __device__ __forceinline__ int key_tile(int b, int i) const {
-    return placed(order + (int64_t)b * sb * (row_tiles() + key_tiles()) + row_tiles() + i, key_tiles());
-  }
+  __device__ __forceinline__ const int32_t* of_set(int b) const { return order + (int64_t)b * sb * (row_tiles() + key_tiles() + 1); }
+  __device__ __forceinline__ int row_tile(int b, int i) const { return placed(of_set(b) + i, row_tiles()); }
+  __device__ __forceinline__ int key_tile(int b, int i) const { return placed(of_set(b) + row_tiles() + i, key_tiles()); }
+  __device__ __forceinline__ int position(int b) const { return of_set(b)[row_tiles() + key_tiles()]; }
   __device__ __forceinline__ static int placed(const int32_t* at, int n) { return __builtin_amdgcn_readfirstlane(min(max(*at, 0), n - 1)); }
   __device__ __forceinline__ const int32_t* tile(int b, int i) const {
     return tiles + ((int64_t)b * sb * n_tiles + i) * WA_RANGE_TILE_INTS;

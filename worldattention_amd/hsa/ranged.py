@@ -29,8 +29,8 @@ class KeyRanges(NamedTuple):
 
     rows: torch.Tensor                    # int32 [B or 1, Lq, 4]: two disjoint runs of keys, the lower one second
     tiles: torch.Tensor                   # int32 [B or 1, ceil(Lq / 64), 12]: what 64 rows see together
-    order: torch.Tensor                   # int32 [B or 1, ceil(Lq / 128) + ceil(Lk / 128)]: tiles of rows and of keys, most work first
-    kv_len: Union[int, torch.Tensor]      # row i sits at key position kv_len - Lq + i
+    order: torch.Tensor                   # int32 [B or 1, ceil(Lq / 128) + ceil(Lk / 128) + 1]: tiles of rows and of keys, most work
+                                          # first, and the first row's position
     q_len: int
     k_len: int
 
@@ -110,8 +110,8 @@ def _make_ranges(batch, q_len, k_len, causal=True, chunk=1, window=None, sink=0,
     if given is not None:
         if given.dim() != 3 or given.shape[0] not in (1, batch) or tuple(given.shape[1:]) != (q_len, 4) or given.dtype is not torch.int32:
             raise ValueError(f"given must be int32 [{batch} or 1, {q_len}, 4], got {given.dtype} {tuple(given.shape)}")
-        given = given.contiguous()
-        sets = given.shape[0]
+        sets = given.shape[0] if kv_t is None else batch
+        given = given.expand(sets, q_len, 4).contiguous()
     elif kv_t is None and prefix_t is None and docs_sb == 0:
         sets = min(1, batch)
     dev = _lib.require_gpu(given, documents, prefix_t, kv_t)
@@ -125,13 +125,13 @@ def _make_ranges(batch, q_len, k_len, causal=True, chunk=1, window=None, sink=0,
         raise ValueError(f"tensors on {dev}, device {device}")
     rows = torch.empty((sets, q_len, 4), dtype=torch.int32, device=dev)
     tiles = torch.empty((sets, -(-q_len // 64), 12), dtype=torch.int32, device=dev)
-    order = torch.empty((sets, -(-q_len // 128) - (-k_len // 128)), dtype=torch.int32, device=dev)
+    order = torch.empty((sets, -(-q_len // 128) - (-k_len // 128) + 1), dtype=torch.int32, device=dev)
     if rows.numel():
         args = _lib.KeyRangesArgs(sets, q_len, k_len, _lib.ptr(kv_t), kv_all, _lib.ptr(given), int(bool(causal)), chunk, window,
                                   sink, _lib.ptr(prefix_t), prefix_all, _lib.ptr(documents), docs_sb, n_borders, rows.data_ptr(),
                                   tiles.data_ptr(), order.data_ptr(), int(in_order))
         _lib.launch("wa_key_ranges", args, dev)
-    return KeyRanges(rows, tiles, order, kv_all if kv_t is None else kv_t, q_len, k_len)
+    return KeyRanges(rows, tiles, order, q_len, k_len)
 
 
 def _ready(t: torch.Tensor) -> torch.Tensor:
@@ -142,10 +142,7 @@ def _ready(t: torch.Tensor) -> torch.Tensor:
 
 
 def _range_args(ranges: KeyRanges):
-    kv = ranges.kv_len
-    tensor = isinstance(kv, torch.Tensor)
-    return (ranges.rows.data_ptr(), ranges.tiles.data_ptr(), ranges.order.data_ptr(), int(ranges.rows.shape[0] > 1), kv.data_ptr() if tensor else None,
-            0 if tensor else kv)
+    return ranges.rows.data_ptr(), ranges.tiles.data_ptr(), ranges.order.data_ptr(), int(ranges.rows.shape[0] > 1)
 
 
 def _forward(q, k, v, slopes, ranges, scale, cap):
@@ -168,9 +165,8 @@ class _Ranged(torch.autograd.Function):
     def forward(ctx, q, k, v, slopes, ranges, scale, cap):
         ctx.set_materialize_grads(False)
         out, lse = _forward(q, k, v, slopes, ranges, scale, cap)
-        held = ranges.kv_len if isinstance(ranges.kv_len, torch.Tensor) else None
-        ctx.save_for_backward(q, k, v, slopes, out, lse, ranges.rows, ranges.tiles, ranges.order, held)
-        ctx.rest = (None if held is not None else ranges.kv_len, ranges.q_len, ranges.k_len, scale, cap)
+        ctx.save_for_backward(q, k, v, slopes, out, lse, *ranges[:3])
+        ctx.rest = (ranges.q_len, ranges.k_len, scale, cap)
         return out, lse
 
     @staticmethod
@@ -179,9 +175,9 @@ class _Ranged(torch.autograd.Function):
         none = (None,) * 3
         if dout is None and dlse is None:
             return None, None, None, None, *none
-        q, k, v, slopes, out, lse, rows, tiles, order, held = ctx.saved_tensors
-        kv_len, q_len, k_len, scale, cap = ctx.rest
-        ranges = KeyRanges(rows, tiles, order, kv_len if held is None else held, q_len, k_len)
+        q, k, v, slopes, out, lse, *ranges = ctx.saved_tensors
+        q_len, k_len, scale, cap = ctx.rest
+        ranges = KeyRanges(*ranges, q_len, k_len)
         dev = q.device
         bsz, n, heads, d = q.shape
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
@@ -230,7 +226,8 @@ def ranged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ranges: 
     A row that sees nothing gets 0 and a log-sum-exp of ``-inf``, and gradients of 0. Differentiable once in ``q``, ``k``, ``v`` and
     ``slopes``, through both results; the gradient of a shared key head is the sum over its query heads. Sums and softmax
     statistics are fp32; weights, and scores' gradients, are rounded to bf16 once, for the products that they enter.
-    Sums run in a fixed order. Keys and values that none of 128 neighbouring rows sees are not read for them; a value that is
+    Sums run in a fixed order. Gradients are formed from the fp32 log-sum-exp, so they lose accuracy where scores pass 2^16 in
+    magnitude. Keys and values that none of 128 neighbouring rows sees are not read for them; a value that is
     not finite reaches, besides the rows that see it, rows that share its tile of 128 rows by 64 keys.
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or v.shape != k.shape:
@@ -246,15 +243,13 @@ def ranged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ranges: 
         raise ValueError(f"ranges of {ranges.rows.shape[0]} sequences, {ranges.q_len} rows and {ranges.k_len} keys do not fit "
                          f"{bsz}, {n} and {k.shape[1]}")
     sets = ranges.rows.shape[0]
-    shapes = ((sets, n, 4), (sets, -(-n // 64), 12), (sets, -(-n // 128) - (-k.shape[1] // 128)))
+    shapes = ((sets, n, 4), (sets, -(-n // 64), 12), (sets, -(-n // 128) - (-k.shape[1] // 128) + 1))
     if any(t.shape != s or t.dtype is not torch.int32 or not t.is_contiguous() for t, s in zip(ranges, shapes)):
         raise ValueError("ranges must be as key_ranges makes them")
     dp = padded_head_dim(d)
     scale, cap = check_scores(d, heads, scale, cap, slopes)
-    if isinstance(ranges.kv_len, torch.Tensor) and tuple(ranges.kv_len.shape) != (bsz,):
-        raise ValueError(f"ranges' kv_len is of {tuple(ranges.kv_len.shape)}, the batch of {bsz}")
     _lib.refuse_tangents(q, k, v, slopes)
-    _lib.require_gpu(q, k, v, slopes, *ranges[:3], ranges.kv_len if isinstance(ranges.kv_len, torch.Tensor) else None)
+    _lib.require_gpu(q, k, v, slopes, *ranges[:3])
     if d != dp:
         q, k, v = (torch.nn.functional.pad(t, (0, dp - d)) for t in (q, k, v))
     q, k, v = _ready(q), _ready(k), _ready(v)
