@@ -299,3 +299,77 @@ def test_a_decoding_step_captured():
             want = step(cache=before)
             assert all(torch.equal(x, y) for x, y in zip(got, want)), turn
             assert all(torch.equal(cache[x].view(torch.uint8), before[x].view(torch.uint8)) for x in ("k", "v", "k_scale", "k_block_sums"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attend_selected_on_an_8bit_cache(dtype):
+    """The choice and the attention in one call, with lengths past the cache too."""
+    cache, g = _filled(2, 700, 2, 128, 64, dtype, seed=14)
+    q = torch.randn(2, 3, 8, 128, generator=g).bfloat16().to(DEV)
+    for lens in ([700, 130], [705, 2]):
+        out, lse, chosen = W.attend_selected(q, cache, _i32(lens), topk=4, local_blocks=2)
+        want = W.select_key_blocks(q, cache["k_block_sums"], _i32([min(x, 700) for x in lens]), block_size=64, topk=4, local_blocks=2)
+        assert torch.equal(chosen.index, want.index) and torch.equal(chosen.num, want.num)
+        _check_attention((out, lse), q, cache, lens, chosen=chosen)
+    with pytest.raises(ValueError, match="scale must be above 0"):
+        W.attend_selected(q, cache, 700, topk=4, scale=-1.0)
+
+
+def test_a_cache_whose_offsets_pass_32_bits():
+    """Codes behind 2^31 bytes and 2^32: written, read and attended to at the far end, alone and as a chunk."""
+    cap, hk, d = (1 << 25) // 8 + 300, 8, 128
+    g = torch.Generator().manual_seed(15)
+    cache = W.new_cache_8bit(1, cap, hk, d)
+    n = 200
+    k, v = (torch.randn(1, n, hk, d, generator=g).bfloat16().to(DEV) for _ in range(2))
+    start = cap - n - 11
+    W.kv_append_8bit(cache, k, v, _i32([start]))
+    first = start // 64 * 64
+    small = W.new_cache_8bit(1, cap - first, hk, d)
+    W.kv_append_8bit(small, k, v, start - first)
+    for x, y in zip(W.kv_read_8bit(cache, first, cap - first), W.kv_read_8bit(small, 0, cap - first)):
+        assert torch.equal(x, y)
+    for rows in (2, 80):
+        q = torch.randn(1, rows, hk, d, generator=g).bfloat16().to(DEV)
+        far = W.attend_8bit(q, cache, _i32([start + n]), window=64)
+        near = W.attend_8bit(q, small, start - first + n, window=64)
+        assert torch.equal(far[1], near[1]) or (far[1] - near[1]).abs().max() <= 2.0 ** -10
+        assert ((far[0] - near[0]).abs().float() <= 2.0 ** -5).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,h", [(1, 17), (4, 8), (8, 8), (16, 4), (64, 1), (65, 1)])
+def test_every_number_of_rows(dtype, d, n, h):
+    """Units of one, two and four row tiles, full and not, several of them, and the chunk."""
+    cache, g = _filled(1, 310, 1, d, 64, dtype, seed=n * h)
+    q = torch.randn(1, n, h, d, generator=g).bfloat16().to(DEV)
+    for kw in ({}, dict(window=40, sink=35, cap=4.0)):
+        _check_attention(W.attend_8bit(q, cache, 301, **kw), q, cache, [301], **kw)
+
+
+def test_prompt_then_single_tokens():
+    """A model's use of it all: a packed training step's attention, its prompt into the cache, drafts that are taken back, single tokens
+    over all, some and the newest of the cache, against the same attention over the keys and values that the codes stand for."""
+    b, h, hk, d, n = 2, 4, 2, 64, 300
+    g = torch.Generator().manual_seed(20)
+    make = lambda m, heads: torch.randn(b, m, heads, d, generator=g).bfloat16().to(DEV)  # noqa: E731
+    q, k, v = make(n, h), make(n, hk), make(n, hk)
+    slopes = torch.tensor([0.1, 0.05, 0.02, 0.01], device=DEV)
+    lens = _i32([n, 211])
+    cache = W.new_cache_8bit(b, 400, hk, d)
+    W.kv_append_8bit(cache, k, v, 0, lengths=lens)
+    held = W.kv_read_8bit(cache, 0, n)
+    prompt = W.ranged_attention(q, *held, W.key_ranges(b, n, n, lengths=lens), cap=20.0, slopes=slopes)
+    chunk, _ = W.attend_8bit(q[:, -80:], cache, n, cap=20.0, slopes=slopes)      # the same tokens, as the chunk of a longer prompt
+    assert torch.equal(prompt[0, -80:], chunk[0])
+    drafts = make(4, hk), make(4, hk)
+    W.kv_append_8bit(cache, *drafts, lens)
+    for step in range(3):
+        new = make(1, hk), make(1, hk)
+        W.kv_append_8bit(cache, *new, lens + step)
+        at = (lens + step + 1).tolist()
+        one = make(1, h)
+        for kw in (dict(cap=20.0, slopes=slopes), dict(window=70, sink=4), dict(chosen=W.select_key_blocks(
+                one, cache["k_block_sums"], lens + step + 1, block_size=64, topk=3))):
+            _check_attention(W.attend_8bit(one, cache, lens + step + 1, **kw), one, cache, at, **kw)

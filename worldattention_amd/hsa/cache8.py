@@ -48,10 +48,6 @@ def new_cache_8bit(batch: int, cap: int, kv_heads: int, head_dim: int, *, block_
             "k_block_sums_block_size": block_size}
 
 
-def is_8bit(kv_cache: dict) -> bool:
-    return "k_scale" in kv_cache
-
-
 def _cache_args(c: dict):
     """``(wa_cache8, its tensors)``."""
     try:
@@ -78,6 +74,11 @@ def _cache_args(c: dict):
         raise ValueError("the cache's tensors must be contiguous, its codes on 16-byte addresses (they are read and written in place)")
     return _lib.Cache8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), _lib.ptr(sums), bsz, cap, hk, d, bs,
                        _CODES[k.dtype]), tensors
+
+
+def check_cache_8bit(kv_cache: dict) -> None:
+    """Refuse a dict that is not as :func:`new_cache_8bit` makes it."""
+    _cache_args(kv_cache)
 
 
 def _start(x, bsz: int, name: str):

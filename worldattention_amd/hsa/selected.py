@@ -195,12 +195,20 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
 def attend_selected(q: torch.Tensor, kv_cache: dict, kv_len: KvLen, *, topk: int, sink_blocks: int = 1,
                     local_blocks: int = 1, scale: Optional[float] = None):
     """``(out, lse, BlockSelection)``: :func:`select_key_blocks` and :func:`selected_attention` on a cache that
-    ``kv_append`` or ``cache_step`` keeps with a ``block_size`` (``kv_cache["k"]``, ``["v"]``, ``["k_block_sums"]``)."""
+    ``kv_append`` or ``cache_step`` keeps with a ``block_size`` (``kv_cache["k"]``, ``["v"]``, ``["k_block_sums"]``), or on an
+    8-bit one (:func:`~worldattention_amd.hsa.cache8.new_cache_8bit`), whose blocks
+    :func:`~worldattention_amd.hsa.cache8.attend_8bit` reads."""
     if "k_block_sums" not in kv_cache or "k_block_sums_block_size" not in kv_cache:
         raise ValueError("kv_cache keeps no k_block_sums: write it with kv_append(..., block_size=...)")
     k, v, sums = kv_cache["k"], kv_cache["v"], kv_cache["k_block_sums"]
     bs = int(kv_cache["k_block_sums_block_size"])
-    _check_cache(k, v)
+    eight = "k_scale" in kv_cache
+    if eight:
+        from .cache8 import attend_8bit, check_cache_8bit
+
+        check_cache_8bit(kv_cache)
+    else:
+        _check_cache(k, v)
     bsz, cap, hk, d = k.shape
     _check_query(q, hk, bsz, d, bs, kv_len)
     _check_sums(sums, "k_block_sums")
@@ -212,5 +220,7 @@ def attend_selected(q: torch.Tensor, kv_cache: dict, kv_len: KvLen, *, topk: int
     _lib.require_gpu(q, k, v, sums, kv_len if isinstance(kv_len, torch.Tensor) else None)
     q = _lib.kernel_ready(q)
     chosen = _select(q, sums, kv_len, bs, int(topk), int(sink_blocks), int(local_blocks), cap)
+    if eight:
+        return (*attend_8bit(q, kv_cache, kv_len, scale=scale or None, chosen=chosen), chosen)
     out, lse = _attend(q, k, v, chosen.index, chosen.num, kv_len, bs, scale)
     return out, lse, chosen
