@@ -16,7 +16,7 @@ import torch
 
 from .. import _lib
 from .ranged import _count, _forward, _make_ranges, check_scores
-from .selected import BlockSelection, KvLen, _no_gradient
+from .selected import BlockSelection, KvLen
 
 __all__ = ["new_cache_8bit", "kv_append_8bit", "kv_read_8bit", "attend_8bit"]
 
@@ -46,6 +46,12 @@ def new_cache_8bit(batch: int, cap: int, kv_heads: int, head_dim: int, *, block_
     return {"k": codes(), "v": codes(), "k_scale": scales(), "v_scale": scales(),
             "k_block_sums": torch.zeros((batch, kv_heads, blocks, head_dim), dtype=torch.float32, device=device),
             "k_block_sums_block_size": block_size}
+
+
+def _no_gradient(*tensors) -> None:
+    _lib.refuse_tangents(*tensors)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("an 8-bit cache takes no gradient: call it under torch.no_grad(), or train with ranged_attention")
 
 
 def _cache_args(c: dict):
@@ -192,7 +198,7 @@ def attend_8bit(q: torch.Tensor, kv_cache: dict, kv_len: KvLen, *, scale: Option
         index, num, topk = index.contiguous(), num.contiguous(), index.shape[3]
     elif sink and not window:
         raise ValueError("sink needs a window (without one every token is seen)")
-    _no_gradient(q, slopes) if slopes is not None else _no_gradient(q)
+    _no_gradient(q, slopes)
     dev = _lib.require_gpu(*tensors, q, slopes, lens, index, num)
     slopes = None if slopes is None else slopes.contiguous()
     if q.numel() == 0:
