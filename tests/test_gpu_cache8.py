@@ -348,6 +348,19 @@ def test_every_number_of_rows(dtype, d, n, h):
         _check_attention(W.attend_8bit(q, cache, 301, **kw), q, cache, [301], **kw)
 
 
+@pytest.mark.parametrize("b,n,h,hk,d,cap,kw", [
+    (2, 1, 4, 2, 128, 4000, {}), (37, 1, 4, 2, 64, 3000, {}), (37, 3, 10, 1, 128, 3000, dict(window=1500, sink=70, cap=9.0)), (5, 2, 21, 3, 64, 2900, {}),
+    (256, 1, 2, 1, 64, 900, dict(window=500)), (257, 1, 2, 1, 64, 900, {}), (9, 8, 8, 1, 128, 2500, {}), (3, 1, 16, 16, 64, 2048, {})])
+def test_ragged_sequences(b, n, h, hk, d, cap, kw):
+    """Tiles shared along all sequences: none, one, the cache's whole length and more, and many in a row that see nothing."""
+    cache, g = _filled(b, cap, hk, d, 64, torch.int8, seed=b + n)
+    q = torch.randn(b, n, h, d, generator=g).bfloat16().to(DEV)
+    lens = torch.randint(0, cap + 1, (b,), generator=g).tolist()
+    some = [0, cap + 5, 1, cap][:b]
+    for lens in (lens, some + [0] * (b - len(some)), [0] * (b - 1) + [cap], [0] * b, [cap] * b, [-3, 31] + [33] * (b - 2)):
+        _check_attention(W.attend_8bit(q, cache, _i32(lens), **kw), q, cache, [min(max(x, 0), cap) for x in lens], **kw)
+
+
 def test_prompt_then_single_tokens():
     """A model's use of it all: a packed training step's attention, its prompt into the cache, drafts that are taken back, single tokens
     over all, some and the newest of the cache, against the same attention over the keys and values that the codes stand for."""

@@ -28,9 +28,24 @@ struct AttendParams {
   const float* slopes;
   int n, H, Hk, nb, shift;        // shift: log2 of a block's tokens
   int units, parts, per;          // row units of (sequence, key head, with lists: query); parts of a unit, tiles of a part
+  int even;                       // workgroups of a key head that run at once and share all sequences' tiles evenly, or 0: units are cut
+  int B;
   Bend bend;
-  float* part;                    // [unit][part][16 RT][D + 2]: maximum, sum, outputs
+  float* part;                    // [unit][part] or, evenly, [workgroup][2], [16 RT][D + 2]: maximum, sum, outputs
 };
+
+// Tiles of a workgroup, of `all` that workgroups share of which `at_once` run at a time: at least two a wave and as many for each of the four. Beyond
+// 64 they come in rounds, up to 8 of them: workgroups that start as others end even out what the memory gives each (32 sequences of 32,760 tokens, 8 key
+// heads: 8 rounds of 64 tiles 392 us, two of 256 or one of 512 430; 4 sequences: one round of 64 61 us, 8 rounds of 8 85).
+constexpr int64_t kRounds = 8;
+// So many neighbouring workgroups take one key head's tiles, then as many the next head's: an XCD, which gets every eighth, works on all
+// heads (32 ragged sequences: 204 us; with a head on each XCD 224, with turns of 8 and 64 207 and 208).
+constexpr int kTurn = 16;
+__host__ __device__ __forceinline__ int share(int64_t all, int64_t at_once) {
+  const int64_t rounds = (all + 64 * at_once - 1) / (64 * at_once), n = at_once * (rounds < 1 ? 1 : rounds > kRounds ? kRounds : rounds);
+  const int64_t each = (all + n - 1) / n;
+  return each < 8 ? 8 : (int)((each + 3) & ~(int64_t)3);
+}
 
 constexpr float kLowest = -3.4028234e38f;   // running maximum before the first key: below every score, and no difference of it is NaN
 constexpr float kSlack = 8.f;               // log2 of the growth that the running maximum lets pass
@@ -59,37 +74,46 @@ struct Unit {
   int b, hk, i0, row0, rows, tiles;   // first query (with lists), first row, rows; tiles in all
   int n0, s1;                         // without lists: the first n0 tiles, then those from s1 on
   int64_t len;
+  __device__ __forceinline__ void held(const AttendParams& p) {
+    const int64_t x = p.kv_len ? (int64_t)p.kv_len[b] : p.kv_len_all;
+    len = min(max(x, (int64_t)0), p.cap);
+  }
+  // Tiles that rows at positions t0 .. t1 see.
+  __device__ __forceinline__ void walk(const AttendParams& p, int64_t t0, int64_t t1) {
+    const int end = (int)((t1 + 32) >> 5);          // tiles that the last row sees
+    if (t1 < 0) {
+      tiles = 0;
+    } else if (p.window > 0 && t0 - p.window + 1 > 0) {
+      n0 = (int)min((int64_t)end, (p.sink + 31) >> 5);
+      s1 = max(n0, (int)((t0 - p.window + 1) >> 5));
+      tiles = n0 + max(0, end - s1);
+    } else {
+      tiles = n0 = end;
+    }
+  }
+  // Tiles that a whole sequence's rows see (without lists).
+  __device__ __forceinline__ int of_sequence(const AttendParams& p, int sequence) {
+    b = sequence;
+    held(p);
+    walk(p, len - p.n, len - 1);
+    return tiles;
+  }
   template <int RT>
-  __device__ __forceinline__ void init(const AttendParams& p, int64_t u) {
-    const int G = p.H / p.Hk, of = p.index ? (G + 16 * RT - 1) / (16 * RT) : p.units;
-    // neighbouring workgroups take the key heads in turn: with eight of them each XCD's L2 sees one head's cache
-    hk = (int)(u % p.Hk);
-    u /= p.Hk;
+  __device__ __forceinline__ void init(const AttendParams& p, unsigned u) {
+    const int G = p.H / p.Hk;
+    const unsigned of = p.index ? (G + 16 * RT - 1) / (16 * RT) : p.units;
+    hk = (int)(u % (unsigned)p.Hk);
+    u /= (unsigned)p.Hk;
     const int chunk = (int)(u % of);
     u /= of;
-    i0 = p.index ? (int)(u % p.n) : 0;
-    b = (int)(p.index ? u / p.n : u);
+    i0 = p.index ? (int)(u % (unsigned)p.n) : 0;
+    b = (int)(p.index ? u / (unsigned)p.n : u);
     row0 = 16 * RT * chunk;
     rows = min(16 * RT, (p.index ? G : p.n * G) - row0);
-    const int64_t held = p.kv_len ? (int64_t)p.kv_len[b] : p.kv_len_all;
-    len = min(max(held, (int64_t)0), p.cap);
+    held(p);
     n0 = s1 = 0;
-    if (p.index) {
-      tiles = max(0, min(p.num[((int64_t)b * p.n + i0) * p.Hk + hk], p.topk)) << (p.shift - 5);
-    } else {
-      const int64_t t0 = len - p.n + row0 / G, t1 = len - p.n + (row0 + rows - 1) / G;   // the rows' positions
-      const int end = (int)((t1 + 32) >> 5);          // tiles that the last row sees
-      if (t1 < 0) {
-        tiles = 0;
-      } else if (p.window > 0 && t0 - p.window + 1 > 0) {
-        n0 = (int)min((int64_t)end, (p.sink + 31) >> 5);
-        s1 = max(n0, (int)((t0 - p.window + 1) >> 5));
-        tiles = n0 + max(0, end - s1);
-      } else {
-        tiles = n0 = end;
-      }
-    }
-    tiles = __builtin_amdgcn_readfirstlane(tiles);
+    if (p.index) tiles = max(0, min(p.num[((int64_t)b * p.n + i0) * p.Hk + hk], p.topk)) << (p.shift - 5);
+    else walk(p, len - p.n + row0 / G, len - p.n + (row0 + rows - 1) / G);
   }
   // Query and head (in its group) of row r of the unit.
   __device__ __forceinline__ int query(const AttendParams& p, int r) const { return p.index ? i0 : (row0 + r) / (p.H / p.Hk); }
@@ -111,14 +135,66 @@ __global__ void __launch_bounds__(256, D == 128 && RT == 4 ? 1 : 2) attend_kerne
   static_assert(NW * 4 * 32 * D >= NW * 16 * (D + 4) * 4, "the waves' outputs fit their drained rings");
   __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * 32 * D];   // of each wave two stages of keys and values; then the waves' outputs
   __shared__ float sm[NW][16], sl[NW][16];
+  __shared__ int s_wave[NW], s_end[256], s_seq;   // where each sequence's tiles end
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, kg = lane >> 4;
-  const int64_t u = blockIdx.x / p.parts;
-  const int part = (int)(blockIdx.x % p.parts);
+  unsigned u;
+  int64_t slot;
+  int t0, t1, head = 0, turn = 0, upto = 0, seq = 0;   // upto: where this workgroup's tiles end among those of all sequences
+  if (p.even) {
+    // Where this workgroup's tiles begin: a sequence a lane, their tiles summed over the workgroup.
+    Unit x;
+    const int mine = tid < p.B ? x.of_sequence(p, tid) : 0;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int below = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += below;
+    }
+    if (lane == 63) s_wave[w] = sum;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int y = 0; y < NW; ++y) {
+      if (y < w) sum += s_wave[y];
+      all += s_wave[y];
+    }
+    const int per = share(all, p.even);
+    const unsigned next = blockIdx.x / kTurn;
+    head = (int)(next % (unsigned)p.Hk);
+    turn = (int)(next / (unsigned)p.Hk * kTurn + blockIdx.x % kTurn);
+    const int64_t at = (int64_t)turn * per;
+    if (at >= all) return;
+    const int begin = (int)at;
+    s_end[tid] = sum;
+    if (begin < sum && begin >= sum - mine) s_seq = tid;
+    __syncthreads();
+    seq = __builtin_amdgcn_readfirstlane(s_seq);
+    upto = (int)min(at + per, (int64_t)all);
+    t0 = begin - (seq ? s_end[seq - 1] : 0);
+  } else {
+    u = blockIdx.x / p.parts;
+    t0 = (int)(blockIdx.x % p.parts) * p.per;
+  }
+  for (bool more = true; more;) {
   Unit unit;
-  unit.init<RT>(p, u);
-  const int t0 = part * p.per, t1 = min(unit.tiles, t0 + p.per);
-  if (t0 >= t1 && part > 0) return;
-  const bool alone = unit.tiles <= p.per;
+  bool alone;
+  if (p.even) {
+    u = (unsigned)seq * p.Hk + head;
+    unit.init<RT>(p, u);
+    unit.tiles = __builtin_amdgcn_readfirstlane(unit.tiles);
+    const int before = __builtin_amdgcn_readfirstlane(seq ? s_end[seq - 1] : 0);
+    t0 = __builtin_amdgcn_readfirstlane(t0);
+    t1 = min(unit.tiles, upto - before);
+    alone = t0 == 0 && t1 == unit.tiles;
+    slot = 2 * ((int64_t)turn * p.Hk + head) + (t0 == 0);   // one sequence at most began before this workgroup's tiles, and one that begins there goes on behind
+  } else {
+    unit.init<RT>(p, u);
+    unit.tiles = __builtin_amdgcn_readfirstlane(unit.tiles);
+    t1 = min(unit.tiles, t0 + p.per);
+    if (t0 >= t1 && t0 > 0) return;
+    alone = unit.tiles <= p.per;
+    slot = blockIdx.x;
+  }
   const int b = unit.b, hk = unit.hk, window = (int)p.window, sink = (int)p.sink;
 
   bf16x8 q[RT][KC];
@@ -361,7 +437,7 @@ __global__ void __launch_bounds__(256, D == 128 && RT == 4 ? 1 : 2) attend_kerne
       if (alone) {
         write_row(p, b, unit.query(p, 16 * x + r), unit.head(p, 16 * x + r), d, sum, top, all);
       } else {
-        float* at = p.part + ((u * p.parts + part) * 16 * RT + 16 * x + r) * (D + 2);
+        float* at = p.part + (slot * 16 * RT + 16 * x + r) * (D + 2);
         at[2 + d] = sum;
         if (d == 0) {
           at[0] = top;
@@ -370,33 +446,69 @@ __global__ void __launch_bounds__(256, D == 128 && RT == 4 ? 1 : 2) attend_kerne
       }
     }
   }
+  more = false;
+  if (p.even && t1 == unit.tiles) {   // on to the next sequence that sees a token
+    const int at = s_end[seq];
+    while (seq + 1 < p.B && s_end[seq + 1] == at) ++seq;
+    ++seq;
+    t0 = 0;
+    more = at < upto;
+    __syncthreads();   // the outputs' places are the rings'
+  }
+  }
 }
 
 // The parts of units that have several, in their order: one wave per row.
 template <int D, int RT>
 __global__ void __launch_bounds__(256) join_kernel(AttendParams p, int64_t units) {
   const int lane = threadIdx.x & 63;
-  const int64_t x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), u = x / (16 * RT);
+  const unsigned x = blockIdx.x * 4 + (threadIdx.x >> 6), u = x / (16 * RT);
   const int r = (int)(x % (16 * RT));
   if (u >= units) return;
   Unit unit;
   unit.init<RT>(p, u);
-  if (r >= unit.rows || unit.tiles <= p.per) return;
-  const int n = (unit.tiles + p.per - 1) / p.per;
-  constexpr int64_t kPart = 16 * RT * (D + 2);
-  const float* at = p.part + (u * p.parts * 16 * RT + r) * (D + 2);
+  if (r >= unit.rows) return;
+  int n;
+  int64_t first, step, second;   // the parts' places: first, then second + step s
+  if (p.even) {
+    int before = 0, all = 0;
+    for (int y = lane; y < p.B; y += 64) {
+      Unit other;
+      const int tiles = other.of_sequence(p, y);
+      all += tiles;
+      before += y < unit.b ? tiles : 0;
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      before += __shfl_xor(before, d, 64);
+      all += __shfl_xor(all, d, 64);
+    }
+    const int per = share(all, p.even), from = before / per;
+    n = unit.tiles ? (before + unit.tiles - 1) / per - from + 1 : 0;
+    if (n == 1) return;
+    first = 2 * ((int64_t)from * p.Hk + unit.hk) + 1;
+    step = 2 * p.Hk;
+    second = first - 1;
+  } else {
+    if (unit.tiles <= p.per) return;
+    n = (unit.tiles + p.per - 1) / p.per;
+    first = second = (int64_t)u * p.parts;
+    step = 1;
+  }
+  auto place = [&](int s) { return p.part + ((s ? second + step * s : first) * 16 * RT + r) * (D + 2); };
   float top = kLowest;
-  for (int s = lane; s < n; s += 64) top = fmaxf(top, at[s * kPart]);
+  for (int s = lane; s < n; s += 64) top = fmaxf(top, place(s)[0]);
   top = wa_wave_max(top);
   float l = 0.f, o[D / 64];
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
 #pragma unroll 4
   for (int s = 0; s < n; ++s) {
-    const float f = __builtin_amdgcn_exp2f(at[s * kPart] - top);
-    l += at[s * kPart + 1] * f;
+    const float* at = place(s);
+    const float f = __builtin_amdgcn_exp2f(at[0] - top);
+    l += at[1] * f;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] += at[s * kPart + 2 + lane + 64 * e] * f;
+    for (int e = 0; e < D / 64; ++e) o[e] += at[2 + lane + 64 * e] * f;
   }
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) write_row(p, unit.b, unit.query(p, r), unit.head(p, r), lane + 64 * e, o[e], top, l);
@@ -406,7 +518,11 @@ __global__ void __launch_bounds__(256) join_kernel(AttendParams p, int64_t units
 struct Cut {
   int rt, units_of;
   int64_t units;
-  int per, parts;
+  int per, parts;      // tiles of a part, parts of a unit; or,
+  int even;            // with sequences cut evenly, workgroups of a key head at once
+  int64_t most, heads; // and in all at most
+  int64_t grid() const { return even ? most * heads : units * parts; }
+  int64_t slots() const { return even ? 2 * grid() : parts > 1 ? units * parts : 0; }
 };
 
 bool sized(const wa_kv8_attend_args& a) {
@@ -427,21 +543,27 @@ Cut cut(const wa_kv8_attend_args& a) {
   // at most: the sinks', and from the first row's window to the last row, each run with a partial tile at either end
   const int64_t seen = a.window > 0 ? std::min(tokens, std::min(a.sink, tokens) + std::min(a.window, tokens) + a.n + 128) : tokens;
   const int64_t tiles = a.index ? a.topk * (a.cache.block_size / 32) : (seen + 31) / 32;
-  // parts of at least 8 tiles (two a wave), about 4,096 workgroups where there is work for them: ragged sequences even out
-  const int64_t want = std::max<int64_t>(1, 4096 / c.units);
-  c.per = (int)std::max<int64_t>(8, (tiles + want - 1) / want);
+  // workgroups that run at once: what the kernels' registers leave of four a CU (D = 64) or, with their codes' stages, two
+  const int64_t at_once = a.cache.D == 128 ? (c.rt == 4 ? 256 : 512) : c.rt == 1 ? 1024 : c.rt == 2 ? 768 : 512;
+  c.per = (int)std::min<int64_t>(share(c.units * tiles, at_once), std::max<int64_t>(8, tiles));
   c.parts = (int)std::max<int64_t>(1, (tiles + c.per - 1) / c.per);
+  // Sequences of lengths that only the GPU knows: cut along all of them, so that workgroups bring as much each (ragged ones of up to 32,768 tokens,
+  // 32 of them, 8 key heads: 204 us; cut by the cache's length into parts of 64 tiles 268).
+  c.heads = a.cache.Hk;
+  const bool ragged = a.kv_len && !a.index && of == 1 && a.cache.B > 1 && a.cache.B <= 256 && c.heads <= at_once;
+  c.even = ragged && a.cache.B * tiles <= INT32_MAX ? (int)(at_once / c.heads) : 0;
+  c.most = (std::min<int64_t>(kRounds * c.even, a.cache.B * tiles / 64 + c.even) + kTurn - 1) / kTurn * kTurn;
   return c;
 }
 
 template <typename Code, int D>
 void launch(const AttendParams& p, const Cut& c, hipStream_t s) {
-  const dim3 grid((unsigned)(c.units * c.parts)), block(256);
+  const dim3 grid((unsigned)c.grid()), block(256);
   const dim3 rows((unsigned)((c.units * 16 * c.rt + 3) / 4));
   if (c.rt == 1) hipLaunchKernelGGL((attend_kernel<Code, D, 1>), grid, block, 0, s, p);
   else if (c.rt == 2) hipLaunchKernelGGL((attend_kernel<Code, D, 2>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((attend_kernel<Code, D, 4>), grid, block, 0, s, p);
-  if (c.parts == 1) return;
+  if (!c.slots()) return;
   if (c.rt == 1) hipLaunchKernelGGL((join_kernel<D, 1>), rows, block, 0, s, p, c.units);
   else if (c.rt == 2) hipLaunchKernelGGL((join_kernel<D, 2>), rows, block, 0, s, p, c.units);
   else hipLaunchKernelGGL((join_kernel<D, 4>), rows, block, 0, s, p, c.units);
@@ -452,7 +574,7 @@ void launch(const AttendParams& p, const Cut& c, hipStream_t s) {
 extern "C" int64_t wa_kv8_attend_workspace_bytes(const wa_kv8_attend_args* a) {
   if (!a || !sized(*a)) return 0;
   const Cut c = cut(*a);
-  return c.parts > 1 ? c.units * c.parts * 16 * c.rt * (a->cache.D + 2) * 4 : 0;
+  return c.slots() * 16 * c.rt * (a->cache.D + 2) * 4;
 }
 
 extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
@@ -472,8 +594,8 @@ extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
   WA_CHECK_ARG(a->scale >= 0.f && a->scale < INFINITY && (a->cap == 0.f || (a->cap >= 1e-6f && a->cap <= 1e6f && a->scale <= 1e30f)),
                "kv8_attend: scale must be finite and not below 0, cap 0 or 1e-6 .. 1e6 (with a scale of at most 1e30)");
   const Cut k = cut(*a);
-  WA_CHECK_ARG(k.units * k.parts <= INT32_MAX && k.units * 16 * k.rt / 4 <= INT32_MAX, "kv8_attend: too many rows");
-  WA_CHECK_ARG(k.parts == 1 || a->workspace, "kv8_attend: a launch of %d parts needs a workspace", k.parts);
+  WA_CHECK_ARG(k.grid() <= INT32_MAX && k.units * k.parts <= INT32_MAX && k.units * 16 * k.rt / 4 <= INT32_MAX, "kv8_attend: too many rows");
+  WA_CHECK_ARG(!k.slots() || a->workspace, "kv8_attend: a launch of %d parts needs a workspace", k.parts);
   AttendParams p{};
   p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.o = (bf16_t*)a->o; p.o_sb = a->o_sb; p.o_st = a->o_st; p.o_sh = a->o_sh;
@@ -485,7 +607,7 @@ extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
   p.slopes = a->slopes;
   p.n = (int)a->n; p.H = (int)a->H; p.Hk = (int)c.Hk;
   p.nb = (int)((c.cap + c.block_size - 1) / c.block_size); p.shift = c.block_size == 64 ? 6 : 7;
-  p.units = k.units_of; p.parts = k.parts; p.per = k.per;
+  p.units = k.units_of; p.parts = k.parts; p.per = k.per; p.even = k.even; p.B = (int)c.B;
   const float scale = a->scale == 0.f ? 1.f / sqrtf((float)c.D) : a->scale;
   p.bend = bend_of(scale, a->cap);
   p.part = (float*)a->workspace;
