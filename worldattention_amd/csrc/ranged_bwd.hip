@@ -33,7 +33,7 @@ struct BwdParams {
   // workspace
   float* lse2;    // [B, H, Lq] log-sum-exp in units of log2; +inf where a row sees nothing: its weights come out 0
   float* on;      // [B, H, Lq] 1, or 0 where a row sees a single key: its weight is 1 whatever the score, and its dS exactly 0
-  float* delta;   // [B, H, Lq] delta * on
+  float* delta;   // [B, H, Lq] delta * on; from the output for dQ, which puts it right for dK
   float* slope_part;   // [H][B * q tiles]
   float* part_kv;      // [parts][dK, dV][B, Lk, Hk, D] fp32, with parts > 1
   int parts;
@@ -160,13 +160,17 @@ struct ColsProduct {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) read(rd, lds, a, i);
   }
-  __device__ __forceinline__ static void run(const TileReads<D>& rd, uint32_t lds, const bf16x8 (&b)[4], f32x16 (&acc)[DT], Operands& a) {
+  // B: one operand, or one and what its rounding left of it.
+  template <int B>
+  __device__ __forceinline__ static void run(const TileReads<D>& rd, uint32_t lds, const bf16x8 (&b)[B][4], f32x16 (&acc)[DT], Operands& a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (i + kAhead < N) read(rd, lds, a, i + kAhead);
       in_order();
 #pragma unroll
-      for (int y = 0; y < 2; ++y) acc[(2 * i + y) % DT] = wa_mfma32(a[i % (kAhead + 1)][y], b[(2 * i + y) / DT], acc[(2 * i + y) % DT]);
+      for (int z = 0; z < B; ++z)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) acc[(2 * i + y) % DT] = wa_mfma32(a[i % (kAhead + 1)][y], b[z][(2 * i + y) / DT], acc[(2 * i + y) % DT]);
       in_order();
     }
   }
@@ -190,14 +194,18 @@ __device__ __forceinline__ void put4(bf16x8& a, int x, const float (&f)[4]) {
   }
 }
 
-
 // Top of a step: this wave's tile loads have landed and its LDS reads returned, then the workgroup's.
 __device__ __forceinline__ void step_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // ---------------------------------------------------------------------------------------------
 // dQ: one workgroup of four waves per 128 rows of a head over the 64-key steps that they see; K and V through two LDS stages each, a row
-// a lane. SLOPES: the slope's gradient besides, from sums over the row's keys of P, P dP, P dist and P dP dist in fp32: with them delta is
-// the row's own sum of P dP instead of one from the rounded output.
+// a lane. delta comes from the output, whose weights and self are rounded to bf16, and is off by 2^-9 / sqrt(keys that count); the rows' sums of
+// dS, which delta makes the log-sum-exp's gradient, tell by how much: delta is put right for the launch behind, which forms dK, and for the
+// slopes' gradients (SLOPES: sums of dS dist and P dist besides). dQ itself takes dS in two bf16 parts, of 16 bits together, so that
+// its only other rounding is its own: one product in four more. Rows of few keys: 2.8e-3 from the exact dQ and dK with one part and the
+// output's delta, 2.4e-3 so (of norms; 1.7e-3 is the results' rounding). 4,680 tokens in 3 frames, 12 heads of 128: dQ 230 us (one
+// part 187); packed documents of 8,190 tokens in all, 16 heads, capped: 152 us (134). A second part only where a weight is above 1/8 cost more
+// in registers than it saved.
 // ---------------------------------------------------------------------------------------------
 template <int D, bool BENT, bool SLOPES>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ranged_dq_kernel(BwdParams p) {
@@ -248,7 +256,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   f32x16 dqacc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) dqacc[t] = f32x16{};
-  float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;   // sums of P, P dP, P dP dist, P dist
+  float left = 0.f, a2 = 0.f, a3 = 0.f;   // sums of dS (before the cap's factor), of dS dist and P dist
 
   RT kt, vt;
   kt.init(p.k_st, w, lane);
@@ -262,16 +270,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   };
   TileReads<D> rd;
   rd.init(lane);
-  auto slopes_of = [&](float pr, float dp, float dist) {
-    const float pd = pr * dp, far = fabsf(dist);
-    a0 += pr;
-    a1 += pd;
-    a2 = fmaf(pd, far, a2);
-    a3 = fmaf(pr, far, a3);
-  };
-  // 32 keys at a time: S^T = K Q^T and dP^T = V dO^T in turn, then dS^T = P^T (dP^T - delta), packed in accumulator order for the next product
+  // 32 keys at a time: S^T = K Q^T and dP^T = V dO^T in turn, then dS^T = P^T (dP^T - delta) and what its rounding leaves, packed in accumulator
+  // order for the next product
   // (both halves' products first, their exponentials after, took 64 more registers than there are).
-  auto half = [&](uint32_t kc, uint32_t vc, int x, int key0, int end, bool whole, bf16x8* dsb) {
+  auto half = [&](uint32_t kc, uint32_t vc, int x, int key0, int end, bool whole, bf16x8* dsb, bf16x8* rest) {
     f32x16 s, dp;
     Operands a;
     auto read = [&](int c) {
@@ -293,31 +295,38 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
       const float far = (float)(key0 - pos);
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        float out[4], pr[4], d[4];
+        float out[4], pr[4], turn[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 4 * r4 + i;
-          float turn = 1.f;
-          d[i] = dp[r];
-          if constexpr (BENT) pr[i] = __builtin_amdgcn_exp2f(bend.bent<decltype(form)::value>(s[r], far + (float)(8 * r4 + i), turn) - lse2);
+          turn[i] = 1.f;
+          if constexpr (BENT) pr[i] = __builtin_amdgcn_exp2f(bend.bent<decltype(form)::value>(s[r], far + (float)(8 * r4 + i), turn[i]) - lse2);
           else pr[i] = __builtin_amdgcn_exp2f(fmaf(s[r], bend.scale2, -lse2));
-          out[i] = pr[i] * fmaf(d[i], on, -dl);
-          if constexpr (BENT) out[i] *= turn;
         }
         if (!whole) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool seen = mine.sees(key0 + 8 * r4 + i);
-            out[i] = seen ? out[i] : 0.f;
-            pr[i] = seen ? pr[i] : 0.f;
-            d[i] = seen ? d[i] : 0.f;
-          }
+          for (int i = 0; i < 4; ++i) pr[i] = mine.sees(key0 + 8 * r4 + i) ? pr[i] : 0.f;
         }
+        // products that are 0 where the weight is: what a masked key holds, NaN too, reaches nothing
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = zero_mul(pr[i], fmaf(dp[4 * r4 + i], on, -dl));
+        left += (out[0] + out[1]) + (out[2] + out[3]);
         if constexpr (SLOPES) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) slopes_of(pr[i], d[i], far + (float)(8 * r4 + i));
+          for (int i = 0; i < 4; ++i) {
+            const float dist = fabsf(far + (float)(8 * r4 + i));
+            a2 = fmaf(out[i], dist, a2);
+            a3 = fmaf(pr[i], dist, a3);
+          }
+        }
+        if constexpr (BENT) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) out[i] = zero_mul(out[i], turn[i]);
         }
         put4(dsb[r4 >> 1], r4 & 1, out);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] -= (float)dsb[r4 >> 1][4 * (r4 & 1) + i];
+        put4(rest[r4 >> 1], r4 & 1, out);
         if constexpr (BENT) in_order();
       }
     };
@@ -337,27 +346,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
     if (t + 1 < st.total) issue(t & 1 ? kv0 : kv1, t + 1);   // the stage of step t - 1
     const int key = st.key(t), end = st.end(t);
     const bool whole = st.whole(key, end);
-    bf16x8 dsb[4];
-    half(kc, vc, 0, key + 4 * g, end, whole, dsb);
-    half(kc, vc, 1, key + 32 + 4 * g, end, whole, dsb + 2);
+    bf16x8 dsb[2][4];
+    half(kc, vc, 0, key + 4 * g, end, whole, dsb[0], dsb[1]);
+    half(kc, vc, 1, key + 32 + 4 * g, end, whole, dsb[0] + 2, dsb[1] + 2);
     // dQ^T[d, q] += K^T dS^T: A by transpose reads, B from registers (a row a lane)
     Operands a;
     ColsProduct<D>::first(rd, kc, a);
     ColsProduct<D>::run(rd, kc, dsb, dqacc, a);
   }
+  // P (dP - delta) sums to the log-sum-exp's gradient: what it is beside that is delta's own error, from the rounded output
+  left += __shfl_xor(left, 32, 64);
+  const float off = on > 0.f ? left - (p.dlse ? p.dlse[srow + row] : 0.f) : 0.f;
+  if (q_ok && g == 0) p.delta[srow + row] = dl + off;
   if constexpr (SLOPES) {
-    a0 += __shfl_xor(a0, 32, 64);
-    a1 += __shfl_xor(a1, 32, 64);
     a2 += __shfl_xor(a2, 32, 64);
     a3 += __shfl_xor(a3, 32, 64);
-    // the log-sum-exp's gradient shifts delta: it is what the rows' delta holds beyond the output's
-    float mine = 0.f;
-    if (a0 > 0.f) {
-      const float shift = p.dlse ? p.dlse[srow + row] : 0.f;
-      mine = on > 0.f ? a2 - (a1 / a0 - shift) * a3 : shift * a3;
-    } else if (a0 != a0) {
-      mine = a0;
-    }
+    const float mine = a2 - off * a3;
     float sum = g == 0 ? mine : 0.f;
     sum = wa_wave_sum(sum);
     if (lane == 0) s_part[w] = sum;
@@ -548,7 +552,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
           issue(t + 2);
           ColsProduct<D>::first(rd, dc, a);   // under the exponentials
           in_order();
-          bf16x8 ab[4];
+          bf16x8 ab[1][4];
           const bool whole = entry >> 20;
           auto weights = [&](auto form) {
             const float far = (float)(key - pos0 - row0 - 4 * g);
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
                 f16x4 p4;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p4[i] = (_Float16)(pr[i] * (BENT ? kLift * turn[i] : kLift));
-                put4(ab[x * 2 + (rq >> 1)], rq & 1, pr);
+                put4(ab[0][x * 2 + (rq >> 1)], rq & 1, pr);
                 s_p[t & 1][kg][x][rq][lane] = p4;
                 if (BENT || rq % 2) in_order();   // few rows' statistics in registers at a time
               }
@@ -604,7 +608,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
           const uint32_t qc = rd.address(s_q + (t & 3) * TILE);
           const float* st_dl = s_stats + (t & 3) * STATS + 64;
           const float* st_on = st_dl + 64;
-          bf16x8 ab[4];
+          bf16x8 ab[1][4];
           Operands a;
           ColsProduct<D>::first(rd, qc, a);
           in_order();
@@ -622,7 +626,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
                 // a product that is 0 where the weight is: what a masked key holds, NaN too, reaches nothing
                 ds[i] = zero_mul((float)p4[i], fmaf(dp[x][r], o4[i], -d4[i]));
               }
-              put4(ab[x * 2 + (rq >> 1)], rq & 1, ds);
+              put4(ab[0][x * 2 + (rq >> 1)], rq & 1, ds);
               if (rq % 2) in_order();
             }
           }
