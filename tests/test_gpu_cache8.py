@@ -361,6 +361,17 @@ def test_ragged_sequences(b, n, h, hk, d, cap, kw):
         _check_attention(W.attend_8bit(q, cache, _i32(lens), **kw), q, cache, [min(max(x, 0), cap) for x in lens], **kw)
 
 
+@pytest.mark.parametrize("n,h,hk", [(127, 1, 1), (128, 2, 2), (129, 1, 1), (32, 8, 2), (33, 8, 2), (43, 3, 1)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_around_the_number_of_rows_that_read_codes(n, h, hk, d):
+    cache, g = _filled(3, 420, hk, d, 64, torch.float8_e4m3fn, seed=n)
+    q = torch.randn(3, n, h, d, generator=g).bfloat16().to(DEV)
+    for kw in ({}, dict(window=70, sink=9, cap=6.0)):
+        lens = [420, n - 3, 131]
+        _check_attention(W.attend_8bit(q, cache, _i32(lens), **kw), q, cache, lens, **kw)
+        _check_attention(W.attend_8bit(q, cache, 300, **kw), q, cache, [300] * 3, **kw)
+
+
 def test_prompt_then_single_tokens():
     """A model's use of it all: a packed training step's attention, its prompt into the cache, drafts that are taken back, single tokens
     over all, some and the newest of the cache, against the same attention over the keys and values that the codes stand for."""
