@@ -971,7 +971,7 @@ typedef struct wa_kv8_append_args {
 int wa_kv8_append(const wa_kv8_append_args* args, void* stream);
 
 /* Tokens [start, start + n) as values, bf16 or fp32 k_out, v_out [B, n, Hk, D] (contiguous); 0 outside the cache. With
- * kv_len (device int32 [B]) or kv_len_all >= 0 only what `last` tokens at the sequence's end see under a window (0:
+ * kv_len (device int32 [B]; at most cap) or kv_len_all >= 0 only what `last` tokens at the sequence's end see under a window (0:
  * everything) with sinks is written; kv_len_all < 0 and no kv_len: everything. */
 typedef struct wa_kv8_read_args {
   wa_cache8 cache;

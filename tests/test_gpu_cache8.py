@@ -372,6 +372,20 @@ def test_around_the_number_of_rows_that_read_codes(n, h, hk, d):
         _check_attention(W.attend_8bit(q, cache, 300, **kw), q, cache, [300] * 3, **kw)
 
 
+@pytest.mark.parametrize("n", [2, 80])
+def test_lengths_past_the_cache_under_a_window(n):
+    """A length past the cache is the cache's, for what a long chunk reads back too: memory that is not written there holds NaN."""
+    b, h, hk, d, cap = 3, 4, 2, 64, 500
+    cache, g = _filled(b, cap, hk, d, 64, torch.int8, seed=41)
+    q = torch.randn(b, n, h, d, generator=g).bfloat16().to(DEV)
+    for kw in (dict(window=30), dict(window=30, sink=7)):
+        for lens, x in (([cap + 40, 400, cap + 5000], None), ([cap + 100] * b, cap + 100)):
+            waste = [torch.full((b, cap, hk, d), math.nan, dtype=torch.bfloat16, device=DEV) for _ in range(4)]
+            del waste
+            got = W.attend_8bit(q, cache, _i32(lens) if x is None else x, **kw)
+            _check_attention(got, q, cache, [min(y, cap) for y in lens], **kw)
+
+
 def test_prompt_then_single_tokens():
     """A model's use of it all: a packed training step's attention, its prompt into the cache, drafts that are taken back, single tokens
     over all, some and the newest of the cache, against the same attention over the keys and values that the codes stand for."""

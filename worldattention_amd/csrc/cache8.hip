@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
   const unsigned row = u >> shift, i = row / (unsigned)p.Hk, h = row % (unsigned)p.Hk, c0 = (u & ((1u << shift) - 1)) * 16;
   const int64_t t = per_sequence(p.start, p.start_all, b) + i;
   if (p.kv_len || p.kv_len_all >= 0) {
-    const int64_t len = per_sequence(p.kv_len, p.kv_len_all, b);
+    const int64_t len = min(per_sequence(p.kv_len, p.kv_len_all, b), p.cap);   // as the attention takes it
     if (t >= len || (p.window > 0 && t >= p.sink && t <= len - p.last - p.window)) return;
   }
   float f[16];
