@@ -184,6 +184,16 @@ def test_read_refuses(start, n, options):
         W.kv_read_8bit(cache(), start, n, **options)
 
 
+@pytest.mark.parametrize("far", [1 << 63, (1 << 64) + 5, -(1 << 64)])
+def test_numbers_that_64_bits_do_not_hold(far):
+    for call in (lambda: W.kv_read_8bit(cache(), far, 4), lambda: W.attend_8bit(zeros(2, 1, 4, 64), cache(), far),
+                 lambda: W.kv_append_8bit(cache(), zeros(2, 1, 2, 64), zeros(2, 1, 2, 64), far), lambda: W.key_ranges(1, 4, 4, kv_len=far),
+                 lambda: W.key_ranges(1, 4, 4, prefix=abs(far)), lambda: W.key_ranges(1, 4, 4, window=abs(far)),
+                 lambda: W.attend_8bit(zeros(2, 1, 4, 64), cache(), 9, window=abs(far))):
+        with pytest.raises(ValueError):
+            call()
+
+
 def lists(b=2, n=1, hk=2, topk=3, dtype=I32):
     return W.BlockSelection(torch.zeros(b, n, hk, topk, dtype=dtype), torch.zeros(b, n, hk, dtype=dtype))
 

@@ -11,8 +11,8 @@ namespace {
 // Rows are (query, head of the group) pairs of one key head; a unit of 16 RT rows walks its tiles of 32 keys once. A part of a unit (the
 // tiles that one workgroup takes) is shared by four waves, tile by tile, each with running maxima and sums of its own. A wave's codes stream through
 // two LDS stages of its own by direct loads, whole rows at a time: a stage is read into registers and filled again, two tiles on, before the tile is
-// used, so a CU has 128 KB on their way (one tile ahead in registers, 64 KB, and rows in halves: 32 ragged sequences of up to 32,768 tokens, 8 key heads,
-// 283 us). Codes become bf16 exactly; a block's scales are wave-uniform factors of the scores and of the weights (powers of two: the weights' rounding
+// used, so a CU has 128 KB on their way (one tile ahead in registers, 64 KB, and rows in halves: 283 us against 265 for 32 ragged sequences of up to
+// 32,768 tokens, 8 key heads, before they shared the workgroups evenly). Codes become bf16 exactly; a block's scales are wave-uniform factors of the scores and of the weights (powers of two: the weights' rounding
 // is that of the plain ones). Products are v_mfma_f32_16x16x32: S^T = K Q^T, O^T += V^T P^T; row a = 4 x + y of the former is key 4 y + x of
 // its 16, which puts value rows that are read together in different banks. Bound by reading the codes.
 // =============================================================================================
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(256, D == 128 && RT == 4 ? 1 : 2) attend_kerne
 
 // The parts of units that have several, in their order: one wave per row.
 template <int D, int RT>
-__global__ void __launch_bounds__(256) join_kernel(AttendParams p, int64_t units) {
+__global__ void __launch_bounds__(256) join_kernel(AttendParams p, unsigned units) {
   const int lane = threadIdx.x & 63;
   const unsigned x = blockIdx.x * 4 + (threadIdx.x >> 6), u = x / (16 * RT);
   const int r = (int)(x % (16 * RT));
@@ -564,9 +564,9 @@ void launch(const AttendParams& p, const Cut& c, hipStream_t s) {
   else if (c.rt == 2) hipLaunchKernelGGL((attend_kernel<Code, D, 2>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((attend_kernel<Code, D, 4>), grid, block, 0, s, p);
   if (!c.slots()) return;
-  if (c.rt == 1) hipLaunchKernelGGL((join_kernel<D, 1>), rows, block, 0, s, p, c.units);
-  else if (c.rt == 2) hipLaunchKernelGGL((join_kernel<D, 2>), rows, block, 0, s, p, c.units);
-  else hipLaunchKernelGGL((join_kernel<D, 4>), rows, block, 0, s, p, c.units);
+  if (c.rt == 1) hipLaunchKernelGGL((join_kernel<D, 1>), rows, block, 0, s, p, (unsigned)c.units);
+  else if (c.rt == 2) hipLaunchKernelGGL((join_kernel<D, 2>), rows, block, 0, s, p, (unsigned)c.units);
+  else hipLaunchKernelGGL((join_kernel<D, 4>), rows, block, 0, s, p, (unsigned)c.units);
 }
 
 }  // namespace
@@ -594,7 +594,7 @@ extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
   WA_CHECK_ARG(a->scale >= 0.f && a->scale < INFINITY && (a->cap == 0.f || (a->cap >= 1e-6f && a->cap <= 1e6f && a->scale <= 1e30f)),
                "kv8_attend: scale must be finite and not below 0, cap 0 or 1e-6 .. 1e6 (with a scale of at most 1e30)");
   const Cut k = cut(*a);
-  WA_CHECK_ARG(k.grid() <= INT32_MAX && k.units * k.parts <= INT32_MAX && k.units * 16 * k.rt / 4 <= INT32_MAX, "kv8_attend: too many rows");
+  WA_CHECK_ARG(k.grid() <= INT32_MAX && k.units * k.parts <= INT32_MAX && k.units * 16 * k.rt <= INT32_MAX, "kv8_attend: too many rows");
   WA_CHECK_ARG(!k.slots() || a->workspace, "kv8_attend: a launch of %d parts needs a workspace", k.parts);
   AttendParams p{};
   p.q = (const bf16_t*)a->q; p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;

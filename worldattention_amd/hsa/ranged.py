@@ -22,6 +22,7 @@ from .block_sparse import padded_head_dim
 __all__ = ["KeyRanges", "key_ranges", "ranged_attention"]
 
 _MOST = 1 << 30      # tokens of a sequence
+_FAR = 1 << 62       # of a whole number, which the kernels take in 64 bits
 
 
 class KeyRanges(NamedTuple):
@@ -36,7 +37,7 @@ class KeyRanges(NamedTuple):
 
 
 def _count(x, name: str, low: int) -> int:
-    if isinstance(x, bool) or int(x) != x or x < low:
+    if isinstance(x, bool) or int(x) != x or not low <= x <= _FAR:
         raise ValueError(f"{name} must be a whole number of at least {low}, got {x}")
     return int(x)
 
@@ -47,6 +48,8 @@ def _per_sequence(x, bsz: int, name: str):
         if tuple(x.shape) != (bsz,) or x.dtype is not torch.int32:
             raise ValueError(f"{name} must be an int or int32 [{bsz}], got {x.dtype} {tuple(x.shape)}")
         return x.contiguous(), 0
+    if abs(int(x)) > _FAR:
+        raise ValueError(f"{name} does not fit 64 bits: {x}")
     return None, int(x)
 
 
