@@ -1,7 +1,7 @@
 // Gradients of the ranged attention (ranged.hip). With P = exp(s - lse), dP = dO V^T and delta = rowsum(O dO) - dlse,
 //   dS = P (dP - delta),  dslope = -sum dS |t - j|,  dx = dS (1 - tanh^2),
 //   dQ = scale dx K,  dK = scale dx^T Q,  dV = P^T dO   (a shared key head: summed over its query heads).
-// Three launches: the rows' statistics, dQ (and the slopes'), dK and dV. The scores are formed again in each of the last two; that costs two
+// Two launches: dQ (with the rows' statistics, and the slopes' gradients), then dK and dV. The scores are formed again in each of the last two; that costs two
 // products more than forming them once, and needs neither atomics nor partial sums of dQ in memory.
 #include <algorithm>
 #include <type_traits>
@@ -38,39 +38,6 @@ struct BwdParams {
   float* part_kv;      // [parts][dK, dV][B, Lk, Hk, D] fp32, with parts > 1
   int parts;
 };
-
-// ---------------------------------------------------------------------------------------------
-// Rows' statistics: D / 8 lanes a row.
-// ---------------------------------------------------------------------------------------------
-template <int D>
-__global__ void __launch_bounds__(256) rows_kernel(BwdParams p, int64_t n_rows) {
-  constexpr int TPR = D / 8;
-  const int64_t u = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;   // (b, token, head): heads lie side by side
-  const int c0 = (threadIdx.x % TPR) * 8;
-  float s = 0.f;
-  int b = 0, i = 0, h = 0;
-  if (u < n_rows) {
-    h = (int)(u % p.H);
-    i = (int)(u / p.H % p.ranges.Lq);
-    b = (int)(u / p.H / p.ranges.Lq);
-    const bf16x8 o = *(const bf16x8*)(p.o + (int64_t)b * p.o_sb + (int64_t)i * p.o_st + (int64_t)h * p.o_sh + c0);
-    const bf16x8 d = *(const bf16x8*)(p.dout + (int64_t)b * p.d_sb + (int64_t)i * p.d_st + (int64_t)h * p.d_sh + c0);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf((float)o[e], (float)d[e], s);
-  }
-#pragma unroll
-  for (int m = TPR / 2; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
-  if (u < n_rows && threadIdx.x % TPR == 0) {
-    const int64_t r = ((int64_t)b * p.H + h) * p.ranges.Lq + i;
-    const int4 runs = p.ranges.row(b, i);
-    const bool one = (runs.y - runs.x) + (runs.w - runs.z) == 1;
-    const float l = p.lse[r], more = p.dlse ? p.dlse[r] : 0.f;
-    const bool none = l == -INFINITY;
-    p.lse2[r] = none ? INFINITY : l * WA_LOG2E;
-    p.on[r] = one ? 0.f : 1.f;
-    p.delta[r] = one || none ? (one && !none ? -more : 0.f) : s - more;
-  }
-}
 
 // A tile of 64 rows streamed into LDS by direct loads (tile.h's layout): rows from `rows` on read as zeros.
 template <int D, int NW>
@@ -229,20 +196,34 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   int4 runs = p.ranges.row(b, row);
   if (!q_ok) runs = int4{0, 0, 0, 0};
   bf16x8 qf[DC], dof[DC];
+  float dl = 0.f;
   {
     const bf16_t* qr = p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)row * p.q_st;
     const bf16_t* dr = p.dout + (int64_t)b * p.d_sb + (int64_t)h * p.d_sh + (int64_t)row * p.d_st;
+    const bf16_t* orow = p.o + (int64_t)b * p.o_sb + (int64_t)h * p.o_sh + (int64_t)row * p.o_st;
 #pragma unroll
     for (int c = 0; c < DC; ++c) {
       const bf16x8 a = *(const bf16x8*)(qr + c * 16 + g * 8);
       const bf16x8 d = *(const bf16x8*)(dr + c * 16 + g * 8);
+      const bf16x8 o = *(const bf16x8*)(orow + c * 16 + g * 8);
       qf[c] = q_ok ? a : bf16x8{};
       dof[c] = q_ok ? d : bf16x8{};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dl = fmaf((float)o[e], (float)d[e], dl);
     }
   }
+  dl += __shfl_xor(dl, 32, 64);
+  // The row's statistics, for the launch behind too: weights of a row that sees nothing come out 0, and of one that sees a single key 1 whatever
+  // its score, so that its dS is 0.
   const int64_t srow = ((int64_t)b * p.H + h) * p.ranges.Lq;
-  float lse2 = q_ok ? p.lse2[srow + row] : INFINITY;
-  float dl = q_ok ? p.delta[srow + row] : 0.f, on = q_ok ? p.on[srow + row] : 0.f;
+  const float lse = p.lse[srow + row], shift = p.dlse ? p.dlse[srow + row] : 0.f;
+  const bool none = !q_ok || lse == -INFINITY, one = (runs.y - runs.x) + (runs.w - runs.z) == 1;
+  float lse2 = none ? INFINITY : lse * WA_LOG2E, on = one || !q_ok ? 0.f : 1.f;
+  dl = none ? 0.f : one ? -shift : dl - shift;
+  if (q_ok && g == 0) {
+    p.lse2[srow + row] = lse2;
+    p.on[srow + row] = on;
+  }
   Bend bend = p.bend;
   int pos = 0;   // the row's position
   if (BENT && p.slopes) {
@@ -356,7 +337,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   }
   // P (dP - delta) sums to the log-sum-exp's gradient: what it is beside that is delta's own error, from the rounded output
   left += __shfl_xor(left, 32, 64);
-  const float off = on > 0.f ? left - (p.dlse ? p.dlse[srow + row] : 0.f) : 0.f;
+  const float off = on > 0.f && lse2 < INFINITY ? left - (p.dlse ? p.dlse[srow + row] : 0.f) : 0.f;
   if (q_ok && g == 0) p.delta[srow + row] = dl + off;
   if constexpr (SLOPES) {
     a2 += __shfl_xor(a2, 32, 64);
@@ -721,8 +702,7 @@ int kv_parts(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk) {
 
 template <int D, bool BENT>
 void launch_bwd(const BwdParams& p, hipStream_t s) {
-  const int64_t n_rows = (int64_t)p.B * p.H * p.ranges.Lq, nq = (p.ranges.Lq + 127) / 128;
-  hipLaunchKernelGGL((rows_kernel<D>), dim3((unsigned)((n_rows + 2048 / D - 1) / (2048 / D))), dim3(256), 0, s, p, n_rows);
+  const int64_t nq = (p.ranges.Lq + 127) / 128;
   const dim3 gq((unsigned)(p.B * p.H * nq)), gk((unsigned)((int64_t)p.B * p.Hk * ((p.ranges.Lk + kKeys - 1) / kKeys) * p.parts));
   if constexpr (BENT) {
     if (p.dslopes) {
