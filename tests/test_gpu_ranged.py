@@ -162,6 +162,16 @@ def test_caps_slopes_and_the_log_sum_exps_gradient(d, cap, slopes, dlse):
           dlse=torch.randn(b, h, n, generator=g).to(DEV) if dlse else None)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("part", [0.1, 0.29, 0.31, 0.49, 0.51, 1.5])
+def test_scores_at_parts_of_the_cap(d, part):
+    """The largest score at some part of the cap, on either side of where a tile's scores take another form of the tanh."""
+    b, n, h, hk = 1, 200, 2, 1
+    q, k, v, do = _inputs(b, n, n, h, hk, d, seed=44, size=1.5)
+    most = (torch.matmul(q.double().transpose(1, 2), k.double().transpose(1, 2).transpose(2, 3).contiguous()) * 0.2).abs().max().item()
+    check(q, k, v, do, _ranges(b, n, n, dict()), OR.seen(b, n, n), cap=most / part, scale=0.2)
+
+
 def test_given_runs_in_attention():
     """Any runs: rows that see nothing between rows that see much, runs that overlap, two far apart."""
     g = torch.Generator().manual_seed(9)

@@ -103,20 +103,21 @@ struct RowRuns {
 // Scores beyond the plain product, in units of log2: cap tanh(x / cap), x = scale s, less the distance's bias. Which form of the tanh is right for all of
 // a wave's scores is asked once for a tile:
 //   kBias   no cap;
-//   kNear   |x| <= cap / 2: tanh(z) = z P(z^2), P of degree 4 fitted to 1.5e-8 of the value (a weighted least-squares fit of tanh(z) / z on
-//           [0, 1/4] with the leading 1 kept), with the scale in its coefficients: six instructions, more exact than kFar and half its work;
+//   kClose  |x| <= 0.3 cap: tanh(z) = z P(z^2), P of degree 3 fitted to 1.2e-8 of the value (a weighted least-squares fit of tanh(z) / z on
+//           [0, 0.09] with the leading 1 kept), with the scale in its coefficients: five instructions (a chunk of 1,024 rows over 8,256 keys: 256 us, 275 with kNear);
+//   kNear   |x| <= cap / 2: the same of degree 4, on [0, 1/4] to 1.5e-8: six instructions, more exact than kFar and half its work;
 //   kFar    e = exp(2 z), r = 1 / (e + 1): tanh = 1 - 2 r, off by a few 2^-24 of the cap wherever z is (e = inf gives r = 0); its derivative
 //           4 e r r, off by a few 2^-24 of itself.
-enum BendForm { kBias, kNear, kFar };
+enum BendForm { kBias, kClose, kNear, kFar };
 struct Bend {
-  float near;                 // largest |s| for kNear (below 0: none; the coefficients' powers of the scale would leave fp32)
+  float close, near;          // largest |s| for kClose and kNear (below 0: none; the coefficients' powers of the scale would leave fp32)
   float scale2, in2, cap2;    // scale log2(e); 2 scale / cap log2(e); cap log2(e) or 0
-  float c[4], icap2;          // kNear's coefficients of s^2 and its powers; 1 / cap2
+  float c[4], c3[3], icap2;   // kNear's and kClose's coefficients of s^2 and its powers; 1 / cap2
   float slope2;               // slope log2(e)
   // The form for scores of at most `most`, the same in all of the wave's lanes.
   __device__ __forceinline__ BendForm form(float most) const {
     if (!(cap2 > 0.f)) return kBias;
-    return __any(most > near) ? kFar : kNear;
+    return !__any(most > close) ? kClose : __any(most > near) ? kFar : kNear;
   }
   // The score before the bias, and the cap's derivative there.
   template <BendForm FORM>
@@ -124,8 +125,9 @@ struct Bend {
     turn = 1.f;
     if constexpr (FORM == kBias) {
       return s * scale2;
-    } else if constexpr (FORM == kNear) {
-      const float u = s * s, y = s * fmaf(u, fmaf(u, fmaf(u, fmaf(u, c[3], c[2]), c[1]), c[0]), scale2), t = y * icap2;
+    } else if constexpr (FORM != kFar) {
+      const float u = s * s, p = FORM == kClose ? fmaf(u, fmaf(u, fmaf(u, c3[2], c3[1]), c3[0]), scale2) : fmaf(u, fmaf(u, fmaf(u, fmaf(u, c[3], c[2]), c[1]), c[0]), scale2);
+      const float y = s * p, t = y * icap2;
       turn = fmaf(-t, t, 1.f);
       return y;
     } else {
@@ -142,14 +144,18 @@ struct Bend {
 static inline Bend bend_of(float scale, float cap) {
   Bend b{};
   b.scale2 = scale * WA_LOG2E;
-  b.near = -1.f;
+  b.close = b.near = -1.f;
   if (cap > 0.f) {
     const float in = scale / cap, u = in * in;
     b.in2 = 2.f * in * WA_LOG2E;
     b.cap2 = cap * WA_LOG2E;
     b.icap2 = 1.f / b.cap2;
     if (in >= 0x1p-15f && in <= 0x1p15f) {   // powers up to the eighth, and |s| <= 2^14, stay normal
+      b.close = 0.3f / in;
       b.near = 0.5f / in;
+      b.c3[0] = -0x1.55549ep-2f * u * b.scale2;
+      b.c3[1] = 0x1.10b012p-3f * u * u * b.scale2;
+      b.c3[2] = -0x1.9c99a8p-5f * u * u * u * b.scale2;
       b.c[0] = -0x1.5554d6p-2f * u * b.scale2;
       b.c[1] = 0x1.10e9fcp-3f * u * u * b.scale2;
       b.c[2] = -0x1.b28c5ep-5f * u * u * u * b.scale2;
@@ -172,6 +178,7 @@ template <BendForm F> struct FormTag { static constexpr BendForm value = F; };
 template <typename Run>
 __device__ __forceinline__ void by_form(BendForm form, const Run& run) {
   if (form == kBias) run(FormTag<kBias>{});
+  else if (form == kClose) run(FormTag<kClose>{});
   else if (form == kNear) run(FormTag<kNear>{});
   else run(FormTag<kFar>{});
 }
