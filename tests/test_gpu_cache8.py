@@ -386,6 +386,35 @@ def test_lengths_past_the_cache_under_a_window(n):
             _check_attention(got, q, cache, [min(y, cap) for y in lens], **kw)
 
 
+def test_ragged_lengths_that_move_between_replays():
+    """Where a captured call's workgroups begin follows the lengths of each replay; two graphs in turn."""
+    b, cap, hk, d = 4, 4000, 2, 128
+    g = torch.Generator().manual_seed(51)
+    sets = []
+    for n, kw in ((1, {}), (3, dict(window=1200, sink=30))):
+        cache, _ = _filled(b, cap, hk, d, 64, torch.int8, seed=n)
+        q = torch.randn(b, n, 6, d, generator=g).bfloat16().to(DEV)
+        lens = _i32([5, 0, 4000, 900])
+        call = lambda cache=cache, q=q, lens=lens, kw=kw: W.attend_8bit(q, cache, lens, **kw)  # noqa: E731
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        sets.append((graph, got, call, cache, q, lens, kw))
+    for now in ([5, 0, 4000, 900], [0, 0, 0, 0], [4000, 4000, 4000, 4000], [1, 3999, 0, 64], [2000, 31, 33, 4005]):
+        for graph, got, call, cache, q, lens, kw in sets:
+            lens.copy_(_i32(now))
+            graph.replay()
+            torch.cuda.synchronize()
+            want = call()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), now
+            _check_attention(got, q, cache, [min(x, cap) for x in now], **kw)
+
+
 def test_prompt_then_single_tokens():
     """A model's use of it all: a packed training step's attention, its prompt into the cache, drafts that are taken back, single tokens
     over all, some and the newest of the cache, against the same attention over the keys and values that the codes stand for."""

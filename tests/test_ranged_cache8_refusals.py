@@ -321,6 +321,28 @@ def test_c_cache_entries_refuse(fn, bad):
     _refused(fn, _filled(cls, {**sizes, "cache": _cache8(), **bad}, optional))
 
 
+BIG = 1 << 40
+
+
+@pytest.mark.parametrize("fn,cls,sizes,optional", [
+    ("wa_ranged_fwd", _lib.RangedFwdArgs, {**ATTENTION, "B": BIG, "H": BIG}, ()),
+    ("wa_ranged_fwd", _lib.RangedFwdArgs, {**ATTENTION, "B": 1 << 20, "Lq": 1 << 30}, ()),
+    ("wa_ranged_bwd", _lib.RangedBwdArgs, {**ATTENTION, "B": BIG, "H": BIG}, ()),
+    ("wa_ranged_bwd", _lib.RangedBwdArgs, {**ATTENTION, "B": 1 << 20, "Lk": 1 << 30}, ()),
+    ("wa_key_ranges", _lib.KeyRangesArgs, dict(B=BIG, Lq=BIG >> 12, Lk=8, chunk=1, n_borders=2), ("given",)),
+    ("wa_key_ranges", _lib.KeyRangesArgs, dict(B=1 << 62, Lq=1 << 30, Lk=8, chunk=1, n_borders=2), ("given",)),
+    ("wa_kv8_append", _lib.Kv8AppendArgs, dict(dtype=_lib.WA_BF16, n=2, cache=_cache8(B=1 << 30, Hk=65536)), ("start",)),
+    ("wa_kv8_append", _lib.Kv8AppendArgs, dict(dtype=_lib.WA_BF16, n=1 << 30, cache=_cache8(B=1 << 20, cap=1 << 30)), ()),
+    ("wa_kv8_read", _lib.Kv8ReadArgs, dict(dtype=_lib.WA_BF16, n=1 << 30, cache=_cache8(Hk=32768)), ()),
+    ("wa_kv8_read", _lib.Kv8ReadArgs, dict(dtype=_lib.WA_BF16, n=2, cache=_cache8(B=65536)), ()),
+    ("wa_kv8_attend", _lib.Kv8AttendArgs, dict(n=1 << 24, H=65536, cache=_cache8(B=1 << 24, Hk=65536)), ("index", "num")),
+    ("wa_kv8_attend", _lib.Kv8AttendArgs, dict(n=1 << 24, H=65536, topk=4, cache=_cache8(B=1 << 24)), ()),
+    ("wa_kv8_attend", _lib.Kv8AttendArgs, dict(n=1 << 20, H=64, cache=_cache8(B=1 << 20)), ("index", "num")),
+])
+def test_c_entries_refuse_sizes_that_no_grid_holds(fn, cls, sizes, optional):
+    _refused(fn, _filled(cls, {**({"scale": 0.1} if "attend" in fn else {}), **sizes}, optional))
+
+
 @pytest.mark.parametrize("fn", ["wa_key_ranges", "wa_ranged_fwd", "wa_ranged_bwd", "wa_kv8_append", "wa_kv8_read", "wa_kv8_attend"])
 def test_c_entries_refuse_null(fn):
     assert getattr(_lib.lib(), fn)(None, None) == _lib.WA_ERR_ARG

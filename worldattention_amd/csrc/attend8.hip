@@ -528,7 +528,8 @@ struct Cut {
 bool sized(const wa_kv8_attend_args& a) {
   const wa_cache8& c = a.cache;
   return c.B >= 1 && a.n >= 1 && c.cap >= 1 && c.cap <= 1 << 30 && c.Hk >= 1 && a.H >= c.Hk && a.H % c.Hk == 0 && a.H <= 65536 && a.n <= 1 << 24 &&
-         c.B <= 1 << 24 && a.n * (a.H / c.Hk) <= INT32_MAX && a.window >= 0 && a.sink >= 0 &&
+         a.n * (a.H / c.Hk) <= INT32_MAX && c.B <= INT32_MAX / c.Hk &&
+         (a.index ? a.n * ((a.H / c.Hk + 15) / 16) : (a.n * (a.H / c.Hk) + 15) / 16) <= INT32_MAX / (c.B * c.Hk) && a.window >= 0 && a.sink >= 0 &&
          (!a.index || (a.topk >= 1 && a.topk <= WA_SELECT_MAX_BLOCKS && a.window == 0));
 }
 

@@ -198,7 +198,7 @@ int check_cache(const char* what, const wa_cache8& c) {
   WA_CHECK_ARG(c.D == 64 || c.D == 128, "%s: head dim must be 64 or 128, got %lld", what, (long long)c.D);
   WA_CHECK_ARG(c.block_size == 64 || c.block_size == 128, "%s: block size must be 64 or 128, got %lld", what, (long long)c.block_size);
   WA_CHECK_ARG(c.code == WA_CODE_INT8 || c.code == WA_CODE_E4M3, "%s: unknown code %d", what, c.code);
-  WA_CHECK_ARG(c.B >= 1 && c.Hk >= 1 && c.cap >= 1 && c.cap <= 1 << 30 && c.B <= INT32_MAX && c.Hk <= 65536, "%s: bad sizes B %lld cap %lld Hk %lld",
+  WA_CHECK_ARG(c.B >= 1 && c.Hk >= 1 && c.cap >= 1 && c.cap <= 1 << 30 && c.Hk <= 65536 && c.B <= INT32_MAX / c.Hk, "%s: bad sizes B %lld cap %lld Hk %lld",
                what, (long long)c.B, (long long)c.cap, (long long)c.Hk);
   WA_CHECK_ARG(c.k && c.v && c.k_scale && c.v_scale && wa_aligned16(c.k) && wa_aligned16(c.v), "%s: null or misaligned cache", what);
   return WA_OK;

@@ -523,7 +523,8 @@ extern "C" int64_t wa_ranged_fwd_workspace_bytes(int64_t B, int64_t H, int64_t, 
 extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   WA_CHECK_ARG(a, "ranged_fwd: null args");
   WA_CHECK_ARG(a->D == 64 || a->D == 128, "ranged_fwd: head dim must be 64 or 128, got %lld", (long long)a->D);
-  WA_CHECK_ARG(a->B >= 1 && a->Lq >= 1 && a->Lk >= 1 && a->Lq <= 1 << 30 && a->Lk <= 1 << 30 && a->Hk >= 1 && a->H >= a->Hk && a->H % a->Hk == 0,
+  WA_CHECK_ARG(a->B >= 1 && a->Lq >= 1 && a->Lk >= 1 && a->Lq <= 1 << 30 && a->Lk <= 1 << 30 && a->Hk >= 1 && a->H >= a->Hk && a->H % a->Hk == 0 &&
+               a->B <= INT32_MAX / a->H,
                "ranged_fwd: bad sizes B %lld Lq %lld Lk %lld heads %lld / %lld", (long long)a->B, (long long)a->Lq, (long long)a->Lk,
                (long long)a->H, (long long)a->Hk);
   WA_CHECK_ARG(a->q && a->k && a->v && a->o && a->lse && a->rows && a->tiles && a->order && wa_aligned16(a->rows), "ranged_fwd: null tensor");
