@@ -989,7 +989,7 @@ int wa_kv8_read(const wa_kv8_read_args* args, void* stream);
  * `sink`. With `index` (int32 [B, n, Hk, topk]) and `num` (int32 [B, n, Hk]) each query and key head attends to the
  * seen tokens of the listed blocks (no window; any lists, as in wa_selected_attn). q, o: bf16 [B, n, H, D], 16-byte
  * aligned rows; lse: fp32 [B, H, n]. A query that sees nothing gets 0 and -inf. Meant for few rows (n H / Hk): each
- * 64 of them read the cache once. The workspace may be NULL where its size is 0. */
+ * 64 of them (D = 128: 32) read the cache once. The workspace may be NULL where its size is 0. */
 typedef struct wa_kv8_attend_args {
   wa_cache8 cache;
   const void* q; int64_t q_sb, q_st, q_sh;

@@ -185,7 +185,8 @@ def _check_attention(got, q, cache, lens, **kw):
     (1, 1, 1, 1, 64, 1, 64, {}), (3, 1, 8, 2, 128, 700, 64, {}), (2, 1, 20, 1, 64, 300, 128, {}), (4, 3, 6, 3, 128, 260, 64, {}),
     (2, 5, 8, 1, 64, 500, 128, dict(cap=9.0)), (1, 16, 4, 1, 128, 333, 64, {}), (2, 9, 7, 7, 64, 200, 64, dict(window=50, sink=3)),
     (1, 1, 48, 1, 128, 900, 64, dict(window=200)), (2, 2, 8, 4, 128, 600, 64, dict(window=90, sink=70)), (2, 33, 2, 1, 64, 400, 64, dict(cap=3.0)),
-    (2, 70, 4, 2, 128, 400, 64, dict(window=120, sink=10, cap=5.0)), (1, 100, 2, 2, 64, 140, 128, {}), (1, 1, 4, 2, 64, 5000, 64, {})])
+    (2, 70, 4, 2, 128, 400, 64, dict(window=120, sink=10, cap=5.0)), (2, 140, 4, 2, 128, 400, 64, dict(window=120, sink=10, cap=5.0)),
+    (1, 100, 2, 2, 64, 140, 128, {}), (1, 270, 2, 2, 64, 300, 128, {}), (3, 131, 6, 3, 128, 200, 64, dict(window=33)), (1, 1, 4, 2, 64, 5000, 64, {})])
 def test_attention_against_the_definition(dtype, b, n, h, hk, d, cap, bs, kw):
     """Ragged lengths: the whole cache, one token, none, around tile and block ends, below the number of queries, past the cache."""
     cache, g = _filled(b, cap, hk, d, bs, dtype, seed=cap)
@@ -214,7 +215,7 @@ def test_chosen_blocks(dtype, d, bs):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,kw", [(2, dict(window=60, sink=5)), (70, dict(window=60, sink=5)), (2, {}), (70, {})])
+@pytest.mark.parametrize("n,kw", [(2, dict(window=60, sink=5)), (70, dict(window=60, sink=5)), (140, dict(window=60, sink=5)), (2, {}), (70, {}), (140, {})])
 def test_nothing_behind_a_sequence_is_used(dtype, n, kw):
     cap = 400
     cache, g = _filled(2, cap, 2, 64, 64, dtype, seed=8)
@@ -238,7 +239,7 @@ def test_a_block_that_is_not_finite_reaches_those_who_see_it():
     assert out[0, :2].isfinite().all() and out[0, 2:].isnan().all() and lse.isfinite().all()
 
 
-@pytest.mark.parametrize("n", [1, 65])
+@pytest.mark.parametrize("n", [1, 65, 130])
 def test_any_strides_of_queries(n):
     cache, g = _filled(2, 300, 2, 64, 64, torch.int8, seed=10)
     wide = torch.randn(2, 4, n + 3, 80, generator=g).bfloat16().to(DEV)
@@ -257,14 +258,16 @@ def test_any_strides_of_queries(n):
 def test_both_ways_agree():
     """The same queries a few at a time over the codes, and all at once over the values read back."""
     cache, g = _filled(2, 500, 2, 128, 64, torch.float8_e4m3fn, seed=12)
-    q = torch.randn(2, 96, 4, 128, generator=g).bfloat16().to(DEV)
+    q = torch.randn(2, 144, 4, 128, generator=g).bfloat16().to(DEV)
     slopes = torch.tensor([0.1, 0.02, 0.3, 0.0], device=DEV)
     kw = dict(cap=8.0, slopes=slopes, window=100, sink=4)
     whole, lse = W.attend_8bit(q, cache, _i32([500, 120]), **kw)
-    for i in range(0, 96, 32):
-        part, part_lse = W.attend_8bit(q[:, i:i + 32], cache, _i32([500 - 64 + i, 120 - 64 + i]), **kw)
-        assert ((part - whole[:, i:i + 32]).abs().float() <= 2.0 ** -5).all()      # values of about 1: two roundings to bf16 of a few weights each
-        assert ((part_lse - lse[:, :, i:i + 32]).abs() <= 2.0 ** -10).all()
+    for i in range(0, 144, 48):
+        part, part_lse = W.attend_8bit(q[:, i:i + 48], cache, _i32([500 - 96 + i, 120 - 96 + i]), **kw)
+        assert ((part - whole[:, i:i + 48]).abs().float() <= 2.0 ** -5).all()      # values of about 1: two roundings to bf16 of a few weights each
+        same = lse[:, :, i:i + 48]
+        none = torch.isinf(same)      # queries before the first token, in both
+        assert torch.equal(none, torch.isinf(part_lse)) and ((part_lse - same).abs()[~none] <= 2.0 ** -10).all()
 
 
 def test_a_decoding_step_captured():
@@ -361,7 +364,7 @@ def test_ragged_sequences(b, n, h, hk, d, cap, kw):
         _check_attention(W.attend_8bit(q, cache, _i32(lens), **kw), q, cache, [min(max(x, 0), cap) for x in lens], **kw)
 
 
-@pytest.mark.parametrize("n,h,hk", [(127, 1, 1), (128, 2, 2), (129, 1, 1), (32, 8, 2), (33, 8, 2), (43, 3, 1)])
+@pytest.mark.parametrize("n,h,hk", [(127, 1, 1), (128, 2, 2), (129, 1, 1), (64, 8, 2), (65, 8, 2), (85, 3, 1), (86, 3, 1), (256, 1, 1), (257, 2, 2)])
 @pytest.mark.parametrize("d", [64, 128])
 def test_around_the_number_of_rows_that_read_codes(n, h, hk, d):
     cache, g = _filled(3, 420, hk, d, 64, torch.float8_e4m3fn, seed=n)
@@ -372,7 +375,7 @@ def test_around_the_number_of_rows_that_read_codes(n, h, hk, d):
         _check_attention(W.attend_8bit(q, cache, 300, **kw), q, cache, [300] * 3, **kw)
 
 
-@pytest.mark.parametrize("n", [2, 80])
+@pytest.mark.parametrize("n", [2, 80, 140])
 def test_lengths_past_the_cache_under_a_window(n):
     """A length past the cache is the cache's, for what a long chunk reads back too: memory that is not written there holds NaN."""
     b, h, hk, d, cap = 3, 4, 2, 64, 500
@@ -428,8 +431,8 @@ def test_prompt_then_single_tokens():
     W.kv_append_8bit(cache, k, v, 0, lengths=lens)
     held = W.kv_read_8bit(cache, 0, n)
     prompt = W.ranged_attention(q, *held, W.key_ranges(b, n, n, lengths=lens), cap=20.0, slopes=slopes)
-    chunk, _ = W.attend_8bit(q[:, -80:], cache, n, cap=20.0, slopes=slopes)      # the same tokens, as the chunk of a longer prompt
-    assert torch.equal(prompt[0, -80:], chunk[0])
+    chunk, _ = W.attend_8bit(q[:, -140:], cache, n, cap=20.0, slopes=slopes)     # the same tokens, as the chunk of a longer prompt
+    assert torch.equal(prompt[0, -140:], chunk[0])
     drafts = make(4, hk), make(4, hk)
     W.kv_append_8bit(cache, *drafts, lens)
     for step in range(3):

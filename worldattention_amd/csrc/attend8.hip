@@ -130,7 +130,7 @@ __device__ __forceinline__ void write_row(const AttendParams& p, int b, int i, i
 }
 
 template <typename Code, int D, int RT>
-__global__ void __launch_bounds__(256, D == 128 && RT == 4 ? 1 : 2) attend_kernel(AttendParams p) {
+__global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
   constexpr int NW = 4, KC = D / 32, VC = D / 16, KL = D / 64;   // key products of a tile half; channels of a value row a lane holds; loads of a key row
   typedef typename ValueRow<D>::type VRow;
   static_assert(NW * 4 * 32 * D >= NW * 16 * (D + 4) * 4, "the waves' outputs fit their drained rings");
@@ -537,7 +537,9 @@ bool sized(const wa_kv8_attend_args& a) {
 Cut cut(const wa_kv8_attend_args& a) {
   Cut c;
   const int64_t G = a.H / a.cache.Hk, rows = a.index ? G : a.n * G;
-  c.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  // 64 rows of a unit take 256 registers at D = 64; at D = 128 they would leave one wave a SIMD (8 sequences of 32,000 tokens, 64 rows of 8 key heads:
+  // two units of 32 rows 197 us, one of 64 283)
+  c.rt = rows <= 16 ? 1 : rows <= 32 || a.cache.D == 128 ? 2 : 4;
   const int64_t of = (rows + 16 * c.rt - 1) / (16 * c.rt);
   c.units_of = (int)of;
   c.units = a.cache.B * a.cache.Hk * of * (a.index ? a.n : 1);
@@ -546,14 +548,15 @@ Cut cut(const wa_kv8_attend_args& a) {
   const int64_t seen = a.window > 0 ? std::min(tokens, std::min(a.sink, tokens) + std::min(a.window, tokens) + a.n + 128) : tokens;
   const int64_t tiles = a.index ? a.topk * (a.cache.block_size / 32) : (seen + 31) / 32;
   // workgroups that run at once: what the kernels' registers leave of four a CU (D = 64) or, with their codes' stages, two
-  const int64_t at_once = a.cache.D == 128 ? (c.rt == 4 ? 256 : 512) : c.rt == 1 ? 1024 : c.rt == 2 ? 768 : 512;
+  const int64_t at_once = a.cache.D == 128 ? 512 : c.rt == 1 ? 1024 : c.rt == 2 ? 768 : 512;
   c.per = (int)std::min<int64_t>(share(c.units * tiles, at_once), std::max<int64_t>(8, tiles));
   c.parts = (int)std::max<int64_t>(1, (tiles + c.per - 1) / c.per);
-  // Sequences of lengths that only the GPU knows: cut along all of them, so that workgroups bring as much each (ragged ones of up to 32,768 tokens,
-  // 32 of them, 8 key heads: 204 us; cut by the cache's length into parts of 64 tiles 268).
+  // Sequences of lengths that only the GPU knows, and more tiles than one round takes: cut along all sequences, so that workgroups bring as much each
+  // (32 ragged ones of up to 32,768 tokens, 8 key heads of 128: 204 us; cut by the cache's length into parts of 64 tiles 268. 32 of 30,000 and heads
+  // of 64: 251 and 311; 16 of 4,000, less than a round: 27 and 23).
   c.heads = a.cache.Hk;
-  const bool ragged = a.kv_len && !a.index && of == 1 && a.cache.B > 1 && a.cache.B <= 256 && c.heads <= at_once;
-  c.even = ragged && a.cache.B * tiles <= INT32_MAX ? (int)(at_once / c.heads) : 0;
+  const bool along = (a.kv_len || c.units * tiles > 64 * at_once) && !a.index && of == 1 && a.cache.B > 1 && a.cache.B <= 256 && c.heads <= at_once;
+  c.even = along && a.cache.B * tiles <= INT32_MAX ? (int)(at_once / c.heads) : 0;
   c.most = (std::min<int64_t>(kRounds * c.even, a.cache.B * tiles / 64 + c.even) + kTurn - 1) / kTurn * kTurn;
   return c;
 }
@@ -564,11 +567,11 @@ void launch(const AttendParams& p, const Cut& c, hipStream_t s) {
   const dim3 rows((unsigned)((c.units * 16 * c.rt + 3) / 4));
   if (c.rt == 1) hipLaunchKernelGGL((attend_kernel<Code, D, 1>), grid, block, 0, s, p);
   else if (c.rt == 2) hipLaunchKernelGGL((attend_kernel<Code, D, 2>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((attend_kernel<Code, D, 4>), grid, block, 0, s, p);
+  else if constexpr (D == 64) hipLaunchKernelGGL((attend_kernel<Code, D, 4>), grid, block, 0, s, p);
   if (!c.slots()) return;
   if (c.rt == 1) hipLaunchKernelGGL((join_kernel<D, 1>), rows, block, 0, s, p, (unsigned)c.units);
   else if (c.rt == 2) hipLaunchKernelGGL((join_kernel<D, 2>), rows, block, 0, s, p, (unsigned)c.units);
-  else hipLaunchKernelGGL((join_kernel<D, 4>), rows, block, 0, s, p, (unsigned)c.units);
+  else if constexpr (D == 64) hipLaunchKernelGGL((join_kernel<D, 4>), rows, block, 0, s, p, (unsigned)c.units);
 }
 
 }  // namespace

@@ -22,10 +22,10 @@ __all__ = ["new_cache_8bit", "kv_append_8bit", "kv_read_8bit", "attend_8bit"]
 
 _CODES = {torch.int8: _lib.WA_CODE_INT8, torch.float8_e4m3fn: _lib.WA_CODE_E4M3}
 
-# Rows of a key head (queries times query heads) up to which attend_8bit reads codes, once for every 64 rows; above, the values are read
-# back to bf16 once. 8 key heads of 128, codes against read back: 128 rows 67 and 106 us over 32,760 tokens, 32 and 46 over 4,096, 484 and 724
-# for 8 sequences of 32,000; 256 rows 126 and 111, 37 and 47.
-_FEW_ROWS = 128
+# Rows of a key head (queries times query heads) up to which attend_8bit reads codes, once for every 32 or 64 rows; above, the values are
+# read back to bf16 once. 8 key heads of 128, codes against read back: 256 rows 96 and 110 us over 32,760 tokens, 30 and 50 over 4,096, 615 and
+# 723 for 8 sequences of 32,000; 512 rows 176 and 121, 39 and 50, 1,065 and 777.
+_FEW_ROWS = 256
 
 
 def new_cache_8bit(batch: int, cap: int, kv_heads: int, head_dim: int, *, block_size: int = 64, dtype=torch.int8,
@@ -168,7 +168,7 @@ def attend_8bit(q: torch.Tensor, kv_cache: dict, kv_len: KvLen, *, scale: Option
     * ``chosen``: a :class:`~worldattention_amd.hsa.selected.BlockSelection` instead (no window): each query and key head attends
       to the seen tokens of its listed blocks (any lists; an id listed twice counts twice).
 
-    Few queries (up to 128 rows, queries times heads, of a key head) and chosen blocks read the codes; a longer chunk reads the
+    Few queries (up to 256 rows, queries times heads, of a key head) and chosen blocks read the codes; a longer chunk reads the
     tokens that it sees back into bf16 once, exactly, and attends to those: two tensors of ``[B, cap, Hk, D]`` while the call
     runs. Sums and softmax statistics are fp32; weights (times the values' scale) round to bf16 once. No gradient.
     """
