@@ -464,7 +464,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
       if (i < limit) {
         const int32_t* r = p.ranges.tile(b, i);
         any = (r[kUpLo] < key_end && r[kUpHi] > key0) || (r[kLowLo] < key_end && r[kLowHi] > key0);
-        const bool whole = (r[kUpIn0] <= key0 && r[kUpIn1] >= key_end) || (r[kLowIn0] <= key0 && r[kLowIn1] >= key_end);
+        // rows from Lq on read as zeros, their log-sum-exp too, and with a negative slope their weights may be infinite: masked, by runs of zeros
+        const bool whole = ((r[kUpIn0] <= key0 && r[kUpIn1] >= key_end) || (r[kLowIn0] <= key0 && r[kLowIn1] >= key_end)) && (i + 1) * 64 <= p.ranges.Lq;
         entry = (i - base) | min(max(min(r[kRowEnd], p.ranges.Lq) - i * 64, 0), 64) << 10 | (whole ? 1 << 20 : 0);
       }
       const uint64_t mask = __ballot(any);
