@@ -443,3 +443,19 @@ def test_prompt_then_single_tokens():
         for kw in (dict(cap=20.0, slopes=slopes), dict(window=70, sink=4), dict(chosen=W.select_key_blocks(
                 one, cache["k_block_sums"], lens + step + 1, block_size=64, topk=3))):
             _check_attention(W.attend_8bit(one, cache, lens + step + 1, **kw), one, cache, at, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,n", [(64, 3), (64, 40), (64, 300), (128, 16), (128, 150)])
+def test_large_caps(dtype, d, n):
+    """Scores far below the cap keep fp32's accuracy, also beside a query whose scores pass it, but for that of the one token that it sees: 0.
+    Codes, and read back."""
+    cache, g = _filled(1, n + 50, 1, d, 64, dtype, seed=n)
+    cache["k"].view(torch.uint8)[:, 0, :, 0] = 0
+    q = torch.randn(1, n, 2, d, generator=g).bfloat16().to(DEV)
+    for cap in (100.0, 1100.0, 1e4, 1e6):
+        far = q.clone()
+        far[:, 0] = 0
+        far[:, 0, :, 0] = 2 * cap * d ** 0.5
+        for x, lens in ((q, n + 50), (far, n)):
+            _check_attention(W.attend_8bit(x, cache, lens, cap=cap), x, cache, [lens], cap=cap)

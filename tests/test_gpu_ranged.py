@@ -382,3 +382,25 @@ def test_scores_at_the_ends_of_fp32():
     k[0, 40, 0, 1] = math.inf
     out = W.ranged_attention(q, k, v, _ranges(1, n, n, dict(documents=[0, 40, 41, 70])))
     assert out[0, 40].isnan().all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cap", [100.0, 1024.0, 1100.0, 3e3, 1e4, 1e5, 1e6])
+@pytest.mark.parametrize("far", [False, True])
+def test_large_caps(d, cap, far):
+    """Scores far below the cap keep fp32's accuracy, also beside a row whose scores pass it, but for that of the one key that it sees: 0."""
+    b, n, h, hk = 1, 200, 2, 1
+    q, k, v, do = _inputs(b, n, n, h, hk, d, seed=52)
+    if far:
+        q[:, 0] = 0
+        q[:, 0, :, 0] = 2 * cap * d ** 0.5
+        k[:, 0, :, 0] = 0
+    check(q, k, v, do, _ranges(b, n, n, dict()), OR.seen(b, n, n), cap=cap, slopes=torch.tensor([0.1, 0.01], device=DEV))
+
+
+@pytest.mark.parametrize("power,cap", [(-100, 5.0), (-60, 1e4), (-13, 1000.0), (-16, 1000.0), (40, 3.0), (80, 1e-6)])
+def test_caps_at_any_scale(power, cap):
+    """Scores of about 1 from small and large products."""
+    b, n, h, hk, d = 1, 130, 2, 1, 64
+    q, k, v, do = _inputs(b, n, n, h, hk, d, seed=53, size=2.0 ** -(power // 2))
+    check(q, k, v, do, _ranges(b, n, n, dict()), OR.seen(b, n, n), scale=2.0 ** (power - 3), cap=cap)

@@ -129,7 +129,7 @@ __device__ __forceinline__ void write_row(const AttendParams& p, int b, int i, i
   if (d == 0) p.lse[((int64_t)b * p.H + h) * p.n + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * WA_LN2;
 }
 
-template <typename Code, int D, int RT>
+template <typename Code, int D, int RT, Bends BENDS>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
   constexpr int NW = 4, KC = D / 32, VC = D / 16, KL = D / 64;   // key products of a tile half; channels of a value row a lane holds; loads of a key row
   typedef typename ValueRow<D>::type VRow;
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
           s[e] = acc[e >> 2][e & 3] * x.ks;
           most = fmaxf(most, fabsf(s[e]));
         }
-        by_form(bend.form(most), [&](auto form) {
+        by_form<BENDS>(bend, most, [&](auto form) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[e] = bend.bent<decltype(form)::value>(s[e], far - (float)(16 * (e >> 2) + 4 * (e & 3)), unused);
         });
@@ -561,17 +561,25 @@ Cut cut(const wa_kv8_attend_args& a) {
   return c;
 }
 
-template <typename Code, int D>
+template <typename Code, int D, Bends BENDS>
 void launch(const AttendParams& p, const Cut& c, hipStream_t s) {
   const dim3 grid((unsigned)c.grid()), block(256);
   const dim3 rows((unsigned)((c.units * 16 * c.rt + 3) / 4));
-  if (c.rt == 1) hipLaunchKernelGGL((attend_kernel<Code, D, 1>), grid, block, 0, s, p);
-  else if (c.rt == 2) hipLaunchKernelGGL((attend_kernel<Code, D, 2>), grid, block, 0, s, p);
-  else if constexpr (D == 64) hipLaunchKernelGGL((attend_kernel<Code, D, 4>), grid, block, 0, s, p);
+  if (c.rt == 1) hipLaunchKernelGGL((attend_kernel<Code, D, 1, BENDS>), grid, block, 0, s, p);
+  else if (c.rt == 2) hipLaunchKernelGGL((attend_kernel<Code, D, 2, BENDS>), grid, block, 0, s, p);
+  else if constexpr (D == 64) hipLaunchKernelGGL((attend_kernel<Code, D, 4, BENDS>), grid, block, 0, s, p);
   if (!c.slots()) return;
   if (c.rt == 1) hipLaunchKernelGGL((join_kernel<D, 1>), rows, block, 0, s, p, (unsigned)c.units);
   else if (c.rt == 2) hipLaunchKernelGGL((join_kernel<D, 2>), rows, block, 0, s, p, (unsigned)c.units);
   else if constexpr (D == 64) hipLaunchKernelGGL((join_kernel<D, 4>), rows, block, 0, s, p, (unsigned)c.units);
+}
+
+template <typename Code>
+void launch(const AttendParams& p, const Cut& c, bool large, int64_t D, hipStream_t s) {
+  if (D == 128 && large) launch<Code, 128, kLargeCaps>(p, c, s);
+  else if (D == 128) launch<Code, 128, kSmallCaps>(p, c, s);
+  else if (large) launch<Code, 64, kLargeCaps>(p, c, s);
+  else launch<Code, 64, kSmallCaps>(p, c, s);
 }
 
 }  // namespace
@@ -617,12 +625,8 @@ extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
   p.bend = bend_of(scale, a->cap);
   p.part = (float*)a->workspace;
   hipStream_t s = (hipStream_t)stream;
-  if (c.code == WA_CODE_INT8) {
-    if (c.D == 128) launch<Int8, 128>(p, k, s);
-    else launch<Int8, 64>(p, k, s);
-  } else {
-    if (c.D == 128) launch<E4m3, 128>(p, k, s);
-    else launch<E4m3, 64>(p, k, s);
-  }
+  const bool large = bends_of(a->cap, a->slopes) == kLargeCaps;
+  if (c.code == WA_CODE_INT8) launch<Int8>(p, k, large, c.D, s);
+  else launch<E4m3>(p, k, large, c.D, s);
   return wa_launch_status("kv8_attend");
 }

@@ -178,7 +178,7 @@ struct FwdParams {
 // Running maximum before the first key: below every score, and finite, so that no difference of it is NaN where a row sees nothing yet.
 constexpr float kNoMax = -3.4028234e38f;
 
-template <int D, bool BENT>
+template <int D, Bends BENT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ranged_fwd_kernel(FwdParams p) {
   constexpr int NW = 4, QT = 1, BM = 32 * NW * QT, DC = D / 16, DT = D / 32, TILE = 64 * D;
   using NT = NextTile<D, NW>;
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
         float most = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(x[r]));
-        by_form(bend.form(most), bend_all);
+        by_form<BENT>(bend, most, bend_all);
         S[KH][qt] = x;
       }
     }
@@ -477,10 +477,11 @@ int fwd_splits(int64_t B, int64_t H, int64_t Lq, int64_t Lk) {
 }
 
 template <int D>
-void launch_fwd(const FwdParams& p, bool bent, hipStream_t s) {
+void launch_fwd(const FwdParams& p, Bends bends, hipStream_t s) {
   const int64_t grid = (int64_t)p.B * p.H * ((p.ranges.Lq + 127) / 128) * p.splits;
-  if (bent) hipLaunchKernelGGL((ranged_fwd_kernel<D, true>), dim3((unsigned)grid), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((ranged_fwd_kernel<D, false>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  if (bends == kPlain) hipLaunchKernelGGL((ranged_fwd_kernel<D, kPlain>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  else if (bends == kSmallCaps) hipLaunchKernelGGL((ranged_fwd_kernel<D, kSmallCaps>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((ranged_fwd_kernel<D, kLargeCaps>), dim3((unsigned)grid), dim3(256), 0, s, p);
   if (p.splits > 1) {
     const int64_t n_rows = (int64_t)p.B * p.H * p.ranges.Lq, per = 2048 / D;
     hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)((n_rows + per - 1) / per)), dim3(256), 0, s, p, n_rows);
@@ -553,8 +554,8 @@ extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   WA_CHECK_ARG(p.splits == 1 || (a->workspace && wa_aligned16(a->workspace)), "ranged_fwd: a launch in %d parts needs a workspace", p.splits);
   p.part_o = (float*)a->workspace;
   p.part_ml = p.part_o + p.splits * a->B * a->H * a->Lq * a->D;
-  const bool bent = a->cap > 0.f || a->slopes;
-  if (a->D == 128) launch_fwd<128>(p, bent, (hipStream_t)stream);
-  else launch_fwd<64>(p, bent, (hipStream_t)stream);
+  const Bends bends = bends_of(a->cap, a->slopes);
+  if (a->D == 128) launch_fwd<128>(p, bends, (hipStream_t)stream);
+  else launch_fwd<64>(p, bends, (hipStream_t)stream);
   return wa_launch_status("ranged_fwd");
 }

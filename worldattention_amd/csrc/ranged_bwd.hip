@@ -178,7 +178,7 @@ __device__ __forceinline__ void step_wait() { asm volatile("s_waitcnt vmcnt(0) l
 // part 187); packed documents of 8,190 tokens in all, 16 heads, capped: 152 us (134). A second part only where a weight is above 1/8 cost more
 // in registers than it saved.
 // ---------------------------------------------------------------------------------------------
-template <int D, bool BENT, bool SLOPES>
+template <int D, Bends BENT, bool SLOPES>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ranged_dq_kernel(BwdParams p) {
   constexpr int NW = 4, DC = D / 16, DT = D / 32, TILE = 64 * D;
   using RT = RowTile<D, NW>;
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
       float most = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[r]));
-      by_form(bend.form(most), weights);
+      by_form<BENT>(bend, most, weights);
     } else {
       weights(FormTag<kBias>{});
     }
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(256) slopes_kernel(BwdParams p, int n) {
 constexpr int kListMax = 1024;   // row tiles listed at a time: 65,536 rows
 constexpr int kKeys = 128;       // of a workgroup, as the order of the key tiles has them
 
-template <int D, bool BENT>
+template <int D, Bends BENT>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) ranged_dkv_kernel(BwdParams p) {
   constexpr int NW = 8, DC = D / 16, DT = D / 32, TILE = 64 * D;
   using RT = RowTile<D, NW>;
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) r
               }
             }
           };
-          if constexpr (BENT) by_form(bend.form(largest<2>(sacc)), weights);
+          if constexpr (BENT) by_form<BENT>(bend, largest<2>(sacc), weights);
           else weights(FormTag<kBias>{});
           // dV^T[d, key] += dO^T P: A by transpose reads, B from registers
           ColsProduct<D>::run(rd, dc, ab, acc, a);
@@ -717,25 +717,31 @@ int kv_parts(int64_t B, int64_t H, int64_t Hk, int64_t Lq, int64_t Lk) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({512 / groups, steps / 4, 8}));
 }
 
-template <int D, bool BENT>
+template <int D, Bends BENT>
 void launch_bwd(const BwdParams& p, hipStream_t s) {
   const int64_t nq = (p.ranges.Lq + 127) / 128;
   const dim3 gq((unsigned)(p.B * p.H * nq)), gk((unsigned)((int64_t)p.B * p.Hk * ((p.ranges.Lk + kKeys - 1) / kKeys) * p.parts));
+  bool slopes = false;
   if constexpr (BENT) {
-    if (p.dslopes) {
-      hipLaunchKernelGGL((ranged_dq_kernel<D, true, true>), gq, dim3(256), 0, s, p);
+    slopes = p.dslopes;
+    if (slopes) {
+      hipLaunchKernelGGL((ranged_dq_kernel<D, BENT, true>), gq, dim3(256), 0, s, p);
       hipLaunchKernelGGL(slopes_kernel, dim3((unsigned)p.H), dim3(256), 0, s, p, (int)(p.B * nq));
-    } else {
-      hipLaunchKernelGGL((ranged_dq_kernel<D, true, false>), gq, dim3(256), 0, s, p);
     }
-  } else {
-    hipLaunchKernelGGL((ranged_dq_kernel<D, false, false>), gq, dim3(256), 0, s, p);
   }
+  if (!slopes) hipLaunchKernelGGL((ranged_dq_kernel<D, BENT, false>), gq, dim3(256), 0, s, p);
   hipLaunchKernelGGL((ranged_dkv_kernel<D, BENT>), gk, dim3(512), 0, s, p);
   if (p.parts > 1) {
     const int64_t size = (int64_t)p.B * p.ranges.Lk * p.Hk * D;
     hipLaunchKernelGGL(parts_kernel, dim3((unsigned)((size / 4 + 255) / 256)), dim3(256), 0, s, p, size);
   }
+}
+
+template <int D>
+void launch_bwd(const BwdParams& p, Bends bends, hipStream_t s) {
+  if (bends == kPlain) launch_bwd<D, kPlain>(p, s);
+  else if (bends == kSmallCaps) launch_bwd<D, kSmallCaps>(p, s);
+  else launch_bwd<D, kLargeCaps>(p, s);
 }
 
 }  // namespace
@@ -790,13 +796,8 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   p.parts = kv_parts(a->B, a->H, a->Hk, a->Lq, a->Lk);
   p.part_kv = (float*)((char*)a->workspace + (n * 12 + a->B * a->H * ((a->Lq + 127) / 128) * 4 + 15) / 16 * 16);
   hipStream_t s = (hipStream_t)stream;
-  const bool bent = a->cap > 0.f || a->slopes;
-  if (a->D == 128) {
-    if (bent) launch_bwd<128, true>(p, s);
-    else launch_bwd<128, false>(p, s);
-  } else {
-    if (bent) launch_bwd<64, true>(p, s);
-    else launch_bwd<64, false>(p, s);
-  }
+  const Bends bends = bends_of(a->cap, a->slopes);
+  if (a->D == 128) launch_bwd<128>(p, bends, s);
+  else launch_bwd<64>(p, bends, s);
   return wa_launch_status("ranged_bwd");
 }

@@ -103,21 +103,32 @@ struct RowRuns {
 // Scores beyond the plain product, in units of log2: cap tanh(x / cap), x = scale s, less the distance's bias. Which form of the tanh is right for all of
 // a wave's scores is asked once for a tile:
 //   kBias   no cap;
-//   kClose  |x| <= 0.3 cap: tanh(z) = z P(z^2), P of degree 3 fitted to 1.2e-8 of the value (a weighted least-squares fit of tanh(z) / z on
-//           [0, 0.09] with the leading 1 kept), with the scale in its coefficients: five instructions (a chunk of 1,024 rows over 8,256 keys: 256 us, 275 with kNear);
-//   kNear   |x| <= cap / 2: the same of degree 4, on [0, 1/4] to 1.5e-8: six instructions, more exact than kFar and half its work;
+//   kClose  |x| <= 0.3 cap: tanh(z) = z P(z^2), P of degree 3 fitted to 1.3e-8 of the value (a weighted least-squares fit of tanh(z) / z on
+//           [0, 0.09] with the leading 1 kept), with the powers of the scale in its coefficients: five instructions (a chunk of 1,024 rows over 8,256
+//           keys: 256 us, 275 with six). Left out where those powers would leave fp32;
+//   kNear   |x| <= cap / 2: the same of degree 4, on [0, 1/4] to 1.7e-8, in z itself, which any scale and cap leave in range: seven instructions;
 //   kFar    e = exp(2 z), r = 1 / (e + 1): tanh = 1 - 2 r, off by a few 2^-24 of the cap wherever z is (e = inf gives r = 0); its derivative
-//           4 e r r, off by a few 2^-24 of itself.
-enum BendForm { kBias, kClose, kNear, kFar };
+//           4 e r r, off by a few 2^-24 of itself;
+//   kBoth   kNear or kFar, score by score: for caps above kFarCap, a few 2^-24 of which (1e-4 there) show in small scores that share a tile with
+//           large ones. 8,190 causal tokens, 16 heads on 4 of 128, scores up to the cap everywhere: forward 488 us, with gradients 2,165; kFar 415
+//           and 1,755. Kernels are built for either side of kFarCap: as a fifth form in one kernel it put the forward's scores in scratch and
+//           cost the attention over codes 4%, whatever the cap.
+enum BendForm { kBias, kClose, kNear, kFar, kBoth };
+enum Bends { kPlain, kSmallCaps, kLargeCaps };   // no cap and no bias; a bias or a cap of at most kFarCap; a cap above it
+constexpr float kFarCap = 1024.f;
+static inline Bends bends_of(float cap, bool bias) { return cap > kFarCap ? kLargeCaps : cap > 0.f || bias ? kSmallCaps : kPlain; }
 struct Bend {
-  float close, near;          // largest |s| for kClose and kNear (below 0: none; the coefficients' powers of the scale would leave fp32)
-  float scale2, in2, cap2;    // scale log2(e); 2 scale / cap log2(e); cap log2(e) or 0
-  float c[4], c3[3], icap2;   // kNear's and kClose's coefficients of s^2 and its powers; 1 / cap2
-  float slope2;               // slope log2(e)
+  float close, near;           // largest |s| for kClose (below 0: none) and kNear
+  float scale2, in, in2, cap2; // scale log2(e); scale / cap; 2 scale / cap log2(e); cap log2(e) or 0
+  float c[4], c3[3], icap2;    // kNear's coefficients of z^2 and kClose's of s^2, and its powers, times scale2; 1 / cap2
+  float slope2;                // slope log2(e)
   // The form for scores of at most `most`, the same in all of the wave's lanes.
+  template <Bends BENDS>
   __device__ __forceinline__ BendForm form(float most) const {
+    if (BENDS == kLargeCaps) return __any(most > near) ? kBoth : kNear;
     if (!(cap2 > 0.f)) return kBias;
-    return !__any(most > close) ? kClose : __any(most > near) ? kFar : kNear;
+    if (!__any(most > close)) return kClose;
+    return __any(most > near) ? kFar : kNear;
   }
   // The score before the bias, and the cap's derivative there.
   template <BendForm FORM>
@@ -125,15 +136,22 @@ struct Bend {
     turn = 1.f;
     if constexpr (FORM == kBias) {
       return s * scale2;
-    } else if constexpr (FORM != kFar) {
-      const float u = s * s, p = FORM == kClose ? fmaf(u, fmaf(u, fmaf(u, c3[2], c3[1]), c3[0]), scale2) : fmaf(u, fmaf(u, fmaf(u, fmaf(u, c[3], c[2]), c[1]), c[0]), scale2);
+    } else if constexpr (FORM == kClose || FORM == kNear) {
+      const float z = FORM == kClose ? s : s * in, u = z * z;
+      const float p = FORM == kClose ? fmaf(u, fmaf(u, fmaf(u, c3[2], c3[1]), c3[0]), scale2) : fmaf(u, fmaf(u, fmaf(u, fmaf(u, c[3], c[2]), c[1]), c[0]), scale2);
       const float y = s * p, t = y * icap2;
       turn = fmaf(-t, t, 1.f);
       return y;
-    } else {
+    } else if constexpr (FORM == kFar) {
       const float e = __builtin_amdgcn_exp2f(s * in2), r = __builtin_amdgcn_rcpf(e + 1.f);
       turn = fminf(e, 0x1p100f) * 4.f * r * r;
       return fmaf(-2.f * cap2, r, cap2);
+    } else {
+      float turn_far;
+      const float y = capped<kNear>(s, turn), far = capped<kFar>(s, turn_far);
+      const bool small = fabsf(s) <= near;
+      turn = small ? turn : turn_far;
+      return small ? y : far;
     }
   }
   template <BendForm FORM>
@@ -147,19 +165,20 @@ static inline Bend bend_of(float scale, float cap) {
   b.close = b.near = -1.f;
   if (cap > 0.f) {
     const float in = scale / cap, u = in * in;
+    b.in = in;
     b.in2 = 2.f * in * WA_LOG2E;
     b.cap2 = cap * WA_LOG2E;
     b.icap2 = 1.f / b.cap2;
-    if (in >= 0x1p-15f && in <= 0x1p15f) {   // powers up to the eighth, and |s| <= 2^14, stay normal
+    b.near = fminf(0.5f / in, 3.4e38f);
+    b.c[0] = -0x1.5554d6p-2f * b.scale2;
+    b.c[1] = 0x1.10e9fcp-3f * b.scale2;
+    b.c[2] = -0x1.b28c5ep-5f * b.scale2;
+    b.c[3] = 0x1.1a7b9cp-6f * b.scale2;
+    if (in >= 0x1p-15f && in <= 0x1p15f) {   // the last coefficient is above 2^-130: even as a subnormal it has the bits that show
       b.close = 0.3f / in;
-      b.near = 0.5f / in;
       b.c3[0] = -0x1.55549ep-2f * u * b.scale2;
       b.c3[1] = 0x1.10b012p-3f * u * u * b.scale2;
       b.c3[2] = -0x1.9c99a8p-5f * u * u * u * b.scale2;
-      b.c[0] = -0x1.5554d6p-2f * u * b.scale2;
-      b.c[1] = 0x1.10e9fcp-3f * u * u * b.scale2;
-      b.c[2] = -0x1.b28c5ep-5f * u * u * u * b.scale2;
-      b.c[3] = 0x1.1a7b9cp-6f * u * u * u * u * b.scale2;
     }
   }
   return b;
@@ -174,12 +193,18 @@ __device__ __forceinline__ float largest(const f32x16 (&s)[N]) {
   return x;
 }
 template <BendForm F> struct FormTag { static constexpr BendForm value = F; };
-// run(FormTag<form>)
-template <typename Run>
-__device__ __forceinline__ void by_form(BendForm form, const Run& run) {
-  if (form == kBias) run(FormTag<kBias>{});
-  else if (form == kClose) run(FormTag<kClose>{});
-  else if (form == kNear) run(FormTag<kNear>{});
-  else run(FormTag<kFar>{});
+// run(FormTag<form>) of the form for scores of at most `most`
+template <Bends BENDS, typename Run>
+__device__ __forceinline__ void by_form(const Bend& bend, float most, const Run& run) {
+  const BendForm form = bend.form<BENDS>(most);
+  if constexpr (BENDS == kLargeCaps) {
+    if (form == kNear) run(FormTag<kNear>{});
+    else run(FormTag<kBoth>{});
+  } else {
+    if (form == kBias) run(FormTag<kBias>{});
+    else if (form == kClose) run(FormTag<kClose>{});
+    else if (form == kNear) run(FormTag<kNear>{});
+    else run(FormTag<kFar>{});
+  }
 }
 }  // namespace
