@@ -25,7 +25,7 @@ def seen(batch, q_len, k_len, *, causal=True, chunk=1, window=None, sink=0, pref
             if not home:
                 continue
             x, y = home[0]
-            for j in range(x, y):
+            for j in range(max(x, 0), y):
                 reached = not causal or (j - x) // chunk <= (t - x) // chunk
                 near = window is None or (j > t - window and (causal or j < t + window))
                 out[b, i, j] = (reached and (near or j - x < sink)) or j - x < listed(prefix, b)

@@ -404,3 +404,13 @@ def test_caps_at_any_scale(power, cap):
     b, n, h, hk, d = 1, 130, 2, 1, 64
     q, k, v, do = _inputs(b, n, n, h, hk, d, seed=53, size=2.0 ** -(power // 2))
     check(q, k, v, do, _ranges(b, n, n, dict()), OR.seen(b, n, n), scale=2.0 ** (power - 3), cap=cap)
+
+
+@pytest.mark.parametrize("rules", RULES)
+def test_documents_that_begin_before_the_first_token(rules):
+    """Chunks, sinks and prefixes count from the document's border, tokens that are no longer held among them."""
+    for documents in ([-5, 40, 70], [-200, -7, 30, 65], [[-3, 66, 70], [0, 9, 70]]):
+        both = {**rules, "documents": documents}
+        got = _ranges(2, 70, 70, both)
+        assert torch.equal(_mask_of(got, 70).expand(2, 70, 70), OR.seen(2, 70, 70, **both)), both
+        _check_tiles(got, 70, 70)

@@ -54,7 +54,7 @@ __device__ int4 by_rules(const RulesParams& p, int b, int i) {
       else hi = mid;
     }
     if (lo == 0 || lo == p.n_docs) return int4{0, 0, 0, 0};
-    first = max((int64_t)d[lo - 1], (int64_t)0);
+    first = (int64_t)d[lo - 1];   // before the first token, too: its chunks, sinks and prefix count from there
     end = min((int64_t)d[lo], len);
   }
   const int64_t reach = p.causal ? min(end, first + ((t - first) / p.chunk + 1) * p.chunk) : end;
