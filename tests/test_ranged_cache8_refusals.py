@@ -346,3 +346,14 @@ def test_c_entries_refuse_sizes_that_no_grid_holds(fn, cls, sizes, optional):
 @pytest.mark.parametrize("fn", ["wa_key_ranges", "wa_ranged_fwd", "wa_ranged_bwd", "wa_kv8_append", "wa_kv8_read", "wa_kv8_attend"])
 def test_c_entries_refuse_null(fn):
     assert getattr(_lib.lib(), fn)(None, None) == _lib.WA_ERR_ARG
+
+
+@pytest.mark.parametrize("x", [2.5, -0.5, math.inf, -math.inf, math.nan, True])
+def test_numbers_that_are_not_whole(x):
+    """Places and lengths are not cut off to whole numbers, and rules that are not numbers of tokens are no other errors."""
+    c, kv = cache(), zeros(2, 3, 2, 64)
+    for call in (lambda: W.key_ranges(2, 8, 8, kv_len=x), lambda: W.kv_append_8bit(c, kv, kv, x), lambda: W.kv_read_8bit(c, x, 3),
+                 lambda: W.kv_read_8bit(c, 0, x), lambda: W.attend_8bit(zeros(2, 1, 4, 64), c, x), lambda: W.key_ranges(2, 8, 8, window=x),
+                 lambda: W.key_ranges(2, 8, 8, prefix=x), lambda: W.key_ranges(x, 8, 8), lambda: W.new_cache_8bit(2, x, 2, 64, device="cpu")):
+        with pytest.raises(ValueError, match="whole number"):
+            call()

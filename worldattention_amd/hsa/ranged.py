@@ -36,8 +36,15 @@ class KeyRanges(NamedTuple):
     k_len: int
 
 
+def _is_whole(x) -> bool:
+    try:
+        return not isinstance(x, bool) and int(x) == x
+    except (OverflowError, ValueError):      # infinities and NaN
+        return False
+
+
 def _count(x, name: str, low: int) -> int:
-    if isinstance(x, bool) or int(x) != x or not low <= x <= _FAR:
+    if not _is_whole(x) or not low <= x <= _FAR:
         raise ValueError(f"{name} must be a whole number of at least {low}, got {x}")
     return int(x)
 
@@ -48,7 +55,9 @@ def _per_sequence(x, bsz: int, name: str):
         if tuple(x.shape) != (bsz,) or x.dtype is not torch.int32:
             raise ValueError(f"{name} must be an int or int32 [{bsz}], got {x.dtype} {tuple(x.shape)}")
         return x.contiguous(), 0
-    if abs(int(x)) > _FAR:
+    if not _is_whole(x):
+        raise ValueError(f"{name} must be a whole number or int32 [{bsz}], got {x}")
+    if abs(x) > _FAR:
         raise ValueError(f"{name} does not fit 64 bits: {x}")
     return None, int(x)
 
