@@ -357,3 +357,9 @@ def test_numbers_that_are_not_whole(x):
                  lambda: W.key_ranges(2, 8, 8, prefix=x), lambda: W.key_ranges(x, 8, 8), lambda: W.new_cache_8bit(2, x, 2, 64, device="cpu")):
         with pytest.raises(ValueError, match="whole number"):
             call()
+
+
+@pytest.mark.parametrize("start_all", [(1 << 63) - 1, (1 << 63) - 2, 1 << 62])
+def test_c_append_refuses_places_whose_end_64_bits_do_not_hold(start_all):
+    cls, sizes, optional = ENTRIES["wa_kv8_append"]
+    _refused("wa_kv8_append", _filled(cls, {**sizes, "cache": _cache8(), "start_all": start_all}, optional))

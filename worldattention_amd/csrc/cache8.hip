@@ -221,8 +221,8 @@ extern "C" int wa_kv8_append(const wa_kv8_append_args* a, void* stream) {
   const wa_cache8& c = a->cache;
   WA_CHECK_ARG(a->n >= 0 && a->n <= c.cap, "kv8_append: %lld tokens do not fit a cache of %lld", (long long)a->n, (long long)c.cap);
   if (a->n == 0) return WA_OK;
-  WA_CHECK_ARG(a->start || (a->start_all >= 0 && a->start_all + a->n <= c.cap), "kv8_append: tokens [%lld, %lld) do not fit a cache of %lld",
-               (long long)a->start_all, (long long)(a->start_all + a->n), (long long)c.cap);
+  WA_CHECK_ARG(a->start || (a->start_all >= 0 && a->start_all <= c.cap - a->n), "kv8_append: %lld tokens from %lld on do not fit a cache of %lld",
+               (long long)a->n, (long long)a->start_all, (long long)c.cap);
   WA_CHECK_ARG(a->dtype == WA_BF16 || a->dtype == WA_F32, "kv8_append: unknown dtype %d", a->dtype);
   const int64_t unit = a->dtype == WA_BF16 ? 8 : 4;
   auto rows16 = [&](const void* x, int64_t sb, int64_t st, int64_t sh) {
