@@ -459,3 +459,20 @@ def test_large_caps(dtype, d, n):
         far[:, 0, :, 0] = 2 * cap * d ** 0.5
         for x, lens in ((q, n + 50), (far, n)):
             _check_attention(W.attend_8bit(x, cache, lens, cap=cap), x, cache, [lens], cap=cap)
+
+
+def test_a_window_that_64_bits_barely_hold():
+    """The library's own call: a window and a number of newest tokens whose sum passes 64 bits are as all tokens."""
+    cache, _ = _filled(1, 130, 1, 64, 64, torch.int8, seed=60)
+    _lib = W.cache8._lib
+    c, _ = W.cache8._cache_args(cache)
+    want = W.kv_read_8bit(cache, 0, 130)
+    most = (1 << 63) - 1
+    for last, window, sink in ((0, 0, 0), (most, most, 0), (most, 5, most), (3, most, most)):
+        k, v = (torch.full((1, 130, 1, 64), math.nan, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        _lib.launch("wa_kv8_read", _lib.Kv8ReadArgs(c, k.data_ptr(), v.data_ptr(), _lib.WA_BF16, 130, None, 0, None, 130, last, window, sink),
+                    k.device)
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1]), (last, window, sink)
+    for start in (most, -most - 1, most - 100):      # all outside the cache: zeros
+        _lib.launch("wa_kv8_read", _lib.Kv8ReadArgs(c, k.data_ptr(), v.data_ptr(), _lib.WA_BF16, 130, None, start, None, -1, 0, 0, 0), k.device)
+        assert (k == 0).all() and (v == 0).all(), start

@@ -265,8 +265,10 @@ extern "C" int wa_kv8_read(const wa_kv8_read_args* a, void* stream) {
   p.code[0] = (const uint8_t*)c.k; p.code[1] = (const uint8_t*)c.v;
   p.scale[0] = c.k_scale; p.scale[1] = c.v_scale;
   p.out[0] = a->k_out; p.out[1] = a->v_out;
-  p.start = a->start; p.start_all = a->start_all; p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all;
-  p.last = a->last; p.window = a->window; p.sink = a->sink; p.cap = c.cap;
+  // beyond any cache numbers count as just beyond it: the kernel's sums of them stay in 64 bits
+  const int64_t far = (int64_t)1 << 31;
+  p.start = a->start; p.start_all = std::min(std::max(a->start_all, -far), far); p.kv_len = a->kv_len; p.kv_len_all = a->kv_len_all;
+  p.last = std::min(a->last, far); p.window = std::min(a->window, far); p.sink = std::min(a->sink, far); p.cap = c.cap;
   p.Hk = (int)c.Hk; p.bs = (int)c.block_size; p.D = (int)c.D;
   p.nb = (int)((c.cap + c.block_size - 1) / c.block_size);
   const int64_t chunks = a->n * c.Hk * (c.D / 16);
