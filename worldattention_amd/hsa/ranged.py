@@ -73,14 +73,15 @@ def key_ranges(batch: int, q_len: int, k_len: int, *, causal: bool = True, chunk
 
     * the keys up to its own; with ``chunk`` > 1 up to the end of its chunk of that many tokens, counted from the
       document's start (the frames of a video); all of them with ``causal=False``;
-    * with ``window`` only those of them less than ``window`` tokens away, and still the document's first ``sink``
-      tokens (as far as the rules above reach);
+    * with ``window``, of the keys before its own only those less than ``window`` tokens back (with ``causal=False`` of those ahead too; a
+      chunk's keys ahead are seen whatever the window), and still the document's first ``sink`` tokens (as far as the rules above
+      reach);
     * the document's first ``prefix`` tokens (int, or int32 ``[B]``) from wherever it sits.
 
     ``documents``: int32 borders on the GPU, ascending, ``[n]`` for all sequences or ``[B, n]`` (repeat the last border
     to fill up a row): document ``d`` is ``[border d, border d + 1)``, and tokens outside all of them are padding that sees
-    nothing and that nothing sees. ``lengths``: int32 ``[B]``, for a padded batch: one document of that many tokens. Without
-    either a sequence is one document. Keys from ``kv_len`` on are seen by no row.
+    nothing and that nothing sees (a document that begins before token 0 keeps its count from there). ``lengths``: int32 ``[B]``, for a
+    padded batch: one document of that many tokens. Without either a sequence is one document. Keys from ``kv_len`` on are seen by no row.
 
     ``given``: int32 ``[B or 1, q_len, 4]`` in place of all rules: rows' runs ``[0, 1)`` and ``[2, 3)`` (clamped to the keys; a
     key in both counts once; positions are used by a bias alone). A batch whose rules do not differ shares one set. Nothing is
