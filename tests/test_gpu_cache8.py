@@ -476,3 +476,41 @@ def test_a_window_that_64_bits_barely_hold():
     for start in (most, -most - 1, most - 100):      # all outside the cache: zeros
         _lib.launch("wa_kv8_read", _lib.Kv8ReadArgs(c, k.data_ptr(), v.data_ptr(), _lib.WA_BF16, 130, None, start, None, -1, 0, 0, 0), k.device)
         assert (k == 0).all() and (v == 0).all(), start
+
+
+def test_a_chunk_over_a_cache_whose_offsets_pass_32_bits():
+    """More rows than read codes: the far end is read back, and attended to at token offsets past 2^31."""
+    cap, hk, d = (1 << 25) // 8 + 300, 8, 128
+    n = W.cache8._FEW_ROWS + 4
+    g = torch.Generator().manual_seed(16)
+    cache = W.new_cache_8bit(1, cap, hk, d)
+    k, v = (torch.randn(1, n, hk, d, generator=g).bfloat16().to(DEV) for _ in range(2))
+    start = cap - n - 11
+    W.kv_append_8bit(cache, k, v, start)
+    first = start // 64 * 64
+    small = W.new_cache_8bit(1, cap - first, hk, d)
+    W.kv_append_8bit(small, k, v, start - first)
+    q = torch.randn(1, n - 1, hk, d, generator=g).bfloat16().to(DEV)
+    assert n - 1 > W.cache8._FEW_ROWS
+    kw = dict(window=40, cap=6.0)     # the first query's window begins among the tokens that were never written, in both
+    far = W.attend_8bit(q, cache, _i32([start + n]), **kw)
+    _check_attention(W.attend_8bit(q, small, start - first + n, **kw), q, small, [start - first + n], **kw)
+    lens = start - first + n
+    want_k, want_v = W.kv_read_8bit(small, 0, small["k"].shape[1], dtype=torch.float32)
+    want, want_lse = OC.attend(q[:, 64:], want_k, want_v, [lens], **kw)
+    mag, _ = OC.attend(q[:, 64:], want_k, want_v.abs(), [lens], **kw)
+    err = (far[0][:, 64:].cpu().double() - want).abs()
+    assert (err <= U * mag + U * want.abs() + 2.0 ** -11 * mag).all()
+    assert ((far[1][:, :, 64:].cpu().double() - want_lse).abs() <= 2.0 ** -12 + 2.0 ** -22 * want_lse.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,h", [(257, 1), (1, 257), (130, 2), (52, 5)])
+def test_every_number_of_rows_that_are_read_back(dtype, d, n, h):
+    """Chunks of just more rows than read codes, one token among them."""
+    assert n * h > W.cache8._FEW_ROWS
+    cache, g = _filled(1, 310, 1, d, 64, dtype, seed=n * h)
+    q = torch.randn(1, n, h, d, generator=g).bfloat16().to(DEV)
+    for kw in ({}, dict(window=40, sink=35, cap=4.0)):
+        _check_attention(W.attend_8bit(q, cache, 301, **kw), q, cache, [301], **kw)
