@@ -551,7 +551,7 @@ Cut cut(const wa_kv8_attend_args& a) {
   const int64_t at_once = a.cache.D == 128 ? 512 : c.rt == 1 ? 1024 : c.rt == 2 ? 768 : 512;
   c.per = (int)std::min<int64_t>(share(c.units * tiles, at_once), std::max<int64_t>(8, tiles));
   c.parts = (int)std::max<int64_t>(1, (tiles + c.per - 1) / c.per);
-  // Sequences of lengths that only the GPU knows, and more tiles than one round takes: cut along all sequences, so that workgroups bring as much each
+  // Sequences of lengths that only the GPU knows, or, whatever the lengths, more tiles than one round takes: cut along all sequences, so that workgroups bring as much each
   // (32 ragged ones of up to 32,768 tokens, 8 key heads of 128: 204 us; cut by the cache's length into parts of 64 tiles 268. 32 of 30,000 and heads
   // of 64: 251 and 311; 16 of 4,000, less than a round: 27 and 23).
   c.heads = a.cache.Hk;

@@ -109,7 +109,10 @@ __global__ void __launch_bounds__(256) ranges_kernel(RulesParams p) {
 
 // The order in which tiles of 128 rows, and of 128 keys, are worked on: those with the most steps first, so that what is left for the end is short
 // (8,190 tokens in 7 uneven documents, 16 heads: forward 115 us, 143 in row order; dK and dV 233, 287). One workgroup for the rows and one for the keys
-// of a set; a tile's place is the number of tiles before it, in ascending order where there are too many to count against each other.
+// of a set; a tile's place is the number of tiles before it, in ascending order where there are too many to count against each other. Once for a batch, it
+// costs 75 us at 32,760 causal rows, 1.3 ms at 131,072 and 22 ms at 524,288 (kOrderMax), about half that or less under windows and documents; it gains each call of uneven
+// documents its last tiles (32,760 rows, 4 heads of 64: 36 us of a forward's 302, 270 of a training call's 1,344; 131,072 rows: 140 of 2,408, 260 of 13,078;
+// 524,288 rows, one head: 0.9 ms of a forward's 9.8), causal masks and windows nothing.
 constexpr int kOrderMax = 4096;
 
 __global__ void __launch_bounds__(1024) order_kernel(Ranges p, RulesParams rules, int32_t* order, int sorted) {

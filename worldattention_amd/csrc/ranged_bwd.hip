@@ -1,8 +1,9 @@
 // Gradients of the ranged attention (ranged.hip). With P = exp(s - lse), dP = dO V^T and delta = rowsum(O dO) - dlse,
 //   dS = P (dP - delta),  dslope = -sum dS |t - j|,  dx = dS (1 - tanh^2),
 //   dQ = scale dx K,  dK = scale dx^T Q,  dV = P^T dO   (a shared key head: summed over its query heads).
-// Two launches: dQ (with the rows' statistics, and the slopes' gradients), then dK and dV. The scores are formed again in each of the last two; that costs two
-// products more than forming them once, and needs neither atomics nor partial sums of dQ in memory.
+// Two launches: dQ (with the rows' statistics, and the slopes' gradients in parts), then dK and dV; one more adds up the slopes' parts, and one
+// those of dK and dV where their steps are cut. Each of the two forms the scores (dQ twice where a row tile has few steps); that costs two
+// products more than forming them once for both, and needs neither atomics nor partial sums of dQ in memory.
 #include <algorithm>
 #include <type_traits>
 
@@ -14,7 +15,7 @@ namespace {
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 // dS is carried with this factor: the weights go from one wave to another as fp16 (11 significant bits), and 2^12 keeps weights down to
-// 2^-26 among its normal numbers. It is taken out where the gradients are written.
+// 2^-26 among its normal numbers (smaller ones are off by up to 2^-37). It is taken out where the gradients are written.
 constexpr float kLift = 4096.f;
 
 // Steps of 128 rows up to which dQ's launch walks them twice, at first for delta alone: rows that see few keys, whose dQ the output's delta leaves

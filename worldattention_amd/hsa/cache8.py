@@ -108,8 +108,8 @@ def kv_append_8bit(kv_cache: dict, k_new: torch.Tensor, v_new: torch.Tensor, wri
     the block keeps their scale or, if it needs a larger one, rounds their codes again at that: an int8 token is off by less
     than one step of its block's scale in all. What the block held behind the written tokens is given up (rejected drafts are
     overwritten this way). ``k_block_sums`` of the touched blocks are those of the keys that the codes stand for. A value that
-    is not finite makes its block's scale NaN, and so every token of the block, until the block is begun anew. Not
-    differentiable; in place, on the current stream, and fit for graph capture.
+    is not finite makes its block's scale NaN, and so every token of the block, until the block is begun anew; finite ones of more than
+    1.9 2^127 may be rounded up to 2^128, which reads as infinite. Not differentiable; in place, on the current stream, and fit for graph capture.
     """
     c, tensors = _cache_args(kv_cache)
     bsz, cap, hk, d = tensors[0].shape

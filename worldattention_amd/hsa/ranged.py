@@ -242,7 +242,9 @@ def ranged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ranges: 
     16 bits for the queries' gradients.
     Sums run in a fixed order. Gradients are formed from the fp32 log-sum-exp, so they lose accuracy where scores pass 2^16 in
     magnitude. Keys and values that none of 128 neighbouring rows sees are not read for them; a value that is
-    not finite reaches, besides the rows that see it, rows that share its tile of 128 rows by 64 keys.
+    not finite reaches, besides the rows that see it, rows that share its tile of 128 rows by 64 keys. In the gradients so do a key, for the
+    queries', and, for the keys' and values' of its tile of 64 rows by 128 keys, a query or an output's gradient (rows behind the last of 64 that
+    sees anything are not read).
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or v.shape != k.shape:
         raise ValueError(f"q must be [B, Lq, H, D] and k, v matching [B, Lk, Hk, D], got {tuple(q.shape)}, {tuple(k.shape)}, "
