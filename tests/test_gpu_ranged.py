@@ -398,7 +398,7 @@ def test_large_caps(d, cap, far):
     check(q, k, v, do, _ranges(b, n, n, dict()), OR.seen(b, n, n), cap=cap, slopes=torch.tensor([0.1, 0.01], device=DEV))
 
 
-@pytest.mark.parametrize("power,cap", [(-100, 5.0), (-60, 1e4), (-13, 1000.0), (-16, 1000.0), (40, 3.0), (80, 1e-6)])
+@pytest.mark.parametrize("power,cap", [(-100, 5.0), (-60, 1e4), (-13, 1000.0), (-16, 1000.0), (40, 3.0), (80, 1e-6), (18, 10.0), (19, 10.0), (21, 10.0), (28, 900.0), (-4, 10.0), (-9, 10.0)])
 def test_caps_at_any_scale(power, cap):
     """Scores of about 1 from small and large products."""
     b, n, h, hk, d = 1, 130, 2, 1, 64

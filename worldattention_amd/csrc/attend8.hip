@@ -575,11 +575,11 @@ void launch(const AttendParams& p, const Cut& c, hipStream_t s) {
 }
 
 template <typename Code>
-void launch(const AttendParams& p, const Cut& c, bool large, int64_t D, hipStream_t s) {
-  if (D == 128 && large) launch<Code, 128, kLargeCaps>(p, c, s);
-  else if (D == 128) launch<Code, 128, kSmallCaps>(p, c, s);
-  else if (large) launch<Code, 64, kLargeCaps>(p, c, s);
-  else launch<Code, 64, kSmallCaps>(p, c, s);
+void launch(const AttendParams& p, const Cut& c, bool other, int64_t D, hipStream_t s) {
+  if (D == 128 && other) launch<Code, 128, kOther>(p, c, s);
+  else if (D == 128) launch<Code, 128, kUsual>(p, c, s);
+  else if (other) launch<Code, 64, kOther>(p, c, s);
+  else launch<Code, 64, kUsual>(p, c, s);
 }
 
 }  // namespace
@@ -625,8 +625,8 @@ extern "C" int wa_kv8_attend(const wa_kv8_attend_args* a, void* stream) {
   p.bend = bend_of(scale, a->cap);
   p.part = (float*)a->workspace;
   hipStream_t s = (hipStream_t)stream;
-  const bool large = bends_of(a->cap, a->slopes) == kLargeCaps;
-  if (c.code == WA_CODE_INT8) launch<Int8>(p, k, large, c.D, s);
-  else launch<E4m3>(p, k, large, c.D, s);
+  const bool other = bends_of(scale, a->cap, a->slopes) == kOther;
+  if (c.code == WA_CODE_INT8) launch<Int8>(p, k, other, c.D, s);
+  else launch<E4m3>(p, k, other, c.D, s);
   return wa_launch_status("kv8_attend");
 }

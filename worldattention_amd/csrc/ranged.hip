@@ -483,8 +483,8 @@ template <int D>
 void launch_fwd(const FwdParams& p, Bends bends, hipStream_t s) {
   const int64_t grid = (int64_t)p.B * p.H * ((p.ranges.Lq + 127) / 128) * p.splits;
   if (bends == kPlain) hipLaunchKernelGGL((ranged_fwd_kernel<D, kPlain>), dim3((unsigned)grid), dim3(256), 0, s, p);
-  else if (bends == kSmallCaps) hipLaunchKernelGGL((ranged_fwd_kernel<D, kSmallCaps>), dim3((unsigned)grid), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((ranged_fwd_kernel<D, kLargeCaps>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  else if (bends == kUsual) hipLaunchKernelGGL((ranged_fwd_kernel<D, kUsual>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((ranged_fwd_kernel<D, kOther>), dim3((unsigned)grid), dim3(256), 0, s, p);
   if (p.splits > 1) {
     const int64_t n_rows = (int64_t)p.B * p.H * p.ranges.Lq, per = 2048 / D;
     hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)((n_rows + per - 1) / per)), dim3(256), 0, s, p, n_rows);
@@ -557,7 +557,7 @@ extern "C" int wa_ranged_fwd(const wa_ranged_fwd_args* a, void* stream) {
   WA_CHECK_ARG(p.splits == 1 || (a->workspace && wa_aligned16(a->workspace)), "ranged_fwd: a launch in %d parts needs a workspace", p.splits);
   p.part_o = (float*)a->workspace;
   p.part_ml = p.part_o + p.splits * a->B * a->H * a->Lq * a->D;
-  const Bends bends = bends_of(a->cap, a->slopes);
+  const Bends bends = bends_of(scale, a->cap, a->slopes);
   if (a->D == 128) launch_fwd<128>(p, bends, (hipStream_t)stream);
   else launch_fwd<64>(p, bends, (hipStream_t)stream);
   return wa_launch_status("ranged_fwd");

@@ -741,8 +741,8 @@ void launch_bwd(const BwdParams& p, hipStream_t s) {
 template <int D>
 void launch_bwd(const BwdParams& p, Bends bends, hipStream_t s) {
   if (bends == kPlain) launch_bwd<D, kPlain>(p, s);
-  else if (bends == kSmallCaps) launch_bwd<D, kSmallCaps>(p, s);
-  else launch_bwd<D, kLargeCaps>(p, s);
+  else if (bends == kUsual) launch_bwd<D, kUsual>(p, s);
+  else launch_bwd<D, kOther>(p, s);
 }
 
 }  // namespace
@@ -797,7 +797,7 @@ extern "C" int wa_ranged_bwd(const wa_ranged_bwd_args* a, void* stream) {
   p.parts = kv_parts(a->B, a->H, a->Hk, a->Lq, a->Lk);
   p.part_kv = (float*)((char*)a->workspace + (n * 12 + a->B * a->H * ((a->Lq + 127) / 128) * 4 + 15) / 16 * 16);
   hipStream_t s = (hipStream_t)stream;
-  const Bends bends = bends_of(a->cap, a->slopes);
+  const Bends bends = bends_of(p.scale, a->cap, a->slopes);
   if (a->D == 128) launch_bwd<128>(p, bends, s);
   else launch_bwd<64>(p, bends, s);
   return wa_launch_status("ranged_bwd");

@@ -104,31 +104,37 @@ struct RowRuns {
 // a wave's scores is asked once for a tile:
 //   kBias   no cap;
 //   kClose  |x| <= 0.3 cap: tanh(z) = z P(z^2), P of degree 3 fitted to 1.3e-8 of the value (a weighted least-squares fit of tanh(z) / z on
-//           [0, 0.09] with the leading 1 kept), with the powers of the scale in its coefficients: five instructions (a chunk of 1,024 rows over 8,256
-//           keys: 256 us, 275 with six). Left out where those powers would leave fp32;
-//   kNear   |x| <= cap / 2: the same of degree 4, on [0, 1/4] to 1.7e-8, in z itself, which any scale and cap leave in range: seven instructions;
+//           [0, 0.09] with the leading 1 kept), with the scale in its coefficients: five instructions (a chunk of 1,024 rows over 8,256 keys: 256 us, 275
+//           with kNear);
+//   kNear   |x| <= cap / 2: the same of degree 4, on [0, 1/4] to 1.7e-8: six instructions, more exact than kFar and half its work;
 //   kFar    e = exp(2 z), r = 1 / (e + 1): tanh = 1 - 2 r, off by a few 2^-24 of the cap wherever z is (e = inf gives r = 0); its derivative
 //           4 e r r, off by a few 2^-24 of itself;
-//   kBoth   kNear or kFar, score by score: for caps above kFarCap, a few 2^-24 of which (1e-4 there) show in small scores that share a tile with
-//           large ones. 8,190 causal tokens, 16 heads on 4 of 128, scores up to the cap everywhere: forward 488 us, with gradients 2,165; kFar 415
-//           and 1,755. Kernels are built for either side of kFarCap: as a fifth form in one kernel it put the forward's scores in scratch and
-//           cost the attention over codes 4%, whatever the cap.
-enum BendForm { kBias, kClose, kNear, kFar, kBoth };
-enum Bends { kPlain, kSmallCaps, kLargeCaps };   // no cap and no bias; a bias or a cap of at most kFarCap; a cap above it
+//   kAny    kNear's polynomial in z itself, which any scale and cap leave in fp32: seven instructions;
+//   kBoth   kAny or kFar, score by score.
+// The last two are of kernels of their own, for caps above kFarCap, a few 2^-24 of which (1e-4 there) show in small scores that share a tile with
+// large ones, and for ratios of scale and cap whose powers leave fp32. 8,190 causal tokens, 16 heads on 4 of 128, a cap of 1,100, scores up to it
+// everywhere: forward 488 us, with gradients 2,165; kFar 415 and 1,755. As further forms of one kernel they put the forward's scores in scratch and cost
+// the attention over codes 4% and learnt slopes 3%, whatever the cap.
+enum BendForm { kBias, kClose, kNear, kFar, kAny, kBoth };
+enum Bends { kPlain, kUsual, kOther };   // kernels of no cap and no bias; of kBias to kFar; of kAny and kBoth
 constexpr float kFarCap = 1024.f;
-static inline Bends bends_of(float cap, bool bias) { return cap > kFarCap ? kLargeCaps : cap > 0.f || bias ? kSmallCaps : kPlain; }
+// Powers of the ratio up to the eighth, times scale2 (at most 2^23), do not pass fp32; where the last coefficient falls below it, scores are below 2^-9 and
+// its term, 2^-14 of them at most, shows nowhere.
+static inline bool usual_cap(float scale, float cap) {
+  return !(cap > 0.f) || (cap <= kFarCap && scale >= 0x1p-15f * cap && scale <= 0x1p12f * cap);
+}
+static inline Bends bends_of(float scale, float cap, bool bias) { return !usual_cap(scale, cap) ? kOther : cap > 0.f || bias ? kUsual : kPlain; }
 struct Bend {
-  float close, near;           // largest |s| for kClose (below 0: none) and kNear
+  float close, near;           // largest |s| for kClose, and for kNear or kAny
   float scale2, in, in2, cap2; // scale log2(e); scale / cap; 2 scale / cap log2(e); cap log2(e) or 0
-  float c[4], c3[3], icap2;    // kNear's coefficients of z^2 and kClose's of s^2, and its powers, times scale2; 1 / cap2
+  float c[4], c3[3], icap2;    // kNear's and kClose's coefficients of s^2 (kAny's of z^2) and its powers, times scale2; 1 / cap2
   float slope2;                // slope log2(e)
   // The form for scores of at most `most`, the same in all of the wave's lanes.
   template <Bends BENDS>
   __device__ __forceinline__ BendForm form(float most) const {
-    if (BENDS == kLargeCaps) return __any(most > near) ? kBoth : kNear;
+    if (BENDS == kOther) return __any(most > near) ? kBoth : kAny;
     if (!(cap2 > 0.f)) return kBias;
-    if (!__any(most > close)) return kClose;
-    return __any(most > near) ? kFar : kNear;
+    return !__any(most > close) ? kClose : __any(most > near) ? kFar : kNear;
   }
   // The score before the bias, and the cap's derivative there.
   template <BendForm FORM>
@@ -136,22 +142,22 @@ struct Bend {
     turn = 1.f;
     if constexpr (FORM == kBias) {
       return s * scale2;
-    } else if constexpr (FORM == kClose || FORM == kNear) {
-      const float z = FORM == kClose ? s : s * in, u = z * z;
+    } else if constexpr (FORM == kBoth) {
+      float turn_far;
+      const float y = capped<kAny>(s, turn), far = capped<kFar>(s, turn_far);
+      const bool small = fabsf(s) <= near;
+      turn = small ? turn : turn_far;
+      return small ? y : far;
+    } else if constexpr (FORM != kFar) {
+      const float z = FORM == kAny ? s * in : s, u = z * z;
       const float p = FORM == kClose ? fmaf(u, fmaf(u, fmaf(u, c3[2], c3[1]), c3[0]), scale2) : fmaf(u, fmaf(u, fmaf(u, fmaf(u, c[3], c[2]), c[1]), c[0]), scale2);
       const float y = s * p, t = y * icap2;
       turn = fmaf(-t, t, 1.f);
       return y;
-    } else if constexpr (FORM == kFar) {
+    } else {
       const float e = __builtin_amdgcn_exp2f(s * in2), r = __builtin_amdgcn_rcpf(e + 1.f);
       turn = fminf(e, 0x1p100f) * 4.f * r * r;
       return fmaf(-2.f * cap2, r, cap2);
-    } else {
-      float turn_far;
-      const float y = capped<kNear>(s, turn), far = capped<kFar>(s, turn_far);
-      const bool small = fabsf(s) <= near;
-      turn = small ? turn : turn_far;
-      return small ? y : far;
     }
   }
   template <BendForm FORM>
@@ -164,22 +170,20 @@ static inline Bend bend_of(float scale, float cap) {
   b.scale2 = scale * WA_LOG2E;
   b.close = b.near = -1.f;
   if (cap > 0.f) {
-    const float in = scale / cap, u = in * in;
+    const float in = scale / cap, u = usual_cap(scale, cap) ? in * in : 1.f;
     b.in = in;
     b.in2 = 2.f * in * WA_LOG2E;
     b.cap2 = cap * WA_LOG2E;
     b.icap2 = 1.f / b.cap2;
+    b.close = 0.3f / in;
     b.near = fminf(0.5f / in, 3.4e38f);
-    b.c[0] = -0x1.5554d6p-2f * b.scale2;
-    b.c[1] = 0x1.10e9fcp-3f * b.scale2;
-    b.c[2] = -0x1.b28c5ep-5f * b.scale2;
-    b.c[3] = 0x1.1a7b9cp-6f * b.scale2;
-    if (in >= 0x1p-15f && in <= 0x1p15f) {   // the last coefficient is above 2^-130: even as a subnormal it has the bits that show
-      b.close = 0.3f / in;
-      b.c3[0] = -0x1.55549ep-2f * u * b.scale2;
-      b.c3[1] = 0x1.10b012p-3f * u * u * b.scale2;
-      b.c3[2] = -0x1.9c99a8p-5f * u * u * u * b.scale2;
-    }
+    b.c3[0] = -0x1.55549ep-2f * u * b.scale2;
+    b.c3[1] = 0x1.10b012p-3f * u * u * b.scale2;
+    b.c3[2] = -0x1.9c99a8p-5f * u * u * u * b.scale2;
+    b.c[0] = -0x1.5554d6p-2f * u * b.scale2;
+    b.c[1] = 0x1.10e9fcp-3f * u * u * b.scale2;
+    b.c[2] = -0x1.b28c5ep-5f * u * u * u * b.scale2;
+    b.c[3] = 0x1.1a7b9cp-6f * u * u * u * u * b.scale2;
   }
   return b;
 }
@@ -197,8 +201,8 @@ template <BendForm F> struct FormTag { static constexpr BendForm value = F; };
 template <Bends BENDS, typename Run>
 __device__ __forceinline__ void by_form(const Bend& bend, float most, const Run& run) {
   const BendForm form = bend.form<BENDS>(most);
-  if constexpr (BENDS == kLargeCaps) {
-    if (form == kNear) run(FormTag<kNear>{});
+  if constexpr (BENDS == kOther) {
+    if (form == kAny) run(FormTag<kAny>{});
     else run(FormTag<kBoth>{});
   } else {
     if (form == kBias) run(FormTag<kBias>{});
