@@ -3,7 +3,7 @@
 Bounds as those of ``test_gpu_ranged.py``, with u = 2^-8 (half a step of bf16): dS is off by P u E (the output's rounding in delta, E = sum
 |o| |do|), by its own rounding u |dS|, and by 2^-11 P (|dP| + |delta|) for the weights (scores of at most 2^8 here); gradients are rounded once more. For
 the keys' gradient the weights pass as fp16 with a factor of 2^12: 2^-11 of a weight, or half of fp16's smallest step, 2^-25 2^-12 = 2^-37,
-where a weight is below 2^-26, as most are where the farthest keys take it all."""
+where a weight times the cap's derivative is below 2^-26, as most are where the farthest keys take it all."""
 import pytest
 import torch
 
@@ -41,7 +41,7 @@ def test_over_a_ragged_last_tile(d, n, h, hk, cap, slopes):
         small = torch.where(p > 0, 2.0 ** -37 * wide, 0.0)
         bent = (turn + 2.0 ** -20) * d ** -0.5
         bounds = [torch.matmul(off * bent, kh.abs()).transpose(1, 2),
-                  group(torch.matmul(((off + small) * bent).transpose(-1, -2).contiguous(), qh.abs())),
+                  group(torch.matmul((off * bent + small * d ** -0.5).transpose(-1, -2).contiguous(), qh.abs())),
                   group(torch.matmul(p.transpose(-1, -2).contiguous(), doh.abs())) * (U + 2.0 ** -11),
                   (2.0 ** -11 * p * wide * far).sum((0, 2, 3))]
     for name, got, w, bound in zip(("dq", "dk", "dv", "dslopes"), grads, want, bounds):

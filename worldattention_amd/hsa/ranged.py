@@ -239,7 +239,8 @@ def ranged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ranges: 
     A row that sees nothing gets 0 and a log-sum-exp of ``-inf``, and gradients of 0. Differentiable once in ``q``, ``k``, ``v`` and
     ``slopes``, through both results; the gradient of a shared key head is the sum over its query heads. Sums and softmax
     statistics are fp32; weights are rounded to bf16 once, for the product that they enter, scores' gradients to bf16 for the keys' and to
-    16 bits for the queries' gradients.
+    16 bits for the queries' gradients (for the keys', weights times the cap's derivative below 2^-26
+    are off by up to 2^-37).
     Sums run in a fixed order. Gradients are formed from the fp32 log-sum-exp, so they lose accuracy where scores pass 2^16 in
     magnitude. Keys and values that none of 128 neighbouring rows sees are not read for them; a value that is
     not finite reaches, besides the rows that see it, rows that share its tile of 128 rows by 64 keys. In the gradients so do a key, for the
